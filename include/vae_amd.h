@@ -558,6 +558,36 @@ int vae_adamw_step_bf16(float* params, const float* grads, float* exp_avg, float
 int vae_l1_penalty(const float* params, float* grads, int64_t n, const vae_adamw_segment* segments, int n_segments,
                    double grad_coeff, float* workspace, int64_t workspace_bytes, float* sum_out, void* stream);
 
+/* ---- AdamW over many separate tensors ----------------------------------------------------------
+ * One step (same update as vae_adamw_step: decoupled decay, bias correction, optional clipping by the global norm) over
+ * n_tensors contiguous tensors of fp32, bf16 or fp16, each with a gradient of its own type.  The moments are flat: tensor k
+ * owns the blocks of VAE_ADAMW_BLOCK elements from tensors[k].first_block on (the last one padded), n_blocks in all.
+ * state_bits = 32: exp_avg / exp_avg_sq are float (n_blocks * VAE_ADAMW_BLOCK).
+ * state_bits = 8: they are OCP e4m3 bytes, exp_avg_sq holds the ROOT of the second moment, and a code times
+ * scales[block] (exp_avg) / scales[n_blocks + block] (exp_avg_sq) is the value.  The first moment is rounded to nearest, the
+ * root up or down at random from a hash of (seed, step, flat element index): the same call gives the same bits.  A block with
+ * a moment that is not finite decodes as NaN throughout.
+ * master (nullable): float weights in the state's layout, which are updated instead; params receive their rounding and are
+ * not read.  Weights are rounded to nearest.  A norm that is not finite reaches every weight, as with
+ * torch.nn.utils.clip_grad_norm_.  Tensors that share memory with each other or with the state are rejected, and so are
+ * tensors that share blocks.  The tensor array is read during the call only.
+ * workspace: needed when max_grad_norm > 0 or grad_norm_out is not null.                                            */
+#define VAE_ADAMW_BLOCK 256
+enum { VAE_ADAMW_F32 = 0, VAE_ADAMW_BF16 = 1, VAE_ADAMW_F16 = 2 };
+typedef struct {
+  void* param;
+  const void* grad;
+  int64_t n;
+  int64_t first_block;
+  float weight_decay;
+  int32_t dtype;
+} vae_adamw_tensor;
+int64_t vae_adamw_multi_workspace_bytes(int64_t n_tensors);
+int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensors, int state_bits, void* exp_avg, void* exp_avg_sq,
+                    float* scales, int64_t n_blocks, float* master, double lr, double beta1, double beta2, double eps,
+                    int64_t step, double max_grad_norm, double grad_scale, uint64_t seed, void* workspace,
+                    int64_t workspace_bytes, float* grad_norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

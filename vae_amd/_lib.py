@@ -17,6 +17,9 @@ X_F32, X_U8 = 0, 1   # enum { VAE_X_F32, VAE_X_U8 } of include/vae_amd.h
 
 # name -> (restype, argtypes); mirrors include/vae_amd.h one to one
 SIGNATURES = {
+    "vae_adamw_multi_workspace_bytes": (_i64, [_i64]),
+    "vae_adamw_multi": (_i32, [_ptr, _i64, _i32, _ptr, _ptr, _ptr, _i64, _ptr, C.c_double, C.c_double, C.c_double, C.c_double, _i64,
+                               C.c_double, C.c_double, C.c_uint64, _ptr, _i64, _ptr, _ptr]),
     "vae_version": (_i32, []),
     "vae_arch": (C.c_char_p, []),
     "vae_last_error": (C.c_char_p, []),
@@ -112,6 +115,12 @@ _fp = C.POINTER(C.c_float)
 class AdamWSegment(C.Structure):
     """vae_adamw_segment of include/vae_amd.h"""
     _fields_ = [("begin", C.c_int64), ("end", C.c_int64), ("weight_decay", C.c_float)]
+
+
+class AdamWTensor(C.Structure):
+    """vae_adamw_tensor of include/vae_amd.h"""
+    _fields_ = [("param", _ptr), ("grad", _ptr), ("n", C.c_int64), ("first_block", C.c_int64), ("weight_decay", C.c_float),
+                ("dtype", C.c_int32)]
 
 
 class StepConfig(C.Structure):

@@ -11,7 +11,8 @@ of steps already taken, exactly like ``LambdaLR`` stepped once per optimiser ste
 from __future__ import annotations
 
 import ctypes as C
-from typing import Callable, Dict, Iterable, List, Optional, Tuple
+import struct
+from typing import Callable, Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -215,3 +216,191 @@ class L1Penalty:
                                      self.total.data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream))
         _lib.check(rc, "l1_penalty")
         return self.total[0]
+
+
+ADAMW_BLOCK = 256                      # VAE_ADAMW_BLOCK: elements of a block of the flat state
+_ADAMW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def adamw_blocks(n: int) -> int:
+    """Blocks of the flat state that a tensor of ``n`` elements owns."""
+    return -(-n // ADAMW_BLOCK)
+
+
+def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], exp_avg: torch.Tensor,
+                        exp_avg_sq: torch.Tensor, *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.998),
+                        eps: float = 1e-7, weight_decay: Union[float, Sequence[float]] = 0.0, scales: Optional[torch.Tensor] = None,
+                        master: Optional[torch.Tensor] = None, max_grad_norm: float = 0.0, grad_scale: float = 1.0, seed: int = 0,
+                        return_norm: bool = False) -> Optional[torch.Tensor]:
+    """One AdamW step in place over ``params`` (contiguous fp32 / bf16 / fp16 tensors on one GPU) in one launch for every 96 of
+    them (include/vae_amd.h, ``vae_adamw_multi``).  A parameter whose gradient is None is left alone, with its state.
+
+    The state is flat, in the order of ``params``: every tensor starts a new block of ``ADAMW_BLOCK`` elements.  fp32
+    ``exp_avg`` / ``exp_avg_sq``: 32-bit moments.  float8_e4m3fn ones: 8-bit moments, where ``exp_avg_sq`` holds the ROOT of
+    the second moment and a code times ``scales[0 | 1, block]`` is the value; the root is rounded at random by
+    ``(seed, step, element)``, so equal calls give equal bits.  ``master``: fp32 weights in the same layout, which are updated in
+    the parameters' place; the parameters then receive their rounding.  Start all of them at zero (``master``: at the
+    parameters).
+
+    ``step`` counts from 1.  ``weight_decay``: one value, or one for each tensor.  ``max_grad_norm`` > 0 clips by the norm over
+    all gradients; ``return_norm`` returns that norm (of ``grad_scale`` times the gradients, before clipping) as a 1-element
+    tensor.  The learning rate and the step count are host values: a captured graph would repeat them, so capturing raises."""
+    lib = _lib.load()
+    n = len(params)
+    if len(grads) != n:
+        raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(grads)} grads")
+    dev = exp_avg.device
+    if dev.type != "cuda":
+        raise RuntimeError("vae_amd.optim.multi_tensor_adamw_: the state must live on the GPU (no CPU fallback)")
+    bits = 8 if exp_avg.dtype == torch.float8_e4m3fn else 32
+    if exp_avg.dtype not in (torch.float8_e4m3fn, torch.float32) or exp_avg_sq.dtype != exp_avg.dtype:
+        raise TypeError("vae_amd.optim.multi_tensor_adamw_: exp_avg and exp_avg_sq must both be float32 or both float8_e4m3fn")
+    if isinstance(weight_decay, (int, float)):
+        decay: Sequence[float] = [float(weight_decay)] * n
+    else:
+        decay = weight_decay
+        if len(decay) != n:
+            raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(decay)} weight decays")
+    table: List[Union[int, float]] = []
+    at = live = 0
+    for p, g, wd in zip(params, grads, decay):
+        count = p.numel()
+        if g is not None and count:
+            kind = _ADAMW_DTYPES.get(p.dtype)
+            if kind is None or g.dtype != p.dtype:
+                raise TypeError(f"vae_amd.optim.multi_tensor_adamw_: a parameter of {p.dtype} with a gradient of {g.dtype}; "
+                                "float32, bfloat16 and float16 are supported, both of the same type")
+            if p.device != dev or g.device != dev:
+                raise RuntimeError(f"vae_amd.optim.multi_tensor_adamw_: parameters, gradients and state must be on {dev}")
+            if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
+                raise ValueError("vae_amd.optim.multi_tensor_adamw_: parameters and gradients must be contiguous and of one shape")
+            table += (p.data_ptr(), g.data_ptr(), count, at, wd, kind)
+            live += 1
+        at += -(-count // ADAMW_BLOCK)
+    for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
+        if t is None:
+            continue
+        if t.numel() != at * ADAMW_BLOCK or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {name} must hold {at * ADAMW_BLOCK} contiguous elements on {dev}")
+    if master is not None and master.dtype != torch.float32:
+        raise TypeError("vae_amd.optim.multi_tensor_adamw_: master must be float32")
+    if bits == 8:
+        if scales is None or scales.dtype != torch.float32 or scales.numel() != 2 * at or scales.device != dev or not scales.is_contiguous():
+            raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: 8-bit moments need contiguous float32 scales (2, {at}) on {dev}")
+    clip = max_grad_norm > 0 or return_norm
+    norm = None
+    with torch.cuda.device(dev):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("vae_amd.optim.multi_tensor_adamw_: step and learning rate are host values; a captured step would repeat them")
+        if return_norm:
+            norm = torch.zeros(1, dtype=torch.float32, device=dev)
+        if not live:
+            return norm
+        nbytes = lib.vae_adamw_multi_workspace_bytes(live) if clip else 0
+        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev) if clip else None
+        rc = lib.vae_adamw_multi(struct.pack("=" + "QQqqfi" * live, *table), live, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+                                 scales.data_ptr() if bits == 8 else None, at, None if master is None else master.data_ptr(), float(lr),
+                                 float(betas[0]), float(betas[1]), float(eps), int(step), float(max_grad_norm), float(grad_scale),
+                                 int(seed) & (2 ** 64 - 1), None if ws is None else ws.data_ptr(), nbytes,
+                                 None if norm is None else norm.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "multi_tensor_adamw_")
+    return norm
+
+
+class MultiTensorAdamW:
+    """AdamW over separate tensors of any of the three float types, beside ``FusedAdamW`` (which owns ONE fp32 arena): moments
+    in 8 or 32 bits, optional fp32 master weights, the reference's betas / eps by default (task.py:534-553).
+
+    ``params``: an iterable of tensors, or of dicts ``{"params": [...], "weight_decay": ...}``.  ``state_bits`` 8 keeps two bytes
+    and 1/32 of a byte per parameter in place of eight (see ``multi_tensor_adamw_``)."""
+
+    def __init__(self, params: Iterable, lr: float = 5e-4, betas: Tuple[float, float] = (0.9, 0.998), eps: float = 1e-7,
+                 weight_decay: float = 0.0, max_grad_norm: float = 0.0, state_bits: int = 8, master_weights: bool = False,
+                 lr_lambda: Optional[Callable[[int], float]] = None, seed: int = 0):
+        self.params: List[torch.Tensor] = []
+        self.decay: List[float] = []
+        for group in params:
+            members, wd = (list(group["params"]), group.get("weight_decay", weight_decay)) if isinstance(group, dict) else ([group], weight_decay)
+            self.params += members
+            self.decay += [float(wd)] * len(members)
+        if not self.params:
+            raise ValueError("vae_amd: MultiTensorAdamW got no parameters")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("vae_amd: MultiTensorAdamW got a parameter twice")
+        if state_bits not in (8, 32):
+            raise ValueError(f"vae_amd: MultiTensorAdamW: state_bits must be 8 or 32, got {state_bits}")
+        dev = self.params[0].device
+        for p in self.params:
+            if p.dtype not in _ADAMW_DTYPES:
+                raise TypeError(f"vae_amd: MultiTensorAdamW: parameters of {p.dtype} are not supported")
+            if not p.is_contiguous():
+                raise ValueError("vae_amd: MultiTensorAdamW needs contiguous parameters")
+            if not p.is_cuda or p.device != dev:
+                raise RuntimeError("vae_amd: MultiTensorAdamW needs all parameters on one GPU (there is no CPU fallback)")
+        self.base_lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
+        self.max_grad_norm = float(max_grad_norm) if max_grad_norm else 0.0
+        self.lr_lambda, self.seed, self.state_bits = lr_lambda, int(seed), state_bits
+        self.steps = 0
+        self.starts, blocks = [], 0
+        for p in self.params:
+            self.starts.append(blocks * ADAMW_BLOCK)
+            blocks += adamw_blocks(p.numel())
+        kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        self.exp_avg = torch.zeros(blocks * ADAMW_BLOCK, dtype=torch.uint8 if state_bits == 8 else kind, device=dev).view(kind)
+        self.exp_avg_sq = torch.zeros_like(self.exp_avg.view(torch.uint8)).view(kind)
+        self.scales = torch.zeros(2, blocks, dtype=torch.float32, device=dev) if state_bits == 8 else None
+        self.master = None
+        if master_weights:
+            self.master = torch.zeros(blocks * ADAMW_BLOCK, dtype=torch.float32, device=dev)
+            self.refresh_master()
+        self.grad_norm: Optional[torch.Tensor] = None
+
+    def refresh_master(self) -> None:
+        """Take the master weights from the parameters as they are now (after anything but ``step()`` changed them)."""
+        if self.master is not None:
+            for p, b in zip(self.params, self.starts):
+                self.master[b:b + p.numel()].copy_(p.detach().reshape(-1))
+
+    @property
+    def lr(self) -> float:
+        """Learning rate of the NEXT step."""
+        return self.base_lr * (float(self.lr_lambda(self.steps)) if self.lr_lambda is not None else 1.0)
+
+    def zero_grad(self) -> None:
+        for p in self.params:
+            p.grad = None
+
+    def step(self, grad_scale: float = 1.0) -> None:
+        """Update from ``p.grad``; ``grad_norm`` holds the unclipped norm afterwards when clipping is on."""
+        self.grad_norm = multi_tensor_adamw_(self.params, [p.grad for p in self.params], self.exp_avg, self.exp_avg_sq,
+                                             step=self.steps + 1, lr=self.lr, betas=self.betas, eps=self.eps, weight_decay=self.decay,
+                                             scales=self.scales, master=self.master, max_grad_norm=self.max_grad_norm,
+                                             grad_scale=grad_scale, seed=self.seed, return_norm=self.max_grad_norm > 0)
+        self.steps += 1
+
+    def moments(self, index: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """-> (exp_avg, exp_avg_sq) of parameter ``index`` in fp32 and in its shape, whatever they are held in."""
+        p, b = self.params[index], self.starts[index]
+        n = p.numel()
+        m, v = (t[b:b + adamw_blocks(n) * ADAMW_BLOCK].float() for t in (self.exp_avg, self.exp_avg_sq))
+        if self.state_bits == 8:
+            k = b // ADAMW_BLOCK
+            m, v = ((t.view(-1, ADAMW_BLOCK) * s[k:k + adamw_blocks(n), None]).view(-1) for t, s in zip((m, v), self.scales))
+            v = v * v
+        return m[:n].view(p.shape), v[:n].view(p.shape)
+
+    def state_dict(self) -> Dict[str, object]:
+        return {"steps": self.steps, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
+                "master": self.master}
+
+    def load_state_dict(self, sd: Dict[str, object]) -> None:
+        """State of an optimiser over the same parameters with the same ``state_bits``."""
+        mine = {k: getattr(self, k) for k in ("exp_avg", "exp_avg_sq", "scales", "master")}
+        for k, t in mine.items():
+            s = sd[k]
+            if (t is None) != (s is None) or (t is not None and (t.shape != s.shape or t.dtype != s.dtype)):
+                raise ValueError(f"vae_amd: MultiTensorAdamW.load_state_dict: {k} does not fit (other parameters, state_bits or master_weights)")
+        for k, t in mine.items():
+            if t is not None:
+                t.copy_(sd[k])
+        self.steps, self.seed = int(sd["steps"]), int(sd["seed"])
