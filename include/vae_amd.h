@@ -588,6 +588,45 @@ int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensors, int stat
                     int64_t step, double max_grad_norm, double grad_scale, uint64_t seed, void* workspace,
                     int64_t workspace_bytes, float* grad_norm_out, void* stream);
 
+/* ---- norms around a residual block, with its gate and residual scale ---------------------------
+ * u = norm(b) * post_weight + post_bias (b itself where post_weight is null), y = r + scale * act(gate) * u,
+ * h = norm(y) * norm_weight + norm_bias, over N rows of D <= VAE_GATED_NORM_MAX_D columns (LayerNorm or RMS norm, FCLayers'
+ * and ResidualLayer's glue, modules.py:45-71, 112-114).  Rows are fp32, bf16 or fp16 (VAE_ADAMW_F32 / BF16 / F16) with row
+ * strides ld_* in elements; y, h, dr, db and dgate are dense.  The vectors over columns are of the rows' type, or float where
+ * vectors_f32 is set; null ones are 1 (weights, scale) or 0 (biases).  gate: none, one value per row ((N, 1), row stride
+ * ld_gate) or one per element.  y is rounded to its type before h is formed.  Arithmetic and sums in 32 bits.
+ * stats (N, 4) floats, 16-byte aligned: mean and 1 / sigma of b and of y; the forward pass writes it (nullable there), the
+ * backward pass reads it with b, gate, y and the gradients dy, dh (null = 0) and writes dr, db, dgate (nullable) and those of
+ * the column gradients that are not null (same bits every time: no atomics; workspace only for these).                      */
+#define VAE_GATED_NORM_MAX_D 16384
+enum { VAE_NORM_RMS = 0, VAE_NORM_LAYER = 1 };
+enum { VAE_GATE_NONE = 0, VAE_GATE_ROW = 1, VAE_GATE_FULL = 2 };
+enum { VAE_GATE_IDENTITY = 0, VAE_GATE_SIGMOID = 1, VAE_GATE_TANH = 2 };
+typedef struct {
+  int64_t N, D;
+  int32_t dtype, vectors_f32, kind, gate_mode, act;
+  float eps;
+  const void* r;
+  int64_t ld_r;
+  const void* b;
+  int64_t ld_b;
+  const void* gate;
+  int64_t ld_gate;
+  const void *post_weight, *post_bias, *scale, *norm_weight, *norm_bias;
+  void* y;                       /* written by the forward pass, read by the backward pass */
+  void* h;
+  float* stats;
+  const void* dy;
+  int64_t ld_dy;
+  const void* dh;
+  int64_t ld_dh;
+  void *dr, *db, *dgate;
+  void *dnorm_weight, *dnorm_bias, *dscale, *dpost_weight, *dpost_bias;
+} vae_gated_norm;
+int64_t vae_gated_norm_workspace_bytes(int64_t N, int64_t D, int dtype);
+int vae_gated_norm_fwd(const vae_gated_norm* args, void* stream);
+int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,9 @@ X_F32, X_U8 = 0, 1   # enum { VAE_X_F32, VAE_X_U8 } of include/vae_amd.h
 
 # name -> (restype, argtypes); mirrors include/vae_amd.h one to one
 SIGNATURES = {
+    "vae_gated_norm_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "vae_gated_norm_fwd": (_i32, [_ptr, _ptr]),
+    "vae_gated_norm_bwd": (_i32, [_ptr, _ptr, _i64, _ptr]),
     "vae_adamw_multi_workspace_bytes": (_i64, [_i64]),
     "vae_adamw_multi": (_i32, [_ptr, _i64, _i32, _ptr, _ptr, _ptr, _i64, _ptr, C.c_double, C.c_double, C.c_double, C.c_double, _i64,
                                C.c_double, C.c_double, C.c_uint64, _ptr, _i64, _ptr, _ptr]),
@@ -121,6 +124,16 @@ class AdamWTensor(C.Structure):
     """vae_adamw_tensor of include/vae_amd.h"""
     _fields_ = [("param", _ptr), ("grad", _ptr), ("n", C.c_int64), ("first_block", C.c_int64), ("weight_decay", C.c_float),
                 ("dtype", C.c_int32)]
+
+
+class GatedNorm(C.Structure):
+    """vae_gated_norm of include/vae_amd.h"""
+    _fields_ = [("N", _i64), ("D", _i64), ("dtype", C.c_int32), ("vectors_f32", C.c_int32), ("kind", C.c_int32), ("gate_mode", C.c_int32),
+                ("act", C.c_int32), ("eps", _f32), ("r", _ptr), ("ld_r", _i64), ("b", _ptr), ("ld_b", _i64), ("gate", _ptr), ("ld_gate", _i64),
+                ("post_weight", _ptr), ("post_bias", _ptr), ("scale", _ptr), ("norm_weight", _ptr), ("norm_bias", _ptr),
+                ("y", _ptr), ("h", _ptr), ("stats", _ptr), ("dy", _ptr), ("ld_dy", _i64), ("dh", _ptr), ("ld_dh", _i64),
+                ("dr", _ptr), ("db", _ptr), ("dgate", _ptr), ("dnorm_weight", _ptr), ("dnorm_bias", _ptr), ("dscale", _ptr),
+                ("dpost_weight", _ptr), ("dpost_bias", _ptr)]
 
 
 class StepConfig(C.Structure):

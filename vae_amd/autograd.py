@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -141,3 +142,32 @@ class LogLikFn(Function):
             red = ops.colsum_into(dth, torch.zeros(dth.shape[1], dtype=torch.float32, device=dth.device))
             dth = red.view(ctx.theta_shape)
         return None, dmu, dth, dpi, None
+
+
+GATED_NORM_VECTORS = ("post_weight", "post_bias", "scale", "norm_weight", "norm_bias")
+
+
+class GatedResidualNormFn(Function):
+    """(y, h) = (r + scale * act(gate) * norm(b), norm(y)) over rows, in one pass each way (ops.gated_norm_fwd / _bwd).
+    y and the (N, 4) row statistics are kept for the backward pass; r is not."""
+
+    @staticmethod
+    def forward(ctx, r, b, gate, post_weight, post_bias, scale, norm_weight, norm_bias, kind, gate_act, eps):
+        vectors = dict(zip(GATED_NORM_VECTORS, (post_weight, post_bias, scale, norm_weight, norm_bias)))
+        y, h, stats = ops.gated_norm_fwd(r, b, gate, **vectors, kind=kind, gate_act=gate_act, eps=eps)
+        ctx.how = dict(kind=kind, gate_act=gate_act, eps=eps)
+        ctx.save_for_backward(y, b, stats, gate, *vectors.values())
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        y, b, stats, gate, *vectors = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 11
+        dy, dh = (None if t is None else (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()) for t in (dy, dh))
+        names = ("r", "b", "gate") + GATED_NORM_VECTORS
+        want = [n for n, need in zip(names, ctx.needs_input_grad) if need]
+        g = ops.gated_norm_bwd(dy, dh, y, b, stats, gate, **dict(zip(GATED_NORM_VECTORS, vectors)), **ctx.how, want=want)
+        return tuple(g.get(n) if n in want else None for n in names) + (None, None, None)

@@ -1,0 +1,480 @@
+// The two norms around a residual block, its gate and its residual scale in one pass, and the backward pass (gfx950).
+//
+//   u = norm(b) * gp + bp   (or b)        y = r + s * act(gate) * u        h = norm(y) * gn + bn
+//
+// norm is (t - mean) / sqrt(var + eps) or t / sqrt(mean t^2 + eps); y is rounded to its type before h is formed, so that the
+// backward pass, which reads y again, works on the values that the forward pass used.  With dt the gradient that reaches y,
+//
+//   dt = dy + N_y(dh * gn)     dr = dt     dgate = dt * s * u * act'     ds = sum dt * act * u
+//   dgp = sum dt * act * s * nb    dbp = sum dt * act * s    db = N_b(dt * act * s * gp)    dgn = sum dh * ny    dbn = sum dh
+//   N(d) = (d - n * mean(d * n) [- mean d]) / sigma
+//
+// HBM-bound: the forward pass reads r, b and the gate and writes y and h, the backward pass reads y, b, the gate, dy and dh and
+// writes dr, db and dgate, each once: a row lives in registers from its loads to its stores, in 32 bits.  A wave takes a row of
+// up to 64 16-byte pieces, a workgroup of up to 1024 threads a longer one, one to four pieces per thread.  A workgroup walks
+// over rows; the gradients of the vectors over columns are summed in registers over its rows, written once per workgroup, and
+// added up in a second launch in a fixed order (no atomics: same bits every time).
+#include "../../include/vae_amd.h"
+#include "common.h"
+
+namespace {
+
+typedef vae_gated_norm Args;
+constexpr int N_COL = 5;                 // column sums: d gn, d bn, d s, d gp, d bp
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// rows of an odd width start at any element: the hardware takes 16-byte accesses at any address, only the type has to say so
+typedef u4 u4_any __attribute__((aligned(2)));
+
+template <typename T> constexpr int PIECE = 16 / (int)sizeof(T);
+
+template <typename T> union Raw {
+  u4 q;
+  T t[PIECE<T>];
+};
+
+template <typename T> __device__ __forceinline__ Raw<T> load(const T* __restrict__ row, int c, int D) {
+  Raw<T> w;
+  if (c + PIECE<T> <= D) {
+    w.q = *reinterpret_cast<const u4_any*>(row + c);
+  } else {
+    w.q = (u4)0;
+#pragma unroll
+    for (int j = 0; j < PIECE<T>; ++j)
+      if (c + j < D) w.t[j] = row[c + j];
+  }
+  return w;
+}
+template <typename T> __device__ __forceinline__ void store(T* __restrict__ row, int c, int D, const Raw<T>& w) {
+  if (c + PIECE<T> <= D) {
+    *reinterpret_cast<u4_any*>(row + c) = w.q;
+  } else {
+#pragma unroll
+    for (int j = 0; j < PIECE<T>; ++j)
+      if (c + j < D) row[c + j] = w.t[j];
+  }
+}
+// A vector over columns, of the rows' type or float; absent: `none` throughout.  They are read again for every row, with the
+// row's own loads and from the caches: that costs a tenth of what the CU's share of the L2 can deliver, and held in registers
+// in 32 bits they would halve the waves of the backward pass.
+template <typename V, int P> struct Vec {
+  V v[P];
+  __device__ __forceinline__ float operator[](int j) const { return (float)v[j]; }
+};
+template <typename V, int P> __device__ __forceinline__ Vec<V, P> column(const void* p, int c, int D, float none) {
+  union {
+    Vec<V, P> o;
+    u4 q[P * sizeof(V) / 16];
+  } w;
+  const V* src = reinterpret_cast<const V*>(p) + c;
+  if (p && c + P <= D) {
+#pragma unroll
+    for (int i = 0; i < (int)(P * sizeof(V) / 16); ++i) w.q[i] = reinterpret_cast<const u4_any*>(src)[i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < P; ++j) w.o.v[j] = p && c + j < D ? src[j] : (V)none;
+  }
+  return w.o;
+}
+
+// sums of K values over the row's threads: a wave by DPP, a workgroup of NW waves through `red` (one barrier; the caller
+// alternates between two buffers, so that a fast wave does not overwrite what a slow one still reads)
+template <int NW, int K> __device__ __forceinline__ void row_sums(float (&v)[K], float* __restrict__ red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum_dpp(v[k]);
+  if (NW > 1) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[k * NW + w] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) s += red[k * NW + i];
+      v[k] = s;
+    }
+  }
+}
+
+__device__ __forceinline__ float sigmoid_f(float v) { return 1.f / (1.f + expf(-v)); }
+__device__ __forceinline__ void act_of(int act, float g, float& a, float& da) {
+  if (act == VAE_GATE_SIGMOID) {
+    a = sigmoid_f(g);
+    da = a * (1.f - a);
+  } else if (act == VAE_GATE_TANH) {
+    a = tanhf(g);
+    da = 1.f - a * a;
+  } else {
+    a = g;
+    da = 1.f;
+  }
+}
+
+// NW waves share a row (NW = 1: four rows to a workgroup), ITEMS pieces per thread
+template <typename T, typename V, int NW, int ITEMS>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void gated_norm_fwd_kernel(Args a) {
+  constexpr int P = PIECE<T>, TPR = NW * 64, RPW = NW == 1 ? 4 : 1;
+  __shared__ float red[2][2 * NW];
+  const int D = (int)a.D, lane = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const float inv_d = 1.f / (float)D;
+  const bool layer = a.kind == VAE_NORM_LAYER, post = a.post_weight != nullptr;
+  int flip = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPW + (NW == 1 ? threadIdx.x >> 6 : 0); row < a.N; row += (int64_t)gridDim.x * RPW) {
+    const T* rr = reinterpret_cast<const T*>(a.r) + row * a.ld_r;
+    const T* rb = reinterpret_cast<const T*>(a.b) + row * a.ld_b;
+    Raw<T> wr[ITEMS], wb[ITEMS], wg[ITEMS];
+    Vec<V, P> gn[ITEMS], bn[ITEMS], sc[ITEMS], gp[ITEMS], bp[ITEMS];
+    float row_act = 1.f, unused;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * TPR + lane) * P;
+      wb[i] = load(rb, c, D);
+      wr[i] = load(rr, c, D);
+      if (a.gate_mode == VAE_GATE_FULL) wg[i] = load(reinterpret_cast<const T*>(a.gate) + row * a.ld_gate, c, D);
+      gp[i] = column<V, P>(a.post_weight, c, D, 1.f);
+      bp[i] = column<V, P>(a.post_bias, c, D, 0.f);
+      sc[i] = column<V, P>(a.scale, c, D, 1.f);
+      gn[i] = column<V, P>(a.norm_weight, c, D, 1.f);
+      bn[i] = column<V, P>(a.norm_bias, c, D, 0.f);
+    }
+    if (a.gate_mode == VAE_GATE_ROW) act_of(a.act, (float)reinterpret_cast<const T*>(a.gate)[row * a.ld_gate], row_act, unused);
+    // mean and 1 / sigma of the block's output, from its deviations
+    float x[ITEMS][P];
+    auto moments = [&](float& mean, float& inv) {
+      mean = 0.f;
+      if (layer) {
+        float s[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+          for (int j = 0; j < P; ++j) s[0] += x[i][j];             // columns past D hold 0
+        row_sums<NW, 1>(s, red[flip]);
+        flip ^= 1;
+        mean = s[0] * inv_d;
+      }
+      float s[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const float d = (i * TPR + lane) * P + j < D ? x[i][j] - mean : 0.f;
+          s[0] = fmaf(d, d, s[0]);
+        }
+      row_sums<NW, 1>(s, red[flip]);
+      flip ^= 1;
+      inv = 1.f / sqrtf(s[0] * inv_d + a.eps);
+    };
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) x[i][j] = (float)wb[i].t[j];
+    float mean_b = 0.f, inv_b = 1.f, mean_y, inv_y;
+    if (post) moments(mean_b, inv_b);
+    T* ry = reinterpret_cast<T*>(a.y) + row * a.D;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * TPR + lane) * P;
+      Raw<T> wy;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        float u = x[i][j], act = row_act;
+        if (post) u = fmaf((u - mean_b) * inv_b, gp[i][j], bp[i][j]);
+        if (a.gate_mode == VAE_GATE_FULL) act_of(a.act, (float)wg[i].t[j], act, unused);
+        wy.t[j] = (T)fmaf(u * sc[i][j], act, (float)wr[i].t[j]);
+        x[i][j] = c + j < D ? (float)wy.t[j] : 0.f;
+      }
+      store(ry, c, D, wy);
+    }
+    moments(mean_y, inv_y);
+    T* rh = reinterpret_cast<T*>(a.h) + row * a.D;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * TPR + lane) * P;
+      Raw<T> wh;
+#pragma unroll
+      for (int j = 0; j < P; ++j) wh.t[j] = (T)fmaf((x[i][j] - mean_y) * inv_y, gn[i][j], bn[i][j]);
+      store(rh, c, D, wh);
+    }
+    if (a.stats && lane == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(mean_b, inv_b, mean_y, inv_y);
+  }
+}
+
+template <typename T, typename V, int NW, int ITEMS>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64) void gated_norm_bwd_kernel(Args a, float* __restrict__ partial) {
+  constexpr int P = PIECE<T>, TPR = NW * 64, RPW = NW == 1 ? 4 : 1;
+  __shared__ float red[2][3 * NW];
+  const int D = (int)a.D, lane = NW == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const float inv_d = 1.f / (float)D;
+  const bool layer = a.kind == VAE_NORM_LAYER, post = a.post_weight != nullptr;
+  float acc[N_COL][ITEMS][P];
+#pragma unroll
+  for (int k = 0; k < N_COL; ++k)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) acc[k][i][j] = 0.f;
+  int flip = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPW + (NW == 1 ? threadIdx.x >> 6 : 0); row < a.N; row += (int64_t)gridDim.x * RPW) {
+    Raw<T> wy[ITEMS], wb[ITEMS], wg[ITEMS], wdy[ITEMS], wdh[ITEMS];
+    Vec<V, P> gn[ITEMS], sc[ITEMS], gp[ITEMS], bp[ITEMS];
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);       // mean_b, inv_b, mean_y, inv_y
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * TPR + lane) * P;
+      wy[i] = load(reinterpret_cast<const T*>(a.y) + row * a.D, c, D);
+      wdh[i].q = wdy[i].q = (u4)0;
+      if (a.dh) wdh[i] = load(reinterpret_cast<const T*>(a.dh) + row * a.ld_dh, c, D);
+      if (a.dy) wdy[i] = load(reinterpret_cast<const T*>(a.dy) + row * a.ld_dy, c, D);
+      wb[i] = load(reinterpret_cast<const T*>(a.b) + row * a.ld_b, c, D);
+      if (a.gate_mode == VAE_GATE_FULL) wg[i] = load(reinterpret_cast<const T*>(a.gate) + row * a.ld_gate, c, D);
+      gn[i] = column<V, P>(a.norm_weight, c, D, 1.f);
+      sc[i] = column<V, P>(a.scale, c, D, 1.f);
+      gp[i] = column<V, P>(a.post_weight, c, D, 1.f);
+      bp[i] = column<V, P>(a.post_bias, c, D, 0.f);
+    }
+    float row_act = 1.f, row_dact = 0.f;
+    if (a.gate_mode == VAE_GATE_ROW) act_of(a.act, (float)reinterpret_cast<const T*>(a.gate)[row * a.ld_gate], row_act, row_dact);
+    float s1[2] = {0.f, 0.f};
+    float t[ITEMS][P];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {                               // past D: dh is 0, and with it every term
+        const float dh = (float)wdh[i].t[j], ny = ((float)wy[i].t[j] - st.z) * st.w, dn = dh * gn[i][j];
+        acc[0][i][j] = fmaf(dh, ny, acc[0][i][j]);
+        acc[1][i][j] += dh;
+        s1[0] = fmaf(dn, ny, s1[0]);
+        s1[1] += dn;
+      }
+    row_sums<NW, 2>(s1, red[flip]);
+    flip ^= 1;
+    const float c1 = s1[0] * inv_d, c2 = layer ? s1[1] * inv_d : 0.f;
+    float s2[3] = {0.f, 0.f, 0.f};
+    T* rdr = reinterpret_cast<T*>(a.dr) + row * a.D;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * TPR + lane) * P;
+      Raw<T> wdr, wdg;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float ny = ((float)wy[i].t[j] - st.z) * st.w, dn = (float)wdh[i].t[j] * gn[i][j];
+        const float dt = c + j < D ? (float)wdy[i].t[j] + (dn - ny * c1 - c2) * st.w : 0.f;
+        wdr.t[j] = (T)dt;
+        const float nb = post ? ((float)wb[i].t[j] - st.x) * st.y : (float)wb[i].t[j];
+        const float u = post ? fmaf(nb, gp[i][j], bp[i][j]) : nb;
+        float act = row_act, dact = row_dact;
+        if (a.gate_mode == VAE_GATE_FULL) act_of(a.act, (float)wg[i].t[j], act, dact);
+        const float dk = dt * u * sc[i][j];
+        wdg.t[j] = (T)(dk * dact);
+        s2[2] += dk;
+        const float e = dt * act;
+        acc[2][i][j] = fmaf(e, u, acc[2][i][j]);
+        const float es = e * sc[i][j], d = es * gp[i][j];
+        acc[3][i][j] = fmaf(es, nb, acc[3][i][j]);
+        acc[4][i][j] += es;
+        t[i][j] = post ? d : es;
+        s2[0] = fmaf(d, nb, s2[0]);
+        s2[1] += d;
+      }
+      store(rdr, c, D, wdr);
+      if (a.gate_mode == VAE_GATE_FULL && a.dgate) store(reinterpret_cast<T*>(a.dgate) + row * a.D, c, D, wdg);
+    }
+    float c3 = 0.f, c4 = 0.f;
+    if (post || a.gate_mode == VAE_GATE_ROW) {
+      row_sums<NW, 3>(s2, red[flip]);
+      flip ^= 1;
+      c3 = post ? s2[0] * inv_d : 0.f;
+      c4 = post && layer ? s2[1] * inv_d : 0.f;
+      if (a.gate_mode == VAE_GATE_ROW && a.dgate && lane == 0) reinterpret_cast<T*>(a.dgate)[row] = (T)(s2[2] * row_dact);
+    }
+    T* rdb = reinterpret_cast<T*>(a.db) + row * a.D;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      Raw<T> w;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float nb = ((float)wb[i].t[j] - st.x) * st.y;
+        w.t[j] = (T)(post ? (t[i][j] - nb * c3 - c4) * st.y : t[i][j]);
+      }
+      store(rdb, (i * TPR + lane) * P, D, w);
+    }
+  }
+  if (!partial) return;
+  // this workgroup's sums: partial[column sum][workgroup][D]
+  const bool want[N_COL] = {a.dnorm_weight != nullptr, a.dnorm_bias != nullptr, a.dscale != nullptr, a.dpost_weight != nullptr,
+                            a.dpost_bias != nullptr};
+  if (NW == 1) {                                                  // four waves hold the same columns: waves 1..3 hand theirs over
+    __shared__ float part[3][64 * P];
+    const int w = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < N_COL; ++k) {
+      if (!want[k]) continue;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        __syncthreads();
+        if (w)
+#pragma unroll
+          for (int j = 0; j < P; ++j) part[w - 1][j * 64 + lane] = acc[k][i][j];
+        __syncthreads();
+        if (!w) {
+          const int c = (i * TPR + lane) * P;
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            const float s = ((acc[k][i][j] + part[0][j * 64 + lane]) + part[1][j * 64 + lane]) + part[2][j * 64 + lane];
+            if (c + j < D) partial[((int64_t)k * gridDim.x + blockIdx.x) * D + c + j] = s;
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N_COL; ++k) {
+      if (!want[k]) continue;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = (i * TPR + lane) * P;
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (c + j < D) partial[((int64_t)k * gridDim.x + blockIdx.x) * D + c + j] = acc[k][i][j];
+      }
+    }
+  }
+}
+
+// out[k][c] = sum over the workgroups' partials: 64 columns to a workgroup of 16 waves, each of which adds every 16th partial,
+// eight loads in flight; the 16 sums are added in order
+struct Outs {
+  void* out[N_COL];
+  int elem;                              // VAE_ADAMW_F32 / BF16 / F16
+};
+__global__ __launch_bounds__(1024) void gated_norm_cols_kernel(const float* __restrict__ partial, int groups, int D, Outs o) {
+  __shared__ float red[16][64];
+  const int k = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  if (!o.out[k]) return;
+  float s = 0.f;
+  if (c < D) {
+    const float* p = partial + (int64_t)k * groups * D + c;
+    int g = w;
+    for (; g + 7 * 16 < groups; g += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)(g + 16 * i) * D];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+    for (; g < groups; g += 16) s += p[(int64_t)g * D];
+  }
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < D) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x & 63];
+    if (o.elem == VAE_ADAMW_F32) reinterpret_cast<float*>(o.out[k])[c] = s;
+    else if (o.elem == VAE_ADAMW_BF16) reinterpret_cast<__bf16*>(o.out[k])[c] = (__bf16)s;
+    else reinterpret_cast<_Float16*>(o.out[k])[c] = (_Float16)s;
+  }
+}
+
+// waves per row and pieces per thread for a row of `pieces` 16-byte pieces: the fewest waves that hold one piece per thread,
+// which keeps the backward pass's column sums at 5 * 8 registers; beyond 16 waves more pieces
+struct Shape {
+  int nw, items;
+};
+Shape shape_of(int64_t pieces) {
+  if (pieces <= 64) return {1, 1};
+  if (pieces <= 128) return {2, 1};
+  if (pieces <= 256) return {4, 1};
+  if (pieces <= 512) return {8, 1};
+  if (pieces <= 1024) return {16, 1};
+  if (pieces <= 2048) return {16, 2};
+  return {16, 4};
+}
+int groups_of(int64_t rows, const Shape& s) {
+  // as many workgroups as are resident at once (2048 threads to a CU at most, 256 CUs), at least one row each
+  const int64_t need = s.nw == 1 ? (rows + 3) / 4 : rows;
+  const int64_t fit = s.nw <= 4 ? 1024 : s.nw == 8 ? 512 : 256;
+  return (int)(need < fit ? need : fit);
+}
+int64_t pieces_of(int64_t D, int dtype) {
+  const int64_t p = dtype == VAE_ADAMW_F32 ? 4 : 8;
+  return (D + p - 1) / p;
+}
+
+template <typename T, typename V> void launch(const Args& a, bool bwd, float* partial, const Shape& s, int groups, hipStream_t st) {
+#define VAE_GN(NW, ITEMS)                                                                                    \
+  if (s.nw == NW && s.items == ITEMS) {                                                                      \
+    if (bwd) gated_norm_bwd_kernel<T, V, NW, ITEMS><<<groups, NW == 1 ? 256 : NW * 64, 0, st>>>(a, partial);    \
+    else gated_norm_fwd_kernel<T, V, NW, ITEMS><<<groups, NW == 1 ? 256 : NW * 64, 0, st>>>(a);                 \
+    return;                                                                                                  \
+  }
+  VAE_GN(1, 1) VAE_GN(2, 1) VAE_GN(4, 1) VAE_GN(8, 1) VAE_GN(16, 1) VAE_GN(16, 2)
+  if constexpr (sizeof(T) == 4) { VAE_GN(16, 4) }
+#undef VAE_GN
+}
+
+void dispatch(const Args& a, bool bwd, float* partial, hipStream_t st) {
+  const Shape s = shape_of(pieces_of(a.D, a.dtype));
+  const int groups = groups_of(a.N, s);
+  const bool f = a.vectors_f32;
+  if (a.dtype == VAE_ADAMW_F32) launch<float, float>(a, bwd, partial, s, groups, st);
+  else if (a.dtype == VAE_ADAMW_BF16) f ? launch<__bf16, float>(a, bwd, partial, s, groups, st) : launch<__bf16, __bf16>(a, bwd, partial, s, groups, st);
+  else f ? launch<_Float16, float>(a, bwd, partial, s, groups, st) : launch<_Float16, _Float16>(a, bwd, partial, s, groups, st);
+}
+
+int check(const Args* a, const char* who) {
+  VAE_REQUIRE(a, "%s: null arguments", who);
+  VAE_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "%s: unknown dtype %d", who, a->dtype);
+  VAE_REQUIRE(a->N >= 0 && a->D >= 1 && a->D <= VAE_GATED_NORM_MAX_D, "%s: N >= 0 and 1 <= D <= %d needed", who, VAE_GATED_NORM_MAX_D);
+  VAE_REQUIRE(a->kind == VAE_NORM_RMS || a->kind == VAE_NORM_LAYER, "%s: unknown norm %d", who, a->kind);
+  VAE_REQUIRE(a->gate_mode >= VAE_GATE_NONE && a->gate_mode <= VAE_GATE_FULL, "%s: unknown gate mode %d", who, a->gate_mode);
+  VAE_REQUIRE(a->act >= VAE_GATE_IDENTITY && a->act <= VAE_GATE_TANH, "%s: unknown gate activation %d", who, a->act);
+  VAE_REQUIRE(a->eps >= 0, "%s: negative eps", who);
+  VAE_REQUIRE(!a->post_bias || a->post_weight, "%s: post_bias needs post_weight", who);
+  VAE_REQUIRE(a->N == 0 || (a->b && a->y && (a->gate_mode == VAE_GATE_NONE || a->gate)), "%s: null pointer", who);
+  const uintptr_t bad = a->dtype == VAE_ADAMW_F32 ? 3 : 1;
+  const void* rows[] = {a->r, a->b, a->gate, a->y, a->h, a->dy, a->dh, a->dr, a->db, a->dgate};
+  for (const void* p : rows) VAE_REQUIRE((reinterpret_cast<uintptr_t>(p) & bad) == 0, "%s: a pointer is not aligned to its element", who);
+  VAE_REQUIRE((reinterpret_cast<uintptr_t>(a->stats) & 15u) == 0, "%s: stats must be 16-byte aligned", who);
+  return VAE_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t vae_gated_norm_workspace_bytes(int64_t N, int64_t D, int dtype) {
+  if (N < 1 || D < 1 || D > VAE_GATED_NORM_MAX_D || dtype < 0 || dtype > 2) return 0;
+  return (int64_t)N_COL * groups_of(N, shape_of(pieces_of(D, dtype))) * D * (int64_t)sizeof(float);
+}
+
+extern "C" int vae_gated_norm_fwd(const vae_gated_norm* a, void* stream) {
+  if (int rc = check(a, "vae_gated_norm_fwd")) return rc;
+  if (a->N == 0) return VAE_OK;
+  VAE_REQUIRE(a->r && a->h, "vae_gated_norm_fwd: null pointer");
+  dispatch(*a, false, nullptr, (hipStream_t)stream);
+  VAE_CHECK_LAUNCH("vae_gated_norm_fwd");
+  return VAE_OK;
+}
+
+extern "C" int vae_gated_norm_bwd(const vae_gated_norm* a, float* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check(a, "vae_gated_norm_bwd")) return rc;
+  Outs o = {{a->dnorm_weight, a->dnorm_bias, a->dscale, a->dpost_weight, a->dpost_bias}, a->vectors_f32 ? VAE_ADAMW_F32 : a->dtype};
+  bool cols = false;
+  for (void* p : o.out) cols = cols || p;
+  VAE_REQUIRE(a->N > 0, "vae_gated_norm_bwd: no rows");
+  VAE_REQUIRE(a->stats && a->dr && a->db, "vae_gated_norm_bwd: null pointer");
+  VAE_REQUIRE((!a->dpost_weight && !a->dpost_bias) || a->post_weight, "vae_gated_norm_bwd: gradients of a norm that is not there");
+  VAE_REQUIRE(!cols || (workspace && workspace_bytes >= vae_gated_norm_workspace_bytes(a->N, a->D, a->dtype)),
+              "vae_gated_norm_bwd: needs a workspace of vae_gated_norm_workspace_bytes()");
+  hipStream_t st = (hipStream_t)stream;
+  float* partial = cols ? workspace : nullptr;
+  const int groups = groups_of(a->N, shape_of(pieces_of(a->D, a->dtype)));
+  dispatch(*a, true, partial, st);
+  VAE_CHECK_LAUNCH("vae_gated_norm_bwd");
+  if (cols) {
+    gated_norm_cols_kernel<<<dim3((unsigned)((a->D + 63) / 64), N_COL), 1024, 0, st>>>(partial, groups, (int)a->D, o);
+    VAE_CHECK_LAUNCH("vae_gated_norm_bwd");
+  }
+  return VAE_OK;
+}

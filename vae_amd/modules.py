@@ -16,7 +16,7 @@ from torch import nn
 
 from . import ops
 from .autograd import CountLinearFn, GeluLayerNormFn, LinearFn, SoftmaxRateFn
-from .functional import GradReverseLayer
+from .functional import GradReverseLayer, gated_residual_norm
 
 
 def reparameterize_gaussian(mu, var):
@@ -118,6 +118,28 @@ class FCLayers(nn.Module):
             else:
                 x = torch.cat((x, *batch_vars), dim=-1)
         return self._run(x, _count_input, cov)
+
+
+class GatedResidualNorm(nn.Module):
+    """What stands between two residual blocks (role of the glue of ResidualLayer, modules.py:45-71): the norm behind a block,
+    its gate, a residual scale per column, the sum, and the norm ahead of the next block, in one kernel each way.
+
+    ``forward(r, b, gate=None) -> (y, h)``: the new residual stream and the next block's input
+    (``vae_amd.functional.gated_residual_norm``)."""
+
+    def __init__(self, width: int, kind: str = "layer", post_norm: bool = True, residual_scale: Optional[float] = 1.0,
+                 gate_act: str = "sigmoid", bias: bool = True, eps: float = 1e-5):
+        super().__init__()
+        self.kind, self.gate_act, self.eps = kind, gate_act, eps
+        make = lambda v: nn.Parameter(torch.full((width,), float(v)))  # noqa: E731
+        self.norm_weight, self.norm_bias = make(1), make(0) if bias else None
+        self.post_weight, self.post_bias = make(1) if post_norm else None, make(0) if post_norm and bias else None
+        self.scale = make(residual_scale) if residual_scale is not None else None
+
+    def forward(self, r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.Tensor] = None):
+        return gated_residual_norm(r, b, gate, post_weight=self.post_weight, post_bias=self.post_bias, scale=self.scale,
+                                   norm_weight=self.norm_weight, norm_bias=self.norm_bias, kind=self.kind, gate_act=self.gate_act,
+                                   eps=self.eps)
 
 
 class GeneDropout(nn.Module):

@@ -682,3 +682,124 @@ def softmax_rate_bwd(px_scale: torch.Tensor, library: torch.Tensor, d_scale: Opt
     _lib.check(lib.vae_softmax_rate_bwd(_p(px_scale), _p(library), _p(d_scale), _p(d_rate), B, G, _p(dl), G, _p(dlib),
                                         _stream()), "softmax_rate_bwd")
     return dl, dlib
+
+
+FLOAT_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+NORM_KINDS = {"rms": 0, "layer": 1}
+GATE_ACTS = {"identity": 0, "sigmoid": 1, "tanh": 2}
+GATED_NORM_MAX_D = 16384
+
+
+def _gated_norm_args(r, b, gate, vectors, kind, gate_act, eps):
+    """Checks of what both passes of the gated residual norm take -> (filled _lib.GatedNorm, gate mode)."""
+    who = "vae_amd.ops.gated_norm"
+    if kind not in NORM_KINDS:
+        raise ValueError(f"{who}: kind must be one of {sorted(NORM_KINDS)}, got {kind!r}")
+    if gate_act not in GATE_ACTS:
+        raise ValueError(f"{who}: gate_act must be one of {sorted(GATE_ACTS)}, got {gate_act!r}")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps must not be negative, got {eps}")
+    if b.dtype not in FLOAT_DTYPES:
+        raise TypeError(f"{who}: rows of {b.dtype} are not supported (float32, bfloat16, float16)")
+    N, D = b.shape
+    if not 1 <= D <= GATED_NORM_MAX_D:
+        raise ValueError(f"{who}: rows of {D} columns are not supported (1 to {GATED_NORM_MAX_D})")
+    mode = 0
+    if gate is not None:
+        if tuple(gate.shape) == (N, D):
+            mode = 2
+        elif tuple(gate.shape) == (N, 1):
+            mode = 1
+        else:
+            raise ValueError(f"{who}: gate must be {(N, D)} or {(N, 1)}, got {tuple(gate.shape)}")
+    for t, name in ((r, "r"), (b, "b"), (gate, "gate")):
+        if t is None:
+            continue
+        if t.dtype != b.dtype:
+            raise TypeError(f"{who}: {name} is {t.dtype}, the rows are {b.dtype}")
+        if t.dim() != 2 or (t.numel() and t.shape[1] > 1 and t.stride(1) != 1):
+            raise ValueError(f"{who}: {name} must be 2-D with a contiguous last dim, got {tuple(t.shape)} / {t.stride()}")
+        if name == "r" and t.shape != b.shape:
+            raise ValueError(f"{who}: r is {tuple(t.shape)}, b is {tuple(b.shape)}")
+    kinds = {t.dtype for t in vectors.values() if t is not None}
+    if len(kinds) > 1 or not kinds <= {b.dtype, torch.float32}:
+        raise TypeError(f"{who}: the vectors over columns must all be {b.dtype} or all float32, got {sorted(map(str, kinds))}")
+    for name, t in vectors.items():
+        if t is not None and (t.dim() != 1 or t.shape[0] != D or not t.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be a contiguous vector of {D}, got {tuple(t.shape)}")
+    if vectors["post_bias"] is not None and vectors["post_weight"] is None:
+        raise ValueError(f"{who}: post_bias needs post_weight")
+    for t in (r, b, gate, *vectors.values()):
+        if t is not None and (not t.is_cuda or t.device != b.device):
+            raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
+    a = _lib.GatedNorm(N=N, D=D, dtype=FLOAT_DTYPES[b.dtype], vectors_f32=int(kinds == {torch.float32}), kind=NORM_KINDS[kind],
+                       gate_mode=mode, act=GATE_ACTS[gate_act], eps=float(eps), b=b.data_ptr(), ld_b=b.stride(0))
+    if r is not None:
+        a.r, a.ld_r = r.data_ptr(), r.stride(0)
+    if gate is not None:
+        a.gate, a.ld_gate = gate.data_ptr(), gate.stride(0)
+    for name, t in vectors.items():
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    return a, mode
+
+
+def gated_norm_fwd(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
+                   post_bias: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                   norm_weight: Optional[torch.Tensor] = None, norm_bias: Optional[torch.Tensor] = None, kind: str = "rms",
+                   gate_act: str = "sigmoid", eps: float = 1e-5, want_stats: bool = True):
+    """-> (y, h, stats (N, 4) or None): y = r + scale * act(gate) * norm(b), h = norm(y) (include/vae_amd.h, vae_gated_norm)."""
+    lib = _lib.load()
+    vectors = dict(post_weight=post_weight, post_bias=post_bias, scale=scale, norm_weight=norm_weight, norm_bias=norm_bias)
+    a, _ = _gated_norm_args(r, b, gate, vectors, kind, gate_act, eps)
+    with torch.cuda.device(b.device):
+        y, h = torch.empty(b.shape, dtype=b.dtype, device=b.device), torch.empty(b.shape, dtype=b.dtype, device=b.device)
+        stats = torch.empty(b.shape[0], 4, dtype=torch.float32, device=b.device) if want_stats else None
+        a.y, a.h, a.stats = y.data_ptr(), h.data_ptr(), None if stats is None else stats.data_ptr()
+        rc = lib.vae_gated_norm_fwd(C.byref(a), _stream())
+    _lib.check(rc, "gated_norm_fwd")
+    return y, h, stats
+
+
+def gated_norm_bwd(dy: Optional[torch.Tensor], dh: Optional[torch.Tensor], y: torch.Tensor, b: torch.Tensor, stats: torch.Tensor,
+                   gate: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
+                   post_bias: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                   norm_weight: Optional[torch.Tensor] = None, norm_bias: Optional[torch.Tensor] = None, kind: str = "rms",
+                   gate_act: str = "sigmoid", eps: float = 1e-5, want=("gate", "post_weight", "post_bias", "scale", "norm_weight",
+                                                                       "norm_bias")):
+    """-> dict of gradients: r, b, and those of ``want`` whose tensor is given.  ``dy`` / ``dh`` None: zero."""
+    lib = _lib.load()
+    vectors = dict(post_weight=post_weight, post_bias=post_bias, scale=scale, norm_weight=norm_weight, norm_bias=norm_bias)
+    a, mode = _gated_norm_args(None, b, gate, vectors, kind, gate_act, eps)
+    N, D = b.shape
+    for t, name, shape, dtype in ((y, "y", (N, D), b.dtype), (stats, "stats", (N, 4), torch.float32), (dy, "dy", (N, D), b.dtype),
+                                  (dh, "dh", (N, D), b.dtype)):
+        if t is None:
+            continue
+        dense = t.is_contiguous() if name in ("y", "stats") else (D == 1 or N == 0 or t.stride(1) == 1)
+        if tuple(t.shape) != shape or t.dtype != dtype or t.device != b.device or not dense:
+            raise ValueError(f"vae_amd.ops.gated_norm_bwd: {name} must be {shape} {dtype} on {b.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    out = {}
+    with torch.cuda.device(b.device):
+        out["r"], out["b"] = torch.empty(N, D, dtype=b.dtype, device=b.device), torch.empty(N, D, dtype=b.dtype, device=b.device)
+        if gate is not None and "gate" in want:
+            out["gate"] = torch.empty(N, D if mode == 2 else 1, dtype=b.dtype, device=b.device)
+        columns = [k for k, t in vectors.items() if t is not None and k in want]
+        for k in columns:
+            out[k] = (torch.zeros if N == 0 else torch.empty)(D, dtype=vectors[k].dtype, device=b.device)
+        if N == 0:
+            return out
+        for k in columns:
+            setattr(a, "d" + k, out[k].data_ptr())
+        a.y, a.stats, a.dr, a.db = y.data_ptr(), stats.data_ptr(), out["r"].data_ptr(), out["b"].data_ptr()
+        if "gate" in out:
+            a.dgate = out["gate"].data_ptr()
+        if dy is not None:
+            a.dy, a.ld_dy = dy.data_ptr(), dy.stride(0)
+        if dh is not None:
+            a.dh, a.ld_dh = dh.data_ptr(), dh.stride(0)
+        nbytes = lib.vae_gated_norm_workspace_bytes(N, D, a.dtype) if columns else 0
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=b.device) if nbytes else None   # of this call alone: streams and graphs
+        rc = lib.vae_gated_norm_bwd(C.byref(a), _p(ws), nbytes, _stream())
+    _lib.check(rc, "gated_norm_bwd")
+    return out
