@@ -627,6 +627,39 @@ int64_t vae_gated_norm_workspace_bytes(int64_t N, int64_t D, int dtype);
 int vae_gated_norm_fwd(const vae_gated_norm* args, void* stream);
 int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- softmax cross entropy of a linear head, without its logits --------------------------------
+ * Rows x (N, D), class weights matrix w (V, D), bias (V) or null, all of one type (VAE_ADAMW_F32 / BF16 / F16), row strides
+ * in elements; target (N) class indices, contiguous; class_weight (V) floats or null.  With z = x w^T + bias:
+ * loss_i = class_weight[t_i] (logsumexp(z_i) - z_i[t_i]), 0 for rows whose target is ignore_index (nn.CrossEntropyLoss of the
+ * cell-property heads, task.py:129-137, for heads too wide for vae_cell_heads_step).  reduction: VAE_CE_NONE -> loss (N),
+ * VAE_CE_SUM, VAE_CE_MEAN (divided by the sum of the class weights that took part: NaN when no row does) -> loss (1); always
+ * float.  A target that is neither a class nor ignore_index makes its row's loss and gradients NaN.
+ * state: vae_linear_ce_state_bytes(N) bytes that the forward pass writes and the backward pass of the same arguments reads.
+ * The backward pass takes the float gradient of the loss ((N) or (1)) and overwrites the dense dx (N, D), dw (V, D) and dbias
+ * (V) that are not null, of the operands' type.  Ignored rows take no part at all: their dx is 0 and what their x holds
+ * reaches nothing else.  The logits are never in memory; the workspace holds a packed copy of x, for fp32 (and for w that is
+ * not 16-byte aligned with D and its stride multiples of 8) one of w, and up to 512 MiB of logit gradients.  Same bits every
+ * time.                                                                                                                    */
+enum { VAE_CE_NONE = 0, VAE_CE_SUM = 1, VAE_CE_MEAN = 2 };
+typedef struct {
+  int64_t N, D, V;
+  int32_t dtype;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const void* bias;
+  const int64_t* target;
+  const float* class_weight;
+  int64_t ignore_index;
+} vae_linear_ce;
+int64_t vae_linear_ce_state_bytes(int64_t N);
+int64_t vae_linear_ce_workspace_bytes(const vae_linear_ce* args, int backward);
+int vae_linear_ce_fwd(const vae_linear_ce* args, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int vae_linear_ce_bwd(const vae_linear_ce* args, int reduction, const float* grad, const void* state, void* dx, void* dw, void* dbias,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,319 @@
+"""Cross entropy of a linear head without its logits (vae_amd.losses.linear_cross_entropy; C ABI vae_linear_ce_fwd / _bwd)
+against the definition in 64 bits.
+
+Tolerances.  Logits are sums of D products in 32 bits: off by a few 2^-24 of |x| |w| (norms); with the rows made here (logits of
+a few units) the loss is held to 2e-6 of itself plus 1e-6.  A gradient element is a sum of terms whose d has been rounded
+to the operands' type (finfo.eps / 2 of each) and that is rounded itself: its error is at most eps (the sum of the magnitudes of
+its terms) / 2 plus eps / 2 of the result; the bound takes the matrices |d| |w| and |d|^T |x| for the first.  fp32: 32 * 2^-24 of
+the same sums (three-term products are exact to 2^-24, sums run over thousands of terms in blocks).  For every type p itself is
+off by p times the error of z - lse, two values of up to Z = max |z| that are rounded in 32 bits a few times each:
+(8 + 4 Z) 2^-24 p.  At the target p - 1 keeps that error of p however small p - 1 is, so this term takes the matrices of p and
+not those of d."""
+import ctypes as C
+
+import pytest
+import torch
+
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+# ---------------------------------------------------------------------------------------------------- on the CPU
+def test_refusals_of_the_c_entry():
+    from vae_amd import _lib
+    lib = _lib.load()
+    ok = dict(N=4, D=8, V=16, dtype=1, x=4096, ldx=8, w=8192, ldw=8, target=16384, ignore_index=-100)
+
+    def refused(msg, fwd=True, reduction=2, loss=4096, state=4096, ws=4096, n=1 << 40, dx=4096, db=None, **k):
+        a = _lib.LinearCE(**{**ok, **k})
+        rc = lib.vae_linear_ce_fwd(C.byref(a), reduction, loss, state, ws, n, None) if fwd else \
+            lib.vae_linear_ce_bwd(C.byref(a), reduction, loss, state, dx, None, db, ws, n, None)
+        assert rc == 1 and msg in lib.vae_last_error().decode(), lib.vae_last_error()
+
+    for fwd in (True, False):
+        refused("dtype", fwd, dtype=3)
+        refused("at least 1", fwd, N=0)
+        refused("at least 1", fwd, D=0)
+        refused("at least 1", fwd, V=0)
+        refused("at most", fwd, V=(1 << 24) + 1)
+        refused("tiles", fwd, V=1 << 24, N=1 << 24)
+        refused("null pointer", fwd, x=None)
+        refused("null pointer", fwd, w=None)
+        refused("null pointer", fwd, target=None)
+        refused("stride", fwd, ldw=7)
+        refused("stride is too large", fwd, ldw=1 << 22)
+        refused("aligned to its element", fwd, w=8193)
+        refused("unknown reduction", fwd, reduction=3)
+        refused("null pointer", fwd, state=None)
+        refused("null pointer", fwd, loss=None)
+        refused("workspace", fwd, ws=None)
+        refused("workspace", fwd, n=100)
+        refused("workspace", fwd, ws=4100)
+    refused("null pointer", False, dx=None)
+    refused("not there", False, db=4096)
+    assert lib.vae_linear_ce_workspace_bytes(C.byref(_lib.LinearCE(**{**ok, "N": 0})), 0) == -1
+    # the backward workspace is bounded: half a gigabyte of logit gradients, whatever the vocabulary
+    big = _lib.LinearCE(**{**ok, "N": 8192, "D": 4096, "V": 1 << 20, "ldx": 4096, "ldw": 4096})
+    assert lib.vae_linear_ce_workspace_bytes(C.byref(big), 1) < (512 << 20) + 4 * 8192 * 4096 + 2 * 8192 * 4096 + (1 << 20)
+
+
+def test_refusals_of_the_python_entry():
+    from vae_amd.losses import linear_cross_entropy
+    x, w, t = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        linear_cross_entropy(x, w, t)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        linear_cross_entropy(x[:0], w, t[:0])
+    with pytest.raises(ValueError, match="reduction"):
+        linear_cross_entropy(x, w, t, reduction="max")
+    with pytest.raises(ValueError, match="target"):
+        linear_cross_entropy(x, w, t[:2])
+    with pytest.raises(ValueError, match="int64"):
+        linear_cross_entropy(x, w, t.int())
+    with pytest.raises(ValueError, match="x must be"):
+        linear_cross_entropy(x, w[:, :7], t)
+    with pytest.raises(TypeError, match="float64"):
+        linear_cross_entropy(x.double(), w.double(), t)
+    with pytest.raises(TypeError, match="w is"):
+        linear_cross_entropy(x, w.half(), t)
+    with pytest.raises(TypeError, match="bias is"):
+        linear_cross_entropy(x, w, t, bias=torch.zeros(5).half())
+    with pytest.raises(TypeError, match="weight is"):
+        linear_cross_entropy(x, w, t, weight=torch.zeros(5).double())
+    with pytest.raises(ValueError, match="vector of 5"):
+        linear_cross_entropy(x, w, t, weight=torch.zeros(4))
+
+
+# ---------------------------------------------------------------------------------------------------- on the GPU
+def _inputs(n, d, v, dtype, bias, weight, ignored, seed, off=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = DT[dtype]
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    w = (rnd(v, d + off) / d ** 0.5).to(t)[:, off:]
+    target = torch.randint(0, v, (n,), generator=g, device="cuda")
+    x = torch.zeros(n, d + off, dtype=t, device="cuda")[:, off:]
+    x.copy_(rnd(n, d) + 2 * w[target].float())
+    if ignored:
+        target[torch.rand(n, generator=g, device="cuda") < ignored] = -100
+    return dict(x=x, w=w, target=target, bias=(0.5 * rnd(v)).to(t) if bias else None,
+                weight=0.1 + torch.rand(v, generator=g, device="cuda") if weight else None)
+
+
+def _oracle(s, reduction, up=None, ignore=-100):
+    """(loss, {grad: (value, sum of the magnitudes of its terms, error that p brings)}) in 64 bits."""
+    x, w, t = s["x"].double(), s["w"].double(), s["target"]
+    z = x @ w.t() + (0 if s["bias"] is None else s["bias"].double())
+    kept = t != ignore
+    at = t.clamp(min=0)
+    cw = kept.double() * (1 if s["weight"] is None else s["weight"].double()[at])
+    logp = z - torch.logsumexp(z, 1, keepdim=True)
+    nll = torch.where(kept, -logp.gather(1, at[:, None])[:, 0] * cw, torch.zeros_like(cw))
+    loss = {"none": nll, "sum": nll.sum(), "mean": nll.sum() / cw.sum()}[reduction]
+    g = cw * (1.0 if up is None else up.double())
+    g = g / cw.sum() if reduction == "mean" else g
+    d = logp.exp()
+    p = torch.where(kept[:, None], d * g[:, None], torch.zeros_like(d)) * (8 + 4 * z.abs().amax()) * 2.0 ** -24
+    d.scatter_add_(1, at[:, None], -torch.ones_like(d[:, :1]))
+    d = torch.where(kept[:, None], d * g[:, None], torch.zeros_like(d))
+    clean = torch.where(kept[:, None], x, torch.zeros_like(x))
+    return loss, {"x": (d @ w, d.abs() @ w.abs(), p @ w.abs()), "w": (d.t() @ clean, d.abs().t() @ clean.abs(), p.t() @ clean.abs()),
+                  "bias": (d.sum(0), d.abs().sum(0), p.sum(0))}
+
+
+def _check(s, reduction, got_loss, grads, up=None):
+    loss, ref = _oracle(s, reduction, up)
+    assert got_loss.dtype == torch.float32
+    err = (got_loss.double() - loss).abs()
+    assert bool((err <= 2e-6 * loss.abs() + 1e-6 * (1 if reduction != "sum" else len(s["x"]))).all()), float(err.max())
+    t = s["x"].dtype
+    eps = torch.finfo(t).eps / 2
+    for k, g in grads.items():
+        val, mag, off = ref[k]
+        assert g.dtype == t and g.shape == val.shape
+        k_len = s["w"].shape[0] if k == "x" else s["x"].shape[0]
+        tol = off + max(32.0, 2 * (6 * k_len / 16) ** 0.5) * 2.0 ** -24 * mag + (0 if t == torch.float32 else eps * mag + 1.01 * eps * val.abs())
+        if t == torch.float16:
+            tol = tol + 2.0 ** -25          # half the smallest subnormal
+        bad = (g.double() - val).abs() - tol - 1e-30
+        assert float(bad.max()) <= 0, (k, float(bad.max()), float(val.abs().max()))
+
+
+def _run(s, reduction, up=None, **k):
+    from vae_amd.losses import linear_cross_entropy
+    leaf = {k: s[k].detach().requires_grad_() for k in ("x", "w", "bias") if s[k] is not None}
+    loss = linear_cross_entropy(leaf["x"], leaf["w"], s["target"], bias=leaf.get("bias"), weight=s["weight"], reduction=reduction, **k)
+    grads = torch.autograd.grad(loss, list(leaf.values()), up)
+    return loss.detach(), dict(zip(leaf, grads))
+
+
+SHAPES = [(1, 1, 1), (1, 8, 2), (3, 7, 5), (5, 30, 17), (64, 64, 64), (127, 33, 129), (129, 72, 255), (256, 256, 256), (257, 100, 300),
+          (300, 520, 1000), (31, 1000, 4099), (1000, 40, 3), (512, 264, 6000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", SHAPES)
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("bias,weight,ignored", [(False, False, 0.0), (True, True, 0.3)])
+def test_shapes(n, d, v, dtype, bias, weight, ignored):
+    s = _inputs(n, d, v, dtype, bias, weight, ignored, seed=n + d + v)
+    s["target"][0] = v - 1
+    loss, grads = _run(s, "mean")
+    _check(s, "mean", loss, grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_reductions_and_upstream_gradients(dtype, reduction):
+    s = _inputs(200, 96, 700, dtype, True, True, 0.2, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    up = torch.rand(200, generator=g, device="cuda") * 1e-3 if reduction == "none" else torch.tensor(0.25, device="cuda")
+    loss, grads = _run(s, reduction, up)
+    _check(s, reduction, loss, grads, up)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_large_tiles_and_pieces(dtype):
+    """More than 200 tiles of 256 x 256, and (a batch this long) a vocabulary in two pieces."""
+    n, v = (40000, 7000) if dtype == "bf16" else (14000, 6500)
+    s = _inputs(n, 72, v, dtype, True, False, 0.4, seed=9)
+    loss, grads = _run(s, "mean")
+    _check(s, "mean", loss, grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [1, 4, 8])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_strides_and_offsets(off, dtype):
+    """Rows that are views into wider ones, at addresses that are not multiples of 16 bytes."""
+    s = _inputs(70, 64, 300, dtype, False, False, 0.0, seed=off, off=off)
+    assert s["w"].stride(0) == 64 + off and s["x"].stride(0) == 64 + off
+    loss, grads = _run(s, "mean")
+    _check(s, "mean", loss, grads)
+
+
+@pytest.mark.gpu
+def test_leading_dims_transposed_weights_and_broadcast_rows():
+    from vae_amd.losses import linear_cross_entropy
+    s = _inputs(60, 40, 90, "fp32", False, False, 0.0, seed=8)
+    x3, t3 = s["x"].view(5, 12, 40), s["target"].view(5, 12)
+    want = linear_cross_entropy(s["x"], s["w"], s["target"], reduction="none")
+    got = linear_cross_entropy(x3, s["w"].t().contiguous().t(), t3, reduction="none")
+    assert got.shape == (5, 12) and torch.equal(got.view(-1), want)
+    one = s["x"][:1].detach().requires_grad_()
+    linear_cross_entropy(one.expand(60, 40), s["w"], s["target"]).backward()
+    s2 = {**s, "x": s["x"][:1].expand(60, 40)}
+    val, mag, off = (t.sum(0, keepdim=True) for t in _oracle(s2, "mean")[1]["x"])
+    assert bool(((one.grad.double() - val).abs() <= off + 64 * 2.0 ** -24 * mag).all())
+
+
+@pytest.mark.gpu
+def test_ignored_rows_cost_and_spoil_nothing():
+    """Infinities and NaN in ignored rows reach nothing; a batch without rows that count; targets that are no class."""
+    from vae_amd.losses import linear_cross_entropy
+    s = _inputs(300, 64, 500, "bf16", True, False, 0.3, seed=4)
+    loss, grads = _run(s, "mean")
+    dirty = {**s, "x": s["x"].clone()}
+    off = s["target"] == -100
+    dirty["x"][off] = float("nan")
+    dirty["x"][off.nonzero()[0, 0]] = float("inf")
+    loss2, grads2 = _run(dirty, "mean")
+    assert torch.equal(loss, loss2) and all(torch.equal(grads[k], grads2[k]) for k in grads)
+    assert not bool(grads2["x"][off].any())
+    none = {**s, "target": torch.full_like(s["target"], -100)}
+    loss, grads = _run(none, "mean")
+    assert bool(torch.isnan(loss)) and not any(bool(g.any()) for g in grads.values())
+    loss, grads = _run(none, "none", torch.ones(300, device="cuda"))
+    assert not bool(loss.any()) and not any(bool(g.any()) for g in grads.values())
+    bad = {**s, "target": s["target"].clone()}
+    bad["target"][5], bad["target"][7] = 500, -1
+    loss, grads = _run(bad, "none", torch.ones(300, device="cuda"))
+    assert bool(torch.isnan(loss[[5, 7]]).all()) and int(torch.isnan(loss).sum()) == 2
+    assert bool(torch.isnan(grads["x"][[5, 7]]).all()) and int(torch.isnan(grads["x"]).any(1).sum()) == 2 and bool(torch.isnan(grads["w"]).all())
+    other = {**s, "target": torch.where(off, torch.full_like(s["target"], 3), s["target"])}
+    a = linear_cross_entropy(other["x"], other["w"], other["target"], bias=s["bias"], ignore_index=3)
+    assert bool(torch.isfinite(a))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_extreme_logits(dtype):
+    """Logits of hundreds, classes masked by the type's lowest bias, and a row that holds a NaN."""
+    s = _inputs(40, 64, 600, dtype, True, False, 0.0, seed=6)
+    s["x"].mul_(40)
+    s["target"] = (s["x"].double() @ s["w"].double().t()).argmax(1)     # the likely class, so that the loss is of ordinary size
+    s["bias"][100:400] = torch.finfo(DT[dtype]).min
+    s["target"][(s["target"] >= 100) & (s["target"] < 400)] = 5
+    loss, grads = _run(s, "none", torch.ones(40, device="cuda"))
+    ref, _ = _oracle(s, "none")
+    z = (s["x"].double() @ s["w"].double().t()).abs().amax()
+    assert bool(((loss.double() - ref).abs() <= 64 * 2.0 ** -24 * (z + ref.abs())).all())
+    assert all(bool(torch.isfinite(g).all()) for g in grads.values())
+    assert not bool(grads["w"][100:400].any())                           # masked classes have no share at all
+    s["x"][3, 9] = float("nan")
+    loss, grads = _run(s, "none", torch.ones(40, device="cuda"))
+    assert int(torch.isnan(loss).sum()) == 1 and bool(torch.isnan(loss[3])) and int(torch.isnan(grads["x"]).any(1).sum()) == 1
+
+
+@pytest.mark.gpu
+def test_differences():
+    """Central differences of the forward pass in the direction of the gradient (fp32, steps of 2^-6: 1e-2 is wide)."""
+    from vae_amd.losses import linear_cross_entropy
+    s = _inputs(20, 24, 50, "fp32", True, True, 0.2, seed=5)
+    _, grads = _run(s, "sum")
+    for k, g in grads.items():
+        step, dirn = 2.0 ** -6, g / g.norm()
+        val = lambda e: float(linear_cross_entropy(**{k2: (s[k2] + e * dirn if k2 == k else s[k2]) for k2 in ("x", "w", "bias", "target")},  # noqa: E731
+                                                   weight=s["weight"], reduction="sum"))
+        assert abs((val(step) - val(-step)) / (2 * step) / float(g.norm()) - 1) < 1e-2, k
+
+
+@pytest.mark.gpu
+def test_repeats_other_stream_and_graph():
+    s = _inputs(700, 136, 3000, "bf16", True, True, 0.2, seed=11)
+    first = _run(s, "mean")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = _run(s, "mean")
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(first[0], again[0]) and all(torch.equal(first[1][k], again[1][k]) for k in first[1])
+    static = {k: v.clone() for k, v in s.items()}
+    one, up = torch.tensor(1.0, device="cuda"), None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = _run(static, "mean", one)
+    for seed in (12, 13, 14):                                            # another number of ignored rows every time
+        new = _inputs(700, 136, 3000, "bf16", True, True, 0.1 * (seed - 11), seed=seed)
+        for k in static:
+            static[k].copy_(new[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _run(new, "mean", up)
+        assert torch.equal(loss, want[0]) and all(torch.equal(grads[k], want[1][k]) for k in grads)
+
+
+@pytest.mark.gpu
+def test_partial_gradients_empty_and_module():
+    from vae_amd.losses import LinearCrossEntropyLoss, linear_cross_entropy
+    s = _inputs(50, 32, 40, "fp32", True, False, 0.0, seed=2)
+    full = _run(s, "mean")[1]
+    for k in ("x", "w", "bias"):
+        leaf = s[k].detach().requires_grad_()
+        args = {**s, k: leaf}
+        linear_cross_entropy(args["x"], args["w"], s["target"], bias=args["bias"]).backward()
+        assert torch.equal(leaf.grad, full[k])
+    m = LinearCrossEntropyLoss(32, 40).cuda()
+    with torch.no_grad():
+        m.linear.weight.copy_(s["w"])
+        m.linear.bias.copy_(s["bias"])
+    m(s["x"], s["target"]).backward()
+    assert torch.equal(m.linear.weight.grad, full["w"]) and torch.equal(m.linear.bias.grad, full["bias"])
+    e = torch.zeros(0, 32, device="cuda", requires_grad=True)
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    m.zero_grad()
+    loss = linear_cross_entropy(e, m.linear.weight, none, bias=m.linear.bias, reduction="sum")
+    loss.backward()
+    assert float(loss) == 0 and e.grad.shape == (0, 32) and not bool(m.linear.weight.grad.any())
+    assert bool(torch.isnan(m(e, none))) and linear_cross_entropy(e, m.linear.weight, none, reduction="none").shape == (0,)

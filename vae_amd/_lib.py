@@ -17,6 +17,10 @@ X_F32, X_U8 = 0, 1   # enum { VAE_X_F32, VAE_X_U8 } of include/vae_amd.h
 
 # name -> (restype, argtypes); mirrors include/vae_amd.h one to one
 SIGNATURES = {
+    "vae_linear_ce_state_bytes": (_i64, [_i64]),
+    "vae_linear_ce_workspace_bytes": (_i64, [_ptr, _i32]),
+    "vae_linear_ce_fwd": (_i32, [_ptr, _i32, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "vae_linear_ce_bwd": (_i32, [_ptr, _i32, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "vae_gated_norm_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "vae_gated_norm_fwd": (_i32, [_ptr, _ptr]),
     "vae_gated_norm_bwd": (_i32, [_ptr, _ptr, _i64, _ptr]),
@@ -134,6 +138,12 @@ class GatedNorm(C.Structure):
                 ("y", _ptr), ("h", _ptr), ("stats", _ptr), ("dy", _ptr), ("ld_dy", _i64), ("dh", _ptr), ("ld_dh", _i64),
                 ("dr", _ptr), ("db", _ptr), ("dgate", _ptr), ("dnorm_weight", _ptr), ("dnorm_bias", _ptr), ("dscale", _ptr),
                 ("dpost_weight", _ptr), ("dpost_bias", _ptr)]
+
+
+class LinearCE(C.Structure):
+    """vae_linear_ce of include/vae_amd.h"""
+    _fields_ = [("N", _i64), ("D", _i64), ("V", _i64), ("dtype", C.c_int32), ("x", _ptr), ("ldx", _i64), ("w", _ptr), ("ldw", _i64),
+                ("bias", _ptr), ("target", _ptr), ("class_weight", _ptr), ("ignore_index", _i64)]
 
 
 class StepConfig(C.Structure):

@@ -171,3 +171,23 @@ class GatedResidualNormFn(Function):
         want = [n for n, need in zip(names, ctx.needs_input_grad) if need]
         g = ops.gated_norm_bwd(dy, dh, y, b, stats, gate, **dict(zip(GATED_NORM_VECTORS, vectors)), **ctx.how, want=want)
         return tuple(g.get(n) if n in want else None for n in names) + (None, None, None)
+
+
+class LinearCrossEntropyFn(Function):
+    """Cross entropy of the linear head x w^T + bias against class indices without keeping the logits
+    (ops.linear_ce_fwd / linear_ce_bwd): the backward pass forms them again, piece by piece."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, target, weight, ignore_index, reduction):
+        loss, state = ops.linear_ce_fwd(x, w, target, bias, weight, ignore_index, reduction)
+        ctx.save_for_backward(x, w, bias, target, weight, state)
+        ctx.how = (ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, w, bias, target, weight, state = ctx.saved_tensors
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        dx, dw, db = ops.linear_ce_bwd(grad, state, x, w, target, bias, weight, *ctx.how, need_x=nx, need_w=nw, need_bias=nb)
+        return dx, dw, db, None, None, None, None

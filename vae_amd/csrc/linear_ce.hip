@@ -1,0 +1,953 @@
+// Softmax cross entropy of a linear head, z = x W^T + b over N rows and V classes, with its gradients, without the logits
+// ever being in memory (gfx950).
+//
+//   lse_i = log sum_v exp z_iv        nll_i = c[t_i] (lse_i - z_{i, t_i})
+//   d_iv  = g_i c[t_i] (exp(z_iv - lse_i) - [v = t_i])        dx = d W        dW = d^T x        db = sum_i d_i
+//
+// Rows with the ignored target are left out before anything else: the others are gathered, in order, into a packed copy of x
+// (their number stays on the device; tiles and K loops behind it end at once), so that ignored rows cost nothing and what they
+// hold, infinities and NaN included, reaches no gradient.
+//
+// Forward: a tile product of W with the packed x in which a lane owns a row of x and its accumulators run over classes.  The
+// running maximum and sum of a tile are then taken inside a lane's registers, and only one pair per row and 256 classes is
+// written.  Backward, for pieces of the classes whose d fits a fixed workspace: the same product again, whose epilogue turns
+// the logits into d (16 bits), then dx += d W and dW = d^T x.  4 products of 2 N D V operations, of which one is the recompute
+// that stands for keeping N V logits.  Bound by the matrix cores as soon as N and D are a few hundred.
+//
+// Types: bf16 and fp16 multiply as they are, sums in 32 bits; d is rounded to the same type (relative 2^-9 or 2^-12 of each
+// element, independent of each other, so that a sum of them is off by no more than its own rounding).  d is divided by the
+// largest factor g_i c[t_i] for that, and the products are multiplied by it in 32 bits: the term of the target, -1 in nearly
+// every row of a large vocabulary, is then exact, where the rounding of 1 / N itself would shift every gradient by the same
+// 2^-9 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
+// multiplied by 2^14 as well.  fp32 operands are split exactly
+// into three bf16 terms, and the six products that matter run one after the other along K, small ones first: the error
+// is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix instruction would give a sixteenth).
+#include "../../include/vae_amd.h"
+#include "common.h"
+
+#include <math.h>
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+typedef __attribute__((address_space(3))) void* lds_void_ptr;
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef u4 u4_any __attribute__((aligned(2)));          // 16-byte accesses at any element
+
+constexpr int ROW_PAD = 256;                            // packed rows and columns of d come in multiples of this
+constexpr int K_PAD = 64;
+
+// the state of a forward pass that the backward pass reads: int32 / float words
+constexpr int S_KEPT = 0, S_TOTAL = 1, S_ROWS = 4;      // kept rows, sum of c[t], then row index (N) and lse (N) of the kept rows
+
+enum { EPI_STATS = 0, EPI_D = 1, EPI_STORE = 2 };
+
+struct Gemm {
+  const uint16_t *a, *b;        // A: [M][K] (KC) or [K][M] (RC); B: [N][K] or [K][N]; 16-bit elements
+  int64_t lda, ldb;
+  int64_t plane_a, plane_b;     // elements from one bf16 term to the next (fp32 operands)
+  int M, N, K;
+  int segs;                     // 1, or 6 products of bf16 terms
+  const int* dyn;               // kept rows: bounds N, or K (dyn_k)
+  int dyn_k;
+  int split, tiles_m, tiles_n;
+  // EPI_STATS, EPI_D
+  int v0;                       // first class of this piece: class = v0 + m
+  const void* bias;             // of the operands' outer type
+  int bias_f32;
+  const int64_t* target;        // by original row
+  const int* rows;              // original row of a packed row
+  float2* partial;              // (tile_m, N padded): running maximum and sum
+  float* target_logit;          // by packed row
+  const float* lse;             // by packed row
+  const float* g;               // by packed row: upstream * class weight (0: an exactly zero row)
+  const float* d_scale;         // what d is multiplied by, and its reciprocal
+  uint16_t* d;                  // [N padded][ldd], planes at plane_d
+  int64_t ldd, plane_d;
+  // EPI_STORE: out[n][m], final type or float slabs (split, N, M) that are added to when `add`
+  void* out;
+  int64_t ldo;
+  int out_kind;                 // 0 float slab, 1 the final 16-bit type, 2 final float
+  int add;
+};
+
+__device__ __forceinline__ void split3(float v, __bf16& h, __bf16& m, __bf16& l) {
+  h = (__bf16)v;
+  const float r = v - (float)h;
+  m = (__bf16)r;
+  l = (__bf16)(r - (float)m);
+}
+
+// exp to an ulp or so for v <= 88 (common.h's vae_exp_acc, which would turn a NaN into a small number)
+__device__ __forceinline__ float exp_fine(float v) { return v == v ? vae_exp_acc(v) : v; }
+
+// One wave instruction: lane i copies 16 bytes from base + off_i to LDS byte lds + 16 i.  In inline asm so that the compiler
+// does not drain the counter ahead of the next LDS read; the kernel waits itself.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(off), "s"(base), "s"(lds)
+               : "memory");
+}
+template <int LEFT> __device__ __forceinline__ void wait_and_meet() {   // this wave's loads but LEFT have landed, its LDS reads are done
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+template <bool F16> __device__ __forceinline__ f32x16 mma(u4 a, u4 b, f32x16 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  union {
+    __bf16 h[2];
+    _Float16 f[2];
+    uint32_t u;
+  } w;
+  if constexpr (F16) w.f[0] = (_Float16)a, w.f[1] = (_Float16)b;
+  else w.h[0] = (__bf16)a, w.h[1] = (__bf16)b;
+  return w.u;
+}
+
+// Tile product.  B M x B N outputs, W_M x W_N waves, K in steps of BK through STAGES images in LDS, filled by direct loads that
+// run STAGES - 1 steps ahead; one barrier per step.
+//   KC image [rows][BK]: 16-byte chunk c of a row sits at chunk c ^ f(row), so that the 16 rows of a b128 read hit all banks.
+//   RC image [BK][rows]: chunk c of k sits at c ^ 4 (k & 3); fragments by the transposing read, whose 16 lanes take 4 k x 16 rows.
+// Rows and columns of A past its end are clamped to the last one (their products are not stored, or meet zeros in B); B is a
+// packed operand, padded with zeros to whole tiles.
+template <bool F16, bool A_KC, bool B_KC, int BM, int BN, int W_M, int W_N, int BK, int STAGES, int EPI, bool FINE>
+__global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
+  constexpr int NW = W_M * W_N, TM = BM / (32 * W_M), TN = BN / (32 * W_N);
+  constexpr int IMG_A = BM * BK, IMG_B = BN * BK, STAGE = IMG_A + IMG_B;          // elements
+  constexpr int PA = IMG_A * 2 / 1024 / NW, PB = IMG_B * 2 / 1024 / NW;           // 1 KB pieces per wave
+  static_assert(PA >= 1 && PB >= 1, "tile too small for the workgroup");
+  __shared__ __attribute__((aligned(16))) uint16_t smem[STAGES * STAGE];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / W_N, wn = wave % W_N, l31 = lane & 31, h = lane >> 5;
+
+  // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles, and order the tiles in bands of 4 along M, so
+  // that the 32 tiles an XCD works on at a time share 4 blocks of A and 8 of B in its L2.
+  const int total = g.tiles_m * g.tiles_n;
+  int id = blockIdx.x % total;
+  const int part = blockIdx.x / total;
+  {
+    const int q8 = total >> 3, r8 = total & 7, xcd = id & 7;
+    id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (id >> 3);
+  }
+  int tm, tn;
+  {
+    constexpr int BAND = 4;
+    const int band = id / (BAND * g.tiles_n), in = id - band * BAND * g.tiles_n;
+    const int height = min(BAND, g.tiles_m - band * BAND);
+    tm = band * BAND + in % height;
+    tn = in / height;
+  }
+  const int m0 = tm * BM, n0 = tn * BN;
+  int N = g.N, K = g.K;
+  if (g.dyn) {
+    const int kept = __builtin_amdgcn_readfirstlane(*g.dyn);
+    if (g.dyn_k) K = min(K, kept);
+    else N = min(N, kept);
+  }
+  if (n0 >= N) return;
+
+  const int kt1 = (K + BK - 1) / BK, all = kt1 * g.segs, per = (all + g.split - 1) / g.split;
+  const int t_beg = min(part * per, all), t_end = min(t_beg + per, all);
+
+  // ---- loads: per-lane byte offsets from a base that moves with K ----
+  uint32_t off_a[PA], off_b[PB];
+  auto chunk_a = [&](int i, int k_left) -> uint32_t {        // k_left: elements of K from this step on
+    const int piece = wave * PA + i;
+    if (A_KC) {
+      constexpr int CPR = BK / 8;
+      const int row = piece * (64 / CPR) + lane / CPR, swz = BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+      const int c = min((lane % CPR) ^ swz, (k_left + 7) / 8 - 1);
+      return (uint32_t)(((int64_t)(min(m0 + row, g.M - 1) - m0) * g.lda + 8 * c) * 2);
+    }
+    constexpr int CPR = BM / 8;
+    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
+    return (uint32_t)(((int64_t)min(k, k_left - 1) * g.lda + min(8 * c, ((g.M + 7) & ~7) - 8 - m0)) * 2);
+  };
+  auto chunk_b = [&](int i) -> uint32_t {
+    const int piece = wave * PB + i;
+    if (B_KC) {
+      constexpr int CPR = BK / 8;
+      const int row = piece * (64 / CPR) + lane / CPR, swz = BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+      return (uint32_t)(((int64_t)row * g.ldb + 8 * ((lane % CPR) ^ swz)) * 2);
+    }
+    constexpr int CPR = BN / 8;
+    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
+    return (uint32_t)(((int64_t)k * g.ldb + 8 * c) * 2);
+  };
+#pragma unroll
+  for (int i = 0; i < PA; ++i) off_a[i] = chunk_a(i, BK);
+#pragma unroll
+  for (int i = 0; i < PB; ++i) off_b[i] = chunk_b(i);
+
+  const uint16_t* base_a = A_KC ? g.a + (int64_t)m0 * g.lda : g.a + m0;
+  const uint16_t* base_b = B_KC ? g.b + (int64_t)n0 * g.ldb : g.b + n0;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
+  int seg = t_beg / max(kt1, 1), kt = t_beg - seg * kt1;     // of the next step to load
+  auto issue = [&](int stage) {
+    // terms (hi 0, mid 1, lo 2) of the product a * b that segment `seg` forms: mm, hl, lh, hm, mh, hh
+    const int pa = g.segs == 1 ? 0 : (0x102010 >> (20 - 4 * seg)) & 15, pb = g.segs == 1 ? 0 : (0x120100 >> (20 - 4 * seg)) & 15;
+    const int k0 = kt * BK;
+    const uint16_t* sa = base_a + pa * g.plane_a + (A_KC ? (int64_t)k0 : (int64_t)k0 * g.lda);
+    const uint16_t* sb = base_b + pb * g.plane_b + (B_KC ? (int64_t)k0 : (int64_t)k0 * g.ldb);
+    const uint32_t la = lds0 + (uint32_t)stage * (STAGE * 2u) + (uint32_t)wave * (PA * 1024u);
+    const uint32_t lb = lds0 + (uint32_t)stage * (STAGE * 2u) + IMG_A * 2u + (uint32_t)wave * (PB * 1024u);
+    const int left = K - k0;
+    if (left >= BK) {
+#pragma unroll
+      for (int i = 0; i < PA; ++i) dma16(sa, off_a[i], la + i * 1024u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PA; ++i) dma16(sa, chunk_a(i, left), la + i * 1024u);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) dma16(sb, off_b[i], lb + i * 1024u);
+    if (++kt == kt1) kt = 0, ++seg;
+  };
+
+  // ---- fragments ----
+  const int swz = BK == 64 ? (l31 >> 1) & 7 : (l31 >> 2) & 3;
+  const int la = lane & 15, lq = la >> 2, lp = la & 3, lj = lane >> 4;
+  const int kc_a = (wm * 32 * TM + l31) * BK, kc_b = (wn * 32 * TN + l31) * BK;
+  const int rc_k = 8 * (lj >> 1) + lq;
+  const int rc_a = wm * 32 * TM + 16 * (lj & 1) + 4 * lp, rc_b = wn * 32 * TN + 16 * (lj & 1) + 4 * lp;
+  auto frag_kc = [&](const uint16_t* img, int base, int t, int ks) -> u4 {
+    return *reinterpret_cast<const u4*>(img + base + t * 32 * BK + (((2 * ks + h) ^ swz) << 3));
+  };
+  auto frag_rc = [&](const uint16_t* img, int width, int col0, int t, int ks) -> u4 {
+    const int e = col0 + t * 32, col = (((e >> 3) ^ (lq << 2)) << 3) | (e & 7);
+    const uint16_t* p = img + (ks * 16 + rc_k) * width + col;
+    union {
+      s16x4 s[2];
+      u4 v;
+    } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p + 4 * width));
+    return u.v;
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  const int steps = t_end - t_beg;
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < steps) issue(s);
+  int stage = 0, ahead = STAGES - 1;
+  for (int t = 0; t < steps; ++t) {
+    // step t has landed everywhere when the younger steps' loads are all that is out; and everyone is done with step t - 1
+    if (t + STAGES - 2 < steps) wait_and_meet<(STAGES - 2) * (PA + PB)>();
+    else wait_and_meet<0>();
+    if (t + STAGES - 1 < steps) issue(ahead);
+    const uint16_t *sa = smem + stage * STAGE, *sb = sa + IMG_A;
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      u4 a[TM], b[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) a[i] = A_KC ? frag_kc(sa, kc_a, i, ks) : frag_rc(sa, BM, rc_a, i, ks);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) b[j] = B_KC ? frag_kc(sb, kc_b, j, ks) : frag_rc(sb, BN, rc_b, j, ks);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = mma<F16>(a[i], b[j], acc[i][j]);
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+  }
+
+  // acc[i][j][r]: m = m0 + 32 (wm TM + i) + 8 (r / 4) + 4 h + r % 4, n = n0 + 32 (wn TN + j) + l31
+  const int mw = m0 + wm * 32 * TM + 4 * h, nw = n0 + wn * 32 * TN + l31;
+  if constexpr (EPI == EPI_STORE) {
+    const float inv = g.d_scale[1];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = nw + 32 * j;
+      if (n >= N) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = mw + 32 * i + 8 * q;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * inv;
+          if (g.out_kind == 1) {
+            uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + (int64_t)n * g.ldo + m;
+            const uint32_t w[2] = {pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
+            if (m + 4 <= g.M) {
+              typedef uint32_t u2_any __attribute__((ext_vector_type(2), aligned(2)));
+              u2_any t;
+              t[0] = w[0];
+              t[1] = w[1];
+              *reinterpret_cast<u2_any*>(o) = t;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (m + e < g.M) o[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            }
+          } else {
+            float* o = reinterpret_cast<float*>(g.out) + ((int64_t)(g.out_kind == 0 ? part : 0) * g.N + n) * g.ldo + m;
+            typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+            if (m + 4 <= g.M) {
+              f4_any t = {v[0], v[1], v[2], v[3]};
+              if (g.add) t += *reinterpret_cast<f4_any*>(o);
+              *reinterpret_cast<f4_any*>(o) = t;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (m + e < g.M) o[e] = g.add ? o[e] + v[e] : v[e];
+            }
+          }
+        }
+    }
+  } else {
+    if (g.bias) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int v = g.v0 + min(mw + 32 * i + 8 * (r >> 2) + (r & 3), g.M - 1);
+          const float bv = g.bias_f32 ? reinterpret_cast<const float*>(g.bias)[v]
+                           : F16      ? (float)reinterpret_cast<const _Float16*>(g.bias)[v]
+                                      : (float)reinterpret_cast<const __bf16*>(g.bias)[v];
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j][r] += bv;
+        }
+    }
+    constexpr float L2E = 1.44269504088896341f;
+    const bool edge = m0 + BM > g.M;                          // classes past the last one
+    if constexpr (EPI == EPI_STATS) {
+      float2* red = reinterpret_cast<float2*>(smem);          // [W_M][BN]
+      wait_and_meet<0>();
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = nw + 32 * j;
+        const bool real = n < N;
+        // the target's logit, by the lane that holds it
+        const int64_t tt = real ? g.target[g.rows[n]] : -1;
+        const int64_t at = tt - g.v0 - mw;                    // 32 i + 8 (r / 4) + r % 4 where it is ours
+        if (__any(tt >= 0 && at >= 0 && at < 32 * TM)) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (tt >= 0 && at == 32 * i + 8 * (r >> 2) + (r & 3) && tt < g.v0 + g.M) g.target_logit[n] = acc[i][j][r];
+        }
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float ref = top == -INFINITY ? 0.f : top;       // all of them -inf: the sum is 0, not NaN
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+        sum += __shfl_xor(sum, 32, 64);
+        if (h == 0) red[wm * BN + wn * 32 * TN + 32 * j + l31] = make_float2(top, sum);
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < BN; c += 64 * NW) {
+        if (n0 + c >= N) continue;
+        float2 p = red[c];
+#pragma unroll
+        for (int w = 1; w < W_M; ++w) {
+          const float2 o = red[w * BN + c];
+          const float top = fmaxf(p.x, o.x), ref = top == -INFINITY ? 0.f : top;
+          p.y = p.y * exp_fine(p.x - ref) + o.y * exp_fine(o.x - ref);
+          p.x = top;
+        }
+        g.partial[(int64_t)tm * ((g.N + ROW_PAD - 1) / ROW_PAD * ROW_PAD) + n0 + c] = p;
+      }
+    } else {
+      const float scale = *g.d_scale;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = nw + 32 * j;
+        const bool real = n < N;
+        const float gn = real ? g.g[n] * scale : 0.f, lse = real ? g.lse[n] : 0.f;
+        const int64_t tt = real ? g.target[g.rows[n]] : -1, at = tt - g.v0 - mw;
+        const bool hit = __any(tt >= 0 && at >= 0 && at < 32 * TM);
+        const float neg = -lse * L2E;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int m = mw + 32 * i + 8 * q;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float z = acc[i][j][4 * q + e];
+              float p = FINE ? exp_fine(z - lse) : __builtin_amdgcn_exp2f(fmaf(z, L2E, neg));
+              if (hit && at == 32 * i + 8 * q + e) p -= 1.f;
+              v[e] = p * gn;
+              // zero rows are exactly zero, whatever their logits are; classes past the end too
+              if (gn == 0.f || (edge && m + e >= g.M)) v[e] = 0.f;
+            }
+            uint16_t* o = g.d + (int64_t)n * g.ldd + m;       // d is padded to whole tiles
+            if constexpr (FINE) {
+              union {
+                __bf16 t[4];
+                uint2 u;
+              } w[3];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) split3(v[e], w[0].t[e], w[1].t[e], w[2].t[e]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(o + k * g.plane_d) = w[k].u;
+            } else {
+              *reinterpret_cast<uint2*>(o) = make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
+            }
+          }
+      }
+    }
+  }
+}
+
+// Rows that count, in order: rows[0 .. kept), kept, and the sum of their class weights, by one workgroup (8192 targets at a
+// time, 8 per thread).  An ignored row's loss is written as 0 where losses are returned by row.
+__global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict__ target, int N, int V, int64_t ignore,
+                                                       const float* __restrict__ cw, int* __restrict__ state,
+                                                       float* __restrict__ target_logit, float* __restrict__ loss_rows) {
+  __shared__ int wave_n[16];
+  __shared__ double wave_w[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int before = 0;
+  double weight = 0;
+  for (int base = 0; base < N; base += 8192) {
+    const int i0 = base + threadIdx.x * 8;
+    int64_t t[8];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      t[j] = i0 + j < N ? target[i0 + j] : ignore;
+      mine += t[j] != ignore;
+    }
+    int run = mine;                                           // inclusive scan over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(run, o, 64);
+      if (lane >= o) run += u;
+    }
+    __syncthreads();
+    if (lane == 63) wave_n[wave] = run;
+    __syncthreads();
+    int at = before + run - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += wave_n[w];
+      all += wave_n[w];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i0 + j >= N) continue;
+      if (t[j] != ignore) {
+        state[S_ROWS + at] = i0 + j;
+        target_logit[at] = NAN;                               // stays so where the target is no class
+        ++at;
+        weight += t[j] < 0 || t[j] >= V ? (double)NAN : cw ? (double)cw[t[j]] : 1.0;
+      } else if (loss_rows) {
+        loss_rows[i0 + j] = 0.f;
+      }
+    }
+    before += all;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) weight += __shfl_xor(weight, o, 64);
+  __syncthreads();
+  if (lane == 0) wave_w[wave] = weight;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double w = 0;
+    for (int i = 0; i < 16; ++i) w += wave_w[i];
+    state[S_KEPT] = before;
+    reinterpret_cast<float*>(state)[S_TOTAL] = (float)w;
+  }
+}
+
+// out[i][0 .. ldo) = src[rows[i]][0 .. D), zeros behind the last column and the last kept row (up to whole tiles): 8 elements
+// per thread; T = float: three bf16 planes
+template <typename T>
+__global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ src, int64_t ld, int D, const int* __restrict__ state,
+                                                      int n_rows, uint16_t* __restrict__ out, int64_t ldo, int64_t plane) {
+  const int per = (int)(ldo / 8);
+  const int kept = state ? state[S_KEPT] : n_rows;
+  const int padded = state ? (kept + ROW_PAD - 1) / ROW_PAD * ROW_PAD : n_rows;
+  const int64_t all = (int64_t)padded * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 8;
+    constexpr int Q = sizeof(T) / 2;
+    union {
+      T t[8];
+      u4 q[Q];
+    } v;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) v.q[q] = (u4)0;
+    if (row < kept) {
+      const T* p = src + (int64_t)(state ? state[S_ROWS + row] : row) * ld + c;
+      if (c + 8 <= D) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) v.q[q] = reinterpret_cast<const u4_any*>(p)[q];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < D) v.t[j] = p[j];
+      }
+    }
+    uint16_t* o = out + (int64_t)row * ldo + c;
+    if constexpr (sizeof(T) == 4) {
+      union {
+        __bf16 t[8];
+        u4 q;
+      } w[3];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split3(v.t[j], w[0].t[j], w[1].t[j], w[2].t[j]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u4*>(o + k * plane) = w[k].q;
+    } else {
+      *reinterpret_cast<u4*>(o) = v.q[0];
+    }
+  }
+}
+
+// the partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row
+__global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restrict__ partial, int tiles, int64_t ldp,
+                                                         int* __restrict__ state, int N, const int64_t* __restrict__ target, int V,
+                                                         const float* __restrict__ cw, const float* __restrict__ target_logit,
+                                                         float* __restrict__ nll, float* __restrict__ loss_rows) {
+  __shared__ float2 red[8][32];
+  const int kept = state[S_KEPT];
+  const int row = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  if (blockIdx.x * 32 >= kept) return;
+  float top = -INFINITY, sum = 0.f;
+  if (row < kept) {
+    for (int t = part; t < tiles; t += 64) {                  // eight loads in flight
+      float2 p[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) p[u] = t + 8 * u < tiles ? partial[(int64_t)(t + 8 * u) * ldp + row] : make_float2(-INFINITY, 0.f);
+      float m = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) m = fmaxf(m, p[u].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+      sum *= exp_fine(top - ref);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += p[u].y * exp_fine(p[u].x - ref);
+      top = m;
+    }
+  }
+  red[part][threadIdx.x & 31] = make_float2(top, sum);
+  __syncthreads();
+  if (part || row >= kept) return;
+  float m = top;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i][threadIdx.x].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += red[i][threadIdx.x].y * exp_fine(red[i][threadIdx.x].x - ref);
+  const float lse = m + logf(sum);
+  reinterpret_cast<float*>(state)[S_ROWS + N + row] = lse;
+  const int orig = state[S_ROWS + row];
+  const int64_t t = target[orig];
+  const float v = (lse - target_logit[row]) * (!cw || t < 0 || t >= V ? 1.f : cw[t]);
+  if (loss_rows) loss_rows[orig] = v;
+  else nll[row] = v;
+}
+__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ nll, const int* __restrict__ state, int mean,
+                                                         float* __restrict__ loss) {
+  __shared__ double red[16];
+  const int kept = state[S_KEPT];
+  double s = 0;
+  for (int i = threadIdx.x; i < kept; i += 1024) s += (double)nll[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0;
+    for (int i = 0; i < 16; ++i) s += red[i];
+    *loss = (float)(mean ? s / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : s);
+  }
+}
+
+// g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to)
+__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up, int reduction, const int* __restrict__ state,
+                                                           const int64_t* __restrict__ target, int V, const float* __restrict__ cw,
+                                                           float to, float* __restrict__ g, float* __restrict__ d_scale) {
+  __shared__ float red[16];
+  const int kept = state[S_KEPT];
+  const float total = reinterpret_cast<const float*>(state)[S_TOTAL];
+  float top = 0.f;
+  for (int i = threadIdx.x; i < kept; i += 1024) {
+    const int orig = state[S_ROWS + i];
+    const int64_t t = target[orig];
+    float v = reduction == VAE_CE_NONE ? up[orig] : up[0];
+    if (t < 0 || t >= V) v = NAN;
+    else if (cw) v *= cw[t];
+    if (reduction == VAE_CE_MEAN) v /= total;
+    g[i] = v;
+    top = fmaxf(top, fabsf(v));
+  }
+  top = block_max<16>(top, red);
+  if (threadIdx.x == 0) {
+    const bool usable = top > 1e-30f && top < INFINITY;       // (nothing to do without a gradient; infinities reach the result)
+    d_scale[0] = usable ? to / top : 1.f;
+    d_scale[1] = usable ? top / to : 1.f;
+  }
+}
+
+// dx: the slabs (S, N, D) of a packed row added in order and put at its original row; ignored rows are zero.  A workgroup per
+// row, four columns per thread.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ slabs, int S, int64_t slab, int N, int D,
+                                                    const int* __restrict__ state, const int64_t* __restrict__ target, int64_t ignore,
+                                                    T* __restrict__ dx) {
+  typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+  const int kept = state[S_KEPT];
+  for (int row = blockIdx.x; row < kept; row += gridDim.x) {
+    T* o = dx + (int64_t)state[S_ROWS + row] * D;
+    const float* p = slabs + (int64_t)row * D;
+    for (int c = threadIdx.x * 4; c < D; c += 1024) {
+      if (c + 4 <= D) {
+        f4_any s = {0.f, 0.f, 0.f, 0.f};
+        int k = 0;
+        for (; k + 4 <= S; k += 4) {
+          f4_any v[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f4_any*>(p + (k + u) * slab + c);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s += v[u];
+        }
+        for (; k < S; ++k) s += *reinterpret_cast<const f4_any*>(p + k * slab + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[c + e] = (T)s[e];
+      } else {
+        for (int e = c; e < D; ++e) {
+          float s = 0.f;
+          for (int k = 0; k < S; ++k) s += p[k * slab + e];
+          o[e] = (T)s;
+        }
+      }
+    }
+  }
+  for (int row = blockIdx.x; row < N; row += gridDim.x) {
+    if (target[row] != ignore) continue;
+    for (int c = threadIdx.x; c < D; c += 256) dx[(int64_t)row * D + c] = (T)0;
+  }
+}
+
+// db[v] = sum over the kept rows of d: 64 classes to a workgroup, 16 waves over the rows, added in order
+template <int KIND>   // 0: three bf16 planes -> float, 1: bf16, 2: fp16
+__global__ __launch_bounds__(1024) void ce_bias_kernel(const uint16_t* __restrict__ d, int64_t ldd, int64_t plane, const int* __restrict__ state,
+                                                       int V, const float* __restrict__ d_scale, void* __restrict__ out) {
+  __shared__ float red[16][64];
+  const int v = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, kept = state[S_KEPT];
+  float s = 0.f;
+  for (int n = w; n < kept; n += 16 * 8) {
+    float t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int row = n + 16 * u;
+      t[u] = 0.f;
+      if (row < kept && v < V) {
+        const uint16_t* p = d + (int64_t)row * ldd + v;
+        if (KIND == 2) t[u] = (float)__builtin_bit_cast(_Float16, *p);
+        else t[u] = (float)__builtin_bit_cast(__bf16, *p);
+        if (KIND == 0) t[u] += (float)__builtin_bit_cast(__bf16, p[plane]) + (float)__builtin_bit_cast(__bf16, p[2 * plane]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += t[u];
+  }
+  red[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w || v >= V) return;
+  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+  s *= d_scale[1];
+  if (KIND == 0) reinterpret_cast<float*>(out)[v] = s;
+  else if (KIND == 1) reinterpret_cast<__bf16*>(out)[v] = (__bf16)s;
+  else reinterpret_cast<_Float16*>(out)[v] = (_Float16)s;
+}
+
+// ---- host ----
+int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
+struct Plan {
+  bool f32, pack_w;
+  int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
+  int64_t planes;
+  int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
+  int split;                                          // slabs of dx
+  // byte offsets in the workspaces
+  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, bytes;
+};
+
+constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
+
+Plan plan_of(const vae_linear_ce* a, bool bwd) {
+  Plan p;
+  p.f32 = a->dtype == VAE_ADAMW_F32;
+  p.planes = p.f32 ? 3 : 1;
+  p.n_pad = up_to(a->N, ROW_PAD);
+  p.d_pad = up_to(a->D, K_PAD);
+  p.pack_w = p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w);
+  p.ldw = p.pack_w ? p.d_pad : a->ldw;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up_to(bytes, 256);
+    return o;
+  };
+  p.x = take(p.planes * p.n_pad * p.d_pad * 2);
+  p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
+  if (!bwd) {
+    p.partial = take(up_to(a->V, 128) / 128 * p.n_pad * 8);
+    p.tlogit = take(p.n_pad * 4);
+    p.nll = take(p.n_pad * 4);
+  } else {
+    p.g = take(p.n_pad * 4);
+    p.scale = take(8);
+    const int64_t fit = D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256, most = up_to(a->V, 256);
+    p.piece = fit < 256 ? 256 : fit < most ? fit : most;
+    // pieces of equal length
+    const int64_t pieces = (most + p.piece - 1) / p.piece;
+    p.piece = up_to((most + pieces - 1) / pieces, 256);
+    p.d = take(p.planes * p.n_pad * p.piece * 2);
+    // dx has N x D outputs and a sum over the classes: where its tiles do not fill the chip the sum is split
+    const int64_t tiles = (p.n_pad / 128) * ((a->D + 127) / 128);
+    int64_t s = 512 / tiles;
+    const int64_t steps = p.piece / 32 * (p.f32 ? 6 : 1);
+    if (s > steps / 16) s = steps / 16;
+    p.split = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    p.slabs = take((int64_t)p.split * p.n_pad * a->D * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+template <bool F16, bool A_KC, bool B_KC, int EPI, bool FINE> void launch_gemm(Gemm g, bool big, hipStream_t st) {
+  const int b = big ? 256 : 128;
+  g.tiles_m = (g.M + b - 1) / b;
+  g.tiles_n = (g.N + b - 1) / b;
+  const uint32_t grid = (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
+  if (big) head_gemm_kernel<F16, A_KC, B_KC, 256, 256, 2, 4, 32, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);
+  else head_gemm_kernel<F16, A_KC, B_KC, 128, 128, 2, 2, 32, 4, EPI, FINE><<<grid, 256, 0, st>>>(g);
+}
+template <bool A_KC, bool B_KC, int EPI> void gemm(const Gemm& g, int dtype, bool big, hipStream_t st) {
+  if (dtype == VAE_ADAMW_F32) launch_gemm<false, A_KC, B_KC, EPI, EPI != EPI_STORE>(g, big, st);
+  else if (dtype == VAE_ADAMW_BF16) launch_gemm<false, A_KC, B_KC, EPI, false>(g, big, st);
+  else launch_gemm<true, A_KC, B_KC, EPI, false>(g, big, st);
+}
+// 256 x 256 tiles once they fill the chip; below that 128 x 128 ones, two workgroups to a CU
+bool big_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 200; }
+
+void pack(const void* src, int64_t ld, int64_t D, const int* state, int64_t rows, int64_t padded, uint16_t* out, int64_t ldo, int64_t plane,
+          int dtype, hipStream_t st) {
+  const int64_t work = padded * (ldo / 8) / 256 + 1;
+  const int grid = (int)(work < 4096 ? work : 4096);
+  if (dtype == VAE_ADAMW_F32) ce_pack_kernel<float><<<grid, 256, 0, st>>>((const float*)src, ld, (int)D, state, (int)rows, out, ldo, plane);
+  else ce_pack_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)src, ld, (int)D, state, (int)rows, out, ldo, plane);
+}
+
+int check(const vae_linear_ce* a, const char* who) {
+  VAE_REQUIRE(a, "%s: null arguments", who);
+  VAE_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "%s: unknown dtype %d", who, a->dtype);
+  VAE_REQUIRE(a->N >= 1 && a->D >= 1 && a->V >= 1, "%s: N, D and V must be at least 1", who);
+  VAE_REQUIRE(a->N <= (1ll << 24) && a->D <= (1ll << 20) && a->V <= (1ll << 24), "%s: at most 2^24 rows, 2^20 columns and 2^24 classes", who);
+  VAE_REQUIRE((a->N + 127) / 128 * ((a->V + 127) / 128) < (1ll << 30), "%s: more than 2^30 tiles", who);
+  VAE_REQUIRE(a->x && a->w && a->target, "%s: null pointer", who);
+  VAE_REQUIRE((a->N == 1 || a->ldx >= 0) && (a->V == 1 || a->ldw >= a->D), "%s: bad row stride", who);
+  VAE_REQUIRE(a->ldw < (1ll << 22) && a->ldx < (1ll << 40), "%s: a row stride is too large", who);
+  const uintptr_t bad = a->dtype == VAE_ADAMW_F32 ? 3 : 1;
+  VAE_REQUIRE(((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->w) | reinterpret_cast<uintptr_t>(a->bias)) & bad) == 0,
+              "%s: a pointer is not aligned to its element", who);
+  return VAE_OK;
+}
+
+Gemm logits_gemm(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state) {
+  Gemm g = {};
+  g.a = p.pack_w ? reinterpret_cast<const uint16_t*>(ws + p.w) : reinterpret_cast<const uint16_t*>(a->w);
+  g.lda = p.ldw;
+  g.plane_a = a->V * p.d_pad;
+  g.b = reinterpret_cast<const uint16_t*>(ws + p.x);
+  g.ldb = p.d_pad;
+  g.plane_b = p.n_pad * p.d_pad;
+  g.M = (int)a->V;
+  g.N = (int)a->N;
+  g.K = (int)(p.pack_w ? p.d_pad : a->D);
+  g.segs = p.f32 ? 6 : 1;
+  g.split = 1;
+  g.dyn = state + S_KEPT;
+  g.bias = a->bias;
+  g.bias_f32 = p.f32;
+  g.target = a->target;
+  g.rows = state + S_ROWS;
+  return g;
+}
+
+}  // namespace
+
+extern "C" int64_t vae_linear_ce_state_bytes(int64_t N) { return (S_ROWS + 2 * N) * 4; }
+
+extern "C" int64_t vae_linear_ce_workspace_bytes(const vae_linear_ce* a, int backward) {
+  if (check(a, "vae_linear_ce_workspace_bytes")) return -1;
+  return plan_of(a, backward != 0).bytes;
+}
+
+extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* loss, void* state, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  if (int rc = check(a, "vae_linear_ce_fwd")) return rc;
+  VAE_REQUIRE(reduction >= VAE_CE_NONE && reduction <= VAE_CE_MEAN, "vae_linear_ce_fwd: unknown reduction %d", reduction);
+  VAE_REQUIRE(loss && state, "vae_linear_ce_fwd: null pointer");
+  const Plan p = plan_of(a, false);
+  VAE_REQUIRE(workspace && vae_aligned16(workspace) && workspace_bytes >= p.bytes,
+              "vae_linear_ce_fwd: needs a 16-byte aligned workspace of vae_linear_ce_workspace_bytes()");
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  int* s = reinterpret_cast<int*>(state);
+  hipStream_t st = (hipStream_t)stream;
+  float *tl = reinterpret_cast<float*>(ws + p.tlogit), *nll = reinterpret_cast<float*>(ws + p.nll);
+  float* by_row = reduction == VAE_CE_NONE ? loss : nullptr;
+  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, by_row);
+  VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+  pack(a->x, a->ldx, a->D, s, a->N, p.n_pad, reinterpret_cast<uint16_t*>(ws + p.x), p.d_pad, p.n_pad * p.d_pad, a->dtype, st);
+  if (p.pack_w) pack(a->w, a->ldw, a->D, nullptr, a->V, a->V, reinterpret_cast<uint16_t*>(ws + p.w), p.d_pad, a->V * p.d_pad, a->dtype, st);
+  VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+  Gemm g = logits_gemm(a, p, ws, s);
+  g.partial = reinterpret_cast<float2*>(ws + p.partial);
+  g.target_logit = tl;
+  const bool big = big_tiles(g.M, g.N);
+  gemm<true, true, EPI_STATS>(g, a->dtype, big, st);
+  VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+  const int b = big ? 256 : 128;
+  ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->target,
+                                                                  (int)a->V, a->class_weight, tl, nll, by_row);
+  if (!by_row) ce_reduce_kernel<<<1, 1024, 0, st>>>(nll, s, reduction == VAE_CE_MEAN, loss);
+  VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+  return VAE_OK;
+}
+
+extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const float* grad, const void* state, void* dx, void* dw, void* dbias,
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = check(a, "vae_linear_ce_bwd")) return rc;
+  VAE_REQUIRE(reduction >= VAE_CE_NONE && reduction <= VAE_CE_MEAN, "vae_linear_ce_bwd: unknown reduction %d", reduction);
+  VAE_REQUIRE(grad && state && (dx || dw || dbias), "vae_linear_ce_bwd: null pointer");
+  VAE_REQUIRE(!dbias || a->bias, "vae_linear_ce_bwd: a gradient of a bias that is not there");
+  const Plan p = plan_of(a, true);
+  VAE_REQUIRE(workspace && vae_aligned16(workspace) && workspace_bytes >= p.bytes,
+              "vae_linear_ce_bwd: needs a 16-byte aligned workspace of vae_linear_ce_workspace_bytes()");
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  const int* s = reinterpret_cast<const int*>(state);
+  hipStream_t st = (hipStream_t)stream;
+  float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs);
+  uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
+  const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
+  ce_upstream_kernel<<<1, 1024, 0, st>>>(grad, reduction, s, a->target, (int)a->V, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale);
+  VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+  pack(a->x, a->ldx, a->D, s, a->N, p.n_pad, xp, p.d_pad, p.n_pad * p.d_pad, a->dtype, st);
+  if (p.pack_w) pack(a->w, a->ldw, a->D, nullptr, a->V, a->V, reinterpret_cast<uint16_t*>(ws + p.w), p.d_pad, a->V * p.d_pad, a->dtype, st);
+  VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+  for (int64_t v0 = 0; v0 < a->V; v0 += p.piece) {
+    const int64_t n_v = a->V - v0 < p.piece ? a->V - v0 : p.piece;
+    Gemm z = logits_gemm(a, p, ws, s);
+    const uint16_t* w0 = z.a + v0 * z.lda;
+    z.a = w0;
+    z.M = (int)n_v;
+    z.v0 = (int)v0;
+    z.lse = reinterpret_cast<const float*>(s) + S_ROWS + a->N;
+    z.g = gr;
+    z.d_scale = scale;
+    z.d = d;
+    z.ldd = p.piece;
+    z.plane_d = plane_d;
+    gemm<true, true, EPI_D>(z, a->dtype, big_tiles(z.M, z.N), st);
+    VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    if (dx) {                                           // dx (N, D) += d (N, n_v) W (n_v, D)
+      Gemm g = {};
+      g.a = w0;
+      g.lda = z.lda;
+      g.plane_a = z.plane_a;
+      g.b = d;
+      g.ldb = p.piece;
+      g.plane_b = plane_d;
+      g.M = (int)a->D;
+      g.N = (int)a->N;
+      g.K = (int)n_v;
+      g.segs = z.segs;
+      g.dyn = s + S_KEPT;
+      g.d_scale = scale;
+      g.out = slabs;
+      g.ldo = a->D;
+      g.out_kind = 0;
+      g.add = v0 > 0;
+      const bool big = big_tiles(g.M, g.N);
+      g.split = big ? 1 : p.split;
+      gemm<false, true, EPI_STORE>(g, a->dtype, big, st);
+      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    }
+    if (dw) {                                           // dW (n_v, D) = d^T (n_v, N) x (N, D)
+      Gemm g = {};
+      g.a = xp;
+      g.lda = p.d_pad;
+      g.plane_a = p.n_pad * p.d_pad;
+      g.b = d;
+      g.ldb = p.piece;
+      g.plane_b = plane_d;
+      g.M = (int)a->D;
+      g.N = (int)n_v;
+      g.K = (int)a->N;
+      g.segs = z.segs;
+      g.split = 1;
+      g.dyn = s + S_KEPT;
+      g.dyn_k = 1;
+      g.d_scale = scale;
+      g.out = reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize;
+      g.ldo = a->D;
+      g.out_kind = p.f32 ? 2 : 1;
+      gemm<false, false, EPI_STORE>(g, a->dtype, big_tiles(g.M, g.N), st);
+      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    }
+    if (dbias) {
+      const unsigned grid = (unsigned)((n_v + 63) / 64);
+      void* o = reinterpret_cast<uint8_t*>(dbias) + v0 * esize;
+      if (p.f32) ce_bias_kernel<0><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
+      else if (a->dtype == VAE_ADAMW_BF16) ce_bias_kernel<1><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
+      else ce_bias_kernel<2><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
+      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    }
+  }
+  if (dx) {
+    const int S = big_tiles(a->D, a->N) ? 1 : p.split;
+    const int rows = (int)(a->N < 4096 ? a->N : 4096);
+#define VAE_DX(T) ce_dx_kernel<T><<<rows, 256, 0, st>>>(slabs, S, a->N * a->D, (int)a->N, (int)a->D, s, a->target, a->ignore_index, (T*)dx)
+    if (p.f32) VAE_DX(float);
+    else if (a->dtype == VAE_ADAMW_BF16) VAE_DX(__bf16);
+    else VAE_DX(_Float16);
+#undef VAE_DX
+    VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+  }
+  return VAE_OK;
+}

@@ -1,6 +1,9 @@
 """Alternative classification losses and GroupDRO re-weighting with the reference's names and
 call signatures (src/losses.py:9-202).  Off by default in the reference (task.py:133-134,
-config.py:80) and tiny (B x n_classes): plain torch, no kernels."""
+config.py:80) and tiny (B x n_classes): plain torch, no kernels.
+
+``linear_cross_entropy`` / ``LinearCrossEntropyLoss``: the cross entropy of the discrete cell-property heads
+(task.py:129-137) for heads with many classes, on the HIP kernels and without the logits in memory."""
 from __future__ import annotations
 
 from typing import List, Optional
@@ -104,3 +107,48 @@ class GroupDRO:
 
     def get_weights(self, group_idx):
         return torch.from_numpy(np.array([self.weights[g] for g in group_idx]))
+
+
+def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                         weight: Optional[torch.Tensor] = None, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(x @ w.T + bias, target, weight, ignore_index=..., reduction=...)`` as float32, differentiable once in
+    ``x`` (..., D), ``w`` (V, D) and ``bias`` (V), without the (..., V) logits ever being in memory.
+
+    ``x``, ``w`` and ``bias`` are float32, bfloat16 or float16, all of one type; sums, the softmax statistics and the loss are
+    held in 32 bits.  ``target`` (...) int64; ``weight`` (V) float32 class weights.  Rows whose target is ``ignore_index`` take no
+    part: their loss and gradient are 0, and they cost next to nothing.  Any other target outside [0, V) makes its row's loss
+    and gradients NaN (torch stops with a device assertion).  "mean" divides by the sum of the class weights that took part
+    (NaN when none did; the gradients are 0 then)."""
+    from .autograd import LinearCrossEntropyFn
+    if x.dim() < 1 or tuple(target.shape) != tuple(x.shape[:-1]):
+        raise ValueError(f"vae_amd.linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if rows.numel() and rows.stride(1) != 1 and rows.shape[1] > 1:
+        rows = rows.contiguous()
+    if w.dim() == 2 and w.shape[1] > 1 and (w.stride(1) != 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1])):
+        w = w.contiguous()
+    if rows.shape[0] == 0 and w.dim() == 2 and w.shape[1] == rows.shape[1]:   # as torch: nothing, 0 or 0 / 0, with zero gradients
+        if reduction not in ("none", "sum", "mean"):
+            raise ValueError(f"vae_amd.linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+        if not x.is_cuda:
+            raise RuntimeError("vae_amd.linear_cross_entropy: all tensors must live on one GPU (no CPU fallback)")
+        zero = (rows.float().sum() + 0.0 * sum(t.float().flatten()[:1].sum() for t in (w, bias) if t is not None))
+        return rows.float().sum(1).view(target.shape) if reduction == "none" else zero if reduction == "sum" else zero + float("nan")
+    loss = LinearCrossEntropyFn.apply(rows, w, bias, target.reshape(-1), weight, ignore_index, reduction)
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+class LinearCrossEntropyLoss(nn.Module):
+    """A class head and its loss in one: ``forward(x, target)`` is the cross entropy of ``nn.Linear(in_features, num_classes)``
+    on ``x`` (``linear_cross_entropy``); ``weight`` as ``task.class_balance_weights`` makes it."""
+
+    def __init__(self, in_features: int, num_classes: int, bias: bool = True, weight: Optional[torch.Tensor] = None,
+                 ignore_index: int = -100, reduction: str = "mean"):
+        super().__init__()
+        self.linear = nn.Linear(in_features, num_classes, bias=bias)
+        self.register_buffer("weight", weight, persistent=False)
+        self.ignore_index, self.reduction = ignore_index, reduction
+
+    def forward(self, x: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
+        return linear_cross_entropy(x, self.linear.weight, target, bias=self.linear.bias, weight=self.weight,
+                                    ignore_index=self.ignore_index, reduction=self.reduction)

@@ -803,3 +803,86 @@ def gated_norm_bwd(dy: Optional[torch.Tensor], dh: Optional[torch.Tensor], y: to
         rc = lib.vae_gated_norm_bwd(C.byref(a), _p(ws), nbytes, _stream())
     _lib.check(rc, "gated_norm_bwd")
     return out
+
+
+REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction) -> "_lib.LinearCE":
+    who = "vae_amd.ops.linear_ce"
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"{who}: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
+    if x.dtype not in FLOAT_DTYPES:
+        raise TypeError(f"{who}: rows of {x.dtype} are not supported (float32, bfloat16, float16)")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"{who}: x must be (N, D) and w (V, D), got {tuple(x.shape)} and {tuple(w.shape)}")
+    (N, D), V = x.shape, w.shape[0]
+    if N < 1 or D < 1 or V < 1:
+        raise ValueError(f"{who}: no rows, columns or classes in {tuple(x.shape)} x {tuple(w.shape)}")
+    if tuple(target.shape) != (N,) or target.dtype != torch.int64 or not target.is_contiguous():
+        raise ValueError(f"{who}: target must be a contiguous int64 vector of {N}, got {tuple(target.shape)} {target.dtype}")
+    for t, name, shape, dtype in ((w, "w", (V, D), x.dtype), (bias, "bias", (V,), x.dtype), (weight, "weight", (V,), torch.float32)):
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"{who}: {name} is {t.dtype}, {dtype} is needed")
+        if tuple(t.shape) != shape or (name != "w" and not t.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be a contiguous vector of {V}, got {tuple(t.shape)}")
+    for t, name in ((x, "x"), (w, "w")):
+        if D > 1 and t.stride(1) != 1:
+            raise ValueError(f"{who}: {name} must have a contiguous last dim, got strides {t.stride()}")
+    if V > 1 and w.stride(0) < D:
+        raise ValueError(f"{who}: the rows of w overlap (strides {w.stride()})")
+    for t in (x, w, target, bias, weight):
+        if t is not None and (not t.is_cuda or t.device != x.device):
+            raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
+    return _lib.LinearCE(N=N, D=D, V=V, dtype=FLOAT_DTYPES[x.dtype], x=x.data_ptr(), ldx=x.stride(0) if N > 1 else D, w=w.data_ptr(),
+                         ldw=w.stride(0) if V > 1 else D, bias=None if bias is None else bias.data_ptr(), target=target.data_ptr(),
+                         class_weight=None if weight is None else weight.data_ptr(), ignore_index=int(ignore_index))
+
+
+def _linear_ce_workspace(lib, a, backward: int, device) -> Tuple[torch.Tensor, int]:
+    """Scratch of one call alone (torch's allocator keeps it with the stream, and with a captured graph)."""
+    n = lib.vae_linear_ce_workspace_bytes(C.byref(a), backward)
+    if n < 0:
+        raise ValueError(f"vae_amd.ops.linear_ce: {lib.vae_last_error().decode()}")
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def linear_ce_fwd(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  weight: Optional[torch.Tensor] = None, ignore_index: int = -100, reduction: str = "mean"):
+    """-> (loss float32 () or (N,), state for ``linear_ce_bwd``): cross entropy of ``x w^T + bias`` (include/vae_amd.h,
+    vae_linear_ce_fwd)."""
+    lib = _lib.load()
+    a = _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction)
+    with torch.cuda.device(x.device):
+        loss = torch.empty((a.N,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        state = torch.empty(lib.vae_linear_ce_state_bytes(a.N) // 4, dtype=torch.int32, device=x.device)
+        ws, n = _linear_ce_workspace(lib, a, 0, x.device)
+        rc = lib.vae_linear_ce_fwd(C.byref(a), REDUCTIONS[reduction], loss.data_ptr(), state.data_ptr(), ws.data_ptr(), n, _stream())
+    _lib.check(rc, "linear_ce_fwd")
+    return loss, state
+
+
+def linear_ce_bwd(grad: torch.Tensor, state: torch.Tensor, x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
+                  bias: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                  reduction: str = "mean", need_x: bool = True, need_w: bool = True, need_bias: bool = True):
+    """-> (dx, dw, dbias), None where not needed; ``grad``: float32 gradient of the loss."""
+    lib = _lib.load()
+    a = _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction)
+    if grad.dtype != torch.float32 or grad.numel() != (a.N if reduction == "none" else 1) or grad.device != x.device:
+        raise ValueError(f"vae_amd.ops.linear_ce_bwd: grad must be the float32 gradient of the loss, got {tuple(grad.shape)} {grad.dtype}")
+    if state.numel() * 4 != lib.vae_linear_ce_state_bytes(a.N) or state.dtype != torch.int32 or state.device != x.device or not state.is_contiguous():
+        raise ValueError("vae_amd.ops.linear_ce_bwd: state is not that of a forward pass over these rows")
+    grad = grad.contiguous()
+    with torch.cuda.device(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if need_w else None
+        db = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if need_bias and bias is not None else None
+        if dx is None and dw is None and db is None:
+            return None, None, None
+        ws, n = _linear_ce_workspace(lib, a, 1, x.device)
+        rc = lib.vae_linear_ce_bwd(C.byref(a), REDUCTIONS[reduction], grad.data_ptr(), state.data_ptr(), _p(dx), _p(dw), _p(db), ws.data_ptr(),
+                                   n, _stream())
+    _lib.check(rc, "linear_ce_bwd")
+    return dx, dw, db
