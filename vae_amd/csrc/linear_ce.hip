@@ -114,14 +114,15 @@ template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) 
   return w.u;
 }
 
-// Tile product.  B M x B N outputs, W_M x W_N waves, K in steps of BK through STAGES images in LDS, filled by direct loads that
-// run STAGES - 1 steps ahead; one barrier per step.
+// Tile product.  BM x BN outputs, W_M x W_N waves, K in steps of BK through two images in LDS, filled by direct loads; one
+// barrier per step.
 //   KC image [rows][BK]: 16-byte chunk c of a row sits at chunk c ^ f(row), so that the 16 rows of a b128 read hit all banks.
 //   RC image [BK][rows]: chunk c of k sits at c ^ 4 (k & 3); fragments by the transposing read, whose 16 lanes take 4 k x 16 rows.
 // Rows and columns of A past its end are clamped to the last one (their products are not stored, or meet zeros in B); B is a
 // packed operand, padded with zeros to whole tiles.
-template <bool F16, bool A_KC, bool B_KC, int BM, int BN, int W_M, int W_N, int BK, int STAGES, int EPI, bool FINE>
+template <bool F16, bool A_KC, bool B_KC, int BM, int BN, int W_M, int W_N, int EPI, bool FINE>
 __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
+  constexpr int BK = 64, STAGES = 2, SPREAD = 2;
   constexpr int NW = W_M * W_N, TM = BM / (32 * W_M), TN = BN / (32 * W_N);
   constexpr int IMG_A = BM * BK, IMG_B = BN * BK, STAGE = IMG_A + IMG_B;          // elements
   constexpr int PA = IMG_A * 2 / 1024 / NW, PB = IMG_B * 2 / 1024 / NW;           // 1 KB pieces per wave
@@ -160,13 +161,12 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   const int kt1 = (K + BK - 1) / BK, all = kt1 * g.segs, per = (all + g.split - 1) / g.split;
   const int t_beg = min(part * per, all), t_end = min(t_beg + per, all);
 
-  // ---- loads: per-lane byte offsets from a base that moves with K ----
-  uint32_t off_a[PA], off_b[PB];
-  auto chunk_a = [&](int i, int k_left) -> uint32_t {        // k_left: elements of K from this step on
+  // ---- loads: per-lane byte offsets from a base that moves with K; `k_left` elements of K remain from the step on ----
+  auto chunk_a = [&](int i, int k_left) -> uint32_t {
     const int piece = wave * PA + i;
     if (A_KC) {
       constexpr int CPR = BK / 8;
-      const int row = piece * (64 / CPR) + lane / CPR, swz = BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+      const int row = piece * (64 / CPR) + lane / CPR, swz = (row >> 1) & 7;
       const int c = min((lane % CPR) ^ swz, (k_left + 7) / 8 - 1);
       return (uint32_t)(((int64_t)(min(m0 + row, g.M - 1) - m0) * g.lda + 8 * c) * 2);
     }
@@ -178,45 +178,44 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     const int piece = wave * PB + i;
     if (B_KC) {
       constexpr int CPR = BK / 8;
-      const int row = piece * (64 / CPR) + lane / CPR, swz = BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+      const int row = piece * (64 / CPR) + lane / CPR, swz = (row >> 1) & 7;
       return (uint32_t)(((int64_t)row * g.ldb + 8 * ((lane % CPR) ^ swz)) * 2);
     }
     constexpr int CPR = BN / 8;
     const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
     return (uint32_t)(((int64_t)k * g.ldb + 8 * c) * 2);
   };
+  const int k_tail = K - (kt1 - 1) * BK;                     // of the last step: 1 .. BK
+  uint32_t off_a[PA], off_t[PA], off_b[PB];
 #pragma unroll
-  for (int i = 0; i < PA; ++i) off_a[i] = chunk_a(i, BK);
+  for (int i = 0; i < PA; ++i) off_a[i] = chunk_a(i, BK), off_t[i] = chunk_a(i, max(k_tail, 1));
 #pragma unroll
   for (int i = 0; i < PB; ++i) off_b[i] = chunk_b(i);
 
   const uint16_t* base_a = A_KC ? g.a + (int64_t)m0 * g.lda : g.a + m0;
   const uint16_t* base_b = B_KC ? g.b + (int64_t)n0 * g.ldb : g.b + n0;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
-  int seg = t_beg / max(kt1, 1), kt = t_beg - seg * kt1;     // of the next step to load
-  auto issue = [&](int stage) {
+  const int steps = t_end - t_beg;
+  int seg = t_beg / max(kt1, 1), kt = t_beg - seg * kt1, fetched = 0, fill = 0;   // of the next step to load, and its image
+  const uint16_t *sa, *sb;                                              // its base
+  bool tail;
+  auto aim = [&]() {
     // terms (hi 0, mid 1, lo 2) of the product a * b that segment `seg` forms: mm, hl, lh, hm, mh, hh
     const int pa = g.segs == 1 ? 0 : (0x102010 >> (20 - 4 * seg)) & 15, pb = g.segs == 1 ? 0 : (0x120100 >> (20 - 4 * seg)) & 15;
     const int k0 = kt * BK;
-    const uint16_t* sa = base_a + pa * g.plane_a + (A_KC ? (int64_t)k0 : (int64_t)k0 * g.lda);
-    const uint16_t* sb = base_b + pb * g.plane_b + (B_KC ? (int64_t)k0 : (int64_t)k0 * g.ldb);
-    const uint32_t la = lds0 + (uint32_t)stage * (STAGE * 2u) + (uint32_t)wave * (PA * 1024u);
-    const uint32_t lb = lds0 + (uint32_t)stage * (STAGE * 2u) + IMG_A * 2u + (uint32_t)wave * (PB * 1024u);
-    const int left = K - k0;
-    if (left >= BK) {
-#pragma unroll
-      for (int i = 0; i < PA; ++i) dma16(sa, off_a[i], la + i * 1024u);
-    } else {
-#pragma unroll
-      for (int i = 0; i < PA; ++i) dma16(sa, chunk_a(i, left), la + i * 1024u);
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) dma16(sb, off_b[i], lb + i * 1024u);
+    sa = base_a + pa * g.plane_a + (A_KC ? (int64_t)k0 : (int64_t)k0 * g.lda);
+    sb = base_b + pb * g.plane_b + (B_KC ? (int64_t)k0 : (int64_t)k0 * g.ldb);
+    tail = kt == kt1 - 1;
     if (++kt == kt1) kt = 0, ++seg;
+  };
+  auto load = [&](int i) {                                              // piece i of the step aimed at
+    const uint32_t st = lds0 + (uint32_t)fill * (STAGE * 2u);
+    if (i < PA) dma16(sa, tail ? off_t[i] : off_a[i], st + (uint32_t)(wave * PA + i) * 1024u);
+    else dma16(sb, off_b[i - PA], st + IMG_A * 2u + (uint32_t)(wave * PB + i - PA) * 1024u);
   };
 
   // ---- fragments ----
-  const int swz = BK == 64 ? (l31 >> 1) & 7 : (l31 >> 2) & 3;
+  const int swz = (l31 >> 1) & 7;
   const int la = lane & 15, lq = la >> 2, lp = la & 3, lj = lane >> 4;
   const int kc_a = (wm * 32 * TM + l31) * BK, kc_b = (wn * 32 * TN + l31) * BK;
   const int rc_k = 8 * (lj >> 1) + lq;
@@ -244,77 +243,152 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  const int steps = t_end - t_beg;
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < steps) issue(s);
-  int stage = 0, ahead = STAGES - 1;
-  for (int t = 0; t < steps; ++t) {
-    // step t has landed everywhere when the younger steps' loads are all that is out; and everyone is done with step t - 1
-    if (t + STAGES - 2 < steps) wait_and_meet<(STAGES - 2) * (PA + PB)>();
-    else wait_and_meet<0>();
-    if (t + STAGES - 1 < steps) issue(ahead);
-    const uint16_t *sa = smem + stage * STAGE, *sb = sa + IMG_A;
-#pragma unroll
-    for (int ks = 0; ks < BK / 16; ++ks) {
-      u4 a[TM], b[TN];
-#pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = A_KC ? frag_kc(sa, kc_a, i, ks) : frag_rc(sa, BM, rc_a, i, ks);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = B_KC ? frag_kc(sb, kc_b, j, ks) : frag_rc(sb, BN, rc_b, j, ks);
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][j] = mma<F16>(a[i], b[j], acc[i][j]);
+  // Two images: while one is multiplied the other is filled.  The fragments of the next 16 of K are read ahead of the
+  // products of this 16; before the last products of a step its image has been read by everyone, so the step after next is
+  // sent into it between those products.
+  u4 a[2][TM], b[2][TN];
+  constexpr int KS = BK / 16, MMAS = TM * TN, READS = TM + TN, LOADS = PA + PB, HEAD = MMAS / 4;
+  static_assert(KS % 2 == 0 && HEAD >= 1, "fragments alternate between two sets");
+  auto read = [&](int which, int image, int ks, int r) {     // in the order in which the products want them
+    const uint16_t *ia = smem + image * STAGE, *ib = ia + IMG_A;
+    if (r == 0 || r > TM) {
+      const int j = r == 0 ? 0 : r - TM;
+      b[which][j] = B_KC ? frag_kc(ib, kc_b, j, ks) : frag_rc(ib, BN, rc_b, j, ks);
+    } else {
+      a[which][r - 1] = A_KC ? frag_kc(ia, kc_a, r - 1, ks) : frag_rc(ia, BM, rc_a, r - 1, ks);
     }
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+  };
+  for (; fetched < STAGES && fetched < steps; ++fetched, ++fill) {
+    aim();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(i);
+  }
+  if (steps >= STAGES) wait_and_meet<LOADS>();
+  else wait_and_meet<0>();
+#pragma unroll
+  for (int r = 0; r < READS; ++r) read(0, 0, 0, r);
+  // The loads of a step go out over the two phases (16 of K each) that follow the one in which its image became free.  In one
+  // phase they fill the queue of the vector memory unit and hold up the products behind them (1.48 us a step of a 256 x 256
+  // tile), over three or four the last ones arrive late (1.44, 1.52); over two 1.44.  The products alone take 1.25 at the
+  // clock that their power leaves, as do the library's.  K steps of 32 with 3 to 5 images: 1.61 and more.
+  constexpr int LAST = KS - 1, EACH = (LOADS + SPREAD - 1) / SPREAD;
+  static_assert(SPREAD <= KS, "a step's loads are out before the next image becomes free");
+  fill = 0;
+  int image = 0, next = 1;
+  bool more = false;
+  for (int t = 0; t < steps; ++t) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int cur = ks & 1, head = ks == LAST ? HEAD : 0, phase = ks == LAST ? 0 : ks + 1;
+      int r = 0;
+#pragma unroll
+      for (int q = 0; q < MMAS; ++q) {
+        const int i = q % TM, j = q / TM;
+        acc[i][j] = mma<F16>(a[cur][i], b[cur][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (ks == LAST && q == head - 1) {
+          wait_and_meet<0>();                                // the next step is here, and nobody reads this image any more
+          more = t + STAGES < steps;
+          fill = image;
+          if (more) aim();
+        }
+        if (q >= head) {
+          // spread what is to be read and loaded over the products
+          const int done = q - head + 1, of = MMAS - head;
+#pragma unroll
+          for (; r * of < READS * done; ++r) read(cur ^ 1, ks == LAST ? next : image, ks == LAST ? 0 : ks + 1, r);   // (behind the last step: old values)
+          if (phase < SPREAD && more) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+              if (e * of / EACH == done - 1 && phase * EACH + e < LOADS) load(phase * EACH + e);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (ks == LAST) image = next, next ^= 1;
+    }
   }
 
   // acc[i][j][r]: m = m0 + 32 (wm TM + i) + 8 (r / 4) + 4 h + r % 4, n = n0 + 32 (wn TN + j) + l31
   const int mw = m0 + wm * 32 * TM + 4 * h, nw = n0 + wn * 32 * TN + l31;
-  if constexpr (EPI == EPI_STORE) {
-    const float inv = g.d_scale[1];
+  // The waves' outputs go through LDS (the images are done with), where a row n of the tile is contiguous in m, and leave as
+  // whole rows: straight from the registers every store would touch 32 rows.  16-byte chunk c of row n sits at c ^ n (16-bit
+  // elements) or c ^ 2 n (floats), so that neither the writes nor the reads meet in a bank.
+  auto rows_out16 = [&](auto&& value, auto&& send) {         // value(i, j, q) -> 4 packed elements; send(row, chunk, 16 bytes)
+    constexpr int CPR = BM / 8;
+    wait_and_meet<0>();
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = nw + 32 * j;
-      if (n >= N) continue;
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int m = mw + 32 * i + 8 * q;
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * inv;
-          if (g.out_kind == 1) {
-            uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + (int64_t)n * g.ldo + m;
-            const uint32_t w[2] = {pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
-            if (m + 4 <= g.M) {
-              typedef uint32_t u2_any __attribute__((ext_vector_type(2), aligned(2)));
-              u2_any t;
-              t[0] = w[0];
-              t[1] = w[1];
-              *reinterpret_cast<u2_any*>(o) = t;
+          const int row = wn * 32 * TN + 32 * j + l31, c = wm * 4 * TM + 4 * i + q;
+          *reinterpret_cast<uint2*>(smem + row * BM + (((c ^ l31) % CPR) << 3) + 4 * h) = value(i, j, q);
+        }
+    __syncthreads();
+    for (int x = threadIdx.x; x < BN * CPR; x += 64 * NW) {
+      const int row = x / CPR, c = x % CPR;
+      send(row, c, *reinterpret_cast<const u4*>(smem + row * BM + (((c ^ (row & 31)) % CPR) << 3)));
+    }
+  };
+  if constexpr (EPI == EPI_STORE) {
+    const float inv = g.d_scale[1];
+    if (g.out_kind == 1) {
+      uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
+      rows_out16(
+          [&](int i, int j, int q) {
+            return make_uint2(pack2<F16>(acc[i][j][4 * q] * inv, acc[i][j][4 * q + 1] * inv),
+                              pack2<F16>(acc[i][j][4 * q + 2] * inv, acc[i][j][4 * q + 3] * inv));
+          },
+          [&](int row, int c, u4 v) {
+            const int n = n0 + row, m = m0 + 8 * c;
+            if (n >= N || m >= g.M) return;
+            uint16_t* o = out + (int64_t)n * g.ldo + m;
+            if (m + 8 <= g.M) {
+              *reinterpret_cast<u4_any*>(o) = v;
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (m + e < g.M) o[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+              for (int e = 0; e < 8; ++e)
+                if (m + e < g.M) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
             }
+          });
+    } else {
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      typedef f4 f4_any __attribute__((aligned(4)));
+      float *lds = reinterpret_cast<float*>(smem), *out = reinterpret_cast<float*>(g.out) + (int64_t)(g.out_kind == 0 ? part : 0) * g.N * g.ldo;
+      constexpr int CPR = BM / 4, ROWS = 32 * W_N;           // 32 rows of every wave at a time
+      static_assert(ROWS * BM * 4 <= (int)sizeof(smem), "a pass fits");
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        wait_and_meet<0>();
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int c = wm * 8 * TM + 8 * i + 2 * q + h;
+            f4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * inv;
+            *reinterpret_cast<f4*>(lds + (wn * 32 + l31) * BM + (((c ^ (2 * l31)) % CPR) << 2)) = v;
+          }
+        __syncthreads();
+        for (int x = threadIdx.x; x < ROWS * CPR; x += 64 * NW) {
+          const int row = x / CPR, c = x % CPR;
+          f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (2 * (row & 31))) % CPR) << 2));
+          const int n = n0 + (row >> 5) * 32 * TN + 32 * j + (row & 31), m = m0 + 4 * c;
+          if (n >= N || m >= g.M) continue;
+          float* o = out + (int64_t)n * g.ldo + m;
+          if (m + 4 <= g.M) {
+            if (g.add) v += *reinterpret_cast<const f4_any*>(o);
+            *reinterpret_cast<f4_any*>(o) = v;
           } else {
-            float* o = reinterpret_cast<float*>(g.out) + ((int64_t)(g.out_kind == 0 ? part : 0) * g.N + n) * g.ldo + m;
-            typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
-            if (m + 4 <= g.M) {
-              f4_any t = {v[0], v[1], v[2], v[3]};
-              if (g.add) t += *reinterpret_cast<f4_any*>(o);
-              *reinterpret_cast<f4_any*>(o) = t;
-            } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (m + e < g.M) o[e] = g.add ? o[e] + v[e] : v[e];
-            }
+            for (int e = 0; e < 4; ++e)
+              if (m + e < g.M) o[e] = g.add ? o[e] + v[e] : v[e];
           }
         }
+      }
     }
   } else {
     if (g.bias) {
@@ -330,7 +404,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
           for (int j = 0; j < TN; ++j) acc[i][j][r] += bv;
         }
     }
-    constexpr float L2E = 1.44269504088896341f;
+    constexpr float L2E = 1.44269504088896341f;                // (differences first: z may be the type's lowest value)
     const bool edge = m0 + BM > g.M;                          // classes past the last one
     if constexpr (EPI == EPI_STATS) {
       float2* red = reinterpret_cast<float2*>(smem);          // [W_M][BN]
@@ -385,45 +459,53 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
         g.partial[(int64_t)tm * ((g.N + ROW_PAD - 1) / ROW_PAD * ROW_PAD) + n0 + c] = p;
       }
     } else {
-      const float scale = *g.d_scale;
+      const float scale = g.d_scale[0];
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = nw + 32 * j;
         const bool real = n < N;
         const float gn = real ? g.g[n] * scale : 0.f, lse = real ? g.lse[n] : 0.f;
         const int64_t tt = real ? g.target[g.rows[n]] : -1, at = tt - g.v0 - mw;
-        const bool hit = __any(tt >= 0 && at >= 0 && at < 32 * TM);
-        const float neg = -lse * L2E;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int m = mw + 32 * i + 8 * q;
-            float v[4];
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - lse) : __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * L2E);
+        if (__any(tt >= 0 && at >= 0 && at < 32 * TM)) {      // the target is among this wave's classes
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float z = acc[i][j][4 * q + e];
-              float p = FINE ? exp_fine(z - lse) : __builtin_amdgcn_exp2f(fmaf(z, L2E, neg));
-              if (hit && at == 32 * i + 8 * q + e) p -= 1.f;
-              v[e] = p * gn;
-              // zero rows are exactly zero, whatever their logits are; classes past the end too
-              if (gn == 0.f || (edge && m + e >= g.M)) v[e] = 0.f;
-            }
-            uint16_t* o = g.d + (int64_t)n * g.ldd + m;       // d is padded to whole tiles
-            if constexpr (FINE) {
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (at == 32 * i + 8 * (r >> 2) + (r & 3)) acc[i][j][r] -= 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] *= gn;
+        if (edge || __any(gn == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (gn == 0.f || mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
+        rows_out16(
+            [&](int i, int j, int q) {
+              if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack2<F16>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
               union {
                 __bf16 t[4];
                 uint2 u;
-              } w[3];
+              } w;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) split3(v[e], w[0].t[e], w[1].t[e], w[2].t[e]);
-#pragma unroll
-              for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(o + k * g.plane_d) = w[k].u;
-            } else {
-              *reinterpret_cast<uint2*>(o) = make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
-            }
-          }
-      }
+              for (int e = 0; e < 4; ++e) {                   // the term, and what it leaves for the next
+                w.t[e] = (__bf16)acc[i][j][4 * q + e];
+                acc[i][j][4 * q + e] -= (float)w.t[e];
+              }
+              return w.u;
+            },
+            [&](int row, int c, u4 v) { *reinterpret_cast<u4*>(g.d + plane * g.plane_d + (int64_t)(n0 + row) * g.ldd + m0 + 8 * c) = v; });
     }
   }
 }
@@ -740,8 +822,8 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     // dx has N x D outputs and a sum over the classes: where its tiles do not fill the chip the sum is split
     const int64_t tiles = (p.n_pad / 128) * ((a->D + 127) / 128);
     int64_t s = 512 / tiles;
-    const int64_t steps = p.piece / 32 * (p.f32 ? 6 : 1);
-    if (s > steps / 16) s = steps / 16;
+    const int64_t steps = p.piece / 64 * (p.f32 ? 6 : 1);
+    if (s > steps / 8) s = steps / 8;
     p.split = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     p.slabs = take((int64_t)p.split * p.n_pad * a->D * 4);
   }
@@ -754,8 +836,8 @@ template <bool F16, bool A_KC, bool B_KC, int EPI, bool FINE> void launch_gemm(G
   g.tiles_m = (g.M + b - 1) / b;
   g.tiles_n = (g.N + b - 1) / b;
   const uint32_t grid = (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
-  if (big) head_gemm_kernel<F16, A_KC, B_KC, 256, 256, 2, 4, 32, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);
-  else head_gemm_kernel<F16, A_KC, B_KC, 128, 128, 2, 2, 32, 4, EPI, FINE><<<grid, 256, 0, st>>>(g);
+  if (big) head_gemm_kernel<F16, A_KC, B_KC, 256, 256, 2, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);
+  else head_gemm_kernel<F16, A_KC, B_KC, 128, 128, 2, 2, EPI, FINE><<<grid, 256, 0, st>>>(g);
 }
 template <bool A_KC, bool B_KC, int EPI> void gemm(const Gemm& g, int dtype, bool big, hipStream_t st) {
   if (dtype == VAE_ADAMW_F32) launch_gemm<false, A_KC, B_KC, EPI, EPI != EPI_STORE>(g, big, st);
