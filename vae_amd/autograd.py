@@ -144,7 +144,7 @@ class LogLikFn(Function):
         return None, dmu, dth, dpi, None
 
 
-GATED_NORM_VECTORS = ("post_weight", "post_bias", "scale", "norm_weight", "norm_bias")
+_GATED_NORM_GRADS = ("r", "b", "gate") + ops.GATED_NORM_VECTORS
 
 
 class GatedResidualNormFn(Function):
@@ -153,24 +153,25 @@ class GatedResidualNormFn(Function):
 
     @staticmethod
     def forward(ctx, r, b, gate, post_weight, post_bias, scale, norm_weight, norm_bias, kind, gate_act, eps):
-        vectors = dict(zip(GATED_NORM_VECTORS, (post_weight, post_bias, scale, norm_weight, norm_bias)))
-        y, h, stats = ops.gated_norm_fwd(r, b, gate, **vectors, kind=kind, gate_act=gate_act, eps=eps)
-        ctx.how = dict(kind=kind, gate_act=gate_act, eps=eps)
-        ctx.save_for_backward(y, b, stats, gate, *vectors.values())
+        y, h, stats = ops.gated_norm_fwd(r, b, gate, post_weight=post_weight, post_bias=post_bias, scale=scale, norm_weight=norm_weight,
+                                         norm_bias=norm_bias, kind=kind, gate_act=gate_act, eps=eps)
+        ctx.how = (kind, gate_act, eps)
+        ctx.save_for_backward(y, b, stats, gate, post_weight, post_bias, scale, norm_weight, norm_bias)
         ctx.set_materialize_grads(False)
         return y, h
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh):
-        y, b, stats, gate, *vectors = ctx.saved_tensors
+        y, b, stats, gate, post_weight, post_bias, scale, norm_weight, norm_bias = ctx.saved_tensors
         if dy is None and dh is None:
             return (None,) * 11
         dy, dh = (None if t is None else (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()) for t in (dy, dh))
-        names = ("r", "b", "gate") + GATED_NORM_VECTORS
-        want = [n for n, need in zip(names, ctx.needs_input_grad) if need]
-        g = ops.gated_norm_bwd(dy, dh, y, b, stats, gate, **dict(zip(GATED_NORM_VECTORS, vectors)), **ctx.how, want=want)
-        return tuple(g.get(n) if n in want else None for n in names) + (None, None, None)
+        want = [n for n, need in zip(_GATED_NORM_GRADS, ctx.needs_input_grad) if need]
+        kind, gate_act, eps = ctx.how
+        g = ops.gated_norm_bwd(dy, dh, y, b, stats, gate, post_weight=post_weight, post_bias=post_bias, scale=scale,
+                               norm_weight=norm_weight, norm_bias=norm_bias, kind=kind, gate_act=gate_act, eps=eps, want=want)
+        return tuple(g.get(n) if n in want else None for n in _GATED_NORM_GRADS) + (None, None, None)
 
 
 class LinearCrossEntropyFn(Function):

@@ -742,6 +742,25 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ sl
   }
 }
 
+// dW (one piece of classes): its slabs added in order
+template <typename T> __global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ slabs, int S, int64_t n, T* __restrict__ dw) {
+  typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+    if (i + 4 <= n) {
+      f4_any s = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < S; ++k) s += *reinterpret_cast<const f4_any*>(slabs + k * n + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dw[i + e] = (T)s[e];
+    } else {
+      for (int64_t e = i; e < n; ++e) {
+        float s = 0.f;
+        for (int k = 0; k < S; ++k) s += slabs[k * n + e];
+        dw[e] = (T)s;
+      }
+    }
+  }
+}
+
 // db[v] = sum over the kept rows of d: 64 classes to a workgroup, 16 waves over the rows, added in order
 template <int KIND>   // 0: three bf16 planes -> float, 1: bf16, 2: fp16
 __global__ __launch_bounds__(1024) void ce_bias_kernel(const uint16_t* __restrict__ d, int64_t ldd, int64_t plane, const int* __restrict__ state,
@@ -775,17 +794,262 @@ __global__ __launch_bounds__(1024) void ce_bias_kernel(const uint16_t* __restric
   else reinterpret_cast<_Float16*>(out)[v] = (_Float16)s;
 }
 
+// ---- heads of at most 64 classes on at most 64 columns, few rows: the whole pass in one workgroup ----
+// The products are too small for tiles and the dozen launches of the way above would be all that is waited for.  256 rows at a
+// time lie in LDS beside W, in 32 bits whatever the type; four lanes share a row, which they hold in registers, and take every
+// fourth class.  D is padded with zeros to DM columns.
+constexpr int SMALL_V = 64, SMALL_D = 64, SMALL_ROWS = 1024, SMALL_WORK = 1 << 19, CHUNK = 256;
+struct Small {
+  int N, D, V, reduction;
+  int64_t ldx, ldw, ignore;
+  const void *x, *w, *bias;
+  const int64_t* target;
+  const float *cw, *up;
+  int* state;
+  float* loss;
+  void *dx, *dw, *db;
+};
+template <typename T, int DM> struct SmallLds {
+  float w[SMALL_V][DM + 4], x[CHUNK][DM + 4], bias[SMALL_V];
+};
+template <typename T, int DM> __device__ __forceinline__ void small_weights(const Small& a, SmallLds<T, DM>& s) {
+  for (int i = threadIdx.x; i < a.V * DM; i += 1024) {
+    const int v = i / DM, c = i % DM;
+    s.w[v][c] = c < a.D ? (float)reinterpret_cast<const T*>(a.w)[v * a.ldw + c] : 0.f;
+  }
+  if ((int)threadIdx.x < a.V) s.bias[threadIdx.x] = a.bias ? (float)reinterpret_cast<const T*>(a.bias)[threadIdx.x] : 0.f;
+}
+// rows base .. base + CHUNK, ignored ones and those past the end as zeros
+template <typename T, int DM> __device__ __forceinline__ void small_rows(const Small& a, SmallLds<T, DM>& s, int base) {
+  for (int i = threadIdx.x; i < CHUNK * DM; i += 1024) {
+    const int r = i / DM, c = i % DM, row = base + r;
+    const bool real = row < a.N && c < a.D && a.target[row] != a.ignore;
+    s.x[r][c] = real ? (float)reinterpret_cast<const T*>(a.x)[row * a.ldx + c] : 0.f;
+  }
+}
+template <int DM> __device__ __forceinline__ float small_dot(const float (&x)[DM], const float* w, float z) {
+  float p[4] = {z, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < DM; c += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(w + c);
+    p[0] = fmaf(x[c], v.x, p[0]);
+    p[1] = fmaf(x[c + 1], v.y, p[1]);
+    p[2] = fmaf(x[c + 2], v.z, p[2]);
+    p[3] = fmaf(x[c + 3], v.w, p[3]);
+  }
+  return (p[0] + p[1]) + (p[2] + p[3]);
+}
+template <int DM> __device__ __forceinline__ void small_row(const float* src, float (&x)[DM]) {
+#pragma unroll
+  for (int c = 0; c < DM; c += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(src + c);
+    x[c] = v.x;
+    x[c + 1] = v.y;
+    x[c + 2] = v.z;
+    x[c + 3] = v.w;
+  }
+}
+
+template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_fwd_kernel(Small a) {
+  __shared__ __attribute__((aligned(16))) SmallLds<T, DM> s;
+  __shared__ double red[2][16];
+  const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
+  double total = 0, weight = 0;
+  small_weights(a, s);
+  for (int base = 0; base < a.N; base += CHUNK) {
+    __syncthreads();
+    small_rows(a, s, base);
+    __syncthreads();
+    const int row = base + r;
+    const int64_t t = row < a.N ? a.target[row] : a.ignore;
+    const bool kept = row < a.N && t != a.ignore;
+    float x[DM], top = -INFINITY, sum = 0.f, hit = 0.f;
+    small_row(s.x[r], x);
+    for (int v = part; v < a.V; v += 4) {
+      const float z = small_dot(x, s.w[v], s.bias[v]);
+      if (v == t) hit = z;
+      if (z > top) {
+        sum = sum * exp_fine(top - z) + 1.f;
+        top = z;
+      } else if (z != -INFINITY) {                            // (a NaN ends here and stays)
+        sum += exp_fine(z - top);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const float ot = __shfl_xor(top, o, 64), os = __shfl_xor(sum, o, 64), m = fmaxf(top, ot), ref = m == -INFINITY ? 0.f : m;
+      sum = sum * exp_fine(top - ref) + os * exp_fine(ot - ref);
+      top = m;
+      hit += __shfl_xor(hit, o, 64);
+    }
+    if (part || row >= a.N) continue;
+    const float lse = top + logf(sum), c = !kept ? 0.f : t < 0 || t >= a.V ? NAN : a.cw ? a.cw[t] : 1.f;
+    const float loss = kept ? (lse - hit) * c : 0.f;
+    reinterpret_cast<float*>(a.state)[S_ROWS + a.N + row] = lse;
+    if (a.reduction == VAE_CE_NONE) a.loss[row] = loss;
+    total += (double)loss;
+    weight += (double)c;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64), weight += __shfl_xor(weight, o, 64);
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = total, red[1][threadIdx.x >> 6] = weight;
+  __syncthreads();
+  if (threadIdx.x) return;
+  total = weight = 0;
+  for (int i = 0; i < 16; ++i) total += red[0][i], weight += red[1][i];
+  reinterpret_cast<float*>(a.state)[S_TOTAL] = (float)weight;
+  if (a.reduction != VAE_CE_NONE) *a.loss = (float)(a.reduction == VAE_CE_MEAN ? total / weight : total);
+}
+
+template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_bwd_kernel(Small a) {
+  __shared__ __attribute__((aligned(16))) SmallLds<T, DM> s;
+  __shared__ float d[CHUNK][SMALL_V + 1];
+  const int r = threadIdx.x >> 2, part = threadIdx.x & 3;
+  constexpr int QUADS = DM / 4, COLS = DM / 4;
+  // dW: four columns of one class to a thread, the rows shared out among `ways` groups of threads
+  const int outputs = a.V * QUADS;
+  int span = 64;                                              // threads to a group: whole waves
+  while (span < outputs) span <<= 1;
+  const int ways = 1024 / span, way = threadIdx.x / span, o = threadIdx.x % span, ov = o / QUADS, oq = o % QUADS;
+  const bool mine = o < outputs;
+  float4 dw = make_float4(0.f, 0.f, 0.f, 0.f);
+  float db = 0.f;
+  const float total = reinterpret_cast<const float*>(a.state)[S_TOTAL];
+  small_weights(a, s);
+  for (int base = 0; base < a.N; base += CHUNK) {
+    __syncthreads();
+    small_rows(a, s, base);
+    __syncthreads();
+    const int row = base + r;
+    const int64_t t = row < a.N ? a.target[row] : a.ignore;
+    const bool kept = row < a.N && t != a.ignore;
+    float g = 0.f, lse = 0.f;
+    if (kept) {
+      g = (a.reduction == VAE_CE_NONE ? a.up[row] : a.up[0]) * (t < 0 || t >= a.V ? NAN : a.cw ? a.cw[t] : 1.f);
+      if (a.reduction == VAE_CE_MEAN) g /= total;
+      lse = reinterpret_cast<const float*>(a.state)[S_ROWS + a.N + row];
+    }
+    {
+      float x[DM];
+      small_row(s.x[r], x);
+      for (int v = part; v < a.V; v += 4) {
+        const float p = exp_fine(small_dot(x, s.w[v], s.bias[v]) - lse);
+        d[r][v] = g == 0.f ? 0.f : (v == t ? p - 1.f : p) * g;
+      }
+    }
+    __syncthreads();
+    if (a.dx && row < a.N) {
+      float acc[COLS];
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+      if (kept)
+        for (int v = 0; v < a.V; ++v) {
+          const float dv = d[r][v];
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) acc[c] = fmaf(dv, s.w[v][part * COLS + c], acc[c]);
+        }
+      T* out = reinterpret_cast<T*>(a.dx) + (int64_t)row * a.D + part * COLS;
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)
+        if (part * COLS + c < a.D) out[c] = (T)acc[c];
+    }
+    if (mine) {
+      const int rows = min(CHUNK, a.N - base);
+      for (int i = way; i < rows; i += ways) {
+        const float dv = d[i][ov];
+        const float4 x = *reinterpret_cast<const float4*>(&s.x[i][4 * oq]);
+        dw.x = fmaf(dv, x.x, dw.x);
+        dw.y = fmaf(dv, x.y, dw.y);
+        dw.z = fmaf(dv, x.z, dw.z);
+        dw.w = fmaf(dv, x.w, dw.w);
+        db += dv;
+      }
+    }
+  }
+  // the groups' sums, in order
+  __syncthreads();
+  float* part_w = &s.x[0][0];                                 // [1024][5]
+  static_assert(sizeof(s.x) >= 1024 * 5 * 4, "the rows' place holds the groups' sums");
+  {
+    float* p = part_w + threadIdx.x * 5;
+    p[0] = dw.x;
+    p[1] = dw.y;
+    p[2] = dw.z;
+    p[3] = dw.w;
+    p[4] = db;
+  }
+  __syncthreads();
+  if (way || !mine) return;
+  float sum[5] = {};
+  for (int k = 0; k < ways; ++k)
+#pragma unroll
+    for (int e = 0; e < 5; ++e) sum[e] += part_w[(k * span + o) * 5 + e];
+  if (a.dw)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (4 * oq + e < a.D) reinterpret_cast<T*>(a.dw)[ov * a.D + 4 * oq + e] = (T)sum[e];
+  if (a.db && oq == 0) reinterpret_cast<T*>(a.db)[ov] = (T)sum[4];
+}
+
+// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 512 x 64 x 64,
+// 2^21 products, in 115 against 97).
+bool small_head(const vae_linear_ce* a) {
+  return a->V <= SMALL_V && a->D <= SMALL_D && a->N <= SMALL_ROWS && a->N * a->V * a->D <= SMALL_WORK;
+}
+Small small_args(const vae_linear_ce* a, int reduction, void* state) {
+  return {(int)a->N, (int)a->D, (int)a->V, reduction, a->ldx, a->ldw, a->ignore_index, a->x, a->w, a->bias, a->target, a->class_weight,
+          nullptr, reinterpret_cast<int*>(state), nullptr, nullptr, nullptr, nullptr};
+}
+template <typename T> void launch_small(const Small& s, bool bwd, hipStream_t st) {
+  if (s.D <= 32) {
+    if (bwd) ce_small_bwd_kernel<T, 32><<<1, 1024, 0, st>>>(s);
+    else ce_small_fwd_kernel<T, 32><<<1, 1024, 0, st>>>(s);
+  } else {
+    if (bwd) ce_small_bwd_kernel<T, 64><<<1, 1024, 0, st>>>(s);
+    else ce_small_fwd_kernel<T, 64><<<1, 1024, 0, st>>>(s);
+  }
+}
+void small(const Small& s, int dtype, bool bwd, hipStream_t st) {
+  if (dtype == VAE_ADAMW_F32) launch_small<float>(s, bwd, st);
+  else if (dtype == VAE_ADAMW_BF16) launch_small<__bf16>(s, bwd, st);
+  else launch_small<_Float16>(s, bwd, st);
+}
+
 // ---- host ----
 int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
+// Tiles of 256 x 256 (one workgroup to a CU) or 128 x 128 (two), and into how many parts the sum over K is split where the
+// tiles do not fill the chip: the least of rounds * (steps * c + f) + the slabs' traffic, with c and f as measured in bf16 (a
+// step of 64 of K takes 1.45 us in a large tile and 0.8 in each of two small ones; starting and ending a tile 8 and 6 us).
+struct Tiles {
+  bool big;
+  int split;
+};
+Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool always_slabs) {
+  Tiles best = {true, 1};
+  double least = 1e30;
+  const int64_t steps = (k + 63) / 64 * (f32 ? 6 : 1);
+  for (int big = 0; big < 2; ++big) {
+    const int64_t b = big ? 256 : 128, tiles = ((m + b - 1) / b) * ((n + b - 1) / b), slots = big ? 256 : 512;
+    for (int s = 1; s <= may_split; s += s < 4 ? 1 : s < 16 ? 2 : 8) {
+      const int64_t per = (steps + s - 1) / s;
+      if (s > 1 && per < 4) break;
+      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.45 : 0.8) + (big ? 8.0 : 6.0));
+      if (always_slabs || s > 1) t += 3.0 + (double)s * (double)m * (double)n * 8.0 / 4.5e6;
+      if (t < least) least = t, best = {big != 0, s};
+    }
+  }
+  return best;
+}
 
 struct Plan {
   bool f32, pack_w;
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
   int64_t planes;
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
-  int split;                                          // slabs of dx
+  Tiles z_tiles, d_tiles, dx_tiles, dw_tiles;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, bytes;
+  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, slabs_w, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
@@ -807,6 +1071,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.x = take(p.planes * p.n_pad * p.d_pad * 2);
   p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
   if (!bwd) {
+    p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32, 1, false);
     p.partial = take(up_to(a->V, 128) / 128 * p.n_pad * 8);
     p.tlogit = take(p.n_pad * 4);
     p.nll = take(p.n_pad * 4);
@@ -819,13 +1084,11 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     const int64_t pieces = (most + p.piece - 1) / p.piece;
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
-    // dx has N x D outputs and a sum over the classes: where its tiles do not fill the chip the sum is split
-    const int64_t tiles = (p.n_pad / 128) * ((a->D + 127) / 128);
-    int64_t s = 512 / tiles;
-    const int64_t steps = p.piece / 64 * (p.f32 ? 6 : 1);
-    if (s > steps / 8) s = steps / 8;
-    p.split = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-    p.slabs = take((int64_t)p.split * p.n_pad * a->D * 4);
+    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false);
+    p.dx_tiles = tiles_for(a->D, a->N, p.piece, p.f32, 64, true);
+    p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
+    p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
+    p.slabs_w = take(p.dw_tiles.split > 1 ? (int64_t)p.dw_tiles.split * p.piece * a->D * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -844,9 +1107,6 @@ template <bool A_KC, bool B_KC, int EPI> void gemm(const Gemm& g, int dtype, boo
   else if (dtype == VAE_ADAMW_BF16) launch_gemm<false, A_KC, B_KC, EPI, false>(g, big, st);
   else launch_gemm<true, A_KC, B_KC, EPI, false>(g, big, st);
 }
-// 256 x 256 tiles once they fill the chip; below that 128 x 128 ones, two workgroups to a CU
-bool big_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 200; }
-
 void pack(const void* src, int64_t ld, int64_t D, const int* state, int64_t rows, int64_t padded, uint16_t* out, int64_t ldo, int64_t plane,
           int dtype, hipStream_t st) {
   const int64_t work = padded * (ldo / 8) / 256 + 1;
@@ -897,6 +1157,7 @@ extern "C" int64_t vae_linear_ce_state_bytes(int64_t N) { return (S_ROWS + 2 * N
 
 extern "C" int64_t vae_linear_ce_workspace_bytes(const vae_linear_ce* a, int backward) {
   if (check(a, "vae_linear_ce_workspace_bytes")) return -1;
+  if (small_head(a)) return 0;
   return plan_of(a, backward != 0).bytes;
 }
 
@@ -905,6 +1166,13 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   if (int rc = check(a, "vae_linear_ce_fwd")) return rc;
   VAE_REQUIRE(reduction >= VAE_CE_NONE && reduction <= VAE_CE_MEAN, "vae_linear_ce_fwd: unknown reduction %d", reduction);
   VAE_REQUIRE(loss && state, "vae_linear_ce_fwd: null pointer");
+  if (small_head(a)) {
+    Small m = small_args(a, reduction, state);
+    m.loss = loss;
+    small(m, a->dtype, false, (hipStream_t)stream);
+    VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+    return VAE_OK;
+  }
   const Plan p = plan_of(a, false);
   VAE_REQUIRE(workspace && vae_aligned16(workspace) && workspace_bytes >= p.bytes,
               "vae_linear_ce_fwd: needs a 16-byte aligned workspace of vae_linear_ce_workspace_bytes()");
@@ -921,7 +1189,7 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   Gemm g = logits_gemm(a, p, ws, s);
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
   g.target_logit = tl;
-  const bool big = big_tiles(g.M, g.N);
+  const bool big = p.z_tiles.big;
   gemm<true, true, EPI_STATS>(g, a->dtype, big, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   const int b = big ? 256 : 128;
@@ -938,6 +1206,16 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   VAE_REQUIRE(reduction >= VAE_CE_NONE && reduction <= VAE_CE_MEAN, "vae_linear_ce_bwd: unknown reduction %d", reduction);
   VAE_REQUIRE(grad && state && (dx || dw || dbias), "vae_linear_ce_bwd: null pointer");
   VAE_REQUIRE(!dbias || a->bias, "vae_linear_ce_bwd: a gradient of a bias that is not there");
+  if (small_head(a)) {
+    Small m = small_args(a, reduction, const_cast<void*>(state));
+    m.up = grad;
+    m.dx = dx;
+    m.dw = dw;
+    m.db = dbias;
+    small(m, a->dtype, true, (hipStream_t)stream);
+    VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    return VAE_OK;
+  }
   const Plan p = plan_of(a, true);
   VAE_REQUIRE(workspace && vae_aligned16(workspace) && workspace_bytes >= p.bytes,
               "vae_linear_ce_bwd: needs a 16-byte aligned workspace of vae_linear_ce_workspace_bytes()");
@@ -965,7 +1243,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.d = d;
     z.ldd = p.piece;
     z.plane_d = plane_d;
-    gemm<true, true, EPI_D>(z, a->dtype, big_tiles(z.M, z.N), st);
+    gemm<true, true, EPI_D>(z, a->dtype, p.d_tiles.big, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     if (dx) {                                           // dx (N, D) += d (N, n_v) W (n_v, D)
       Gemm g = {};
@@ -985,9 +1263,8 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       g.ldo = a->D;
       g.out_kind = 0;
       g.add = v0 > 0;
-      const bool big = big_tiles(g.M, g.N);
-      g.split = big ? 1 : p.split;
-      gemm<false, true, EPI_STORE>(g, a->dtype, big, st);
+      g.split = p.dx_tiles.split;
+      gemm<false, true, EPI_STORE>(g, a->dtype, p.dx_tiles.big, st);
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
     if (dw) {                                           // dW (n_v, D) = d^T (n_v, N) x (N, D)
@@ -1002,14 +1279,23 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       g.N = (int)n_v;
       g.K = (int)a->N;
       g.segs = z.segs;
-      g.split = 1;
+      g.split = p.dw_tiles.split;
       g.dyn = s + S_KEPT;
       g.dyn_k = 1;
       g.d_scale = scale;
-      g.out = reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize;
       g.ldo = a->D;
-      g.out_kind = p.f32 ? 2 : 1;
-      gemm<false, false, EPI_STORE>(g, a->dtype, big_tiles(g.M, g.N), st);
+      void* o = reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize;
+      g.out = g.split > 1 ? ws + p.slabs_w : o;
+      g.out_kind = g.split > 1 ? 0 : p.f32 ? 2 : 1;
+      gemm<false, false, EPI_STORE>(g, a->dtype, p.dw_tiles.big, st);
+      if (g.split > 1) {
+        const float* sw = reinterpret_cast<const float*>(ws + p.slabs_w);
+        const int64_t n = n_v * a->D, work = (n + 1023) / 1024;
+        const int grid = (int)(work < 4096 ? work : 4096);
+        if (p.f32) ce_dw_kernel<float><<<grid, 256, 0, st>>>(sw, g.split, n, (float*)o);
+        else if (a->dtype == VAE_ADAMW_BF16) ce_dw_kernel<__bf16><<<grid, 256, 0, st>>>(sw, g.split, n, (__bf16*)o);
+        else ce_dw_kernel<_Float16><<<grid, 256, 0, st>>>(sw, g.split, n, (_Float16*)o);
+      }
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
     if (dbias) {
@@ -1022,7 +1308,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     }
   }
   if (dx) {
-    const int S = big_tiles(a->D, a->N) ? 1 : p.split;
+    const int S = p.dx_tiles.split;
     const int rows = (int)(a->N < 4096 ? a->N : 4096);
 #define VAE_DX(T) ce_dx_kernel<T><<<rows, 256, 0, st>>>(slabs, S, a->N * a->D, (int)a->N, (int)a->D, s, a->target, a->ignore_index, (T*)dx)
     if (p.f32) VAE_DX(float);

@@ -3,7 +3,8 @@ the forward pass is the identity, the backward pass multiplies the incoming grad
 Host-side plumbing of the module API; the fused step applies the same sign flip through dz_extra.
 
 ``gated_residual_norm``: the norms, gate and residual scale between two residual blocks, on the HIP kernels."""
-from typing import Optional, Tuple
+import functools
+from typing import Callable, Optional, Tuple
 
 import torch
 from torch import nn
@@ -56,19 +57,24 @@ def gated_residual_norm(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.T
     "tanh" or "identity".  Absent vectors are 1 or 0.  Rows are float32, bfloat16 or float16; the vectors are all of that type
     or all float32.  ``y`` is rounded to its type before ``h`` is formed.  Gradients reach every tensor given (once: there
     is no second derivative)."""
-    from .autograd import GatedResidualNormFn
     if b.dim() < 1 or r.shape != b.shape:
         raise ValueError(f"vae_amd.gated_residual_norm: r is {tuple(r.shape)}, b is {tuple(b.shape)}")
     if gate is not None and tuple(gate.shape[:-1]) != tuple(b.shape[:-1]):
         raise ValueError(f"vae_amd.gated_residual_norm: gate is {tuple(gate.shape)}, b is {tuple(b.shape)}")
 
-    def rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-        if t is None:
-            return None
-        if t.dim() != 2:
-            t = t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(0, 0)
-        return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
-
-    y, h = GatedResidualNormFn.apply(rows(r), rows(b), rows(gate), post_weight, post_bias, scale, norm_weight, norm_bias, kind,
-                                     gate_act, eps)
+    y, h = _gated_residual_norm()(_rows(r), _rows(b), None if gate is None else _rows(gate), post_weight, post_bias, scale, norm_weight,
+                                  norm_bias, kind, gate_act, eps)
     return (y, h) if b.dim() == 2 else (y.view(b.shape), h.view(b.shape))
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """(..., D) as (rows, D) with a contiguous last dim."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(0, 0)
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+@functools.lru_cache(maxsize=None)
+def _gated_residual_norm() -> Callable:
+    from .autograd import GatedResidualNormFn          # (modules that need no kernels import this one)
+    return GatedResidualNormFn.apply

@@ -7,6 +7,7 @@ dimension is contiguous; there is no CPU fallback -- CPU tensors raise.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -690,8 +691,36 @@ GATE_ACTS = {"identity": 0, "sigmoid": 1, "tanh": 2}
 GATED_NORM_MAX_D = 16384
 
 
-def _gated_norm_args(r, b, gate, vectors, kind, gate_act, eps):
-    """Checks of what both passes of the gated residual norm take -> (filled _lib.GatedNorm, gate mode)."""
+# what the C side reads as vae_gated_norm (include/vae_amd.h): packed at once, a ctypes structure costs three times that
+_GATED_NORM = struct.Struct("=2q5if26Q")
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _Here:
+    """Nothing to do: the tensors' device is the current one."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def _on(device: torch.device):
+    """Context in which ``device`` is the current one (a launch goes to its stream)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _gated_norm_checks(r, b, gate, vectors, kind, gate_act, eps) -> Tuple[int, int]:
+    """Checks of what the gated residual norm takes -> (gate mode, whether the vectors are float32)."""
     who = "vae_amd.ops.gated_norm"
     if kind not in NORM_KINDS:
         raise ValueError(f"{who}: kind must be one of {sorted(NORM_KINDS)}, got {kind!r}")
@@ -699,49 +728,49 @@ def _gated_norm_args(r, b, gate, vectors, kind, gate_act, eps):
         raise ValueError(f"{who}: gate_act must be one of {sorted(GATE_ACTS)}, got {gate_act!r}")
     if not eps >= 0:
         raise ValueError(f"{who}: eps must not be negative, got {eps}")
-    if b.dtype not in FLOAT_DTYPES:
-        raise TypeError(f"{who}: rows of {b.dtype} are not supported (float32, bfloat16, float16)")
-    N, D = b.shape
+    dtype, shape, device = b.dtype, b.shape, b.device
+    if dtype not in FLOAT_DTYPES:
+        raise TypeError(f"{who}: rows of {dtype} are not supported (float32, bfloat16, float16)")
+    N, D = shape
     if not 1 <= D <= GATED_NORM_MAX_D:
         raise ValueError(f"{who}: rows of {D} columns are not supported (1 to {GATED_NORM_MAX_D})")
     mode = 0
     if gate is not None:
-        if tuple(gate.shape) == (N, D):
-            mode = 2
-        elif tuple(gate.shape) == (N, 1):
-            mode = 1
-        else:
+        width = gate.shape[1] if gate.dim() == 2 and gate.shape[0] == N else -1
+        if width != D and width != 1:
             raise ValueError(f"{who}: gate must be {(N, D)} or {(N, 1)}, got {tuple(gate.shape)}")
+        mode = 2 if width == D else 1
+    if r is not None and r.shape != shape:
+        raise ValueError(f"{who}: r is {tuple(r.shape)}, b is {tuple(shape)}")
     for t, name in ((r, "r"), (b, "b"), (gate, "gate")):
         if t is None:
             continue
-        if t.dtype != b.dtype:
-            raise TypeError(f"{who}: {name} is {t.dtype}, the rows are {b.dtype}")
-        if t.dim() != 2 or (t.numel() and t.shape[1] > 1 and t.stride(1) != 1):
+        if t.dtype != dtype:
+            raise TypeError(f"{who}: {name} is {t.dtype}, the rows are {dtype}")
+        if t.stride(1) != 1 and t.shape[1] > 1 and t.numel():
             raise ValueError(f"{who}: {name} must be 2-D with a contiguous last dim, got {tuple(t.shape)} / {t.stride()}")
-        if name == "r" and t.shape != b.shape:
-            raise ValueError(f"{who}: r is {tuple(t.shape)}, b is {tuple(b.shape)}")
-    kinds = {t.dtype for t in vectors.values() if t is not None}
-    if len(kinds) > 1 or not kinds <= {b.dtype, torch.float32}:
-        raise TypeError(f"{who}: the vectors over columns must all be {b.dtype} or all float32, got {sorted(map(str, kinds))}")
-    for name, t in vectors.items():
-        if t is not None and (t.dim() != 1 or t.shape[0] != D or not t.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be a contiguous vector of {D}, got {tuple(t.shape)}")
-    if vectors["post_bias"] is not None and vectors["post_weight"] is None:
-        raise ValueError(f"{who}: post_bias needs post_weight")
-    for t in (r, b, gate, *vectors.values()):
-        if t is not None and (not t.is_cuda or t.device != b.device):
+        if t.device != device:
             raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
-    a = _lib.GatedNorm(N=N, D=D, dtype=FLOAT_DTYPES[b.dtype], vectors_f32=int(kinds == {torch.float32}), kind=NORM_KINDS[kind],
-                       gate_mode=mode, act=GATE_ACTS[gate_act], eps=float(eps), b=b.data_ptr(), ld_b=b.stride(0))
-    if r is not None:
-        a.r, a.ld_r = r.data_ptr(), r.stride(0)
-    if gate is not None:
-        a.gate, a.ld_gate = gate.data_ptr(), gate.stride(0)
-    for name, t in vectors.items():
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    return a, mode
+    of = None
+    for t, name in zip(vectors, GATED_NORM_VECTORS):
+        if t is None:
+            continue
+        if of is None:
+            of = t.dtype
+        if t.dtype != of or (of != dtype and of != torch.float32):
+            raise TypeError(f"{who}: the vectors over columns must all be {dtype} or all float32, got {name} {t.dtype}")
+        if t.shape != (D,) or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be a contiguous vector of {D}, got {tuple(t.shape)}")
+        if t.device != device:
+            raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
+    if vectors[1] is not None and vectors[0] is None:
+        raise ValueError(f"{who}: post_bias needs post_weight")
+    if not b.is_cuda:
+        raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
+    return mode, int(of == torch.float32)
+
+
+GATED_NORM_VECTORS = ("post_weight", "post_bias", "scale", "norm_weight", "norm_bias")
 
 
 def gated_norm_fwd(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
@@ -750,14 +779,18 @@ def gated_norm_fwd(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.Tensor
                    gate_act: str = "sigmoid", eps: float = 1e-5, want_stats: bool = True):
     """-> (y, h, stats (N, 4) or None): y = r + scale * act(gate) * norm(b), h = norm(y) (include/vae_amd.h, vae_gated_norm)."""
     lib = _lib.load()
-    vectors = dict(post_weight=post_weight, post_bias=post_bias, scale=scale, norm_weight=norm_weight, norm_bias=norm_bias)
-    a, _ = _gated_norm_args(r, b, gate, vectors, kind, gate_act, eps)
-    with torch.cuda.device(b.device):
-        y, h = torch.empty(b.shape, dtype=b.dtype, device=b.device), torch.empty(b.shape, dtype=b.dtype, device=b.device)
-        stats = torch.empty(b.shape[0], 4, dtype=torch.float32, device=b.device) if want_stats else None
-        a.y, a.h, a.stats = y.data_ptr(), h.data_ptr(), None if stats is None else stats.data_ptr()
-        rc = lib.vae_gated_norm_fwd(C.byref(a), _stream())
-    _lib.check(rc, "gated_norm_fwd")
+    vectors = (post_weight, post_bias, scale, norm_weight, norm_bias)
+    mode, f32 = _gated_norm_checks(r, b, gate, vectors, kind, gate_act, eps)
+    (N, D), device = b.shape, b.device
+    with _on(device):
+        y, h = torch.empty((N, D), dtype=b.dtype, device=device), torch.empty((N, D), dtype=b.dtype, device=device)
+        stats = torch.empty((N, 4), dtype=torch.float32, device=device) if want_stats else None
+        rc = lib.vae_gated_norm_fwd(_GATED_NORM.pack(
+            N, D, FLOAT_DTYPES[b.dtype], f32, NORM_KINDS[kind], mode, GATE_ACTS[gate_act], eps, r.data_ptr(), r.stride(0), b.data_ptr(),
+            b.stride(0), _at(gate), 0 if gate is None else gate.stride(0), *map(_at, vectors), y.data_ptr(), h.data_ptr(), _at(stats),
+            0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "gated_norm_fwd")
     return y, h, stats
 
 
@@ -765,85 +798,96 @@ def gated_norm_bwd(dy: Optional[torch.Tensor], dh: Optional[torch.Tensor], y: to
                    gate: Optional[torch.Tensor] = None, *, post_weight: Optional[torch.Tensor] = None,
                    post_bias: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
                    norm_weight: Optional[torch.Tensor] = None, norm_bias: Optional[torch.Tensor] = None, kind: str = "rms",
-                   gate_act: str = "sigmoid", eps: float = 1e-5, want=("gate", "post_weight", "post_bias", "scale", "norm_weight",
-                                                                       "norm_bias")):
+                   gate_act: str = "sigmoid", eps: float = 1e-5, want=("gate",) + GATED_NORM_VECTORS):
     """-> dict of gradients: r, b, and those of ``want`` whose tensor is given.  ``dy`` / ``dh`` None: zero."""
     lib = _lib.load()
-    vectors = dict(post_weight=post_weight, post_bias=post_bias, scale=scale, norm_weight=norm_weight, norm_bias=norm_bias)
-    a, mode = _gated_norm_args(None, b, gate, vectors, kind, gate_act, eps)
-    N, D = b.shape
-    for t, name, shape, dtype in ((y, "y", (N, D), b.dtype), (stats, "stats", (N, 4), torch.float32), (dy, "dy", (N, D), b.dtype),
-                                  (dh, "dh", (N, D), b.dtype)):
+    vectors = (post_weight, post_bias, scale, norm_weight, norm_bias)
+    mode, f32 = _gated_norm_checks(None, b, gate, vectors, kind, gate_act, eps)
+    (N, D), dtype, device = b.shape, b.dtype, b.device
+    for t, name, shape, of in ((y, "y", (N, D), dtype), (stats, "stats", (N, 4), torch.float32), (dy, "dy", (N, D), dtype),
+                               (dh, "dh", (N, D), dtype)):
         if t is None:
             continue
         dense = t.is_contiguous() if name in ("y", "stats") else (D == 1 or N == 0 or t.stride(1) == 1)
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != b.device or not dense:
-            raise ValueError(f"vae_amd.ops.gated_norm_bwd: {name} must be {shape} {dtype} on {b.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    out = {}
-    with torch.cuda.device(b.device):
-        out["r"], out["b"] = torch.empty(N, D, dtype=b.dtype, device=b.device), torch.empty(N, D, dtype=b.dtype, device=b.device)
+        if t.shape != shape or t.dtype != of or t.device != device or not dense:
+            raise ValueError(f"vae_amd.ops.gated_norm_bwd: {name} must be {shape} {of} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    with _on(device):
+        dr, db = torch.empty((N, D), dtype=dtype, device=device), torch.empty((N, D), dtype=dtype, device=device)
+        out = {"r": dr, "b": db}
+        dgate = None
         if gate is not None and "gate" in want:
-            out["gate"] = torch.empty(N, D if mode == 2 else 1, dtype=b.dtype, device=b.device)
-        columns = [k for k, t in vectors.items() if t is not None and k in want]
-        for k in columns:
-            out[k] = (torch.zeros if N == 0 else torch.empty)(D, dtype=vectors[k].dtype, device=b.device)
+            out["gate"] = dgate = torch.empty((N, D if mode == 2 else 1), dtype=dtype, device=device)
+        # the gradients of the vectors are rows of one allocation; dnorm_weight, dnorm_bias, dscale, dpost_weight, dpost_bias
+        names = [k for k, t in zip(GATED_NORM_VECTORS, vectors) if t is not None and k in want]
+        at = dict.fromkeys(GATED_NORM_VECTORS, 0)
+        nbytes, ws = 0, 0
+        if names:
+            sums = (torch.empty if N else torch.zeros)((len(names), D), dtype=torch.float32 if f32 else dtype, device=device)
+            out.update(zip(names, sums.unbind(0)))
+            for k in names:
+                at[k] = out[k].data_ptr()
         if N == 0:
             return out
-        for k in columns:
-            setattr(a, "d" + k, out[k].data_ptr())
-        a.y, a.stats, a.dr, a.db = y.data_ptr(), stats.data_ptr(), out["r"].data_ptr(), out["b"].data_ptr()
-        if "gate" in out:
-            a.dgate = out["gate"].data_ptr()
-        if dy is not None:
-            a.dy, a.ld_dy = dy.data_ptr(), dy.stride(0)
-        if dh is not None:
-            a.dh, a.ld_dh = dh.data_ptr(), dh.stride(0)
-        nbytes = lib.vae_gated_norm_workspace_bytes(N, D, a.dtype) if columns else 0
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=b.device) if nbytes else None   # of this call alone: streams and graphs
-        rc = lib.vae_gated_norm_bwd(C.byref(a), _p(ws), nbytes, _stream())
-    _lib.check(rc, "gated_norm_bwd")
+        if names:                                       # scratch of this call alone: streams and captured graphs share none
+            nbytes = lib.vae_gated_norm_workspace_bytes(N, D, FLOAT_DTYPES[dtype])
+            scratch = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+            ws = scratch.data_ptr()
+        rc = lib.vae_gated_norm_bwd(_GATED_NORM.pack(
+            N, D, FLOAT_DTYPES[dtype], f32, NORM_KINDS[kind], mode, GATE_ACTS[gate_act], eps, 0, 0, b.data_ptr(), b.stride(0), _at(gate),
+            0 if gate is None else gate.stride(0), *map(_at, vectors), y.data_ptr(), 0, stats.data_ptr(), _at(dy),
+            0 if dy is None else dy.stride(0), _at(dh), 0 if dh is None else dh.stride(0), dr.data_ptr(), db.data_ptr(), _at(dgate),
+            at["norm_weight"], at["norm_bias"], at["scale"], at["post_weight"], at["post_bias"]), ws, nbytes, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "gated_norm_bwd")
     return out
 
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
-def _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction) -> "_lib.LinearCE":
+# vae_linear_ce of include/vae_amd.h
+_LINEAR_CE = struct.Struct("=3qi4x7Qq")
+
+
+def _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction) -> bytes:
     who = "vae_amd.ops.linear_ce"
     if reduction not in REDUCTIONS:
         raise ValueError(f"{who}: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
-    if x.dtype not in FLOAT_DTYPES:
-        raise TypeError(f"{who}: rows of {x.dtype} are not supported (float32, bfloat16, float16)")
+    dtype, device = x.dtype, x.device
+    if dtype not in FLOAT_DTYPES:
+        raise TypeError(f"{who}: rows of {dtype} are not supported (float32, bfloat16, float16)")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"{who}: x must be (N, D) and w (V, D), got {tuple(x.shape)} and {tuple(w.shape)}")
     (N, D), V = x.shape, w.shape[0]
     if N < 1 or D < 1 or V < 1:
         raise ValueError(f"{who}: no rows, columns or classes in {tuple(x.shape)} x {tuple(w.shape)}")
-    if tuple(target.shape) != (N,) or target.dtype != torch.int64 or not target.is_contiguous():
+    if target.shape != (N,) or target.dtype != torch.int64 or not target.is_contiguous():
         raise ValueError(f"{who}: target must be a contiguous int64 vector of {N}, got {tuple(target.shape)} {target.dtype}")
-    for t, name, shape, dtype in ((w, "w", (V, D), x.dtype), (bias, "bias", (V,), x.dtype), (weight, "weight", (V,), torch.float32)):
+    if w.dtype != dtype:
+        raise TypeError(f"{who}: w is {w.dtype}, {dtype} is needed")
+    for t, name, of in ((bias, "bias", dtype), (weight, "weight", torch.float32)):
         if t is None:
             continue
-        if t.dtype != dtype:
-            raise TypeError(f"{who}: {name} is {t.dtype}, {dtype} is needed")
-        if tuple(t.shape) != shape or (name != "w" and not t.is_contiguous()):
+        if t.dtype != of:
+            raise TypeError(f"{who}: {name} is {t.dtype}, {of} is needed")
+        if t.shape != (V,) or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be a contiguous vector of {V}, got {tuple(t.shape)}")
-    for t, name in ((x, "x"), (w, "w")):
-        if D > 1 and t.stride(1) != 1:
-            raise ValueError(f"{who}: {name} must have a contiguous last dim, got strides {t.stride()}")
-    if V > 1 and w.stride(0) < D:
-        raise ValueError(f"{who}: the rows of w overlap (strides {w.stride()})")
-    for t in (x, w, target, bias, weight):
-        if t is not None and (not t.is_cuda or t.device != x.device):
+        if t.device != device:
             raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
-    return _lib.LinearCE(N=N, D=D, V=V, dtype=FLOAT_DTYPES[x.dtype], x=x.data_ptr(), ldx=x.stride(0) if N > 1 else D, w=w.data_ptr(),
-                         ldw=w.stride(0) if V > 1 else D, bias=None if bias is None else bias.data_ptr(), target=target.data_ptr(),
-                         class_weight=None if weight is None else weight.data_ptr(), ignore_index=int(ignore_index))
+    if D > 1 and (x.stride(1) != 1 or w.stride(1) != 1):
+        raise ValueError(f"{who}: x and w must have a contiguous last dim, got strides {x.stride()} and {w.stride()}")
+    ldw = w.stride(0) if V > 1 else D
+    if ldw < D:
+        raise ValueError(f"{who}: the rows of w overlap (strides {w.stride()})")
+    if not x.is_cuda or w.device != device or target.device != device:
+        raise RuntimeError(f"{who}: all tensors must live on one GPU (no CPU fallback)")
+    return _LINEAR_CE.pack(N, D, V, FLOAT_DTYPES[dtype], x.data_ptr(), x.stride(0) if N > 1 else D, w.data_ptr(), ldw, _at(bias),
+                           target.data_ptr(), _at(weight), int(ignore_index))
 
 
-def _linear_ce_workspace(lib, a, backward: int, device) -> Tuple[torch.Tensor, int]:
+def _linear_ce_workspace(lib, a: bytes, backward: int, device) -> Tuple[torch.Tensor, int]:
     """Scratch of one call alone (torch's allocator keeps it with the stream, and with a captured graph)."""
-    n = lib.vae_linear_ce_workspace_bytes(C.byref(a), backward)
+    n = lib.vae_linear_ce_workspace_bytes(a, backward)
     if n < 0:
         raise ValueError(f"vae_amd.ops.linear_ce: {lib.vae_last_error().decode()}")
     return torch.empty(n, dtype=torch.uint8, device=device), n
@@ -855,12 +899,14 @@ def linear_ce_fwd(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, bias: 
     vae_linear_ce_fwd)."""
     lib = _lib.load()
     a = _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction)
-    with torch.cuda.device(x.device):
-        loss = torch.empty((a.N,) if reduction == "none" else (), dtype=torch.float32, device=x.device)
-        state = torch.empty(lib.vae_linear_ce_state_bytes(a.N) // 4, dtype=torch.int32, device=x.device)
-        ws, n = _linear_ce_workspace(lib, a, 0, x.device)
-        rc = lib.vae_linear_ce_fwd(C.byref(a), REDUCTIONS[reduction], loss.data_ptr(), state.data_ptr(), ws.data_ptr(), n, _stream())
-    _lib.check(rc, "linear_ce_fwd")
+    N, device = x.shape[0], x.device
+    with _on(device):
+        loss = torch.empty((N,) if reduction == "none" else (), dtype=torch.float32, device=device)
+        state = torch.empty(lib.vae_linear_ce_state_bytes(N) // 4, dtype=torch.int32, device=device)
+        ws, n = _linear_ce_workspace(lib, a, 0, device)
+        rc = lib.vae_linear_ce_fwd(a, REDUCTIONS[reduction], loss.data_ptr(), state.data_ptr(), ws.data_ptr(), n, _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "linear_ce_fwd")
     return loss, state
 
 
@@ -870,19 +916,21 @@ def linear_ce_bwd(grad: torch.Tensor, state: torch.Tensor, x: torch.Tensor, w: t
     """-> (dx, dw, dbias), None where not needed; ``grad``: float32 gradient of the loss."""
     lib = _lib.load()
     a = _linear_ce_args(x, w, target, bias, weight, ignore_index, reduction)
-    if grad.dtype != torch.float32 or grad.numel() != (a.N if reduction == "none" else 1) or grad.device != x.device:
+    N, device = x.shape[0], x.device
+    if grad.dtype != torch.float32 or grad.numel() != (N if reduction == "none" else 1) or grad.device != device:
         raise ValueError(f"vae_amd.ops.linear_ce_bwd: grad must be the float32 gradient of the loss, got {tuple(grad.shape)} {grad.dtype}")
-    if state.numel() * 4 != lib.vae_linear_ce_state_bytes(a.N) or state.dtype != torch.int32 or state.device != x.device or not state.is_contiguous():
+    if state.numel() * 4 != lib.vae_linear_ce_state_bytes(N) or state.dtype != torch.int32 or state.device != device or not state.is_contiguous():
         raise ValueError("vae_amd.ops.linear_ce_bwd: state is not that of a forward pass over these rows")
     grad = grad.contiguous()
-    with torch.cuda.device(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if need_w else None
-        db = torch.empty(bias.shape, dtype=x.dtype, device=x.device) if need_bias and bias is not None else None
+    with _on(device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+        dw = torch.empty(w.shape, dtype=x.dtype, device=device) if need_w else None
+        db = torch.empty(bias.shape, dtype=x.dtype, device=device) if need_bias and bias is not None else None
         if dx is None and dw is None and db is None:
             return None, None, None
-        ws, n = _linear_ce_workspace(lib, a, 1, x.device)
-        rc = lib.vae_linear_ce_bwd(C.byref(a), REDUCTIONS[reduction], grad.data_ptr(), state.data_ptr(), _p(dx), _p(dw), _p(db), ws.data_ptr(),
-                                   n, _stream())
-    _lib.check(rc, "linear_ce_bwd")
+        ws, n = _linear_ce_workspace(lib, a, 1, device)
+        rc = lib.vae_linear_ce_bwd(a, REDUCTIONS[reduction], grad.data_ptr(), state.data_ptr(), _at(dx), _at(dw), _at(db), ws.data_ptr(), n,
+                                   _raw_stream(device.index))
+    if rc:
+        _lib.check(rc, "linear_ce_bwd")
     return dx, dw, db

@@ -18,6 +18,7 @@ import torch
 
 from . import _lib
 from .arena import ParamArena
+from .ops import _on, _raw_stream
 
 
 def reference_weight_decay(name: str, weight_decay: float) -> float:
@@ -266,15 +267,15 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
     for p, g, wd in zip(params, grads, decay):
         count = p.numel()
         if g is not None and count:
-            kind = _ADAMW_DTYPES.get(p.dtype)
-            if kind is None or g.dtype != p.dtype:
+            dtype = p.dtype
+            if dtype not in _ADAMW_DTYPES or g.dtype != dtype:
                 raise TypeError(f"vae_amd.optim.multi_tensor_adamw_: a parameter of {p.dtype} with a gradient of {g.dtype}; "
                                 "float32, bfloat16 and float16 are supported, both of the same type")
             if p.device != dev or g.device != dev:
                 raise RuntimeError(f"vae_amd.optim.multi_tensor_adamw_: parameters, gradients and state must be on {dev}")
             if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
                 raise ValueError("vae_amd.optim.multi_tensor_adamw_: parameters and gradients must be contiguous and of one shape")
-            table += (p.data_ptr(), g.data_ptr(), count, at, wd, kind)
+            table += (p.data_ptr(), g.data_ptr(), count, at, wd, _ADAMW_DTYPES[dtype])
             live += 1
         at += -(-count // ADAMW_BLOCK)
     for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
@@ -289,7 +290,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
             raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: 8-bit moments need contiguous float32 scales (2, {at}) on {dev}")
     clip = max_grad_norm > 0 or return_norm
     norm = None
-    with torch.cuda.device(dev):
+    with _on(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("vae_amd.optim.multi_tensor_adamw_: step and learning rate are host values; a captured step would repeat them")
         if return_norm:
@@ -302,7 +303,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
                                  scales.data_ptr() if bits == 8 else None, at, None if master is None else master.data_ptr(), float(lr),
                                  float(betas[0]), float(betas[1]), float(eps), int(step), float(max_grad_norm), float(grad_scale),
                                  int(seed) & (2 ** 64 - 1), None if ws is None else ws.data_ptr(), nbytes,
-                                 None if norm is None else norm.data_ptr(), torch.cuda.current_stream().cuda_stream)
+                                 None if norm is None else norm.data_ptr(), _raw_stream(dev.index))
     _lib.check(rc, "multi_tensor_adamw_")
     return norm
 
