@@ -20,7 +20,7 @@
 // every row of a large vocabulary, is then exact, where the rounding of 1 / N itself would shift every gradient by the same
 // 2^-9 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
 // multiplied by 2^14 as well.  fp32 operands are split exactly
-// into three bf16 terms, and the six products that matter run one after the other along K, small ones first: the error
+// into three bf16 terms, and for every 64 of K the six products that matter run one after the other: the error
 // is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix instruction would give a sixteenth).
 #include "../../include/vae_amd.h"
 #include "common.h"
@@ -132,14 +132,16 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / W_N, wn = wave % W_N, l31 = lane & 31, h = lane >> 5;
 
-  // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles, and order the tiles in bands of 4 along M, so
-  // that the 32 tiles an XCD works on at a time share 4 blocks of A and 8 of B in its L2.
+  // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles (all tiles of one part of K, where K is split),
+  // and order the tiles in bands of 4 along M, so that the 32 tiles an XCD works on at a time share 4 blocks of A and 8 of B in
+  // its L2.
   const int total = g.tiles_m * g.tiles_n;
-  int id = blockIdx.x % total;
-  const int part = blockIdx.x / total;
+  int id, part;
   {
-    const int q8 = total >> 3, r8 = total & 7, xcd = id & 7;
-    id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (id >> 3);
+    const int all_wg = (int)gridDim.x, q8 = all_wg >> 3, r8 = all_wg & 7, xcd = blockIdx.x & 7;
+    const int lin = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + ((int)blockIdx.x >> 3);
+    part = lin / total;
+    id = lin - part * total;
   }
   int tm, tn;
   {
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   const uint16_t* base_b = B_KC ? g.b + (int64_t)n0 * g.ldb : g.b + n0;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
   const int steps = t_end - t_beg;
-  int seg = t_beg / max(kt1, 1), kt = t_beg - seg * kt1, fetched = 0, fill = 0;   // of the next step to load, and its image
+  int kt = t_beg / g.segs, seg = t_beg - kt * g.segs, fetched = 0, fill = 0;   // of the next step to load, and its image
   const uint16_t *sa, *sb;                                              // its base
   bool tail;
   auto aim = [&]() {
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     sa = base_a + pa * g.plane_a + (A_KC ? (int64_t)k0 : (int64_t)k0 * g.lda);
     sb = base_b + pb * g.plane_b + (B_KC ? (int64_t)k0 : (int64_t)k0 * g.ldb);
     tail = kt == kt1 - 1;
-    if (++kt == kt1) kt = 0, ++seg;
+    if (++seg == g.segs) seg = 0, ++kt;                                 // (a block's terms stay in the L2 for all its products)
   };
   auto load = [&](int i) {                                              // piece i of the step aimed at
     const uint32_t st = lds0 + (uint32_t)fill * (STAGE * 2u);
@@ -742,56 +744,60 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ sl
   }
 }
 
-// dW (one piece of classes): its slabs added in order
-template <typename T> __global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ slabs, int S, int64_t n, T* __restrict__ dw) {
+// dW or db of one piece of classes: the slabs added in order
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ slabs, int S, int64_t slab, int64_t n, T* __restrict__ dw) {
   typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
     if (i + 4 <= n) {
       f4_any s = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < S; ++k) s += *reinterpret_cast<const f4_any*>(slabs + k * n + i);
+      for (int k = 0; k < S; ++k) s += *reinterpret_cast<const f4_any*>(slabs + k * slab + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dw[i + e] = (T)s[e];
     } else {
       for (int64_t e = i; e < n; ++e) {
         float s = 0.f;
-        for (int k = 0; k < S; ++k) s += slabs[k * n + e];
+        for (int k = 0; k < S; ++k) s += slabs[k * slab + e];
         dw[e] = (T)s;
       }
     }
   }
 }
 
-// db[v] = sum over the kept rows of d: 64 classes to a workgroup, 16 waves over the rows, added in order
+// db[v] = sum over the kept rows of d, of the y-th of gridDim.y runs of rows: 256 classes to a workgroup, 8 per thread, 32 rows
+// at a time, whose sums are added in order.  One run: the result; several: slabs (runs, classes in whole blocks) for ce_dw_kernel to add.
 template <int KIND>   // 0: three bf16 planes -> float, 1: bf16, 2: fp16
 __global__ __launch_bounds__(1024) void ce_bias_kernel(const uint16_t* __restrict__ d, int64_t ldd, int64_t plane, const int* __restrict__ state,
-                                                       int V, const float* __restrict__ d_scale, void* __restrict__ out) {
-  __shared__ float red[16][64];
-  const int v = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, kept = state[S_KEPT];
-  float s = 0.f;
-  for (int n = w; n < kept; n += 16 * 8) {
-    float t[8];
+                                                       int V, const float* __restrict__ d_scale, float* __restrict__ slabs, void* __restrict__ out) {
+  __shared__ float red[32][257];
+  const int v = blockIdx.x * 256 + (threadIdx.x & 31) * 8, r = threadIdx.x >> 5, kept = state[S_KEPT];
+  const int run = (kept + (int)gridDim.y - 1) / (int)gridDim.y, end = min((int)(blockIdx.y + 1) * run, kept);
+  float s[8] = {};
+  for (int n = blockIdx.y * run + r; n < end; n += 32) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int row = n + 16 * u;
-      t[u] = 0.f;
-      if (row < kept && v < V) {
-        const uint16_t* p = d + (int64_t)row * ldd + v;
-        if (KIND == 2) t[u] = (float)__builtin_bit_cast(_Float16, *p);
-        else t[u] = (float)__builtin_bit_cast(__bf16, *p);
-        if (KIND == 0) t[u] += (float)__builtin_bit_cast(__bf16, p[plane]) + (float)__builtin_bit_cast(__bf16, p[2 * plane]);
+    for (int k = 0; k < (KIND == 0 ? 3 : 1); ++k) {          // (d is padded to whole tiles of classes)
+      const u4 q = *reinterpret_cast<const u4*>(d + k * plane + (int64_t)n * ldd + v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint16_t b = (uint16_t)(q[j >> 1] >> (16 * (j & 1)));
+        if (KIND == 2) s[j] += (float)__builtin_bit_cast(_Float16, b);
+        else s[j] += (float)__builtin_bit_cast(__bf16, b);
       }
     }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) s += t[u];
   }
-  red[w][threadIdx.x & 63] = s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[r][(threadIdx.x & 31) * 8 + j] = s[j];
   __syncthreads();
-  if (w || v >= V) return;
-  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
-  s *= d_scale[1];
-  if (KIND == 0) reinterpret_cast<float*>(out)[v] = s;
-  else if (KIND == 1) reinterpret_cast<__bf16*>(out)[v] = (__bf16)s;
-  else reinterpret_cast<_Float16*>(out)[v] = (_Float16)s;
+  const int c = threadIdx.x, at = blockIdx.x * 256 + c;
+  if (c >= 256) return;
+  float t = 0.f;
+  for (int i = 0; i < 32; ++i) t += red[i][c];
+  t *= d_scale[1];
+  if (gridDim.y > 1) slabs[(int64_t)blockIdx.y * gridDim.x * 256 + at] = t;
+  else if (at >= V) return;
+  else if (KIND == 0) reinterpret_cast<float*>(out)[at] = t;
+  else if (KIND == 1) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
+  else reinterpret_cast<_Float16*>(out)[at] = (_Float16)t;
 }
 
 // ---- heads of at most 64 classes on at most 64 columns, few rows: the whole pass in one workgroup ----
@@ -991,8 +997,8 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_b
   if (a.db && oq == 0) reinterpret_cast<T*>(a.db)[ov] = (T)sum[4];
 }
 
-// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 512 x 64 x 64,
-// 2^21 products, in 115 against 97).
+// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 1024 x 30 x 17 in 63 against 80, 512 x 64 x 64,
+// 2^21 products, in 115 against 74).
 bool small_head(const vae_linear_ce* a) {
   return a->V <= SMALL_V && a->D <= SMALL_D && a->N <= SMALL_ROWS && a->N * a->V * a->D <= SMALL_WORK;
 }
@@ -1042,6 +1048,14 @@ Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool a
   return best;
 }
 
+// runs of rows that the bias gradient of `wide` blocks of 256 classes is summed in: enough for two workgroups to a CU, of 128
+// rows at least
+int64_t bias_runs(int64_t n, int64_t wide) {
+  int64_t r = 512 / wide;
+  if (r > n / 128) r = n / 128;
+  return r < 1 ? 1 : r;
+}
+
 struct Plan {
   bool f32, pack_w;
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
@@ -1049,7 +1063,7 @@ struct Plan {
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
   Tiles z_tiles, d_tiles, dx_tiles, dw_tiles;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, slabs_w, bytes;
+  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, slabs_w, slabs_b, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
@@ -1089,6 +1103,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
     p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
     p.slabs_w = take(p.dw_tiles.split > 1 ? (int64_t)p.dw_tiles.split * p.piece * a->D * 4 : 0);
+    p.slabs_b = take(a->bias ? 512 * 256 * 4 : 0);           // bias_runs() * blocks <= 512
   }
   p.bytes = at;
   return p;
@@ -1107,6 +1122,14 @@ template <bool A_KC, bool B_KC, int EPI> void gemm(const Gemm& g, int dtype, boo
   else if (dtype == VAE_ADAMW_BF16) launch_gemm<false, A_KC, B_KC, EPI, false>(g, big, st);
   else launch_gemm<true, A_KC, B_KC, EPI, false>(g, big, st);
 }
+void add_slabs(const float* slabs, int S, int64_t slab, int64_t n, void* out, int dtype, hipStream_t st) {
+  const int64_t work = (n + 1023) / 1024;
+  const int grid = (int)(work < 4096 ? work : 4096);
+  if (dtype == VAE_ADAMW_F32) ce_dw_kernel<float><<<grid, 256, 0, st>>>(slabs, S, slab, n, (float*)out);
+  else if (dtype == VAE_ADAMW_BF16) ce_dw_kernel<__bf16><<<grid, 256, 0, st>>>(slabs, S, slab, n, (__bf16*)out);
+  else ce_dw_kernel<_Float16><<<grid, 256, 0, st>>>(slabs, S, slab, n, (_Float16*)out);
+}
+
 void pack(const void* src, int64_t ld, int64_t D, const int* state, int64_t rows, int64_t padded, uint16_t* out, int64_t ldo, int64_t plane,
           int dtype, hipStream_t st) {
   const int64_t work = padded * (ldo / 8) / 256 + 1;
@@ -1290,20 +1313,19 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       gemm<false, false, EPI_STORE>(g, a->dtype, p.dw_tiles.big, st);
       if (g.split > 1) {
         const float* sw = reinterpret_cast<const float*>(ws + p.slabs_w);
-        const int64_t n = n_v * a->D, work = (n + 1023) / 1024;
-        const int grid = (int)(work < 4096 ? work : 4096);
-        if (p.f32) ce_dw_kernel<float><<<grid, 256, 0, st>>>(sw, g.split, n, (float*)o);
-        else if (a->dtype == VAE_ADAMW_BF16) ce_dw_kernel<__bf16><<<grid, 256, 0, st>>>(sw, g.split, n, (__bf16*)o);
-        else ce_dw_kernel<_Float16><<<grid, 256, 0, st>>>(sw, g.split, n, (_Float16*)o);
+        add_slabs(sw, g.split, n_v * a->D, n_v * a->D, o, a->dtype, st);
       }
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
     if (dbias) {
-      const unsigned grid = (unsigned)((n_v + 63) / 64);
+      const int64_t wide = (n_v + 255) / 256;
+      const dim3 grid((unsigned)wide, (unsigned)bias_runs(a->N, wide));
       void* o = reinterpret_cast<uint8_t*>(dbias) + v0 * esize;
-      if (p.f32) ce_bias_kernel<0><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
-      else if (a->dtype == VAE_ADAMW_BF16) ce_bias_kernel<1><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
-      else ce_bias_kernel<2><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, o);
+      float* sb = reinterpret_cast<float*>(ws + p.slabs_b);
+      if (p.f32) ce_bias_kernel<0><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
+      else if (a->dtype == VAE_ADAMW_BF16) ce_bias_kernel<1><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
+      else ce_bias_kernel<2><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
+      if (grid.y > 1) add_slabs(sb, (int)grid.y, wide * 256, n_v, o, a->dtype, st);
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
   }
