@@ -42,7 +42,7 @@ constexpr int ROW_PAD = 256;                            // packed rows and colum
 constexpr int K_PAD = 64;
 
 // the state of a forward pass that the backward pass reads: int32 / float words
-constexpr int S_KEPT = 0, S_TOTAL = 1, S_ROWS = 4;      // kept rows, sum of c[t], then row index (N) and lse (N) of the kept rows
+constexpr int S_KEPT = 0, S_TOTAL = 1, S_ROWS = 4;      // kept rows, sum of c[t]; row index, class (-1: none) and lse, N each, of the kept rows
 
 enum { EPI_STATS = 0, EPI_D = 1, EPI_STORE = 2 };
 
@@ -59,8 +59,7 @@ struct Gemm {
   int v0;                       // first class of this piece: class = v0 + m
   const void* bias;             // of the operands' outer type
   int bias_f32;
-  const int64_t* target;        // by original row
-  const int* rows;              // original row of a packed row
+  const int* classes;           // by packed row
   float2* partial;              // (tile_m, N padded): running maximum and sum
   float* target_logit;          // by packed row
   const float* lse;             // by packed row
@@ -82,8 +81,15 @@ __device__ __forceinline__ void split3(float v, __bf16& h, __bf16& m, __bf16& l)
   l = (__bf16)(r - (float)m);
 }
 
-// exp to an ulp or so for v <= 88 (common.h's vae_exp_acc, which would turn a NaN into a small number)
-__device__ __forceinline__ float exp_fine(float v) { return v == v ? vae_exp_acc(v) : v; }
+// exp to an ulp or so for v <= 88, 0 far below, NaN for NaN: the rounding error of v * log2 e is fed back
+__device__ __forceinline__ float exp_fine(float v) {
+  v = v < -100.f ? -100.f : v;
+  const float t = v * 1.44269504088896341f;
+  float r = fmaf(v, 1.44269504088896341f, -t);
+  r = fmaf(v, 1.925963033500011e-8f, r);
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, r * 0.69314718055994531f, e);
+}
 
 // One wave instruction: lane i copies 16 bytes from base + off_i to LDS byte lds + 16 i.  In inline asm so that the compiler
 // does not drain the counter ahead of the next LDS read; the kernel waits itself.
@@ -237,6 +243,19 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     return u.v;
   };
 
+  // what the epilogue needs of this lane's rows, asked for now
+  int cls[TN];
+  float lse[TN], gn[TN];
+  if constexpr (EPI != EPI_STORE) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + (wn * TN + j) * 32 + l31;
+      const bool real = n < N;
+      cls[j] = real ? g.classes[n] : -1;
+      lse[j] = EPI == EPI_D && real ? g.lse[n] : 0.f;
+      gn[j] = EPI == EPI_D && real ? g.g[n] : 0.f;
+    }
+  }
   f32x16 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -406,7 +425,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
           for (int j = 0; j < TN; ++j) acc[i][j][r] += bv;
         }
     }
-    constexpr float L2E = 1.44269504088896341f;                // (differences first: z may be the type's lowest value)
+    constexpr float L2E = 1.44269504088896341f;                // (with |ref| below 1e37 a z of the type's lowest value gives 0)
     const bool edge = m0 + BM > g.M;                          // classes past the last one
     if constexpr (EPI == EPI_STATS) {
       float2* red = reinterpret_cast<float2*>(smem);          // [W_M][BN]
@@ -414,16 +433,14 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = nw + 32 * j;
-        const bool real = n < N;
-        // the target's logit, by the lane that holds it
-        const int64_t tt = real ? g.target[g.rows[n]] : -1;
-        const int64_t at = tt - g.v0 - mw;                    // 32 i + 8 (r / 4) + r % 4 where it is ours
-        if (__any(tt >= 0 && at >= 0 && at < 32 * TM)) {
+        const int at = cls[j] - g.v0 - mw;                    // 32 i + 8 (r / 4) + r % 4 where the target's logit is ours
+        if (__any(at >= 0 && at < 32 * TM)) {
+          float hit = 0.f;
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (tt >= 0 && at == 32 * i + 8 * (r >> 2) + (r & 3) && tt < g.v0 + g.M) g.target_logit[n] = acc[i][j][r];
+            for (int r = 0; r < 16; ++r) hit = at == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : hit;
+          if (at >= 0 && at < 32 * TM && !(at & 4)) g.target_logit[n] = hit;   // (at & 4: it is the other half wave's)
         }
         if (edge) {
 #pragma unroll
@@ -440,10 +457,18 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float ref = top == -INFINITY ? 0.f : top;       // all of them -inf: the sum is 0, not NaN
         float sum = 0.f;
+        if (!FINE && __all(fabsf(ref) < 1e37f)) {
+          const float neg = -ref * L2E;
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+        } else {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+        }
         sum += __shfl_xor(sum, 32, 64);
         if (h == 0) red[wm * BN + wn * 32 * TN + 32 * j + l31] = make_float2(top, sum);
       }
@@ -464,15 +489,21 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
       const float scale = g.d_scale[0];
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int n = nw + 32 * j;
-        const bool real = n < N;
-        const float gn = real ? g.g[n] * scale : 0.f, lse = real ? g.lse[n] : 0.f;
-        const int64_t tt = real ? g.target[g.rows[n]] : -1, at = tt - g.v0 - mw;
+        const float gs = gn[j] * scale, ref = lse[j];
+        const int at = cls[j] - g.v0 - mw;
+        if (!FINE && __all(fabsf(ref) < 1e37f)) {
+          const float neg = -ref * L2E;
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+          for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - lse) : __builtin_amdgcn_exp2f((acc[i][j][r] - lse) * L2E);
-        if (__any(tt >= 0 && at >= 0 && at < 32 * TM)) {      // the target is among this wave's classes
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+        } else {
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+        }
+        if (__any(at >= 0 && at < 32 * TM)) {                 // the target is among this wave's classes
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -482,13 +513,13 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] *= gn;
-        if (edge || __any(gn == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
+          for (int r = 0; r < 16; ++r) acc[i][j][r] *= gs;
+        if (edge || __any(gs == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (gn == 0.f || mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = 0.f;
+              if (gs == 0.f || mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = 0.f;
         }
       }
 #pragma unroll
@@ -551,6 +582,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
       if (i0 + j >= N) continue;
       if (t[j] != ignore) {
         state[S_ROWS + at] = i0 + j;
+        state[S_ROWS + N + at] = t[j] < 0 || t[j] >= V ? -1 : (int)t[j];
         target_logit[at] = NAN;                               // stays so where the target is no class
         ++at;
         weight += t[j] < 0 || t[j] >= V ? (double)NAN : cw ? (double)cw[t[j]] : 1.0;
@@ -620,8 +652,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ src,
 
 // the partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row
 __global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restrict__ partial, int tiles, int64_t ldp,
-                                                         int* __restrict__ state, int N, const int64_t* __restrict__ target, int V,
-                                                         const float* __restrict__ cw, const float* __restrict__ target_logit,
+                                                         int* __restrict__ state, int N, const float* __restrict__ cw, const float* __restrict__ target_logit,
                                                          float* __restrict__ nll, float* __restrict__ loss_rows) {
   __shared__ float2 red[8][32];
   const int kept = state[S_KEPT];
@@ -654,10 +685,9 @@ __global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restric
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum += red[i][threadIdx.x].y * exp_fine(red[i][threadIdx.x].x - ref);
   const float lse = m + logf(sum);
-  reinterpret_cast<float*>(state)[S_ROWS + N + row] = lse;
-  const int orig = state[S_ROWS + row];
-  const int64_t t = target[orig];
-  const float v = (lse - target_logit[row]) * (!cw || t < 0 || t >= V ? 1.f : cw[t]);
+  reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
+  const int orig = state[S_ROWS + row], t = state[S_ROWS + N + row];
+  const float v = (lse - target_logit[row]) * (!cw || t < 0 ? 1.f : cw[t]);
   if (loss_rows) loss_rows[orig] = v;
   else nll[row] = v;
 }
@@ -679,18 +709,17 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
 }
 
 // g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to)
-__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up, int reduction, const int* __restrict__ state,
-                                                           const int64_t* __restrict__ target, int V, const float* __restrict__ cw,
+__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up, int reduction, const int* __restrict__ state, int N,
+                                                           const float* __restrict__ cw,
                                                            float to, float* __restrict__ g, float* __restrict__ d_scale) {
   __shared__ float red[16];
   const int kept = state[S_KEPT];
   const float total = reinterpret_cast<const float*>(state)[S_TOTAL];
   float top = 0.f;
   for (int i = threadIdx.x; i < kept; i += 1024) {
-    const int orig = state[S_ROWS + i];
-    const int64_t t = target[orig];
+    const int orig = state[S_ROWS + i], t = state[S_ROWS + N + i];
     float v = reduction == VAE_CE_NONE ? up[orig] : up[0];
-    if (t < 0 || t >= V) v = NAN;
+    if (t < 0) v = NAN;
     else if (cw) v *= cw[t];
     if (reduction == VAE_CE_MEAN) v /= total;
     g[i] = v;
@@ -891,7 +920,7 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_f
     if (part || row >= a.N) continue;
     const float lse = top + logf(sum), c = !kept ? 0.f : t < 0 || t >= a.V ? NAN : a.cw ? a.cw[t] : 1.f;
     const float loss = kept ? (lse - hit) * c : 0.f;
-    reinterpret_cast<float*>(a.state)[S_ROWS + a.N + row] = lse;
+    reinterpret_cast<float*>(a.state)[S_ROWS + 2 * a.N + row] = lse;
     if (a.reduction == VAE_CE_NONE) a.loss[row] = loss;
     total += (double)loss;
     weight += (double)c;
@@ -933,7 +962,7 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_b
     if (kept) {
       g = (a.reduction == VAE_CE_NONE ? a.up[row] : a.up[0]) * (t < 0 || t >= a.V ? NAN : a.cw ? a.cw[t] : 1.f);
       if (a.reduction == VAE_CE_MEAN) g /= total;
-      lse = reinterpret_cast<const float*>(a.state)[S_ROWS + a.N + row];
+      lse = reinterpret_cast<const float*>(a.state)[S_ROWS + 2 * a.N + row];
     }
     {
       float x[DM];
@@ -1169,14 +1198,13 @@ Gemm logits_gemm(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* 
   g.dyn = state + S_KEPT;
   g.bias = a->bias;
   g.bias_f32 = p.f32;
-  g.target = a->target;
-  g.rows = state + S_ROWS;
+  g.classes = state + S_ROWS + a->N;
   return g;
 }
 
 }  // namespace
 
-extern "C" int64_t vae_linear_ce_state_bytes(int64_t N) { return (S_ROWS + 2 * N) * 4; }
+extern "C" int64_t vae_linear_ce_state_bytes(int64_t N) { return (S_ROWS + 3 * N) * 4; }
 
 extern "C" int64_t vae_linear_ce_workspace_bytes(const vae_linear_ce* a, int backward) {
   if (check(a, "vae_linear_ce_workspace_bytes")) return -1;
@@ -1216,8 +1244,8 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   gemm<true, true, EPI_STATS>(g, a->dtype, big, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   const int b = big ? 256 : 128;
-  ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->target,
-                                                                  (int)a->V, a->class_weight, tl, nll, by_row);
+  ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->class_weight, tl,
+                                                                  nll, by_row);
   if (!by_row) ce_reduce_kernel<<<1, 1024, 0, st>>>(nll, s, reduction == VAE_CE_MEAN, loss);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   return VAE_OK;
@@ -1248,7 +1276,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
-  ce_upstream_kernel<<<1, 1024, 0, st>>>(grad, reduction, s, a->target, (int)a->V, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale);
+  ce_upstream_kernel<<<1, 1024, 0, st>>>(grad, reduction, s, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale);
   VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
   pack(a->x, a->ldx, a->D, s, a->N, p.n_pad, xp, p.d_pad, p.n_pad * p.d_pad, a->dtype, st);
   if (p.pack_w) pack(a->w, a->ldw, a->D, nullptr, a->V, a->V, reinterpret_cast<uint16_t*>(ws + p.w), p.d_pad, a->V * p.d_pad, a->dtype, st);
@@ -1260,7 +1288,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.a = w0;
     z.M = (int)n_v;
     z.v0 = (int)v0;
-    z.lse = reinterpret_cast<const float*>(s) + S_ROWS + a->N;
+    z.lse = reinterpret_cast<const float*>(s) + S_ROWS + 2 * a->N;
     z.g = gr;
     z.d_scale = scale;
     z.d = d;
