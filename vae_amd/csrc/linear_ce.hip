@@ -1055,12 +1055,14 @@ int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
 
 // Tiles of 256 x 256 (one workgroup to a CU) or 128 x 128 (two), and into how many parts the sum over K is split where the
 // tiles do not fill the chip: the least of rounds * (steps * c + f) + the slabs' traffic, with c and f as measured in bf16 (a
-// step of 64 of K takes 1.45 us in a large tile and 0.8 in each of two small ones; starting and ending a tile 8 and 6 us).
+// step of 64 of K takes 1.45 us in a large tile and 0.8 in each of two small ones; starting and ending a tile 8 and 6 us, and
+// 40 where a large tile of fp32 logits is turned into three terms of d, for which its registers do not suffice: 79 us for
+// 512 x 20000 x 256, 59 in small tiles).
 struct Tiles {
   bool big;
   int split;
 };
-Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool always_slabs) {
+Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool always_slabs, double end_big = 8.0) {
   Tiles best = {true, 1};
   double least = 1e30;
   const int64_t steps = (k + 63) / 64 * (f32 ? 6 : 1);
@@ -1069,7 +1071,7 @@ Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool a
     for (int s = 1; s <= may_split; s += s < 4 ? 1 : s < 16 ? 2 : 8) {
       const int64_t per = (steps + s - 1) / s;
       if (s > 1 && per < 4) break;
-      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.45 : 0.8) + (big ? 8.0 : 6.0));
+      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.45 : 0.8) + (big ? end_big : 6.0));
       if (always_slabs || s > 1) t += 3.0 + (double)s * (double)m * (double)n * 8.0 / 4.5e6;
       if (t < least) least = t, best = {big != 0, s};
     }
@@ -1127,7 +1129,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     const int64_t pieces = (most + p.piece - 1) / p.piece;
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
-    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false);
+    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false, p.f32 ? 40.0 : 8.0);
     p.dx_tiles = tiles_for(a->D, a->N, p.piece, p.f32, 64, true);
     p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
     p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
