@@ -173,11 +173,10 @@ def test_reductions_and_upstream_gradients(dtype, reduction, d, v):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-def test_large_tiles_and_pieces(dtype):
-    """More than 200 tiles of 256 x 256, and (a batch this long) a vocabulary in two pieces."""
-    n, v = (40000, 7000) if dtype == "bf16" else (14000, 6500)
-    s = _inputs(n, 72, v, dtype, True, False, 0.4, seed=9)
+@pytest.mark.parametrize("n,d,v,dtype", [(40000, 72, 7000, "bf16"), (14000, 72, 6500, "fp32"), (8000, 520, 7100, "bf16"), (8200, 328, 7000, "fp16")])
+def test_large_tiles_and_pieces(n, d, v, dtype):
+    """Hundreds of tiles of 256 x 256, few and many steps of K, and (the longest batches) a vocabulary in two pieces."""
+    s = _inputs(n, d, v, dtype, True, False, 0.4, seed=9)
     loss, grads = _run(s, "mean")
     _check(s, "mean", loss, grads)
 

@@ -29,7 +29,7 @@
 
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -104,9 +104,11 @@ template <int LEFT> __device__ __forceinline__ void wait_and_meet() {   // this 
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-template <bool F16> __device__ __forceinline__ f32x16 mma(u4 a, u4 b, f32x16 c) {
-  if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+// 16 x 16 x 32: with operands in registers alone this instruction sustains 1985 TFLOP/s in bf16 on random data where the
+// 32 x 32 x 16 one, of the same peak, sustains 1264 (the clock gives way to its power).
+template <bool F16> __device__ __forceinline__ f32x4 mma(u4 a, u4 b, f32x4 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -120,23 +122,29 @@ template <bool F16> __device__ __forceinline__ uint32_t pack2(float a, float b) 
   return w.u;
 }
 
+__device__ __forceinline__ int rc_swizzle(int k) { return (k & 3) << 2 | (k >> 3 & 1) << 1; }
+
 // Tile product.  BM x BN outputs, W_M x W_N waves, K in steps of BK through two images in LDS, filled by direct loads; one
 // barrier per step.
 //   KC image [rows][BK]: 16-byte chunk c of a row sits at chunk c ^ f(row), so that the 16 rows of a b128 read hit all banks.
-//   RC image [BK][rows]: chunk c of k sits at c ^ 4 (k & 3); fragments by the transposing read, whose 16 lanes take 4 k x 16 rows.
+//   RC image [BK][rows]: chunk c of k sits at c ^ f(k); fragments by the transposing read, whose 16 lanes take 4 k x 16 rows: f
+//   spreads the 8 values of k that half a wave reads over the banks.
+// The largest tile's step of 64 takes 1.4 us = 1.5 PFLOP/s over the chip (bf16, 8192 x 16384 from K 1024 to 4096; an image of
+// 32 of K in four stages, a third image for B alone, two 256 x 128 workgroups to a CU and 128 x 128 in four waves were all
+// slower), what a tile starts and ends with 8 to 12 us.
 // Rows and columns of A past its end are clamped to the last one (their products are not stored, or meet zeros in B); B is a
 // packed operand, padded with zeros to whole tiles.
 template <bool F16, bool A_KC, bool B_KC, int BM, int BN, int W_M, int W_N, int EPI, bool FINE>
 __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
-  constexpr int BK = 64, STAGES = 2, SPREAD = 2;
-  constexpr int NW = W_M * W_N, TM = BM / (32 * W_M), TN = BN / (32 * W_N);
+  constexpr int BK = 64, STAGES = 2;
+  constexpr int NW = W_M * W_N, TM = BM / (16 * W_M), TN = BN / (16 * W_N);
   constexpr int IMG_A = BM * BK, IMG_B = BN * BK, STAGE = IMG_A + IMG_B;          // elements
   constexpr int PA = IMG_A * 2 / 1024 / NW, PB = IMG_B * 2 / 1024 / NW;           // 1 KB pieces per wave
   static_assert(PA >= 1 && PB >= 1, "tile too small for the workgroup");
   __shared__ __attribute__((aligned(16))) uint16_t smem[STAGES * STAGE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / W_N, wn = wave % W_N, l31 = lane & 31, h = lane >> 5;
+  const int wm = wave / W_N, wn = wave % W_N, l15 = lane & 15, lj = lane >> 4;
 
   // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles (all tiles of one part of K, where K is split),
   // and order the tiles in bands of 4 along M, so that the 32 tiles an XCD works on at a time share 4 blocks of A and 8 of B in
@@ -179,7 +187,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
       return (uint32_t)(((int64_t)(min(m0 + row, g.M - 1) - m0) * g.lda + 8 * c) * 2);
     }
     constexpr int CPR = BM / 8;
-    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
+    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ rc_swizzle(k);
     return (uint32_t)(((int64_t)min(k, k_left - 1) * g.lda + min(8 * c, ((g.M + 7) & ~7) - 8 - m0)) * 2);
   };
   auto chunk_b = [&](int i) -> uint32_t {
@@ -190,7 +198,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
       return (uint32_t)(((int64_t)row * g.ldb + 8 * ((lane % CPR) ^ swz)) * 2);
     }
     constexpr int CPR = BN / 8;
-    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ ((k & 3) << 2);
+    const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ rc_swizzle(k);
     return (uint32_t)(((int64_t)k * g.ldb + 8 * c) * 2);
   };
   const int k_tail = K - (kt1 - 1) * BK;                     // of the last step: 1 .. BK
@@ -222,18 +230,16 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     else dma16(sb, off_b[i - PA], st + IMG_A * 2u + (uint32_t)(wave * PB + i - PA) * 1024u);
   };
 
-  // ---- fragments ----
-  const int swz = (l31 >> 1) & 7;
-  const int la = lane & 15, lq = la >> 2, lp = la & 3, lj = lane >> 4;
-  const int kc_a = (wm * 32 * TM + l31) * BK, kc_b = (wn * 32 * TN + l31) * BK;
-  const int rc_k = 8 * (lj >> 1) + lq;
-  const int rc_a = wm * 32 * TM + 16 * (lj & 1) + 4 * lp, rc_b = wn * 32 * TN + 16 * (lj & 1) + 4 * lp;
+  // ---- fragments: 16 rows, 32 of K, 8 consecutive ones to a lane ----
+  const int swz = (l15 >> 1) & 7, lq = l15 >> 2, lp = l15 & 3;
+  const int kc_a = (wm * 16 * TM + l15) * BK, kc_b = (wn * 16 * TN + l15) * BK;
+  const int rc_k = 8 * lj + lq, rc_f = rc_swizzle(rc_k) << 3;
+  const int rc_a = wm * 16 * TM + 4 * lp, rc_b = wn * 16 * TN + 4 * lp;
   auto frag_kc = [&](const uint16_t* img, int base, int t, int ks) -> u4 {
-    return *reinterpret_cast<const u4*>(img + base + t * 32 * BK + (((2 * ks + h) ^ swz) << 3));
+    return *reinterpret_cast<const u4*>(img + base + t * 16 * BK + (((4 * ks + lj) ^ swz) << 3));
   };
   auto frag_rc = [&](const uint16_t* img, int width, int col0, int t, int ks) -> u4 {
-    const int e = col0 + t * 32, col = (((e >> 3) ^ (lq << 2)) << 3) | (e & 7);
-    const uint16_t* p = img + (ks * 16 + rc_k) * width + col;
+    const uint16_t* p = img + (ks * 32 + rc_k) * width + ((col0 + t * 16) ^ rc_f);
     union {
       s16x4 s[2];
       u4 v;
@@ -249,35 +255,34 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   if constexpr (EPI != EPI_STORE) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 32 + l31;
+      const int n = n0 + (wn * TN + j) * 16 + l15;
       const bool real = n < N;
       cls[j] = real ? g.classes[n] : -1;
       lse[j] = EPI == EPI_D && real ? g.lse[n] : 0.f;
       gn[j] = EPI == EPI_D && real ? g.g[n] : 0.f;
     }
   }
-  f32x16 acc[TM][TN];
+  f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4)0.f;
 
-  // Two images: while one is multiplied the other is filled.  The fragments of the next 16 of K are read ahead of the
-  // products of this 16; before the last products of a step its image has been read by everyone, so the step after next is
-  // sent into it between those products.
-  u4 a[2][TM], b[2][TN];
-  constexpr int KS = BK / 16, MMAS = TM * TN, READS = TM + TN, LOADS = PA + PB, HEAD = MMAS / 4;
-  static_assert(KS % 2 == 0 && HEAD >= 1, "fragments alternate between two sets");
-  auto read = [&](int which, int image, int ks, int r) {     // in the order in which the products want them
-    const uint16_t *ia = smem + image * STAGE, *ib = ia + IMG_A;
-    if (r == 0 || r > TM) {
-      const int j = r == 0 ? 0 : r - TM;
-      b[which][j] = B_KC ? frag_kc(ib, kc_b, j, ks) : frag_rc(ib, BN, rc_b, j, ks);
-    } else {
-      a[which][r - 1] = A_KC ? frag_kc(ia, kc_a, r - 1, ks) : frag_rc(ia, BM, rc_a, r - 1, ks);
-    }
+  // Two images: while one is multiplied the other is filled.  In each half of a step (32 of K) the fragment of A is read again,
+  // for the next half, as soon as its products are issued, and B's beside the one in use.  After the first products of the
+  // second half a step's image has been read by everyone, and the step after next is sent into it, piece by piece between the
+  // products of that half: all at once the pieces fill the queue of the vector memory unit and hold up what comes behind them,
+  // and over three quarters or five of a half they took 2 and 5 % longer.
+  u4 a[TM], b[2][TN];
+  constexpr int LOADS = PA + PB;
+  static_assert(TN <= TM, "a fragment of B for every block of products");
+  auto read_a = [&](int image, int ks, int i) {
+    const uint16_t* img = smem + image * STAGE;
+    a[i] = A_KC ? frag_kc(img, kc_a, i, ks) : frag_rc(img, BM, rc_a, i, ks);
+  };
+  auto read_b = [&](int which, int image, int ks, int j) {
+    const uint16_t* img = smem + image * STAGE + IMG_A;
+    b[which][j] = B_KC ? frag_kc(img, kc_b, j, ks) : frag_rc(img, BN, rc_b, j, ks);
   };
   for (; fetched < STAGES && fetched < steps; ++fetched, ++fill) {
     aim();
@@ -287,70 +292,59 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   if (steps >= STAGES) wait_and_meet<LOADS>();
   else wait_and_meet<0>();
 #pragma unroll
-  for (int r = 0; r < READS; ++r) read(0, 0, 0, r);
-  // The loads of a step go out over the two phases (16 of K each) that follow the one in which its image became free.  In one
-  // phase they fill the queue of the vector memory unit and hold up the products behind them (1.48 us a step of a 256 x 256
-  // tile), over three or four the last ones arrive late (1.44, 1.52); over two 1.44.  The products alone take 1.25 at the
-  // clock that their power leaves, as do the library's.  K steps of 32 with 3 to 5 images: 1.61 and more.
-  constexpr int LAST = KS - 1, EACH = (LOADS + SPREAD - 1) / SPREAD;
-  static_assert(SPREAD <= KS, "a step's loads are out before the next image becomes free");
-  fill = 0;
-  int image = 0, next = 1;
+  for (int j = 0; j < TN; ++j) read_b(0, 0, 0, j);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) read_a(0, 0, i);
+  int image = 0;
   bool more = false;
   for (int t = 0; t < steps; ++t) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int cur = ks & 1, head = ks == LAST ? HEAD : 0, phase = ks == LAST ? 0 : ks + 1;
-      int r = 0;
+    for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int q = 0; q < MMAS; ++q) {
-        const int i = q % TM, j = q / TM;
-        acc[i][j] = mma<F16>(a[cur][i], b[cur][j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (ks == LAST && q == head - 1) {
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mma<F16>(a[i], b[ks][j], acc[i][j]);
+        if (ks && i == 0) {
           wait_and_meet<0>();                                // the next step is here, and nobody reads this image any more
           more = t + STAGES < steps;
           fill = image;
           if (more) aim();
         }
-        if (q >= head) {
-          // spread what is to be read and loaded over the products
-          const int done = q - head + 1, of = MMAS - head;
+        const int from = ks ? image ^ 1 : image;             // (behind the last step: old values)
+        read_a(from, ks ^ 1, i);
 #pragma unroll
-          for (; r * of < READS * done; ++r) read(cur ^ 1, ks == LAST ? next : image, ks == LAST ? 0 : ks + 1, r);   // (behind the last step: old values)
-          if (phase < SPREAD && more) {
+        for (int j = 0; j < TN; ++j)
+          if (j * TM / TN == i) read_b(ks ^ 1, from, ks ^ 1, j);
+        if (ks && more) {
 #pragma unroll
-            for (int e = 0; e < EACH; ++e)
-              if (e * of / EACH == done - 1 && phase * EACH + e < LOADS) load(phase * EACH + e);
-          }
-          __builtin_amdgcn_sched_barrier(0);
+          for (int e = 0; e < LOADS; ++e)
+            if (e * TM / LOADS == i) load(e);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (ks == LAST) image = next, next ^= 1;
     }
+    image ^= 1;
   }
 
-  // acc[i][j][r]: m = m0 + 32 (wm TM + i) + 8 (r / 4) + 4 h + r % 4, n = n0 + 32 (wn TN + j) + l31
-  const int mw = m0 + wm * 32 * TM + 4 * h, nw = n0 + wn * 32 * TN + l31;
+  // acc[i][j][r]: m = m0 + 16 (wm TM + i) + 4 lj + r, n = n0 + 16 (wn TN + j) + l15
+  const int mw = m0 + wm * 16 * TM + 4 * lj, nw = n0 + wn * 16 * TN + l15;
   // The waves' outputs go through LDS (the images are done with), where a row n of the tile is contiguous in m, and leave as
-  // whole rows: straight from the registers every store would touch 32 rows.  16-byte chunk c of row n sits at c ^ n (16-bit
-  // elements) or c ^ 2 n (floats), so that neither the writes nor the reads meet in a bank.
-  auto rows_out16 = [&](auto&& value, auto&& send) {         // value(i, j, q) -> 4 packed elements; send(row, chunk, 16 bytes)
+  // whole rows: straight from the registers every store would touch 16 rows.  16-byte chunk c of row n sits at c ^ 2 n (16-bit
+  // elements) or c ^ 4 n (floats), so that neither the writes nor the reads meet in a bank.
+  auto rows_out16 = [&](auto&& value, auto&& send) {         // value(i, j) -> 4 packed elements; send(row, chunk, 16 bytes)
     constexpr int CPR = BM / 8;
     wait_and_meet<0>();
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int row = wn * 32 * TN + 32 * j + l31, c = wm * 4 * TM + 4 * i + q;
-          *reinterpret_cast<uint2*>(smem + row * BM + (((c ^ l31) % CPR) << 3) + 4 * h) = value(i, j, q);
-        }
+      for (int i = 0; i < TM; ++i) {
+        const int row = wn * 16 * TN + 16 * j + l15, c = wm * 2 * TM + 2 * i + (lj >> 1);
+        *reinterpret_cast<uint2*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3) + 4 * (lj & 1)) = value(i, j);
+      }
     __syncthreads();
     for (int x = threadIdx.x; x < BN * CPR; x += 64 * NW) {
       const int row = x / CPR, c = x % CPR;
-      send(row, c, *reinterpret_cast<const u4*>(smem + row * BM + (((c ^ (row & 31)) % CPR) << 3)));
+      send(row, c, *reinterpret_cast<const u4*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3)));
     }
   };
   if constexpr (EPI == EPI_STORE) {
@@ -358,9 +352,8 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     if (g.out_kind == 1) {
       uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
       rows_out16(
-          [&](int i, int j, int q) {
-            return make_uint2(pack2<F16>(acc[i][j][4 * q] * inv, acc[i][j][4 * q + 1] * inv),
-                              pack2<F16>(acc[i][j][4 * q + 2] * inv, acc[i][j][4 * q + 3] * inv));
+          [&](int i, int j) {
+            return make_uint2(pack2<F16>(acc[i][j][0] * inv, acc[i][j][1] * inv), pack2<F16>(acc[i][j][2] * inv, acc[i][j][3] * inv));
           },
           [&](int row, int c, u4 v) {
             const int n = n0 + row, m = m0 + 8 * c;
@@ -379,25 +372,22 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
       typedef f4 f4_any __attribute__((aligned(4)));
       float *lds = reinterpret_cast<float*>(smem), *out = reinterpret_cast<float*>(g.out) + (int64_t)(g.out_kind == 0 ? part : 0) * g.N * g.ldo;
       constexpr int CPR = BM / 4, ROWS = 32 * W_N;           // 32 rows of every wave at a time
-      static_assert(ROWS * BM * 4 <= (int)sizeof(smem), "a pass fits");
+      static_assert(ROWS * BM * 4 <= (int)sizeof(smem) && TN % 2 == 0, "a pass fits");
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
+      for (int j0 = 0; j0 < TN; j0 += 2) {
         wait_and_meet<0>();
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int j = j0; j < j0 + 2; ++j)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = wm * 8 * TM + 8 * i + 2 * q + h;
-            f4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e] * inv;
-            *reinterpret_cast<f4*>(lds + (wn * 32 + l31) * BM + (((c ^ (2 * l31)) % CPR) << 2)) = v;
+          for (int i = 0; i < TM; ++i) {
+            const int row = wn * 32 + 16 * (j - j0) + l15, c = wm * 4 * TM + 4 * i + lj;
+            *reinterpret_cast<f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2)) = acc[i][j] * inv;
           }
         __syncthreads();
         for (int x = threadIdx.x; x < ROWS * CPR; x += 64 * NW) {
           const int row = x / CPR, c = x % CPR;
-          f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (2 * (row & 31))) % CPR) << 2));
-          const int n = n0 + (row >> 5) * 32 * TN + 32 * j + (row & 31), m = m0 + 4 * c;
+          f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2));
+          const int n = n0 + (row >> 5) * 16 * TN + 16 * j0 + (row & 31), m = m0 + 4 * c;
           if (n >= N || m >= g.M) continue;
           float* o = out + (int64_t)n * g.ldo + m;
           if (m + 4 <= g.M) {
@@ -416,8 +406,8 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = g.v0 + min(mw + 32 * i + 8 * (r >> 2) + (r & 3), g.M - 1);
+        for (int r = 0; r < 4; ++r) {
+          const int v = g.v0 + min(mw + 16 * i + r, g.M - 1);
           const float bv = g.bias_f32 ? reinterpret_cast<const float*>(g.bias)[v]
                            : F16      ? (float)reinterpret_cast<const _Float16*>(g.bias)[v]
                                       : (float)reinterpret_cast<const __bf16*>(g.bias)[v];
@@ -432,28 +422,29 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
       wait_and_meet<0>();
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const int n = nw + 32 * j;
-        const int at = cls[j] - g.v0 - mw;                    // 32 i + 8 (r / 4) + r % 4 where the target's logit is ours
-        if (__any(at >= 0 && at < 32 * TM)) {
+        const int n = nw + 16 * j;
+        const int at = cls[j] - g.v0 - mw;                    // 16 i + r where the target's logit is ours
+        if (__any(at >= 0 && at < 16 * TM)) {
           float hit = 0.f;
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) hit = at == 32 * i + 8 * (r >> 2) + (r & 3) ? acc[i][j][r] : hit;
-          if (at >= 0 && at < 32 * TM && !(at & 4)) g.target_logit[n] = hit;   // (at & 4: it is the other half wave's)
+            for (int r = 0; r < 4; ++r) hit = at == 16 * i + r ? acc[i][j][r] : hit;
+          if (at >= 0 && at < 16 * TM && !(at & 12)) g.target_logit[n] = hit;   // (at & 12: it is another lane's)
         }
         if (edge) {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = -INFINITY;
+            for (int r = 0; r < 4; ++r)
+              if (mw + 16 * i + r >= g.M) acc[i][j][r] = -INFINITY;
         }
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float ref = top == -INFINITY ? 0.f : top;       // all of them -inf: the sum is 0, not NaN
         float sum = 0.f;
@@ -462,15 +453,16 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+            for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
         } else {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+            for (int r = 0; r < 4; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
         }
+        sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        if (h == 0) red[wm * BN + wn * 32 * TN + 32 * j + l31] = make_float2(top, sum);
+        if (lj == 0) red[wm * BN + wn * 16 * TN + 16 * j + l15] = make_float2(top, sum);
       }
       __syncthreads();
       for (int c = threadIdx.x; c < BN; c += 64 * NW) {
@@ -496,45 +488,45 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
         } else {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+            for (int r = 0; r < 4; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
         }
-        if (__any(at >= 0 && at < 32 * TM)) {                 // the target is among this wave's classes
+        if (__any(at >= 0 && at < 16 * TM)) {                 // the target is among this wave's classes
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (at == 32 * i + 8 * (r >> 2) + (r & 3)) acc[i][j][r] -= 1.f;
+            for (int r = 0; r < 4; ++r)
+              if (at == 16 * i + r) acc[i][j][r] -= 1.f;
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] *= gs;
+          for (int r = 0; r < 4; ++r) acc[i][j][r] *= gs;
         if (edge || __any(gs == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (gs == 0.f || mw + 32 * i + 8 * (r >> 2) + (r & 3) >= g.M) acc[i][j][r] = 0.f;
+            for (int r = 0; r < 4; ++r)
+              if (gs == 0.f || mw + 16 * i + r >= g.M) acc[i][j][r] = 0.f;
         }
       }
 #pragma unroll
       for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
         rows_out16(
-            [&](int i, int j, int q) {
-              if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][4 * q], acc[i][j][4 * q + 1]), pack2<F16>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
+            [&](int i, int j) {
+              if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][0], acc[i][j][1]), pack2<F16>(acc[i][j][2], acc[i][j][3]));
               union {
                 __bf16 t[4];
                 uint2 u;
               } w;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {                   // the term, and what it leaves for the next
-                w.t[e] = (__bf16)acc[i][j][4 * q + e];
-                acc[i][j][4 * q + e] -= (float)w.t[e];
+                w.t[e] = (__bf16)acc[i][j][e];
+                acc[i][j][e] -= (float)w.t[e];
               }
               return w.u;
             },
@@ -1026,8 +1018,8 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_b
   if (a.db && oq == 0) reinterpret_cast<T*>(a.db)[ov] = (T)sum[4];
 }
 
-// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 1024 x 30 x 17 in 63 against 80, 512 x 64 x 64,
-// 2^21 products, in 115 against 74).
+// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 1024 x 30 x 17
+// in 63 against 80, 512 x 64 x 64, 2^21 products, in 115 against 74).
 bool small_head(const vae_linear_ce* a) {
   return a->V <= SMALL_V && a->D <= SMALL_D && a->N <= SMALL_ROWS && a->N * a->V * a->D <= SMALL_WORK;
 }
@@ -1054,10 +1046,12 @@ void small(const Small& s, int dtype, bool bwd, hipStream_t st) {
 int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
 
 // Tiles of 256 x 256 (one workgroup to a CU) or 128 x 128 (two), and into how many parts the sum over K is split where the
-// tiles do not fill the chip: the least of rounds * (steps * c + f) + the slabs' traffic, with c and f as measured in bf16 (a
-// step of 64 of K takes 1.45 us in a large tile and 0.8 in each of two small ones; starting and ending a tile 8 and 6 us, and
-// 40 where a large tile of fp32 logits is turned into three terms of d, for which its registers do not suffice: 79 us for
-// 512 x 20000 x 256, 59 in small tiles).
+// tiles do not fill the chip: the least of rounds * (steps * c + f) + the slabs' traffic, with c and f as measured in bf16: a
+// step of 64 of K takes 1.4 us in a large tile and 0.9 in each of two small ones; starting and ending a tile 8 and 6 us, 12
+// where a large tile of logits is turned into d, and 55 where it is turned into three terms of d, for which its registers do
+// not suffice.  Large against small, rows x D x classes: 8192 x 4096 x 16384 bf16 loss 0.84 and 1.05 ms, 8192 x 1024 x 16384
+// 290 and 356 us; d of 2048 x 256 x 20000 bf16 57 and 50, fp32 264 and 190, of 512 x 256 x 20000 fp32 90 and 67; dx of 2048 x
+// 1024 x 8192 fp32 171 and 213.
 struct Tiles {
   bool big;
   int split;
@@ -1071,7 +1065,7 @@ Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool a
     for (int s = 1; s <= may_split; s += s < 4 ? 1 : s < 16 ? 2 : 8) {
       const int64_t per = (steps + s - 1) / s;
       if (s > 1 && per < 4) break;
-      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.45 : 0.8) + (big ? end_big : 6.0));
+      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.4 : 0.9) + (big ? end_big : 6.0));
       if (always_slabs || s > 1) t += 3.0 + (double)s * (double)m * (double)n * 8.0 / 4.5e6;
       if (t < least) least = t, best = {big != 0, s};
     }
@@ -1129,7 +1123,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     const int64_t pieces = (most + p.piece - 1) / p.piece;
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
-    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false, p.f32 ? 40.0 : 8.0);
+    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false, p.f32 ? 55.0 : 12.0);
     p.dx_tiles = tiles_for(a->D, a->N, p.piece, p.f32, 64, true);
     p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
     p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
