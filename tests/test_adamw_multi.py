@@ -15,9 +15,10 @@ BLOCK = 256
 
 
 # ---------------------------------------------------------------------------------------------------- on the CPU
-def _args(lib_mod, tensors, bits=32, n_blocks=8, ptr=1 << 20, scales=None, master=None, step=1, lr=1e-3, clip=0.0, ws=None, wsb=0):
+def _args(lib_mod, tensors, bits=32, n_blocks=8, ptr=1 << 20, scales=None, master=None, step=1, lr=1e-3, clip=0.0, ws=None, wsb=0,
+          wide=1 << 20):
     arr = (lib_mod.AdamWTensor * max(1, len(tensors)))(*tensors)
-    return (arr, len(tensors), bits, C.c_void_p(ptr), C.c_void_p(ptr + (1 << 20)), scales, n_blocks, master, lr, 0.9, 0.99, 1e-8, step,
+    return (arr, len(tensors), bits, C.c_void_p(ptr), C.c_void_p(ptr + wide), scales, n_blocks, master, lr, 0.9, 0.99, 1e-8, step,
             clip, 1.0, 0, ws, wsb, None, None)
 
 
@@ -48,6 +49,10 @@ def test_refusals_of_the_c_entry():
     refused("overlap", [ok, ok])
     refused("overlap", [T((1 << 20) + 512, base, 4, 0, 0.0, 0)])                # a parameter inside exp_avg
     refused("share blocks", [ok, T(base + 4096, base, 4, 0, 0.0, 0)])
+    refused("the gradient overlaps", [ok, T(base + 4096, base + 396, 4, 1, 0.0, 0)])      # a gradient inside another parameter
+    refused("the gradient overlaps", [T(base, base, 4, 0, 0.0, 0)])
+    refused("the gradient overlaps", [T(base, (1 << 20) + 8188, 4, 0, 0.0, 0)])           # ... or at the end of exp_avg
+    refused("2^37", [T(base, base + (1 << 41), 1 << 38, 0, 0.0, 1)], n_blocks=1 << 30, ptr=1 << 43, wide=1 << 42)
     refused("scales", [ok], bits=8)
     refused("16-byte aligned", [ok], ptr=(1 << 20) + 4)
     refused("workspace", [ok], clip=1.0)
@@ -271,3 +276,26 @@ def test_every_e4m3_rounding():
     inv = (torch.ones(1, device="cuda") * 448).reciprocal() * 448
     want = (g * inv).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(m.float(), want.float())
+
+
+@pytest.mark.gpu
+def test_a_step_shows_in_the_version_of_what_it_changed():
+    """A backward pass that saved weights from before a step must not run on the new ones."""
+    from vae_amd.optim import MultiTensorAdamW
+    w, idle = (torch.ones(5, 5, device="cuda", requires_grad=True) for _ in range(2))
+    x = torch.ones(2, 5, device="cuda", requires_grad=True)
+    old = (x @ w + x @ idle).sum()
+    w.grad = torch.ones_like(w)
+    MultiTensorAdamW([w, idle], state_bits=32).step()
+    assert idle._version == 0
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        old.backward()
+
+
+@pytest.mark.gpu
+def test_two_parameters_may_share_a_gradient():
+    from vae_amd.optim import MultiTensorAdamW
+    a, b = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    a.grad = b.grad = torch.randn(300, device="cuda")
+    MultiTensorAdamW([a, b], state_bits=32).step()
+    assert torch.equal(a, b) and not bool((a == 1).all())

@@ -333,10 +333,11 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
   VAE_REQUIRE(!clip || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0 &&
                         workspace_bytes >= vae_adamw_multi_workspace_bytes(n_tensors)),
               "vae_adamw_multi: clipping needs an 8-byte aligned workspace of vae_adamw_multi_workspace_bytes()");
-  // what is written must be disjoint: two updates of one element would race
-  Span* spans = new (std::nothrow) Span[2 * n_tensors + 5];
+  // what is written must be disjoint, and no gradient may lie in it: two accesses to one element would race
+  Span* spans = new (std::nothrow) Span[2 * n_tensors + 4];
   VAE_REQUIRE(spans, "vae_adamw_multi: out of host memory");
-  int64_t total = 0, n_spans = 0;
+  Span* blocks = spans + n_tensors + 4;
+  int64_t total = 0, n_spans = 0, n_live = 0;
   const char* bad = nullptr;
   long long bad_at = 0;
   const int64_t per = state_bits == 8 ? 1 : 4;
@@ -353,9 +354,16 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
     else if (!(t.weight_decay >= 0)) bad = "negative weight decay";
     else if (t.n) {
       spans[n_spans++] = {pb, pb + (uintptr_t)(t.n * esize)};
+      blocks[n_live++] = {(uintptr_t)t.first_block, (uintptr_t)(t.first_block + (t.n + BLK - 1) / BLK)};
       total += t.n;
     }
   }
+  const auto disjoint = [](Span* s, int64_t n) {
+    std::sort(s, s + n, [](const Span& a, const Span& b) { return a.b < b.b; });
+    for (int64_t i = 1; i < n; ++i)
+      if (s[i].b < s[i - 1].e) return false;
+    return true;
+  };
   if (!bad) {
     auto add = [&](const void* q, int64_t bytes) {
       if (q) spans[n_spans++] = {reinterpret_cast<uintptr_t>(q), reinterpret_cast<uintptr_t>(q) + (uintptr_t)bytes};
@@ -364,18 +372,15 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
     add(exp_avg_sq, n_blocks * BLK * per);
     if (state_bits == 8) add(scales, 2 * n_blocks * 4);
     add(master, n_blocks * BLK * 4);
-    std::sort(spans, spans + n_spans, [](const Span& a, const Span& b) { return a.b < b.b; });
-    for (int64_t i = 1; i < n_spans && !bad; ++i)
-      if (spans[i].b < spans[i - 1].e) bad = "params and state overlap in memory", bad_at = -1;
+    if (!disjoint(spans, n_spans)) bad = "params and state overlap in memory", bad_at = -1;
+    else if (!disjoint(blocks, n_live)) bad = "two tensors share blocks of the state", bad_at = -1;
+    else if (total > 1ll << 37) bad = "more than 2^37 elements", bad_at = -1;      // (a launch's grid holds what 96 of them need)
   }
-  if (!bad) {   // the same for the ranges of the flat state
-    n_spans = 0;
-    for (int64_t k = 0; k < n_tensors; ++k)
-      if (tensors[k].n)
-        spans[n_spans++] = {(uintptr_t)tensors[k].first_block, (uintptr_t)(tensors[k].first_block + (tensors[k].n + BLK - 1) / BLK)};
-    std::sort(spans, spans + n_spans, [](const Span& a, const Span& b) { return a.b < b.b; });
-    for (int64_t i = 1; i < n_spans && !bad; ++i)
-      if (spans[i].b < spans[i - 1].e) bad = "two tensors share blocks of the state", bad_at = -1;
+  for (int64_t k = 0; k < n_tensors && !bad; ++k) {
+    const vae_adamw_tensor& t = tensors[k];
+    const uintptr_t b = reinterpret_cast<uintptr_t>(t.grad), e = b + (uintptr_t)(t.n * (t.dtype == VAE_ADAMW_F32 ? 4 : 2));
+    const Span* after = std::lower_bound(spans, spans + n_spans, e, [](const Span& s, uintptr_t x) { return s.b < x; });
+    if (t.n && after != spans && after[-1].e > b) bad = "the gradient overlaps what is written", bad_at = (long long)k;
   }
   delete[] spans;
   VAE_REQUIRE(!bad, "vae_adamw_multi: tensor %lld: %s", bad_at, bad);
@@ -409,10 +414,8 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
       for (; k < n_tensors && t.count < PER_LAUNCH; ++k) {
         const vae_adamw_tensor& e = tensors[k];
         if (e.n == 0) continue;
-        const int64_t c = (e.n + chunk - 1) / chunk;
-        if (t.count && chunks + c > 0x7fffffffll) break;
         const int i = t.count++;
-        chunks += c;
+        chunks += (e.n + chunk - 1) / chunk;
         t.p[i] = e.param;
         t.g[i] = e.grad;
         t.n[i] = e.n;

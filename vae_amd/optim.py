@@ -263,7 +263,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
         if len(decay) != n:
             raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(decay)} weight decays")
     table: List[Union[int, float]] = []
-    at = live = 0
+    at, live = 0, []
     for p, g, wd in zip(params, grads, decay):
         count = p.numel()
         if g is not None and count:
@@ -276,7 +276,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
             if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
                 raise ValueError("vae_amd.optim.multi_tensor_adamw_: parameters and gradients must be contiguous and of one shape")
             table += (p.data_ptr(), g.data_ptr(), count, at, wd, _ADAMW_DTYPES[dtype])
-            live += 1
+            live.append(p)
         at += -(-count // ADAMW_BLOCK)
     for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
         if t is None:
@@ -297,14 +297,15 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
             norm = torch.zeros(1, dtype=torch.float32, device=dev)
         if not live:
             return norm
-        nbytes = lib.vae_adamw_multi_workspace_bytes(live) if clip else 0
+        nbytes = lib.vae_adamw_multi_workspace_bytes(len(live)) if clip else 0
         ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev) if clip else None
-        rc = lib.vae_adamw_multi(struct.pack("=" + "QQqqfi" * live, *table), live, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+        rc = lib.vae_adamw_multi(struct.pack("=" + "QQqqfi" * len(live), *table), len(live), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
                                  scales.data_ptr() if bits == 8 else None, at, None if master is None else master.data_ptr(), float(lr),
                                  float(betas[0]), float(betas[1]), float(eps), int(step), float(max_grad_norm), float(grad_scale),
                                  int(seed) & (2 ** 64 - 1), None if ws is None else ws.data_ptr(), nbytes,
                                  None if norm is None else norm.data_ptr(), _raw_stream(dev.index))
     _lib.check(rc, "multi_tensor_adamw_")
+    torch.autograd.graph.increment_version(live)       # a backward pass that saved the old values then says so
     return norm
 
 
