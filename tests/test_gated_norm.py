@@ -42,6 +42,8 @@ def test_refusals_of_the_c_entry():
     refused("null pointer", gate_mode=1)
     refused("null pointer", h=None)
     refused("aligned", r=4098)
+    refused("vector is not aligned", scale=4098)
+    refused("vector is not aligned", dtype=1, vectors_f32=1, norm_weight=4098)
     refused("stats", stats=4100)
     refused("null pointer", bwd=True)
     full = dict(stats=65536, dr=4096, db=4096)
@@ -294,3 +296,27 @@ def test_non_finite_rows_stay_in_their_rows():
         assert torch.equal(c[[0, 1, 3, 5]], o[[0, 1, 3, 5]])
         assert bool(torch.isnan(o[2]).all())
     assert bool(torch.isinf(got[0][4, 299])) and not bool(torch.isfinite(got[1][4]).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [40, 1000])
+def test_gradients_of_vectors_that_are_taken_as_one_or_zero(d):
+    """The C entry gives them as well: the gradient of an absent bias of the second norm is the sum of dh over the rows."""
+    from vae_amd import _lib
+    lib, n = _lib.load(), 9
+    x = _inputs(n, d, "fp32", None, False, False, False, False, seed=3)[0]
+    from vae_amd import ops
+    y, h, stats = ops.gated_norm_fwd(x["r"], x["b"])
+    dh = torch.randn(n, d, device="cuda")
+    dr, db, out = torch.empty_like(y), torch.empty_like(y), torch.full((3, d), float("nan"), device="cuda")
+    nbytes = lib.vae_gated_norm_workspace_bytes(n, d, 0)
+    ws = torch.full((nbytes // 4,), float("nan"), device="cuda")
+    a = _lib.GatedNorm(N=n, D=d, dtype=0, kind=0, gate_mode=0, act=0, eps=1e-5, r=x["r"].data_ptr(), ld_r=d, b=x["b"].data_ptr(), ld_b=d,
+                       y=y.data_ptr(), h=h.data_ptr(), stats=stats.data_ptr(), dh=dh.data_ptr(), ld_dh=d, dr=dr.data_ptr(),
+                       db=db.data_ptr(), dnorm_weight=out[0].data_ptr(), dnorm_bias=out[1].data_ptr(), dscale=out[2].data_ptr())
+    assert lib.vae_gated_norm_bwd(C.byref(a), ws.data_ptr(), nbytes, None) == 0
+    torch.cuda.synchronize()
+    ny = y.double() / (y.double().square().mean(1, keepdim=True) + 1e-5).sqrt()
+    for got, ref in ((out[0], dh.double() * ny), (out[1], dh.double()), (out[2], dr.double() * x["b"].double())):
+        tol = 2e-5 * float(ref.abs().max()) + 128 * 2.0 ** -24 * ref.abs().sum(0)        # (as the gradients of the vectors above)
+        assert bool(((got.double() - ref.sum(0)).abs() <= tol).all())

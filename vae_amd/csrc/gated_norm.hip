@@ -312,8 +312,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, FWD_WAVES) void gated_norm
   }
 }
 
-// BIAS: whether either norm has one; without, their column sums are not carried.  WAVES: least waves per SIMD, which bounds
-// the registers.
+// BIAS: whether a gradient of either norm's bias is asked for; without, their column sums are not carried.
 template <typename T, typename V, int NW, int ITEMS, bool BIAS>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, bwd_waves(NW)) void gated_norm_bwd_kernel(Args a, float* __restrict__ partial) {
   constexpr int P = PIECE<T>, TPR = NW * 64, RPW = NW == 1 ? 4 : 1;
@@ -553,7 +552,7 @@ int64_t pieces_of(int64_t D, int dtype) {
 template <typename T, typename V> void launch(const Args& a, bool bwd, float* partial, const Shape& s, int groups, hipStream_t st) {
 #define VAE_GN(NW, ITEMS)                                                                                    \
   if (s.nw == NW && s.items == ITEMS) {                                                                      \
-    if (bwd && (a.norm_bias || a.post_bias))                                                                 \
+    if (bwd && (a.dnorm_bias || a.dpost_bias))                                                               \
       gated_norm_bwd_kernel<T, V, NW, ITEMS, true><<<groups, NW == 1 ? 256 : NW * 64, 0, st>>>(a, partial);  \
     else if (bwd)                                                                                            \
       gated_norm_bwd_kernel<T, V, NW, ITEMS, false><<<groups, NW == 1 ? 256 : NW * 64, 0, st>>>(a, partial); \
@@ -588,6 +587,10 @@ int check(const Args* a, const char* who) {
   const uintptr_t bad = a->dtype == VAE_ADAMW_F32 ? 3 : 1;
   const void* rows[] = {a->r, a->b, a->gate, a->y, a->h, a->dy, a->dh, a->dr, a->db, a->dgate};
   for (const void* p : rows) VAE_REQUIRE((reinterpret_cast<uintptr_t>(p) & bad) == 0, "%s: a pointer is not aligned to its element", who);
+  const void* vectors[] = {a->norm_weight, a->norm_bias, a->scale, a->post_weight, a->post_bias, a->dnorm_weight, a->dnorm_bias, a->dscale,
+                           a->dpost_weight, a->dpost_bias};
+  for (const void* p : vectors)
+    VAE_REQUIRE((reinterpret_cast<uintptr_t>(p) & (a->vectors_f32 ? 3 : bad)) == 0, "%s: a vector is not aligned to its element", who);
   VAE_REQUIRE((reinterpret_cast<uintptr_t>(a->stats) & 15u) == 0, "%s: stats must be 16-byte aligned", who);
   return VAE_OK;
 }
