@@ -36,6 +36,9 @@ def test_refusals_of_the_c_entry():
         refused("at least 1", fwd, V=0)
         refused("at most", fwd, V=(1 << 24) + 1)
         refused("tiles", fwd, V=1 << 24, N=1 << 24)
+        refused("128 classes", fwd, V=1 << 20, N=1 << 18)
+        refused("128 columns", fwd, D=1 << 20, N=1 << 18, ldw=1 << 20, ldx=1 << 20)
+        refused("128 columns", fwd, D=1 << 20, V=1 << 18, ldw=1 << 20, ldx=1 << 20)
         refused("null pointer", fwd, x=None)
         refused("null pointer", fwd, w=None)
         refused("null pointer", fwd, target=None)
@@ -79,6 +82,8 @@ def test_refusals_of_the_python_entry():
         linear_cross_entropy(x, w, t, bias=torch.zeros(5).half())
     with pytest.raises(TypeError, match="weight is"):
         linear_cross_entropy(x, w, t, weight=torch.zeros(5).double())
+    with pytest.raises(ValueError, match="not differentiable"):
+        linear_cross_entropy(x, w, t, weight=torch.zeros(5, requires_grad=True))
     with pytest.raises(ValueError, match="vector of 5"):
         linear_cross_entropy(x, w, t, weight=torch.zeros(4))
 
@@ -320,3 +325,6 @@ def test_partial_gradients_empty_and_module():
     loss.backward()
     assert float(loss.detach()) == 0 and e.grad.shape == (0, 32) and not bool(m.linear.weight.grad.any())
     assert bool(torch.isnan(m(e, none))) and linear_cross_entropy(e, m.linear.weight, none, reduction="none").shape == (0,)
+    weighted = LinearCrossEntropyLoss(32, 40, weight=torch.rand(40, device="cuda")).cuda().bfloat16()    # takes the weights along
+    weighted(s["x"].bfloat16(), s["target"]).backward()
+    assert weighted.linear.weight.grad.dtype == torch.bfloat16

@@ -1064,7 +1064,7 @@ Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool a
     const int64_t b = big ? 256 : 128, tiles = ((m + b - 1) / b) * ((n + b - 1) / b), slots = big ? 256 : 512;
     for (int s = 1; s <= may_split; s += s < 4 ? 1 : s < 16 ? 2 : 8) {
       const int64_t per = (steps + s - 1) / s;
-      if (s > 1 && per < 4) break;
+      if (s > 1 && (per < 4 || tiles * s >= 1 << 24)) break;
       double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.4 : 0.9) + (big ? end_big : 6.0));
       if (always_slabs || s > 1) t += 3.0 + (double)s * (double)m * (double)n * 8.0 / 4.5e6;
       if (t < least) least = t, best = {big != 0, s};
@@ -1168,7 +1168,10 @@ int check(const vae_linear_ce* a, const char* who) {
   VAE_REQUIRE(a->dtype >= 0 && a->dtype <= 2, "%s: unknown dtype %d", who, a->dtype);
   VAE_REQUIRE(a->N >= 1 && a->D >= 1 && a->V >= 1, "%s: N, D and V must be at least 1", who);
   VAE_REQUIRE(a->N <= (1ll << 24) && a->D <= (1ll << 20) && a->V <= (1ll << 24), "%s: at most 2^24 rows, 2^20 columns and 2^24 classes", who);
-  VAE_REQUIRE((a->N + 127) / 128 * ((a->V + 127) / 128) < (1ll << 30), "%s: more than 2^30 tiles", who);
+  // (a launch holds 2^32 threads: 2^24 tiles of 256)
+  VAE_REQUIRE((a->N + 127) / 128 * ((a->V + 127) / 128) < (1ll << 24), "%s: more than 2^24 tiles of 128 rows and 128 classes", who);
+  VAE_REQUIRE((a->N + 127) / 128 * ((a->D + 127) / 128) < (1ll << 24), "%s: more than 2^24 tiles of 128 rows and 128 columns", who);
+  VAE_REQUIRE((a->V + 127) / 128 * ((a->D + 127) / 128) < (1ll << 24), "%s: more than 2^24 tiles of 128 classes and 128 columns", who);
   VAE_REQUIRE(a->x && a->w && a->target, "%s: null pointer", who);
   VAE_REQUIRE((a->N == 1 || a->ldx >= 0) && (a->V == 1 || a->ldw >= a->D), "%s: bad row stride", who);
   VAE_REQUIRE(a->ldw < (1ll << 22) && a->ldx < (1ll << 40), "%s: a row stride is too large", who);

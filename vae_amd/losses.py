@@ -118,10 +118,13 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
     held in 32 bits.  ``target`` (...) int64; ``weight`` (V) float32 class weights.  Rows whose target is ``ignore_index`` take no
     part: their loss and gradient are 0, and they cost next to nothing.  Any other target outside [0, V) makes its row's loss
     and gradients NaN (torch stops with a device assertion).  "mean" divides by the sum of the class weights that took part
-    (NaN when none did; the gradients are 0 then)."""
+    (NaN when none did; the gradients are 0 then).  A class is ruled out by a bias of -inf or of the type's lowest value; what
+    an infinity in ``w`` or in a row of ``x`` that takes part reaches is infinite or NaN."""
     from .autograd import LinearCrossEntropyFn
     if x.dim() < 1 or tuple(target.shape) != tuple(x.shape[:-1]):
         raise ValueError(f"vae_amd.linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if weight is not None and weight.requires_grad:
+        raise ValueError("vae_amd.linear_cross_entropy: weight is not differentiable (as in torch); detach it")
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.numel() and rows.stride(1) != 1 and rows.shape[1] > 1:
         rows = rows.contiguous()
@@ -150,5 +153,6 @@ class LinearCrossEntropyLoss(nn.Module):
         self.ignore_index, self.reduction = ignore_index, reduction
 
     def forward(self, x: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
-        return linear_cross_entropy(x, self.linear.weight, target, bias=self.linear.bias, weight=self.weight,
+        weight = None if self.weight is None else self.weight.float()        # (.to(dtype) takes the buffer along)
+        return linear_cross_entropy(x, self.linear.weight, target, bias=self.linear.bias, weight=weight,
                                     ignore_index=self.ignore_index, reduction=self.reduction)
