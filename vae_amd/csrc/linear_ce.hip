@@ -141,54 +141,57 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   constexpr int IMG_A = BM * BK, IMG_B = BN * BK, STAGE = IMG_A + IMG_B;          // elements
   constexpr int PA = IMG_A * 2 / 1024 / NW, PB = IMG_B * 2 / 1024 / NW;           // 1 KB pieces per wave
   static_assert(PA >= 1 && PB >= 1, "tile too small for the workgroup");
-  __shared__ __attribute__((aligned(16))) uint16_t smem[STAGES * STAGE];
+  // Workgroups whose epilogue leaves the images alone stay for several tiles and send for the next one's first steps during the
+  // last ones of the tile before: 250 -> 242 us for 4093 x 1000 x 30011, 473 -> 464 for 2048 x 2048 x 65536.
+  constexpr bool STAY = EPI == EPI_STATS;
+  __shared__ __attribute__((aligned(16))) uint16_t smem[STAGES * STAGE + (STAY ? W_M * BN * 4 : 0)];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / W_N, wn = wave % W_N, l15 = lane & 15, lj = lane >> 4;
 
-  // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles (all tiles of one part of K, where K is split),
-  // and order the tiles in bands of 4 along M, so that the 32 tiles an XCD works on at a time share 4 blocks of A and 8 of B in
-  // its L2.
-  const int total = g.tiles_m * g.tiles_n;
-  int id, part;
-  {
-    const int all_wg = (int)gridDim.x, q8 = all_wg >> 3, r8 = all_wg & 7, xcd = blockIdx.x & 7;
-    const int lin = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + ((int)blockIdx.x >> 3);
-    part = lin / total;
-    id = lin - part * total;
-  }
-  int tm, tn;
-  {
-    constexpr int BAND = 4;
-    const int band = id / (BAND * g.tiles_n), in = id - band * BAND * g.tiles_n;
-    const int height = min(BAND, g.tiles_m - band * BAND);
-    tm = band * BAND + in % height;
-    tn = in / height;
-  }
-  const int m0 = tm * BM, n0 = tn * BN;
-  int N = g.N, K = g.K;
+  int N = g.N, K = g.K, tiles_n = g.tiles_n;
   if (g.dyn) {
     const int kept = __builtin_amdgcn_readfirstlane(*g.dyn);
     if (g.dyn_k) K = min(K, kept);
-    else N = min(N, kept);
+    else N = min(N, kept), tiles_n = (N + BN - 1) / BN;
   }
-  if (n0 >= N) return;
+  // Workgroups go round the 8 XCDs: give each XCD a run of consecutive tiles (all tiles of one part of K, where K is split),
+  // which its workgroups take in turn, and order the tiles in bands of 4 along M, so that the 32 tiles an XCD works on at a time
+  // share 4 blocks of A and 8 of B in its L2.
+  const int total = g.tiles_m * tiles_n;
+  int id, end, turn;
+  {
+    const int all = total * g.split, q8 = all >> 3, r8 = all & 7, xcd = blockIdx.x & 7, beg = xcd * q8 + min(xcd, r8);
+    id = beg + ((int)blockIdx.x >> 3);
+    end = beg + q8 + (xcd < r8 ? 1 : 0);
+    turn = ((int)gridDim.x + 7 - xcd) >> 3;
+  }
+  if (id >= end) return;
+  const int part = id / total;                               // of K (which is split only where a workgroup has one tile)
+  auto place = [&](int tile, int& m0, int& n0) {
+    constexpr int BAND = 4;
+    const int at = tile % total, band = at / (BAND * tiles_n), in = at - band * BAND * tiles_n;
+    const int height = min(BAND, g.tiles_m - band * BAND);
+    m0 = (band * BAND + in % height) * BM;
+    n0 = in / height * BN;
+  };
 
-  const int kt1 = (K + BK - 1) / BK, all = kt1 * g.segs, per = (all + g.split - 1) / g.split;
-  const int t_beg = min(part * per, all), t_end = min(t_beg + per, all);
+  const int kt1 = (K + BK - 1) / BK, all_k = kt1 * g.segs, per = (all_k + g.split - 1) / g.split;
+  const int t_beg = min(part * per, all_k), steps = min(t_beg + per, all_k) - t_beg;
 
   // ---- loads: per-lane byte offsets from a base that moves with K; `k_left` elements of K remain from the step on ----
+  int f_m0, f_n0;                                            // the tile that is being loaded: ahead of the one in work at its end
   auto chunk_a = [&](int i, int k_left) -> uint32_t {
     const int piece = wave * PA + i;
     if (A_KC) {
       constexpr int CPR = BK / 8;
       const int row = piece * (64 / CPR) + lane / CPR, swz = (row >> 1) & 7;
       const int c = min((lane % CPR) ^ swz, (k_left + 7) / 8 - 1);
-      return (uint32_t)(((int64_t)(min(m0 + row, g.M - 1) - m0) * g.lda + 8 * c) * 2);
+      return (uint32_t)(((int64_t)(min(f_m0 + row, g.M - 1) - f_m0) * g.lda + 8 * c) * 2);
     }
     constexpr int CPR = BM / 8;
     const int k = piece * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ rc_swizzle(k);
-    return (uint32_t)(((int64_t)min(k, k_left - 1) * g.lda + min(8 * c, ((g.M + 7) & ~7) - 8 - m0)) * 2);
+    return (uint32_t)(((int64_t)min(k, k_left - 1) * g.lda + min(8 * c, ((g.M + 7) & ~7) - 8 - f_m0)) * 2);
   };
   auto chunk_b = [&](int i) -> uint32_t {
     const int piece = wave * PB + i;
@@ -203,19 +206,31 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   };
   const int k_tail = K - (kt1 - 1) * BK;                     // of the last step: 1 .. BK
   uint32_t off_a[PA], off_t[PA], off_b[PB];
+  auto offsets = [&]() {
 #pragma unroll
-  for (int i = 0; i < PA; ++i) off_a[i] = chunk_a(i, BK), off_t[i] = chunk_a(i, max(k_tail, 1));
+    for (int i = 0; i < PA; ++i) off_a[i] = chunk_a(i, BK), off_t[i] = chunk_a(i, max(k_tail, 1));
 #pragma unroll
-  for (int i = 0; i < PB; ++i) off_b[i] = chunk_b(i);
-
-  const uint16_t* base_a = A_KC ? g.a + (int64_t)m0 * g.lda : g.a + m0;
-  const uint16_t* base_b = B_KC ? g.b + (int64_t)n0 * g.ldb : g.b + n0;
+    for (int i = 0; i < PB; ++i) off_b[i] = chunk_b(i);
+  };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
-  const int steps = t_end - t_beg;
-  int kt = t_beg / g.segs, seg = t_beg - kt * g.segs, fetched = 0, fill = 0;   // of the next step to load, and its image
+  const uint16_t *base_a, *base_b;
+  int kt, seg, f_id = id, f_steps = 0, fill = 0;             // of the next step to load; steps loaded of its tile; its image
+  auto start = [&]() {
+    place(f_id, f_m0, f_n0);
+    base_a = A_KC ? g.a + (int64_t)f_m0 * g.lda : g.a + f_m0;
+    base_b = B_KC ? g.b + (int64_t)f_n0 * g.ldb : g.b + f_n0;
+    kt = t_beg / g.segs;
+    seg = t_beg - kt * g.segs;
+    f_steps = 0;
+    offsets();
+  };
+  start();
   const uint16_t *sa, *sb;                                              // its base
   bool tail;
+  auto more = [&]() { return f_steps < steps || (STAY && f_id + turn < end); };
   auto aim = [&]() {
+    if (STAY && f_steps == steps) f_id += turn, start();    // on to the next tile
+    ++f_steps;
     // terms (hi 0, mid 1, lo 2) of the product a * b that segment `seg` forms: mm, hl, lh, hm, mh, hh
     const int pa = g.segs == 1 ? 0 : (0x102010 >> (20 - 4 * seg)) & 15, pb = g.segs == 1 ? 0 : (0x120100 >> (20 - 4 * seg)) & 15;
     const int k0 = kt * BK;
@@ -249,30 +264,13 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     return u.v;
   };
 
-  // what the epilogue needs of this lane's rows, asked for now
-  int cls[TN];
-  float lse[TN], gn[TN];
-  if constexpr (EPI != EPI_STORE) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + (wn * TN + j) * 16 + l15;
-      const bool real = n < N;
-      cls[j] = real ? g.classes[n] : -1;
-      lse[j] = EPI == EPI_D && real ? g.lse[n] : 0.f;
-      gn[j] = EPI == EPI_D && real ? g.g[n] : 0.f;
-    }
-  }
-  f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4)0.f;
-
   // Two images: while one is multiplied the other is filled.  In each half of a step (32 of K) the fragment of A is read again,
   // for the next half, as soon as its products are issued, and B's beside the one in use.  After the first products of the
   // second half a step's image has been read by everyone, and the step after next is sent into it, piece by piece between the
   // products of that half: all at once the pieces fill the queue of the vector memory unit and hold up what comes behind them,
   // and over three quarters or five of a half they took 2 and 5 % longer.
+  // The steps run on from one tile to the next: the last two of a tile send for the first two of the next one, which are on
+  // their way during its epilogue.
   u4 a[TM], b[2][TN];
   constexpr int LOADS = PA + PB;
   static_assert(TN <= TM, "a fragment of B for every block of products");
@@ -284,254 +282,279 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
     const uint16_t* img = smem + image * STAGE + IMG_A;
     b[which][j] = B_KC ? frag_kc(img, kc_b, j, ks) : frag_rc(img, BN, rc_b, j, ks);
   };
-  for (; fetched < STAGES && fetched < steps; ++fetched, ++fill) {
+  int fetched = 0;
+  for (; fetched < STAGES && more(); ++fetched, ++fill) {
     aim();
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) load(i);
   }
-  if (steps >= STAGES) wait_and_meet<LOADS>();
+  if (fetched == STAGES) wait_and_meet<LOADS>();
   else wait_and_meet<0>();
-#pragma unroll
-  for (int j = 0; j < TN; ++j) read_b(0, 0, 0, j);
-#pragma unroll
-  for (int i = 0; i < TM; ++i) read_a(0, 0, i);
   int image = 0;
-  bool more = false;
-  for (int t = 0; t < steps; ++t) {
+  for (; id < end; id += turn) {
+    int m0, n0;
+    place(id, m0, n0);
+    // what the epilogue needs of this lane's rows, asked for now
+    int cls[TN];
+    float lse[TN], gn[TN];
+    if constexpr (EPI != EPI_STORE) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma<F16>(a[i], b[ks][j], acc[i][j]);
-        if (ks && i == 0) {
-          wait_and_meet<0>();                                // the next step is here, and nobody reads this image any more
-          more = t + STAGES < steps;
-          fill = image;
-          if (more) aim();
-        }
-        const int from = ks ? image ^ 1 : image;             // (behind the last step: old values)
-        read_a(from, ks ^ 1, i);
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          if (j * TM / TN == i) read_b(ks ^ 1, from, ks ^ 1, j);
-        if (ks && more) {
-#pragma unroll
-          for (int e = 0; e < LOADS; ++e)
-            if (e * TM / LOADS == i) load(e);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + (wn * TN + j) * 16 + l15;
+        const bool real = n < N;
+        cls[j] = real ? g.classes[n] : -1;
+        lse[j] = EPI == EPI_D && real ? g.lse[n] : 0.f;
+        gn[j] = EPI == EPI_D && real ? g.g[n] : 0.f;
       }
     }
-    image ^= 1;
-  }
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4)0.f;
 
-  // acc[i][j][r]: m = m0 + 16 (wm TM + i) + 4 lj + r, n = n0 + 16 (wn TN + j) + l15
-  const int mw = m0 + wm * 16 * TM + 4 * lj, nw = n0 + wn * 16 * TN + l15;
-  // The waves' outputs go through LDS (the images are done with), where a row n of the tile is contiguous in m, and leave as
-  // whole rows: straight from the registers every store would touch 16 rows.  16-byte chunk c of row n sits at c ^ 2 n (16-bit
-  // elements) or c ^ 4 n (floats), so that neither the writes nor the reads meet in a bank.
-  auto rows_out16 = [&](auto&& value, auto&& send) {         // value(i, j) -> 4 packed elements; send(row, chunk, 16 bytes)
-    constexpr int CPR = BM / 8;
-    wait_and_meet<0>();
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j) read_b(0, image, 0, j);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = wn * 16 * TN + 16 * j + l15, c = wm * 2 * TM + 2 * i + (lj >> 1);
-        *reinterpret_cast<uint2*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3) + 4 * (lj & 1)) = value(i, j);
-      }
-    __syncthreads();
-    for (int x = threadIdx.x; x < BN * CPR; x += 64 * NW) {
-      const int row = x / CPR, c = x % CPR;
-      send(row, c, *reinterpret_cast<const u4*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3)));
-    }
-  };
-  if constexpr (EPI == EPI_STORE) {
-    const float inv = g.d_scale[1];
-    if (g.out_kind == 1) {
-      uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
-      rows_out16(
-          [&](int i, int j) {
-            return make_uint2(pack2<F16>(acc[i][j][0] * inv, acc[i][j][1] * inv), pack2<F16>(acc[i][j][2] * inv, acc[i][j][3] * inv));
-          },
-          [&](int row, int c, u4 v) {
-            const int n = n0 + row, m = m0 + 8 * c;
-            if (n >= N || m >= g.M) return;
-            uint16_t* o = out + (int64_t)n * g.ldo + m;
-            if (m + 8 <= g.M) {
-              *reinterpret_cast<u4_any*>(o) = v;
-            } else {
+    for (int i = 0; i < TM; ++i) read_a(image, 0, i);
+    bool send = false;
+    for (int t = 0; t < steps; ++t) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (m + e < g.M) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
-            }
-          });
-    } else {
-      typedef float f4 __attribute__((ext_vector_type(4)));
-      typedef f4 f4_any __attribute__((aligned(4)));
-      float *lds = reinterpret_cast<float*>(smem), *out = reinterpret_cast<float*>(g.out) + (int64_t)(g.out_kind == 0 ? part : 0) * g.N * g.ldo;
-      constexpr int CPR = BM / 4, ROWS = 32 * W_N;           // 32 rows of every wave at a time
-      static_assert(ROWS * BM * 4 <= (int)sizeof(smem) && TN % 2 == 0, "a pass fits");
+      for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int j0 = 0; j0 < TN; j0 += 2) {
-        wait_and_meet<0>();
+        for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int j = j0; j < j0 + 2; ++j)
-#pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            const int row = wn * 32 + 16 * (j - j0) + l15, c = wm * 4 * TM + 4 * i + lj;
-            *reinterpret_cast<f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2)) = acc[i][j] * inv;
+          for (int j = 0; j < TN; ++j) acc[i][j] = mma<F16>(a[i], b[ks][j], acc[i][j]);
+          if (ks && i == 0) {
+            wait_and_meet<0>();                                // the next step is here, and nobody reads this image any more
+            send = more();
+            fill = image;
+            if (send) aim();
           }
-        __syncthreads();
-        for (int x = threadIdx.x; x < ROWS * CPR; x += 64 * NW) {
-          const int row = x / CPR, c = x % CPR;
-          f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2));
-          const int n = n0 + (row >> 5) * 16 * TN + 16 * j0 + (row & 31), m = m0 + 4 * c;
-          if (n >= N || m >= g.M) continue;
-          float* o = out + (int64_t)n * g.ldo + m;
-          if (m + 4 <= g.M) {
-            if (g.add) v += *reinterpret_cast<const f4_any*>(o);
-            *reinterpret_cast<f4_any*>(o) = v;
-          } else {
+          const int from = ks ? image ^ 1 : image;             // (behind the last step: old values)
+          read_a(from, ks ^ 1, i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (m + e < g.M) o[e] = g.add ? o[e] + v[e] : v[e];
+          for (int j = 0; j < TN; ++j)
+            if (j * TM / TN == i) read_b(ks ^ 1, from, ks ^ 1, j);
+          if (ks && send) {
+#pragma unroll
+            for (int e = 0; e < LOADS; ++e)
+              if (e * TM / LOADS == i) load(e);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      image ^= 1;
     }
-  } else {
-    if (g.bias) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int v = g.v0 + min(mw + 16 * i + r, g.M - 1);
-          const float bv = g.bias_f32 ? reinterpret_cast<const float*>(g.bias)[v]
-                           : F16      ? (float)reinterpret_cast<const _Float16*>(g.bias)[v]
-                                      : (float)reinterpret_cast<const __bf16*>(g.bias)[v];
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j][r] += bv;
-        }
-    }
-    constexpr float L2E = 1.44269504088896341f;                // (with |ref| below 1e37 a z of the type's lowest value gives 0)
-    const bool edge = m0 + BM > g.M;                          // classes past the last one
-    if constexpr (EPI == EPI_STATS) {
-      float2* red = reinterpret_cast<float2*>(smem);          // [W_M][BN]
+
+    // acc[i][j][r]: m = m0 + 16 (wm TM + i) + 4 lj + r, n = n0 + 16 (wn TN + j) + l15
+    const int mw = m0 + wm * 16 * TM + 4 * lj, nw = n0 + wn * 16 * TN + l15;
+    // The waves' outputs go through LDS (the images are done with), where a row n of the tile is contiguous in m, and leave as
+    // whole rows: straight from the registers every store would touch 16 rows.  16-byte chunk c of row n sits at c ^ 2 n (16-bit
+    // elements) or c ^ 4 n (floats), so that neither the writes nor the reads meet in a bank.
+    auto rows_out16 = [&](auto&& value, auto&& send_row) {         // value(i, j) -> 4 packed elements; send_row(row, chunk, 16 bytes)
+      constexpr int CPR = BM / 8;
       wait_and_meet<0>();
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = nw + 16 * j;
-        const int at = cls[j] - g.v0 - mw;                    // 16 i + r where the target's logit is ours
-        if (__any(at >= 0 && at < 16 * TM)) {
-          float hit = 0.f;
+      for (int j = 0; j < TN; ++j)
 #pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) hit = at == 16 * i + r ? acc[i][j][r] : hit;
-          if (at >= 0 && at < 16 * TM && !(at & 12)) g.target_logit[n] = hit;   // (at & 12: it is another lane's)
+        for (int i = 0; i < TM; ++i) {
+          const int row = wn * 16 * TN + 16 * j + l15, c = wm * 2 * TM + 2 * i + (lj >> 1);
+          *reinterpret_cast<uint2*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3) + 4 * (lj & 1)) = value(i, j);
         }
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (mw + 16 * i + r >= g.M) acc[i][j][r] = -INFINITY;
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float ref = top == -INFINITY ? 0.f : top;       // all of them -inf: the sum is 0, not NaN
-        float sum = 0.f;
-        if (!FINE && __all(fabsf(ref) < 1e37f)) {
-          const float neg = -ref * L2E;
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
-        } else {
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
-        }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (lj == 0) red[wm * BN + wn * 16 * TN + 16 * j + l15] = make_float2(top, sum);
-      }
       __syncthreads();
-      for (int c = threadIdx.x; c < BN; c += 64 * NW) {
-        if (n0 + c >= N) continue;
-        float2 p = red[c];
-#pragma unroll
-        for (int w = 1; w < W_M; ++w) {
-          const float2 o = red[w * BN + c];
-          const float top = fmaxf(p.x, o.x), ref = top == -INFINITY ? 0.f : top;
-          p.y = p.y * exp_fine(p.x - ref) + o.y * exp_fine(o.x - ref);
-          p.x = top;
-        }
-        g.partial[(int64_t)tm * ((g.N + ROW_PAD - 1) / ROW_PAD * ROW_PAD) + n0 + c] = p;
+      for (int x = threadIdx.x; x < BN * CPR; x += 64 * NW) {
+        const int row = x / CPR, c = x % CPR;
+        send_row(row, c, *reinterpret_cast<const u4*>(smem + row * BM + (((c ^ (2 * row)) % CPR) << 3)));
       }
-    } else {
-      const float scale = g.d_scale[0];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const float gs = gn[j] * scale, ref = lse[j];
-        const int at = cls[j] - g.v0 - mw;
-        if (!FINE && __all(fabsf(ref) < 1e37f)) {
-          const float neg = -ref * L2E;
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
-        } else {
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
-        }
-        if (__any(at >= 0 && at < 16 * TM)) {                 // the target is among this wave's classes
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (at == 16 * i + r) acc[i][j][r] -= 1.f;
-        }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] *= gs;
-        if (edge || __any(gs == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
-#pragma unroll
-          for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (gs == 0.f || mw + 16 * i + r >= g.M) acc[i][j][r] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
+    };
+    if constexpr (EPI == EPI_STORE) {
+      const float inv = g.d_scale[1];
+      if (g.out_kind == 1) {
+        uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
         rows_out16(
             [&](int i, int j) {
-              if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][0], acc[i][j][1]), pack2<F16>(acc[i][j][2], acc[i][j][3]));
-              union {
-                __bf16 t[4];
-                uint2 u;
-              } w;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {                   // the term, and what it leaves for the next
-                w.t[e] = (__bf16)acc[i][j][e];
-                acc[i][j][e] -= (float)w.t[e];
-              }
-              return w.u;
+              return make_uint2(pack2<F16>(acc[i][j][0] * inv, acc[i][j][1] * inv), pack2<F16>(acc[i][j][2] * inv, acc[i][j][3] * inv));
             },
-            [&](int row, int c, u4 v) { *reinterpret_cast<u4*>(g.d + plane * g.plane_d + (int64_t)(n0 + row) * g.ldd + m0 + 8 * c) = v; });
+            [&](int row, int c, u4 v) {
+              const int n = n0 + row, m = m0 + 8 * c;
+              if (n >= N || m >= g.M) return;
+              uint16_t* o = out + (int64_t)n * g.ldo + m;
+              if (m + 8 <= g.M) {
+                *reinterpret_cast<u4_any*>(o) = v;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (m + e < g.M) o[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+              }
+            });
+      } else {
+        typedef float f4 __attribute__((ext_vector_type(4)));
+        typedef f4 f4_any __attribute__((aligned(4)));
+        float *lds = reinterpret_cast<float*>(smem), *out = reinterpret_cast<float*>(g.out) + (int64_t)(g.out_kind == 0 ? part : 0) * g.N * g.ldo;
+        constexpr int CPR = BM / 4, ROWS = 32 * W_N;           // 32 rows of every wave at a time
+        static_assert(ROWS * BM * 4 <= (int)sizeof(smem) && TN % 2 == 0, "a pass fits");
+#pragma unroll
+        for (int j0 = 0; j0 < TN; j0 += 2) {
+          wait_and_meet<0>();
+#pragma unroll
+          for (int j = j0; j < j0 + 2; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+              const int row = wn * 32 + 16 * (j - j0) + l15, c = wm * 4 * TM + 4 * i + lj;
+              *reinterpret_cast<f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2)) = acc[i][j] * inv;
+            }
+          __syncthreads();
+          for (int x = threadIdx.x; x < ROWS * CPR; x += 64 * NW) {
+            const int row = x / CPR, c = x % CPR;
+            f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2));
+            const int n = n0 + (row >> 5) * 16 * TN + 16 * j0 + (row & 31), m = m0 + 4 * c;
+            if (n >= N || m >= g.M) continue;
+            float* o = out + (int64_t)n * g.ldo + m;
+            if (m + 4 <= g.M) {
+              if (g.add) v += *reinterpret_cast<const f4_any*>(o);
+              *reinterpret_cast<f4_any*>(o) = v;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (m + e < g.M) o[e] = g.add ? o[e] + v[e] : v[e];
+            }
+          }
+        }
+      }
+    } else {
+      if (g.bias) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int v = g.v0 + min(mw + 16 * i + r, g.M - 1);
+            const float bv = g.bias_f32 ? reinterpret_cast<const float*>(g.bias)[v]
+                             : F16      ? (float)reinterpret_cast<const _Float16*>(g.bias)[v]
+                                        : (float)reinterpret_cast<const __bf16*>(g.bias)[v];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j][r] += bv;
+          }
+      }
+      constexpr float L2E = 1.44269504088896341f;                // (with |ref| below 1e37 a z of the type's lowest value gives 0)
+      const bool edge = m0 + BM > g.M;                          // classes past the last one
+      if constexpr (EPI == EPI_STATS) {
+        float2* red = reinterpret_cast<float2*>(smem + STAGES * STAGE);          // [W_M][BN]
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int n = nw + 16 * j;
+          const int at = cls[j] - g.v0 - mw;                    // 16 i + r where the target's logit is ours
+          if (__any(at >= 0 && at < 16 * TM)) {
+            float hit = 0.f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) hit = at == 16 * i + r ? acc[i][j][r] : hit;
+            if (at >= 0 && at < 16 * TM && !(at & 12)) g.target_logit[n] = hit;   // (at & 12: it is another lane's)
+          }
+          if (edge) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (mw + 16 * i + r >= g.M) acc[i][j][r] = -INFINITY;
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float ref = top == -INFINITY ? 0.f : top;       // all of them -inf: the sum is 0, not NaN
+          float sum = 0.f;
+          if (!FINE && __all(fabsf(ref) < 1e37f)) {
+            const float neg = -ref * L2E;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+          } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sum += FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+          }
+          sum += __shfl_xor(sum, 16, 64);
+          sum += __shfl_xor(sum, 32, 64);
+          if (lj == 0) red[wm * BN + wn * 16 * TN + 16 * j + l15] = make_float2(top, sum);
+        }
+        wait_and_meet<63>();
+        for (int c = threadIdx.x; c < BN; c += 64 * NW) {
+          if (n0 + c >= N) continue;
+          float2 p = red[c];
+#pragma unroll
+          for (int w = 1; w < W_M; ++w) {
+            const float2 o = red[w * BN + c];
+            const float top = fmaxf(p.x, o.x), ref = top == -INFINITY ? 0.f : top;
+            p.y = p.y * exp_fine(p.x - ref) + o.y * exp_fine(o.x - ref);
+            p.x = top;
+          }
+          g.partial[(int64_t)(m0 / BM) * ((g.N + ROW_PAD - 1) / ROW_PAD * ROW_PAD) + n0 + c] = p;
+        }
+      } else {
+        const float scale = g.d_scale[0];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const float gs = gn[j] * scale, ref = lse[j];
+          const int at = cls[j] - g.v0 - mw;
+          if (!FINE && __all(fabsf(ref) < 1e37f)) {
+            const float neg = -ref * L2E;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], L2E, neg));
+          } else {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][r] = FINE ? exp_fine(acc[i][j][r] - ref) : __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * L2E);
+          }
+          if (__any(at >= 0 && at < 16 * TM)) {                 // the target is among this wave's classes
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (at == 16 * i + r) acc[i][j][r] -= 1.f;
+          }
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][r] *= gs;
+          if (edge || __any(gs == 0.f)) {                       // rows without a gradient and classes past the end: exactly zero
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (gs == 0.f || mw + 16 * i + r >= g.M) acc[i][j][r] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
+          rows_out16(
+              [&](int i, int j) {
+                if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][0], acc[i][j][1]), pack2<F16>(acc[i][j][2], acc[i][j][3]));
+                union {
+                  __bf16 t[4];
+                  uint2 u;
+                } w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {                   // the term, and what it leaves for the next
+                  w.t[e] = (__bf16)acc[i][j][e];
+                  acc[i][j][e] -= (float)w.t[e];
+                }
+                return w.u;
+              },
+              [&](int row, int c, u4 v) { *reinterpret_cast<u4*>(g.d + plane * g.plane_d + (int64_t)(n0 + row) * g.ldd + m0 + 8 * c) = v; });
+      }
     }
+    if (!STAY) return;
+    offsets();                                                  // (formed again rather than held through the epilogue)
   }
 }
 
@@ -1138,7 +1161,9 @@ template <bool F16, bool A_KC, bool B_KC, int EPI, bool FINE> void launch_gemm(G
   const int b = big ? 256 : 128;
   g.tiles_m = (g.M + b - 1) / b;
   g.tiles_n = (g.N + b - 1) / b;
-  const uint32_t grid = (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
+  uint32_t grid = (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
+  const uint32_t resident = big ? 256 : 512;
+  if (EPI == EPI_STATS && grid > resident) grid = resident;                    // workgroups that stay, as many as are resident
   if (big) head_gemm_kernel<F16, A_KC, B_KC, 256, 256, 2, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);
   else head_gemm_kernel<F16, A_KC, B_KC, 128, 128, 2, 2, EPI, FINE><<<grid, 256, 0, st>>>(g);
 }
