@@ -620,16 +620,53 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
   }
 }
 
+// g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to); by one workgroup
+struct Upstream {
+  const float* up;                                            // null: nothing to do
+  const int* state;
+  int reduction, N;
+  const float* cw;
+  float to;
+  float *g, *d_scale;
+};
+__device__ __forceinline__ void upstream(const Upstream& u) {
+  __shared__ float red[16];
+  const int kept = u.state[S_KEPT];
+  const float total = reinterpret_cast<const float*>(u.state)[S_TOTAL];
+  float top = 0.f;
+  for (int i = threadIdx.x; i < kept; i += 1024) {
+    const int orig = u.state[S_ROWS + i], t = u.state[S_ROWS + u.N + i];
+    float v = u.reduction == VAE_CE_NONE ? u.up[orig] : u.up[0];
+    if (t < 0) v = NAN;
+    else if (u.cw) v *= u.cw[t];
+    if (u.reduction == VAE_CE_MEAN) v /= total;
+    u.g[i] = v;
+    top = fmaxf(top, fabsf(v));
+  }
+  top = block_max<16>(top, red);
+  if (threadIdx.x == 0) {
+    const bool usable = top > 1e-30f && top < INFINITY;       // (nothing to do without a gradient; infinities reach the result)
+    u.d_scale[0] = usable ? u.to / top : 1.f;
+    u.d_scale[1] = usable ? top / u.to : 1.f;
+  }
+}
+
 // out[i][0 .. ldo) = src[rows[i]][0 .. D), zeros behind the last column and the last kept row (up to whole tiles): 8 elements
 // per thread; T = float: three bf16 planes
-template <typename T>
-__global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ src, int64_t ld, int D, const int* __restrict__ state,
-                                                      int n_rows, uint16_t* __restrict__ out, int64_t ldo, int64_t plane) {
+struct Pack {
+  const void* src;
+  int64_t ld;
+  const int* state;                                           // null: all rows as they are
+  int rows, blocks;
+  uint16_t* out;
+  int64_t plane;
+};
+template <typename T> __device__ __forceinline__ void pack_rows(const Pack& p, int block, int D, int64_t ldo) {
   const int per = (int)(ldo / 8);
-  const int kept = state ? state[S_KEPT] : n_rows;
-  const int padded = state ? (kept + ROW_PAD - 1) / ROW_PAD * ROW_PAD : n_rows;
+  const int kept = p.state ? p.state[S_KEPT] : p.rows;
+  const int padded = p.state ? (kept + ROW_PAD - 1) / ROW_PAD * ROW_PAD : p.rows;
   const int64_t all = (int64_t)padded * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = (int64_t)block * 1024 + threadIdx.x; i < all; i += (int64_t)p.blocks * 1024) {
     const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 8;
     constexpr int Q = sizeof(T) / 2;
     union {
@@ -639,17 +676,17 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ src,
 #pragma unroll
     for (int q = 0; q < Q; ++q) v.q[q] = (u4)0;
     if (row < kept) {
-      const T* p = src + (int64_t)(state ? state[S_ROWS + row] : row) * ld + c;
+      const T* from = reinterpret_cast<const T*>(p.src) + (int64_t)(p.state ? p.state[S_ROWS + row] : row) * p.ld + c;
       if (c + 8 <= D) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) v.q[q] = reinterpret_cast<const u4_any*>(p)[q];
+        for (int q = 0; q < Q; ++q) v.q[q] = reinterpret_cast<const u4_any*>(from)[q];
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (c + j < D) v.t[j] = p[j];
+          if (c + j < D) v.t[j] = from[j];
       }
     }
-    uint16_t* o = out + (int64_t)row * ldo + c;
+    uint16_t* o = p.out + (int64_t)row * ldo + c;
     if constexpr (sizeof(T) == 4) {
       union {
         __bf16 t[8];
@@ -658,11 +695,18 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(const T* __restrict__ src,
 #pragma unroll
       for (int j = 0; j < 8; ++j) split3(v.t[j], w[0].t[j], w[1].t[j], w[2].t[j]);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) *reinterpret_cast<u4*>(o + k * plane) = w[k].q;
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u4*>(o + k * p.plane) = w[k].q;
     } else {
       *reinterpret_cast<u4*>(o) = v.q[0];
     }
   }
+}
+// All that comes ahead of the products, in one launch: the row factors, x, and w where it has to be packed.
+template <typename T> __global__ __launch_bounds__(1024) void ce_pack_kernel(Upstream u, Pack x, Pack w, int D, int64_t ldo) {
+  int block = blockIdx.x;
+  if (u.up && block-- == 0) upstream(u);
+  else if (block < x.blocks) pack_rows<T>(x, block, D, ldo);
+  else pack_rows<T>(w, block - x.blocks, D, ldo);
 }
 
 // the partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row
@@ -720,31 +764,6 @@ __global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict
     s = 0;
     for (int i = 0; i < 16; ++i) s += red[i];
     *loss = (float)(mean ? s / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : s);
-  }
-}
-
-// g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to)
-__global__ __launch_bounds__(1024) void ce_upstream_kernel(const float* __restrict__ up, int reduction, const int* __restrict__ state, int N,
-                                                           const float* __restrict__ cw,
-                                                           float to, float* __restrict__ g, float* __restrict__ d_scale) {
-  __shared__ float red[16];
-  const int kept = state[S_KEPT];
-  const float total = reinterpret_cast<const float*>(state)[S_TOTAL];
-  float top = 0.f;
-  for (int i = threadIdx.x; i < kept; i += 1024) {
-    const int orig = state[S_ROWS + i], t = state[S_ROWS + N + i];
-    float v = reduction == VAE_CE_NONE ? up[orig] : up[0];
-    if (t < 0) v = NAN;
-    else if (cw) v *= cw[t];
-    if (reduction == VAE_CE_MEAN) v /= total;
-    g[i] = v;
-    top = fmaxf(top, fabsf(v));
-  }
-  top = block_max<16>(top, red);
-  if (threadIdx.x == 0) {
-    const bool usable = top > 1e-30f && top < INFINITY;       // (nothing to do without a gradient; infinities reach the result)
-    d_scale[0] = usable ? to / top : 1.f;
-    d_scale[1] = usable ? top / to : 1.f;
   }
 }
 
@@ -1180,12 +1199,16 @@ void add_slabs(const float* slabs, int S, int64_t slab, int64_t n, void* out, in
   else ce_dw_kernel<_Float16><<<grid, 256, 0, st>>>(slabs, S, slab, n, (_Float16*)out);
 }
 
-void pack(const void* src, int64_t ld, int64_t D, const int* state, int64_t rows, int64_t padded, uint16_t* out, int64_t ldo, int64_t plane,
-          int dtype, hipStream_t st) {
-  const int64_t work = padded * (ldo / 8) / 256 + 1;
-  const int grid = (int)(work < 4096 ? work : 4096);
-  if (dtype == VAE_ADAMW_F32) ce_pack_kernel<float><<<grid, 256, 0, st>>>((const float*)src, ld, (int)D, state, (int)rows, out, ldo, plane);
-  else ce_pack_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t*)src, ld, (int)D, state, (int)rows, out, ldo, plane);
+void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, const Upstream& u, hipStream_t st) {
+  auto blocks = [&](int64_t rows) {
+    const int64_t b = (rows * (p.d_pad / 8) + 1023) / 1024;
+    return (int)(b < 1024 ? b : 1024);
+  };
+  const Pack x = {a->x, a->ldx, state, (int)a->N, blocks(p.n_pad), reinterpret_cast<uint16_t*>(ws + p.x), p.n_pad * p.d_pad};
+  const Pack w = {a->w, a->ldw, nullptr, (int)a->V, p.pack_w ? blocks(a->V) : 0, reinterpret_cast<uint16_t*>(ws + p.w), a->V * p.d_pad};
+  const int grid = (u.up ? 1 : 0) + x.blocks + w.blocks;
+  if (p.f32) ce_pack_kernel<float><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
+  else ce_pack_kernel<uint16_t><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
 }
 
 int check(const vae_linear_ce* a, const char* who) {
@@ -1258,8 +1281,7 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   float* by_row = reduction == VAE_CE_NONE ? loss : nullptr;
   ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, by_row);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
-  pack(a->x, a->ldx, a->D, s, a->N, p.n_pad, reinterpret_cast<uint16_t*>(ws + p.x), p.d_pad, p.n_pad * p.d_pad, a->dtype, st);
-  if (p.pack_w) pack(a->w, a->ldw, a->D, nullptr, a->V, a->V, reinterpret_cast<uint16_t*>(ws + p.w), p.d_pad, a->V * p.d_pad, a->dtype, st);
+  pack(a, p, ws, s, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   Gemm g = logits_gemm(a, p, ws, s);
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
@@ -1300,10 +1322,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
-  ce_upstream_kernel<<<1, 1024, 0, st>>>(grad, reduction, s, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale);
-  VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
-  pack(a->x, a->ldx, a->D, s, a->N, p.n_pad, xp, p.d_pad, p.n_pad * p.d_pad, a->dtype, st);
-  if (p.pack_w) pack(a->w, a->ldw, a->D, nullptr, a->V, a->V, reinterpret_cast<uint16_t*>(ws + p.w), p.d_pad, a->V * p.d_pad, a->dtype, st);
+  pack(a, p, ws, s, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
   for (int64_t v0 = 0; v0 < a->V; v0 += p.piece) {
     const int64_t n_v = a->V - v0 < p.piece ? a->V - v0 : p.piece;
