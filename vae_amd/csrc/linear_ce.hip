@@ -67,6 +67,7 @@ struct Gemm {
   const float* d_scale;         // what d is multiplied by, and its reciprocal
   uint16_t* d;                  // [N padded][ldd], planes at plane_d
   int64_t ldd, plane_d;
+  float* d_sums;                // null, or (tile_n, ldd): sums of d over a tile's rows
   // EPI_STORE: out[n][m], final type or float slabs (split, N, M) that are added to when `add`
   void* out;
   int64_t ldo;
@@ -89,6 +90,17 @@ __device__ __forceinline__ float exp_fine(float v) {
   r = fmaf(v, 1.925963033500011e-8f, r);
   const float e = __builtin_amdgcn_exp2f(t);
   return fmaf(e, r * 0.69314718055994531f, e);
+}
+
+// sum over 16 consecutive lanes, in all of them
+template <int CTRL> __device__ __forceinline__ float dpp_f(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v += dpp_f<0xB1>(v);                                        // quad_perm [1, 0, 3, 2]
+  v += dpp_f<0x4E>(v);                                        // quad_perm [2, 3, 0, 1]
+  v += dpp_f<0x124>(v);                                       // row_ror:4
+  return v + dpp_f<0x128>(v);                                 // row_ror:8
 }
 
 // One wave instruction: lane i copies 16 bytes from base + off_i to LDS byte lds + 16 i.  In inline asm so that the compiler
@@ -534,8 +546,29 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
                 if (gs == 0.f || mw + 16 * i + r >= g.M) acc[i][j][r] = 0.f;
           }
         }
+      if (g.d_sums) {                                         // (of d as it is, before its rounding)
+        float* red = reinterpret_cast<float*>(smem);          // [W_N][BM]
+        wait_and_meet<0>();
 #pragma unroll
-        for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) s += acc[i][j][r];
+            s = row16_sum(s);
+            if (l15 == 0) red[wn * BM + wm * 16 * TM + 16 * i + 4 * lj + r] = s;
+          }
+        wait_and_meet<0>();
+        for (int c = threadIdx.x; c < BM; c += 64 * NW) {
+          float s = 0.f;
+#pragma unroll
+          for (int w = 0; w < W_N; ++w) s += red[w * BM + c];
+          g.d_sums[(int64_t)(n0 / BN) * g.ldd + m0 + c] = s;
+        }
+      }
+#pragma unroll
+      for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
           rows_out16(
               [&](int i, int j) {
                 if constexpr (!FINE) return make_uint2(pack2<F16>(acc[i][j][0], acc[i][j][1]), pack2<F16>(acc[i][j][2], acc[i][j][3]));
@@ -807,7 +840,7 @@ __global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ sl
   }
 }
 
-// dW or db of one piece of classes: the slabs added in order
+// dW of one piece of classes: the slabs added in order
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ slabs, int S, int64_t slab, int64_t n, T* __restrict__ dw) {
   typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -827,40 +860,32 @@ __global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ sl
   }
 }
 
-// db[v] = sum over the kept rows of d, of the y-th of gridDim.y runs of rows: 256 classes to a workgroup, 8 per thread, 32 rows
-// at a time, whose sums are added in order.  One run: the result; several: slabs (runs, classes in whole blocks) for ce_dw_kernel to add.
-template <int KIND>   // 0: three bf16 planes -> float, 1: bf16, 2: fp16
-__global__ __launch_bounds__(1024) void ce_bias_kernel(const uint16_t* __restrict__ d, int64_t ldd, int64_t plane, const int* __restrict__ state,
-                                                       int V, const float* __restrict__ d_scale, float* __restrict__ slabs, void* __restrict__ out) {
-  __shared__ float red[32][257];
-  const int v = blockIdx.x * 256 + (threadIdx.x & 31) * 8, r = threadIdx.x >> 5, kept = state[S_KEPT];
-  const int run = (kept + (int)gridDim.y - 1) / (int)gridDim.y, end = min((int)(blockIdx.y + 1) * run, kept);
-  float s[8] = {};
-  for (int n = blockIdx.y * run + r; n < end; n += 32) {
+// db[v] = the sums of d over the rows of every tile, added up: 64 classes to a workgroup of 16 waves, each of which adds every
+// 16th tile, eight loads in flight; the 16 sums are added in order
+template <typename T>
+__global__ __launch_bounds__(1024) void ce_bias_kernel(const float* __restrict__ sums, int64_t ld, const int* __restrict__ state, int rows, int V,
+                                                       const float* __restrict__ d_scale, T* __restrict__ out) {
+  __shared__ float red[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, tiles = (state[S_KEPT] + rows - 1) / rows;
+  float s = 0.f;
+  if (c < V) {
+    const float* p = sums + c;
+    int t = w;
+    for (; t + 7 * 16 < tiles; t += 8 * 16) {
+      float v[8];
 #pragma unroll
-    for (int k = 0; k < (KIND == 0 ? 3 : 1); ++k) {          // (d is padded to whole tiles of classes)
-      const u4 q = *reinterpret_cast<const u4*>(d + k * plane + (int64_t)n * ldd + v);
+      for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)(t + 16 * i) * ld];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint16_t b = (uint16_t)(q[j >> 1] >> (16 * (j & 1)));
-        if (KIND == 2) s[j] += (float)__builtin_bit_cast(_Float16, b);
-        else s[j] += (float)__builtin_bit_cast(__bf16, b);
-      }
+      for (int i = 0; i < 8; ++i) s += v[i];
     }
+    for (; t < tiles; t += 16) s += p[(int64_t)t * ld];
   }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) red[r][(threadIdx.x & 31) * 8 + j] = s[j];
+  red[w][threadIdx.x & 63] = s;
   __syncthreads();
-  const int c = threadIdx.x, at = blockIdx.x * 256 + c;
-  if (c >= 256) return;
-  float t = 0.f;
-  for (int i = 0; i < 32; ++i) t += red[i][c];
-  t *= d_scale[1];
-  if (gridDim.y > 1) slabs[(int64_t)blockIdx.y * gridDim.x * 256 + at] = t;
-  else if (at >= V) return;
-  else if (KIND == 0) reinterpret_cast<float*>(out)[at] = t;
-  else if (KIND == 1) reinterpret_cast<__bf16*>(out)[at] = (__bf16)t;
-  else reinterpret_cast<_Float16*>(out)[at] = (_Float16)t;
+  if (w || c >= V) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+  out[c] = (T)(s * d_scale[1]);
 }
 
 // ---- heads of at most 64 classes on at most 64 columns, few rows: the whole pass in one workgroup ----
@@ -1115,14 +1140,6 @@ Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool a
   return best;
 }
 
-// runs of rows that the bias gradient of `wide` blocks of 256 classes is summed in: enough for two workgroups to a CU, of 128
-// rows at least
-int64_t bias_runs(int64_t n, int64_t wide) {
-  int64_t r = 512 / wide;
-  if (r > n / 128) r = n / 128;
-  return r < 1 ? 1 : r;
-}
-
 struct Plan {
   bool f32, pack_w;
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
@@ -1130,7 +1147,7 @@ struct Plan {
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
   Tiles z_tiles, d_tiles, dx_tiles, dw_tiles;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, nll, g, scale, d, slabs, slabs_w, slabs_b, bytes;
+  int64_t x, w, partial, tlogit, nll, g, scale, d, d_sums, slabs, slabs_w, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
@@ -1170,7 +1187,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
     p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
     p.slabs_w = take(p.dw_tiles.split > 1 ? (int64_t)p.dw_tiles.split * p.piece * a->D * 4 : 0);
-    p.slabs_b = take(a->bias ? 512 * 256 * 4 : 0);           // bias_runs() * blocks <= 512
+    p.d_sums = take(a->bias ? p.n_pad / (p.d_tiles.big ? 256 : 128) * p.piece * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -1319,7 +1336,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   const int* s = reinterpret_cast<const int*>(state);
   hipStream_t st = (hipStream_t)stream;
-  float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs);
+  float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs), *sums = reinterpret_cast<float*>(ws + p.d_sums);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
   pack(a, p, ws, s, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
@@ -1337,6 +1354,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.d = d;
     z.ldd = p.piece;
     z.plane_d = plane_d;
+    z.d_sums = dbias ? sums : nullptr;
     gemm<true, true, EPI_D>(z, a->dtype, p.d_tiles.big, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     if (dx) {                                           // dx (N, D) += d (N, n_v) W (n_v, D)
@@ -1389,14 +1407,13 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
     if (dbias) {
-      const int64_t wide = (n_v + 255) / 256;
-      const dim3 grid((unsigned)wide, (unsigned)bias_runs(a->N, wide));
-      void* o = reinterpret_cast<uint8_t*>(dbias) + v0 * esize;
-      float* sb = reinterpret_cast<float*>(ws + p.slabs_b);
-      if (p.f32) ce_bias_kernel<0><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
-      else if (a->dtype == VAE_ADAMW_BF16) ce_bias_kernel<1><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
-      else ce_bias_kernel<2><<<grid, 1024, 0, st>>>(d, p.piece, plane_d, s, (int)n_v, scale, sb, o);
-      if (grid.y > 1) add_slabs(sb, (int)grid.y, wide * 256, n_v, o, a->dtype, st);
+      const unsigned grid = (unsigned)((n_v + 63) / 64);
+      const int rows = p.d_tiles.big ? 256 : 128;
+#define VAE_DB(T) ce_bias_kernel<T><<<grid, 1024, 0, st>>>(sums, p.piece, s, rows, (int)n_v, scale, (T*)dbias + v0)
+      if (p.f32) VAE_DB(float);
+      else if (a->dtype == VAE_ADAMW_BF16) VAE_DB(__bf16);
+      else VAE_DB(_Float16);
+#undef VAE_DB
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     }
   }
