@@ -42,7 +42,7 @@ constexpr int ROW_PAD = 256;                            // packed rows and colum
 constexpr int K_PAD = 64;
 
 // the state of a forward pass that the backward pass reads: int32 / float words
-constexpr int S_KEPT = 0, S_TOTAL = 1, S_ROWS = 4;      // kept rows, sum of c[t]; row index, class (-1: none) and lse, N each, of the kept rows
+constexpr int S_KEPT = 0, S_TOTAL = 1, S_DONE = 2, S_ROWS = 4;   // kept rows, sum of c[t], finished workgroups; row index, class (-1: none) and lse, N each, of the kept rows
 
 enum { EPI_STATS = 0, EPI_D = 1, EPI_STORE = 2 };
 
@@ -146,8 +146,9 @@ __device__ __forceinline__ int rc_swizzle(int k) { return (k & 3) << 2 | (k >> 3
 // slower), what a tile starts and ends with 8 to 12 us.
 // Rows and columns of A past its end are clamped to the last one (their products are not stored, or meet zeros in B); B is a
 // packed operand, padded with zeros to whole tiles.
+constexpr int lds_elements(int bm, int bn, int w_m, int epi) { return 2 * 64 * (bm + bn) + (epi == EPI_STATS ? w_m * bn * 4 : 0); }
 template <bool F16, bool A_KC, bool B_KC, int BM, int BN, int W_M, int W_N, int EPI, bool FINE>
-__global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
+__device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int blocks) {
   constexpr int BK = 64, STAGES = 2;
   constexpr int NW = W_M * W_N, TM = BM / (16 * W_M), TN = BN / (16 * W_N);
   constexpr int IMG_A = BM * BK, IMG_B = BN * BK, STAGE = IMG_A + IMG_B;          // elements
@@ -156,8 +157,6 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   // Workgroups whose epilogue leaves the images alone stay for several tiles and send for the next one's first steps during the
   // last ones of the tile before: 250 -> 242 us for 4093 x 1000 x 30011, 473 -> 464 for 2048 x 2048 x 65536.
   constexpr bool STAY = EPI == EPI_STATS;
-  __shared__ __attribute__((aligned(16))) uint16_t smem[STAGES * STAGE + (STAY ? W_M * BN * 4 : 0)];
-
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / W_N, wn = wave % W_N, l15 = lane & 15, lj = lane >> 4;
 
@@ -173,10 +172,10 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   const int total = g.tiles_m * tiles_n;
   int id, end, turn;
   {
-    const int all = total * g.split, q8 = all >> 3, r8 = all & 7, xcd = blockIdx.x & 7, beg = xcd * q8 + min(xcd, r8);
-    id = beg + ((int)blockIdx.x >> 3);
+    const int all = total * g.split, q8 = all >> 3, r8 = all & 7, xcd = block & 7, beg = xcd * q8 + min(xcd, r8);
+    id = beg + (block >> 3);
     end = beg + q8 + (xcd < r8 ? 1 : 0);
-    turn = ((int)gridDim.x + 7 - xcd) >> 3;
+    turn = (blocks + 7 - xcd) >> 3;
   }
   if (id >= end) return;
   const int part = id / total;                               // of K (which is split only where a workgroup has one tile)
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
         typedef f4 f4_any __attribute__((aligned(4)));
         float *lds = reinterpret_cast<float*>(smem), *out = reinterpret_cast<float*>(g.out) + (int64_t)(g.out_kind == 0 ? part : 0) * g.N * g.ldo;
         constexpr int CPR = BM / 4, ROWS = 32 * W_N;           // 32 rows of every wave at a time
-        static_assert(ROWS * BM * 4 <= (int)sizeof(smem) && TN % 2 == 0, "a pass fits");
+        static_assert(ROWS * BM * 2 <= STAGES * STAGE && TN % 2 == 0, "a pass fits");
 #pragma unroll
         for (int j0 = 0; j0 < TN; j0 += 2) {
           wait_and_meet<0>();
@@ -591,6 +590,20 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_gemm_kernel(Gemm g) {
   }
 }
 
+template <bool F16, int BM, int BN, int W_M, int W_N, int EPI, bool FINE>
+__global__ __launch_bounds__(64 * W_M * W_N, 2) void head_logits_kernel(Gemm g) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem[lds_elements(BM, BN, W_M, EPI)];
+  head_gemm<F16, true, true, BM, BN, W_M, W_N, EPI, FINE>(g, smem, blockIdx.x, gridDim.x);
+}
+// dx and dW of a piece of classes, in one launch: neither fills the chip to its end.  `dx_blocks`: a multiple of 8
+template <bool F16, int BM, int BN, int W_M, int W_N>
+__global__ __launch_bounds__(64 * W_M * W_N, 2) void head_grads_kernel(Gemm dx, Gemm dw, int dx_blocks) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem[lds_elements(BM, BN, W_M, EPI_STORE)];
+  const int block = blockIdx.x;
+  if (block < dx_blocks) head_gemm<F16, false, true, BM, BN, W_M, W_N, EPI_STORE, false>(dx, smem, block, dx_blocks);
+  else head_gemm<F16, false, false, BM, BN, W_M, W_N, EPI_STORE, false>(dw, smem, block - dx_blocks, (int)gridDim.x - dx_blocks);
+}
+
 // Rows that count, in order: rows[0 .. kept), kept, and the sum of their class weights, by one workgroup (8192 targets at a
 // time, 8 per thread).  An ignored row's loss is written as 0 where losses are returned by row.
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict__ target, int N, int V, int64_t ignore,
@@ -649,6 +662,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
     double w = 0;
     for (int i = 0; i < 16; ++i) w += wave_w[i];
     state[S_KEPT] = before;
+    state[S_DONE] = 0;
     reinterpret_cast<float*>(state)[S_TOTAL] = (float)w;
   }
 }
@@ -742,14 +756,17 @@ template <typename T> __global__ __launch_bounds__(1024) void ce_pack_kernel(Ups
   else pack_rows<T>(w, block - x.blocks, D, ldo);
 }
 
-// the partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row
-__global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restrict__ partial, int tiles, int64_t ldp,
-                                                         int* __restrict__ state, int N, const float* __restrict__ cw, const float* __restrict__ target_logit,
-                                                         float* __restrict__ nll, float* __restrict__ loss_rows) {
+// The partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row.
+// Sum and mean: the workgroup that finishes last adds up what all of them left, in order (same bits every time).
+__global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restrict__ partial, int tiles, int64_t ldp, int* __restrict__ state,
+                                                         int N, const float* __restrict__ cw, const float* __restrict__ target_logit,
+                                                         int reduction, double* __restrict__ sums, float* __restrict__ loss) {
   __shared__ float2 red[8][32];
-  const int kept = state[S_KEPT];
+  __shared__ double red64[4];
+  __shared__ bool last;
+  const int kept = state[S_KEPT], blocks = max((kept + 31) / 32, 1);
   const int row = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
-  if (blockIdx.x * 32 >= kept) return;
+  if ((int)blockIdx.x >= blocks) return;
   float top = -INFINITY, sum = 0.f;
   if (row < kept) {
     for (int t = part; t < tiles; t += 64) {                  // eight loads in flight
@@ -768,124 +785,146 @@ __global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restric
   }
   red[part][threadIdx.x & 31] = make_float2(top, sum);
   __syncthreads();
-  if (part || row >= kept) return;
-  float m = top;
+  double share = 0;
+  if (part == 0 && row < kept) {
+    float m = top;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i][threadIdx.x].x);
-  const float ref = m == -INFINITY ? 0.f : m;
-  sum = 0.f;
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i][threadIdx.x].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum += red[i][threadIdx.x].y * exp_fine(red[i][threadIdx.x].x - ref);
-  const float lse = m + logf(sum);
-  reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
-  const int orig = state[S_ROWS + row], t = state[S_ROWS + N + row];
-  const float v = (lse - target_logit[row]) * (!cw || t < 0 ? 1.f : cw[t]);
-  if (loss_rows) loss_rows[orig] = v;
-  else nll[row] = v;
-}
-__global__ __launch_bounds__(1024) void ce_reduce_kernel(const float* __restrict__ nll, const int* __restrict__ state, int mean,
-                                                         float* __restrict__ loss) {
-  __shared__ double red[16];
-  const int kept = state[S_KEPT];
-  double s = 0;
-  for (int i = threadIdx.x; i < kept; i += 1024) s += (double)nll[i];
+    for (int i = 0; i < 8; ++i) sum += red[i][threadIdx.x].y * exp_fine(red[i][threadIdx.x].x - ref);
+    const float lse = m + logf(sum);
+    reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
+    const int orig = state[S_ROWS + row], t = state[S_ROWS + N + row];
+    const float v = (lse - target_logit[row]) * (!cw || t < 0 ? 1.f : cw[t]);
+    if (reduction == VAE_CE_NONE) loss[orig] = v;
+    share = (double)v;
+  }
+  if (reduction == VAE_CE_NONE) return;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  for (int o = 32; o > 0; o >>= 1) share += __shfl_xor(share, o, 64);
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(sums + blockIdx.x, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(state + S_DONE, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  share = 0;
+  for (int i = threadIdx.x; i < blocks; i += 256) share += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) share += __shfl_xor(share, o, 64);
+  if ((threadIdx.x & 63) == 0) red64[threadIdx.x >> 6] = share;
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = 0;
-    for (int i = 0; i < 16; ++i) s += red[i];
-    *loss = (float)(mean ? s / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : s);
+    share = ((red64[0] + red64[1]) + red64[2]) + red64[3];
+    *loss = (float)(reduction == VAE_CE_MEAN ? share / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : share);
   }
 }
 
-// dx: the slabs (S, N, D) of a packed row added in order and put at its original row; ignored rows are zero.  A workgroup per
-// row, four columns per thread.
-template <typename T>
-__global__ __launch_bounds__(256) void ce_dx_kernel(const float* __restrict__ slabs, int S, int64_t slab, int N, int D,
-                                                    const int* __restrict__ state, const int64_t* __restrict__ target, int64_t ignore,
-                                                    T* __restrict__ dx) {
-  typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
-  const int kept = state[S_KEPT];
-  for (int row = blockIdx.x; row < kept; row += gridDim.x) {
-    T* o = dx + (int64_t)state[S_ROWS + row] * D;
-    const float* p = slabs + (int64_t)row * D;
-    for (int c = threadIdx.x * 4; c < D; c += 1024) {
-      if (c + 4 <= D) {
-        f4_any s = {0.f, 0.f, 0.f, 0.f};
-        int k = 0;
-        for (; k + 4 <= S; k += 4) {
-          f4_any v[4];
+// What is left behind the products of a piece, in one launch:
+//   db: the sums of d over the rows of every tile, added up.  64 classes to a workgroup of 4 waves, each of which adds every
+//       4th tile, eight loads in flight; the 4 sums are added in order
+//   dW: its slabs, where there are several, added in order
+//   dx: behind the last piece, the slabs (S, N, D) of a packed row added in order and put at its original row; ignored rows are
+//       zero.  A workgroup per row, four columns per thread
+struct Finish {
+  int db_blocks, dw_blocks, dx_blocks;
+  const int* state;
+  const float* d_scale;
+  const float* sums;
+  int64_t ld_sums;
+  int sum_rows, V;
+  void* db;
+  const float* dw_slabs;
+  int dw_split;
+  int64_t dw_n;
+  void* dw;
+  const float* dx_slabs;
+  int dx_split, N, D;
+  const int64_t* target;
+  int64_t ignore;
+  void* dx;
+};
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f4_any slab_sum(const float* p, int S, int64_t slab) {
+  f4_any s = {0.f, 0.f, 0.f, 0.f};
+  int k = 0;
+  for (; k + 4 <= S; k += 4) {
+    f4_any v[4];
 #pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f4_any*>(p + (k + u) * slab + c);
+    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f4_any*>(p + (k + u) * slab);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) s += v[u];
-        }
-        for (; k < S; ++k) s += *reinterpret_cast<const f4_any*>(p + k * slab + c);
+    for (int u = 0; u < 4; ++u) s += v[u];
+  }
+  for (; k < S; ++k) s += *reinterpret_cast<const f4_any*>(p + k * slab);
+  return s;
+}
+__device__ __forceinline__ float slab_sum1(const float* p, int S, int64_t slab) {
+  float s = 0.f;
+  for (int k = 0; k < S; ++k) s += p[k * slab];
+  return s;
+}
+template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(Finish f) {
+  __shared__ float red[4][64];
+  int block = blockIdx.x;
+  const int kept = f.state[S_KEPT];
+  if (block < f.db_blocks) {
+    const int c = block * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, tiles = (kept + f.sum_rows - 1) / f.sum_rows;
+    float s = 0.f;
+    if (c < f.V) {
+      const float* p = f.sums + c;
+      int t = w;
+      for (; t + 7 * 4 < tiles; t += 8 * 4) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)(t + 4 * i) * f.ld_sums];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+      }
+      for (; t < tiles; t += 4) s += p[(int64_t)t * f.ld_sums];
+    }
+    red[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w || c >= f.V) return;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) s += red[i][threadIdx.x];
+    reinterpret_cast<T*>(f.db)[c] = (T)(s * f.d_scale[1]);
+    return;
+  }
+  block -= f.db_blocks;
+  if (block < f.dw_blocks) {
+    T* dw = reinterpret_cast<T*>(f.dw);
+    for (int64_t i = ((int64_t)block * 256 + threadIdx.x) * 4; i < f.dw_n; i += (int64_t)f.dw_blocks * 1024) {
+      if (i + 4 <= f.dw_n) {
+        const f4_any s = slab_sum(f.dw_slabs + i, f.dw_split, f.dw_n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dw[i + e] = (T)s[e];
+      } else {
+        for (int64_t e = i; e < f.dw_n; ++e) dw[e] = (T)slab_sum1(f.dw_slabs + e, f.dw_split, f.dw_n);
+      }
+    }
+    return;
+  }
+  block -= f.dw_blocks;
+  const int64_t slab = (int64_t)f.N * f.D;
+  for (int row = block; row < kept; row += f.dx_blocks) {
+    T* o = reinterpret_cast<T*>(f.dx) + (int64_t)f.state[S_ROWS + row] * f.D;
+    const float* p = f.dx_slabs + (int64_t)row * f.D;
+    for (int c = threadIdx.x * 4; c < f.D; c += 1024) {
+      if (c + 4 <= f.D) {
+        const f4_any s = slab_sum(p + c, f.dx_split, slab);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[c + e] = (T)s[e];
       } else {
-        for (int e = c; e < D; ++e) {
-          float s = 0.f;
-          for (int k = 0; k < S; ++k) s += p[k * slab + e];
-          o[e] = (T)s;
-        }
+        for (int e = c; e < f.D; ++e) o[e] = (T)slab_sum1(p + e, f.dx_split, slab);
       }
     }
   }
-  for (int row = blockIdx.x; row < N; row += gridDim.x) {
-    if (target[row] != ignore) continue;
-    for (int c = threadIdx.x; c < D; c += 256) dx[(int64_t)row * D + c] = (T)0;
+  for (int row = block; row < f.N; row += f.dx_blocks) {
+    if (f.target[row] != f.ignore) continue;
+    for (int c = threadIdx.x; c < f.D; c += 256) reinterpret_cast<T*>(f.dx)[(int64_t)row * f.D + c] = (T)0;
   }
-}
-
-// dW of one piece of classes: the slabs added in order
-template <typename T>
-__global__ __launch_bounds__(256) void ce_dw_kernel(const float* __restrict__ slabs, int S, int64_t slab, int64_t n, T* __restrict__ dw) {
-  typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
-    if (i + 4 <= n) {
-      f4_any s = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < S; ++k) s += *reinterpret_cast<const f4_any*>(slabs + k * slab + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dw[i + e] = (T)s[e];
-    } else {
-      for (int64_t e = i; e < n; ++e) {
-        float s = 0.f;
-        for (int k = 0; k < S; ++k) s += slabs[k * slab + e];
-        dw[e] = (T)s;
-      }
-    }
-  }
-}
-
-// db[v] = the sums of d over the rows of every tile, added up: 64 classes to a workgroup of 16 waves, each of which adds every
-// 16th tile, eight loads in flight; the 16 sums are added in order
-template <typename T>
-__global__ __launch_bounds__(1024) void ce_bias_kernel(const float* __restrict__ sums, int64_t ld, const int* __restrict__ state, int rows, int V,
-                                                       const float* __restrict__ d_scale, T* __restrict__ out) {
-  __shared__ float red[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6, tiles = (state[S_KEPT] + rows - 1) / rows;
-  float s = 0.f;
-  if (c < V) {
-    const float* p = sums + c;
-    int t = w;
-    for (; t + 7 * 16 < tiles; t += 8 * 16) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)(t + 16 * i) * ld];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[i];
-    }
-    for (; t < tiles; t += 16) s += p[(int64_t)t * ld];
-  }
-  red[w][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (w || c >= V) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
-  out[c] = (T)(s * d_scale[1]);
 }
 
 // ---- heads of at most 64 classes on at most 64 columns, few rows: the whole pass in one workgroup ----
@@ -1122,22 +1161,18 @@ int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
 struct Tiles {
   bool big;
   int split;
+  int64_t wgs;                                        // workgroups
+  double each, slabs;                                 // us of each, us of the slabs' traffic
 };
-Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, int may_split, bool always_slabs, double end_big = 8.0) {
-  Tiles best = {true, 1};
-  double least = 1e30;
+Tiles tiles_at(bool big, int split, int64_t m, int64_t n, int64_t steps, bool always_slabs, double end_big) {
+  const int64_t b = big ? 256 : 128, tiles = ((m + b - 1) / b) * ((n + b - 1) / b), per = (steps + split - 1) / split;
+  return {big, split, tiles * split, (double)per * (big ? 1.4 : 0.9) + (big ? end_big : 6.0),
+          always_slabs || split > 1 ? 3.0 + (double)split * (double)m * (double)n * 8.0 / 4.5e6 : 0.0};
+}
+Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, double end_big = 8.0) {
   const int64_t steps = (k + 63) / 64 * (f32 ? 6 : 1);
-  for (int big = 0; big < 2; ++big) {
-    const int64_t b = big ? 256 : 128, tiles = ((m + b - 1) / b) * ((n + b - 1) / b), slots = big ? 256 : 512;
-    for (int s = 1; s <= may_split; s += s < 4 ? 1 : s < 16 ? 2 : 8) {
-      const int64_t per = (steps + s - 1) / s;
-      if (s > 1 && (per < 4 || tiles * s >= 1 << 24)) break;
-      double t = (double)((tiles * s + slots - 1) / slots) * ((double)per * (big ? 1.4 : 0.9) + (big ? end_big : 6.0));
-      if (always_slabs || s > 1) t += 3.0 + (double)s * (double)m * (double)n * 8.0 / 4.5e6;
-      if (t < least) least = t, best = {big != 0, s};
-    }
-  }
-  return best;
+  const Tiles small = tiles_at(false, 1, m, n, steps, false, end_big), big = tiles_at(true, 1, m, n, steps, false, end_big);
+  return (double)((small.wgs + 511) / 512) * small.each < (double)((big.wgs + 255) / 256) * big.each ? small : big;
 }
 
 struct Plan {
@@ -1145,12 +1180,38 @@ struct Plan {
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
   int64_t planes;
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
-  Tiles z_tiles, d_tiles, dx_tiles, dw_tiles;
+  Tiles z_tiles, d_tiles;
+  bool grads_big;
+  int dx_split, dw_split;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, nll, g, scale, d, d_sums, slabs, slabs_w, bytes;
+  int64_t x, w, partial, tlogit, sums, g, scale, d, d_sums, slabs, slabs_w, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
+
+// dx and dW share a launch: tiles of one size, each product with its own split.  dx's workgroups come first; those of dW take the
+// slots that are left over in dx's last round, and then all of them.  (512 x 256 x 20000 fp32: 192 workgroups of dx beside 314 of
+// dW on 512 slots, 73 us; one after the other, dx on all slots, 98.)
+void grads_for(const vae_linear_ce* a, Plan& p) {
+  const int64_t kx = (p.piece + 63) / 64 * (p.f32 ? 6 : 1), kw = (a->N + 63) / 64 * (p.f32 ? 6 : 1);
+  double least = 1e30;
+  auto next = [](int s) { return s + (s < 4 ? 1 : s < 16 ? 4 : 8); };
+  for (int big = 0; big < 2; ++big) {
+    const int64_t slots = big ? 256 : 512;
+    for (int sx = 1; sx <= 64 && (sx == 1 || kx / sx >= 4); sx = next(sx)) {
+      const Tiles x = tiles_at(big, sx, a->D, a->N, kx, true, 8.0);
+      if (sx > 1 && x.wgs > 2 * slots) break;
+      for (int sw = 1; sw <= 64 && (sw == 1 || kw / sw >= 4); sw = next(sw)) {
+        const Tiles w = tiles_at(big, sw, a->D, p.piece, kw, false, 8.0);
+        if (sw > 1 && w.wgs > 2 * slots) break;
+        const int64_t over = x.wgs % slots, beside = over ? (slots - over) * (int64_t)(x.each / w.each) : 0;
+        const int64_t left = w.wgs > beside ? w.wgs - beside : 0;
+        const double t = (double)((x.wgs + slots - 1) / slots) * x.each + (double)((left + slots - 1) / slots) * w.each + x.slabs + w.slabs;
+        if (t < least) least = t, p.grads_big = big, p.dx_split = sx, p.dw_split = sw;
+      }
+    }
+  }
+}
 
 Plan plan_of(const vae_linear_ce* a, bool bwd) {
   Plan p;
@@ -1169,10 +1230,10 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.x = take(p.planes * p.n_pad * p.d_pad * 2);
   p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
   if (!bwd) {
-    p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32, 1, false);
+    p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32);
     p.partial = take(up_to(a->V, 128) / 128 * p.n_pad * 8);
     p.tlogit = take(p.n_pad * 4);
-    p.nll = take(p.n_pad * 4);
+    p.sums = take(p.n_pad / 32 * 8);
   } else {
     p.g = take(p.n_pad * 4);
     p.scale = take(8);
@@ -1182,38 +1243,49 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     const int64_t pieces = (most + p.piece - 1) / p.piece;
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
-    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, 1, false, p.f32 ? 55.0 : 12.0);
-    p.dx_tiles = tiles_for(a->D, a->N, p.piece, p.f32, 64, true);
-    p.dw_tiles = tiles_for(a->D, p.piece, a->N, p.f32, 64, false);
-    p.slabs = take((int64_t)p.dx_tiles.split * a->N * a->D * 4);
-    p.slabs_w = take(p.dw_tiles.split > 1 ? (int64_t)p.dw_tiles.split * p.piece * a->D * 4 : 0);
+    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, p.f32 ? 55.0 : 12.0);
+    grads_for(a, p);
+    p.slabs = take((int64_t)p.dx_split * a->N * a->D * 4);
+    p.slabs_w = take(p.dw_split > 1 ? (int64_t)p.dw_split * p.piece * a->D * 4 : 0);
     p.d_sums = take(a->bias ? p.n_pad / (p.d_tiles.big ? 256 : 128) * p.piece * 4 : 0);
   }
   p.bytes = at;
   return p;
 }
 
-template <bool F16, bool A_KC, bool B_KC, int EPI, bool FINE> void launch_gemm(Gemm g, bool big, hipStream_t st) {
+uint32_t tiles_of(Gemm& g, bool big) {
   const int b = big ? 256 : 128;
   g.tiles_m = (g.M + b - 1) / b;
   g.tiles_n = (g.N + b - 1) / b;
-  uint32_t grid = (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
+  return (uint32_t)g.tiles_m * (uint32_t)g.tiles_n * (uint32_t)g.split;
+}
+template <int EPI> void logits(Gemm g, int dtype, bool big, hipStream_t st) {
+  uint32_t grid = tiles_of(g, big);
   const uint32_t resident = big ? 256 : 512;
-  if (EPI == EPI_STATS && grid > resident) grid = resident;                    // workgroups that stay, as many as are resident
-  if (big) head_gemm_kernel<F16, A_KC, B_KC, 256, 256, 2, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);
-  else head_gemm_kernel<F16, A_KC, B_KC, 128, 128, 2, 2, EPI, FINE><<<grid, 256, 0, st>>>(g);
+  if (EPI == EPI_STATS && grid > resident) grid = resident;             // workgroups that stay, as many as are resident
+#define VAE_CE(F16, FINE)                                                                           \
+  if (big) head_logits_kernel<F16, 256, 256, 2, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);             \
+  else head_logits_kernel<F16, 128, 128, 2, 2, EPI, FINE><<<grid, 256, 0, st>>>(g)
+  if (dtype == VAE_ADAMW_F32) { VAE_CE(false, true); }
+  else if (dtype == VAE_ADAMW_BF16) { VAE_CE(false, false); }
+  else { VAE_CE(true, false); }
+#undef VAE_CE
 }
-template <bool A_KC, bool B_KC, int EPI> void gemm(const Gemm& g, int dtype, bool big, hipStream_t st) {
-  if (dtype == VAE_ADAMW_F32) launch_gemm<false, A_KC, B_KC, EPI, EPI != EPI_STORE>(g, big, st);
-  else if (dtype == VAE_ADAMW_BF16) launch_gemm<false, A_KC, B_KC, EPI, false>(g, big, st);
-  else launch_gemm<true, A_KC, B_KC, EPI, false>(g, big, st);
+void gradients(Gemm dx, Gemm dw, bool want_dx, bool want_dw, int dtype, bool big, hipStream_t st) {
+  const uint32_t nx = want_dx ? (tiles_of(dx, big) + 7) / 8 * 8 : 0, grid = nx + (want_dw ? tiles_of(dw, big) : 0);
+#define VAE_CE(F16)                                                                                 \
+  if (big) head_grads_kernel<F16, 256, 256, 2, 4><<<grid, 512, 0, st>>>(dx, dw, (int)nx);           \
+  else head_grads_kernel<F16, 128, 128, 2, 2><<<grid, 256, 0, st>>>(dx, dw, (int)nx)
+  if (dtype == VAE_ADAMW_F16) { VAE_CE(true); }
+  else { VAE_CE(false); }
+#undef VAE_CE
 }
-void add_slabs(const float* slabs, int S, int64_t slab, int64_t n, void* out, int dtype, hipStream_t st) {
-  const int64_t work = (n + 1023) / 1024;
-  const int grid = (int)(work < 4096 ? work : 4096);
-  if (dtype == VAE_ADAMW_F32) ce_dw_kernel<float><<<grid, 256, 0, st>>>(slabs, S, slab, n, (float*)out);
-  else if (dtype == VAE_ADAMW_BF16) ce_dw_kernel<__bf16><<<grid, 256, 0, st>>>(slabs, S, slab, n, (__bf16*)out);
-  else ce_dw_kernel<_Float16><<<grid, 256, 0, st>>>(slabs, S, slab, n, (_Float16*)out);
+void finish(const Finish& f, int dtype, hipStream_t st) {
+  const unsigned grid = (unsigned)(f.db_blocks + f.dw_blocks + f.dx_blocks);
+  if (!grid) return;
+  if (dtype == VAE_ADAMW_F32) ce_finish_kernel<float><<<grid, 256, 0, st>>>(f);
+  else if (dtype == VAE_ADAMW_BF16) ce_finish_kernel<__bf16><<<grid, 256, 0, st>>>(f);
+  else ce_finish_kernel<_Float16><<<grid, 256, 0, st>>>(f);
 }
 
 void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, const Upstream& u, hipStream_t st) {
@@ -1294,9 +1366,8 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   int* s = reinterpret_cast<int*>(state);
   hipStream_t st = (hipStream_t)stream;
-  float *tl = reinterpret_cast<float*>(ws + p.tlogit), *nll = reinterpret_cast<float*>(ws + p.nll);
-  float* by_row = reduction == VAE_CE_NONE ? loss : nullptr;
-  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, by_row);
+  float* tl = reinterpret_cast<float*>(ws + p.tlogit);
+  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, reduction == VAE_CE_NONE ? loss : nullptr);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   pack(a, p, ws, s, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
@@ -1304,12 +1375,11 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
   g.target_logit = tl;
   const bool big = p.z_tiles.big;
-  gemm<true, true, EPI_STATS>(g, a->dtype, big, st);
+  logits<EPI_STATS>(g, a->dtype, big, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   const int b = big ? 256 : 128;
   ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->class_weight, tl,
-                                                                  nll, by_row);
-  if (!by_row) ce_reduce_kernel<<<1, 1024, 0, st>>>(nll, s, reduction == VAE_CE_MEAN, loss);
+                                                                  reduction, reinterpret_cast<double*>(ws + p.sums), loss);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   return VAE_OK;
 }
@@ -1355,76 +1425,77 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.ldd = p.piece;
     z.plane_d = plane_d;
     z.d_sums = dbias ? sums : nullptr;
-    gemm<true, true, EPI_D>(z, a->dtype, p.d_tiles.big, st);
+    logits<EPI_D>(z, a->dtype, p.d_tiles.big, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
-    if (dx) {                                           // dx (N, D) += d (N, n_v) W (n_v, D)
-      Gemm g = {};
-      g.a = w0;
-      g.lda = z.lda;
-      g.plane_a = z.plane_a;
-      g.b = d;
-      g.ldb = p.piece;
-      g.plane_b = plane_d;
-      g.M = (int)a->D;
-      g.N = (int)a->N;
-      g.K = (int)n_v;
-      g.segs = z.segs;
-      g.dyn = s + S_KEPT;
-      g.d_scale = scale;
-      g.out = slabs;
-      g.ldo = a->D;
-      g.out_kind = 0;
-      g.add = v0 > 0;
-      g.split = p.dx_tiles.split;
-      gemm<false, true, EPI_STORE>(g, a->dtype, p.dx_tiles.big, st);
-      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
-    }
-    if (dw) {                                           // dW (n_v, D) = d^T (n_v, N) x (N, D)
-      Gemm g = {};
-      g.a = xp;
-      g.lda = p.d_pad;
-      g.plane_a = p.n_pad * p.d_pad;
-      g.b = d;
-      g.ldb = p.piece;
-      g.plane_b = plane_d;
-      g.M = (int)a->D;
-      g.N = (int)n_v;
-      g.K = (int)a->N;
-      g.segs = z.segs;
-      g.split = p.dw_tiles.split;
-      g.dyn = s + S_KEPT;
-      g.dyn_k = 1;
-      g.d_scale = scale;
-      g.ldo = a->D;
-      void* o = reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize;
-      g.out = g.split > 1 ? ws + p.slabs_w : o;
-      g.out_kind = g.split > 1 ? 0 : p.f32 ? 2 : 1;
-      gemm<false, false, EPI_STORE>(g, a->dtype, p.dw_tiles.big, st);
-      if (g.split > 1) {
-        const float* sw = reinterpret_cast<const float*>(ws + p.slabs_w);
-        add_slabs(sw, g.split, n_v * a->D, n_v * a->D, o, a->dtype, st);
-      }
-      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
-    }
+    Gemm gx = {}, gw = {};
+    // dx (N, D) += d (N, n_v) W (n_v, D)
+    gx.a = w0;
+    gx.lda = z.lda;
+    gx.plane_a = z.plane_a;
+    gx.b = d;
+    gx.ldb = p.piece;
+    gx.plane_b = plane_d;
+    gx.M = (int)a->D;
+    gx.N = (int)a->N;
+    gx.K = (int)n_v;
+    gx.segs = z.segs;
+    gx.dyn = s + S_KEPT;
+    gx.d_scale = scale;
+    gx.out = slabs;
+    gx.ldo = a->D;
+    gx.add = v0 > 0;
+    gx.split = p.dx_split;
+    // dW (n_v, D) = d^T (n_v, N) x (N, D)
+    gw.a = xp;
+    gw.lda = p.d_pad;
+    gw.plane_a = p.n_pad * p.d_pad;
+    gw.b = d;
+    gw.ldb = p.piece;
+    gw.plane_b = plane_d;
+    gw.M = (int)a->D;
+    gw.N = (int)n_v;
+    gw.K = (int)a->N;
+    gw.segs = z.segs;
+    gw.split = p.dw_split;
+    gw.dyn = s + S_KEPT;
+    gw.dyn_k = 1;
+    gw.d_scale = scale;
+    gw.ldo = a->D;
+    uint8_t* o = dw ? reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize : nullptr;
+    gw.out = gw.split > 1 ? ws + p.slabs_w : o;
+    gw.out_kind = gw.split > 1 ? 0 : p.f32 ? 2 : 1;
+    if (dx || dw) gradients(gx, gw, dx, dw, a->dtype, p.grads_big, st);
+    VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    Finish f = {};
+    f.state = s;
+    f.d_scale = scale;
     if (dbias) {
-      const unsigned grid = (unsigned)((n_v + 63) / 64);
-      const int rows = p.d_tiles.big ? 256 : 128;
-#define VAE_DB(T) ce_bias_kernel<T><<<grid, 1024, 0, st>>>(sums, p.piece, s, rows, (int)n_v, scale, (T*)dbias + v0)
-      if (p.f32) VAE_DB(float);
-      else if (a->dtype == VAE_ADAMW_BF16) VAE_DB(__bf16);
-      else VAE_DB(_Float16);
-#undef VAE_DB
-      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+      f.db_blocks = (int)((n_v + 63) / 64);
+      f.sums = sums;
+      f.ld_sums = p.piece;
+      f.sum_rows = p.d_tiles.big ? 256 : 128;
+      f.V = (int)n_v;
+      f.db = reinterpret_cast<uint8_t*>(dbias) + v0 * esize;
     }
-  }
-  if (dx) {
-    const int S = p.dx_tiles.split;
-    const int rows = (int)(a->N < 4096 ? a->N : 4096);
-#define VAE_DX(T) ce_dx_kernel<T><<<rows, 256, 0, st>>>(slabs, S, a->N * a->D, (int)a->N, (int)a->D, s, a->target, a->ignore_index, (T*)dx)
-    if (p.f32) VAE_DX(float);
-    else if (a->dtype == VAE_ADAMW_BF16) VAE_DX(__bf16);
-    else VAE_DX(_Float16);
-#undef VAE_DX
+    if (dw && gw.split > 1) {
+      const int64_t work = (n_v * a->D + 1023) / 1024;
+      f.dw_blocks = (int)(work < 4096 ? work : 4096);
+      f.dw_slabs = reinterpret_cast<const float*>(ws + p.slabs_w);
+      f.dw_split = gw.split;
+      f.dw_n = n_v * a->D;
+      f.dw = o;
+    }
+    if (dx && v0 + n_v == a->V) {
+      f.dx_blocks = (int)(a->N < 4096 ? a->N : 4096);
+      f.dx_slabs = slabs;
+      f.dx_split = p.dx_split;
+      f.N = (int)a->N;
+      f.D = (int)a->D;
+      f.target = a->target;
+      f.ignore = a->ignore_index;
+      f.dx = dx;
+    }
+    finish(f, a->dtype, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
   }
   return VAE_OK;
