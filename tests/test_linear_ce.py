@@ -178,6 +178,19 @@ def test_reductions_and_upstream_gradients(dtype, reduction, d, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", [(70, 3000, 10), (9, 2500, 3001), (600, 1700, 350), (2, 2000, 1025), (4096, 1565, 252), (1, 4096, 1)])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_few_tiles_over_many_features(n, d, v, dtype, reduction):
+    """Logits of a few tiles and long sums, which are split."""
+    s = _inputs(n, d, v, dtype, True, True, 0.2 if n > 9 else 0.0, seed=n + v)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    up = torch.rand(n, generator=g, device="cuda") * 1e-3 if reduction == "none" else torch.tensor(0.5, device="cuda")
+    loss, grads = _run(s, reduction, up)
+    _check(s, reduction, loss, grads, up)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,d,v,dtype", [(40000, 72, 7000, "bf16"), (14000, 72, 6500, "fp32"), (8000, 520, 7100, "bf16"), (8200, 328, 7000, "fp16")])
 def test_large_tiles_and_pieces(n, d, v, dtype):
     """Hundreds of tiles of 256 x 256, few and many steps of K, and (the longest batches) a vocabulary in two pieces."""

@@ -380,7 +380,7 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
       }
     };
     if constexpr (EPI == EPI_STORE) {
-      const float inv = g.d_scale[1];
+      const float inv = g.d_scale ? g.d_scale[1] : 1.f;
       if (g.out_kind == 1) {
         uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
         rows_out16(
@@ -756,14 +756,39 @@ template <typename T> __global__ __launch_bounds__(1024) void ce_pack_kernel(Ups
   else pack_rows<T>(w, block - x.blocks, D, ldo);
 }
 
-// The partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row.
-// Sum and mean: the workgroup that finishes last adds up what all of them left, in order (same bits every time).
+// Sum and mean of the losses: every workgroup leaves the sum of its rows' (`share`, over its threads), and the one that finishes
+// last adds up what all of them left, in order (same bits every time).
+__device__ __forceinline__ double block_sum64(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) v += red[i];
+  return v;
+}
+__device__ __forceinline__ void sum_losses(double share, int blocks, int* state, int reduction, double* sums, float* loss) {
+  __shared__ double red[16];
+  __shared__ bool last;
+  share = block_sum64(share, red);
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(sums + blockIdx.x, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = __hip_atomic_fetch_add(state + S_DONE, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  share = 0;
+  for (int i = threadIdx.x; i < blocks; i += blockDim.x) share += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  share = block_sum64(share, red);
+  if (threadIdx.x == 0) *loss = (float)(reduction == VAE_CE_MEAN ? share / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : share);
+}
+
+// The partial maxima and sums of a row over the tiles -> lse and the row's loss: 32 rows to a workgroup, 8 threads to a row
 __global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restrict__ partial, int tiles, int64_t ldp, int* __restrict__ state,
                                                          int N, const float* __restrict__ cw, const float* __restrict__ target_logit,
                                                          int reduction, double* __restrict__ sums, float* __restrict__ loss) {
   __shared__ float2 red[8][32];
-  __shared__ double red64[4];
-  __shared__ bool last;
   const int kept = state[S_KEPT], blocks = max((kept + 31) / 32, 1);
   const int row = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
   if ((int)blockIdx.x >= blocks) return;
@@ -801,25 +826,133 @@ __global__ __launch_bounds__(256) void ce_combine_kernel(const float2* __restric
     if (reduction == VAE_CE_NONE) loss[orig] = v;
     share = (double)v;
   }
-  if (reduction == VAE_CE_NONE) return;
+  if (reduction != VAE_CE_NONE) sum_losses(share, blocks, state, reduction, sums, loss);
+}
+
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f4_any slab_sum(const float* p, int S, int64_t slab) {
+  f4_any s = {0.f, 0.f, 0.f, 0.f};
+  int k = 0;
+  for (; k + 4 <= S; k += 4) {
+    f4_any v[4];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) share += __shfl_xor(share, o, 64);
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(sums + blockIdx.x, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(state + S_DONE, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
-  }
-  __syncthreads();
-  if (!last) return;
-  share = 0;
-  for (int i = threadIdx.x; i < blocks; i += 256) share += __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f4_any*>(p + (k + u) * slab);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) share += __shfl_xor(share, o, 64);
-  if ((threadIdx.x & 63) == 0) red64[threadIdx.x >> 6] = share;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    share = ((red64[0] + red64[1]) + red64[2]) + red64[3];
-    *loss = (float)(reduction == VAE_CE_MEAN ? share / (double)reinterpret_cast<const float*>(state)[S_TOTAL] : share);
+    for (int u = 0; u < 4; ++u) s += v[u];
   }
+  for (; k < S; ++k) s += *reinterpret_cast<const f4_any*>(p + k * slab);
+  return s;
+}
+__device__ __forceinline__ float slab_sum1(const float* p, int S, int64_t slab) {
+  float s = 0.f;
+  for (int k = 0; k < S; ++k) s += p[k * slab];
+  return s;
+}
+
+// ---- logits whose K was split: slabs (S, N, ldz) of partial logits, by packed row ----
+template <typename T> __device__ __forceinline__ f4_any slab_logits(const float* p, int S, int64_t slab, const T* bias, int c, int V) {
+  f4_any z = slab_sum(p + c, S, slab);                        // (ldz is V, up to whole groups of 4)
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = c + e < V ? z[e] + (bias ? (float)bias[c + e] : 0.f) : -INFINITY;
+  return z;
+}
+// lse and loss: TPR threads to a row
+template <typename T, int TPR>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(const float* __restrict__ slabs, int S, int64_t ldz, const T* __restrict__ bias,
+                                                                            int* __restrict__ state, int N, int V, const float* __restrict__ cw,
+                                                                            int reduction, double* __restrict__ sums, float* __restrict__ loss) {
+  constexpr int RPW = TPR < 256 ? 256 / TPR : 1, WAVES = TPR / 64;
+  static_assert(TPR % 64 == 0, "whole waves");
+  __shared__ float2 red[RPW * WAVES];
+  __shared__ float hits[RPW];
+  const int kept = state[S_KEPT], blocks = max((kept + RPW - 1) / RPW, 1);
+  if ((int)blockIdx.x >= blocks) return;
+  const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, row = blockIdx.x * RPW + sub;
+  const int t = row < kept ? state[S_ROWS + N + row] : -1;
+  if (lane == 0) hits[sub] = NAN;                             // stays so where the target is no class
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+  if (row < kept) {
+    const float* p = slabs + (int64_t)row * ldz;
+    for (int c = lane * 4; c < V; c += TPR * 4) {
+      const f4_any z = slab_logits(p, S, (int64_t)N * ldz, bias, c, V);
+      const float m = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), top), ref = m == -INFINITY ? 0.f : m;
+      sum *= exp_fine(top - ref);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (c + e < V) sum += exp_fine(z[e] - ref);
+        if (c + e == t) hits[sub] = z[e];
+      }
+      top = m;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float ot = __shfl_xor(top, o, 64), os = __shfl_xor(sum, o, 64), m = fmaxf(top, ot), ref = m == -INFINITY ? 0.f : m;
+    sum = sum * exp_fine(top - ref) + os * exp_fine(ot - ref);
+    top = m;
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
+  __syncthreads();
+  double share = 0;
+  if (lane == 0 && row < kept) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, red[sub * WAVES + i].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) sum += red[sub * WAVES + i].y * exp_fine(red[sub * WAVES + i].x - ref);
+    const float lse = m + logf(sum);
+    reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
+    const float v = (lse - hits[sub]) * (!cw || t < 0 ? 1.f : cw[t]);
+    if (reduction == VAE_CE_NONE) loss[state[S_ROWS + row]] = v;
+    share = (double)v;
+  }
+  if (reduction != VAE_CE_NONE) sum_losses(share, blocks, state, reduction, sums, loss);
+}
+// d and the sums of SLAB_ROWS rows of it; zeros behind the last class and the last kept row, up to whole steps of K
+constexpr int SLAB_ROWS = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void ce_slab_d_kernel(const float* __restrict__ slabs, int S, int64_t ldz, const T* __restrict__ bias,
+                                                        const int* __restrict__ state, int N, int V, const float* __restrict__ gs,
+                                                        const float* __restrict__ d_scale, uint16_t* __restrict__ d, int64_t ldd, int64_t plane,
+                                                        float* __restrict__ sums) {
+  const int kept = state[S_KEPT], rows = (kept + 63) / 64 * 64, c = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int first = blockIdx.y * SLAB_ROWS;
+  if (first >= rows || c >= (V + 63) / 64 * 64) return;
+  const float scale = d_scale[0];
+  f4_any total = {0.f, 0.f, 0.f, 0.f};
+  for (int row = first; row < first + SLAB_ROWS; ++row) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const float g = row < kept ? gs[row] * scale : 0.f;
+    if (g != 0.f && c < V) {
+      const f4_any z = slab_logits(slabs + (int64_t)row * ldz, S, (int64_t)N * ldz, bias, c, V);
+      const float lse = reinterpret_cast<const float*>(state)[S_ROWS + 2 * N + row];
+      const int at = state[S_ROWS + N + row] - c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = exp_fine(z[e] - lse);
+        v[e] = c + e < V ? (at == e ? p - 1.f : p) * g : 0.f;
+        total[e] += v[e];
+      }
+    }
+    uint16_t* o = d + (int64_t)row * ldd + c;
+    if constexpr (sizeof(T) == 4) {
+      union {
+        __bf16 t[4];
+        uint2 u;
+      } w[3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split3(v[e], w[0].t[e], w[1].t[e], w[2].t[e]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<uint2*>(o + k * plane) = w[k].u;
+    } else {
+      constexpr bool F16 = __is_same(T, _Float16);
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
+    }
+  }
+  if (sums) *reinterpret_cast<f4_any*>(sums + (int64_t)blockIdx.y * ldd + c) = total;
 }
 
 // What is left behind the products of a piece, in one launch:
@@ -846,25 +979,6 @@ struct Finish {
   int64_t ignore;
   void* dx;
 };
-typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
-__device__ __forceinline__ f4_any slab_sum(const float* p, int S, int64_t slab) {
-  f4_any s = {0.f, 0.f, 0.f, 0.f};
-  int k = 0;
-  for (; k + 4 <= S; k += 4) {
-    f4_any v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f4_any*>(p + (k + u) * slab);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s += v[u];
-  }
-  for (; k < S; ++k) s += *reinterpret_cast<const f4_any*>(p + k * slab);
-  return s;
-}
-__device__ __forceinline__ float slab_sum1(const float* p, int S, int64_t slab) {
-  float s = 0.f;
-  for (int k = 0; k < S; ++k) s += p[k * slab];
-  return s;
-}
 template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(Finish f) {
   __shared__ float red[4][64];
   int block = blockIdx.x;
@@ -1169,10 +1283,21 @@ Tiles tiles_at(bool big, int split, int64_t m, int64_t n, int64_t steps, bool al
   return {big, split, tiles * split, (double)per * (big ? 1.4 : 0.9) + (big ? end_big : 6.0),
           always_slabs || split > 1 ? 3.0 + (double)split * (double)m * (double)n * 8.0 / 4.5e6 : 0.0};
 }
-Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, double end_big = 8.0) {
+// Of the logits (m classes, n rows): tiles that fill the chip finish them in their epilogue; otherwise K is split, and a launch
+// that reads the slabs stands for the epilogue (`launch` us, where it is one more)
+Tiles tiles_for(int64_t m, int64_t n, int64_t k, bool f32, double end_big, double launch) {
   const int64_t steps = (k + 63) / 64 * (f32 ? 6 : 1);
-  const Tiles small = tiles_at(false, 1, m, n, steps, false, end_big), big = tiles_at(true, 1, m, n, steps, false, end_big);
-  return (double)((small.wgs + 511) / 512) * small.each < (double)((big.wgs + 255) / 256) * big.each ? small : big;
+  Tiles best = {};
+  double least = 1e30;
+  for (int big = 0; big < 2; ++big)
+    for (int split = 1; split <= 32 && (split == 1 || steps / split >= 4); split += split < 4 ? 1 : split < 16 ? 4 : 8) {
+      const Tiles t = tiles_at(big, split, m, n, steps, false, split == 1 ? end_big : 8.0);
+      const int64_t slots = big ? 256 : 512;
+      if (split > 1 && t.wgs > slots) break;
+      const double us = (double)((t.wgs + slots - 1) / slots) * t.each + t.slabs + (split > 1 ? launch : 0.0);
+      if (us < least) least = us, best = t;
+    }
+  return best;
 }
 
 struct Plan {
@@ -1180,11 +1305,13 @@ struct Plan {
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
   int64_t planes;
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
-  Tiles z_tiles, d_tiles;
+  Tiles z_tiles, d_tiles;                             // (of a pass)
+  int64_t ldz;                                        // of partial logits
+  int sum_rows;                                       // rows to a sum in d_sums
   bool grads_big;
   int dx_split, dw_split;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, sums, g, scale, d, d_sums, slabs, slabs_w, bytes;
+  int64_t x, w, partial, tlogit, sums, g, scale, z, d, d_sums, slabs, slabs_w, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
@@ -1221,6 +1348,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.d_pad = up_to(a->D, K_PAD);
   p.pack_w = p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w);
   p.ldw = p.pack_w ? p.d_pad : a->ldw;
+  p.ldz = up_to(a->V, 4);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -1230,10 +1358,10 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.x = take(p.planes * p.n_pad * p.d_pad * 2);
   p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
   if (!bwd) {
-    p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32);
-    p.partial = take(up_to(a->V, 128) / 128 * p.n_pad * 8);
+    p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32, 8.0, 0.0);
+    p.partial = take(p.z_tiles.split > 1 ? p.z_tiles.split * a->N * p.ldz * 4 : up_to(a->V, 128) / 128 * p.n_pad * 8);
     p.tlogit = take(p.n_pad * 4);
-    p.sums = take(p.n_pad / 32 * 8);
+    p.sums = take(p.n_pad * 8);
   } else {
     p.g = take(p.n_pad * 4);
     p.scale = take(8);
@@ -1243,11 +1371,13 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     const int64_t pieces = (most + p.piece - 1) / p.piece;
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
-    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, p.f32 ? 55.0 : 12.0);
+    p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, p.f32 ? 55.0 : 12.0, 5.0);
+    p.sum_rows = p.d_tiles.split > 1 ? SLAB_ROWS : p.d_tiles.big ? 256 : 128;
+    p.z = take(p.d_tiles.split > 1 ? p.d_tiles.split * a->N * p.ldz * 4 : 0);
     grads_for(a, p);
     p.slabs = take((int64_t)p.dx_split * a->N * a->D * 4);
     p.slabs_w = take(p.dw_split > 1 ? (int64_t)p.dw_split * p.piece * a->D * 4 : 0);
-    p.d_sums = take(a->bias ? p.n_pad / (p.d_tiles.big ? 256 : 128) * p.piece * 4 : 0);
+    p.d_sums = take(a->bias ? p.n_pad / p.sum_rows * p.piece * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -1266,10 +1396,18 @@ template <int EPI> void logits(Gemm g, int dtype, bool big, hipStream_t st) {
 #define VAE_CE(F16, FINE)                                                                           \
   if (big) head_logits_kernel<F16, 256, 256, 2, 4, EPI, FINE><<<grid, 512, 0, st>>>(g);             \
   else head_logits_kernel<F16, 128, 128, 2, 2, EPI, FINE><<<grid, 256, 0, st>>>(g)
-  if (dtype == VAE_ADAMW_F32) { VAE_CE(false, true); }
+  if (dtype == VAE_ADAMW_F32) { VAE_CE(false, EPI != EPI_STORE); }
   else if (dtype == VAE_ADAMW_BF16) { VAE_CE(false, false); }
   else { VAE_CE(true, false); }
 #undef VAE_CE
+}
+// partial logits, float slabs (split, N, ldz)
+void store_logits(Gemm g, const Tiles& t, int64_t ldz, void* slabs, int dtype, hipStream_t st) {
+  g.split = t.split;
+  g.d_scale = nullptr;
+  g.out = slabs;
+  g.ldo = ldz;
+  logits<EPI_STORE>(g, dtype, t.big, st);
 }
 void gradients(Gemm dx, Gemm dw, bool want_dx, bool want_dw, int dtype, bool big, hipStream_t st) {
   const uint32_t nx = want_dx ? (tiles_of(dx, big) + 7) / 8 * 8 : 0, grid = nx + (want_dw ? tiles_of(dw, big) : 0);
@@ -1375,11 +1513,27 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
   g.target_logit = tl;
   const bool big = p.z_tiles.big;
-  logits<EPI_STATS>(g, a->dtype, big, st);
-  VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
-  const int b = big ? 256 : 128;
-  ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->class_weight, tl,
-                                                                  reduction, reinterpret_cast<double*>(ws + p.sums), loss);
+  double* sums = reinterpret_cast<double*>(ws + p.sums);
+  if (p.z_tiles.split > 1) {
+    store_logits(g, p.z_tiles, p.ldz, ws + p.partial, a->dtype, st);
+    VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+    const float* slabs = reinterpret_cast<const float*>(ws + p.partial);
+#define VAE_CE(T)                                                                                                                     \
+  if (a->V <= 1024) ce_slab_loss_kernel<T, 64><<<(unsigned)((a->N + 3) / 4), 256, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, \
+                                                                                (int)a->N, (int)a->V, a->class_weight, reduction, sums, loss); \
+  else ce_slab_loss_kernel<T, 1024><<<(unsigned)a->N, 1024, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)a->V, \
+                                                                a->class_weight, reduction, sums, loss)
+    if (p.f32) { VAE_CE(float); }
+    else if (a->dtype == VAE_ADAMW_BF16) { VAE_CE(__bf16); }
+    else { VAE_CE(_Float16); }
+#undef VAE_CE
+  } else {
+    logits<EPI_STATS>(g, a->dtype, big, st);
+    VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
+    const int b = big ? 256 : 128;
+    ce_combine_kernel<<<(unsigned)((a->N + 31) / 32), 256, 0, st>>>(g.partial, (int)((a->V + b - 1) / b), p.n_pad, s, (int)a->N, a->class_weight, tl,
+                                                                    reduction, sums, loss);
+  }
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   return VAE_OK;
 }
@@ -1425,7 +1579,20 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.ldd = p.piece;
     z.plane_d = plane_d;
     z.d_sums = dbias ? sums : nullptr;
-    logits<EPI_D>(z, a->dtype, p.d_tiles.big, st);
+    if (p.d_tiles.split > 1) {                          // (one piece: the classes that do not fill the chip)
+      store_logits(z, p.d_tiles, p.ldz, ws + p.z, a->dtype, st);
+      VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+      const dim3 grid((unsigned)((up_to(n_v, 64) + 1023) / 1024), (unsigned)(up_to(a->N, 64) / SLAB_ROWS));
+#define VAE_CE(T)                                                                                                                              \
+  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(reinterpret_cast<const float*>(ws + p.z), p.d_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, \
+                                            gr, scale, d, p.piece, plane_d, dbias ? sums : nullptr)
+      if (p.f32) VAE_CE(float);
+      else if (a->dtype == VAE_ADAMW_BF16) VAE_CE(__bf16);
+      else VAE_CE(_Float16);
+#undef VAE_CE
+    } else {
+      logits<EPI_D>(z, a->dtype, p.d_tiles.big, st);
+    }
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     Gemm gx = {}, gw = {};
     // dx (N, D) += d (N, n_v) W (n_v, D)
@@ -1473,7 +1640,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       f.db_blocks = (int)((n_v + 63) / 64);
       f.sums = sums;
       f.ld_sums = p.piece;
-      f.sum_rows = p.d_tiles.big ? 256 : 128;
+      f.sum_rows = p.sum_rows;
       f.V = (int)n_v;
       f.db = reinterpret_cast<uint8_t*>(dbias) + v0 * esize;
     }
