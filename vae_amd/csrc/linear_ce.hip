@@ -71,6 +71,7 @@ struct Gemm {
   // EPI_STORE: out[n][m], final type or float slabs (split, N, M) that are added to when `add`
   void* out;
   int64_t ldo;
+  const int* rows;              // null, or where row n of the result belongs
   int out_kind;                 // 0 float slab, 1 the final 16-bit type, 2 final float
   int add;
 };
@@ -390,7 +391,7 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
             [&](int row, int c, u4 v) {
               const int n = n0 + row, m = m0 + 8 * c;
               if (n >= N || m >= g.M) return;
-              uint16_t* o = out + (int64_t)n * g.ldo + m;
+              uint16_t* o = out + (int64_t)(g.rows ? g.rows[n] : n) * g.ldo + m;
               if (m + 8 <= g.M) {
                 *reinterpret_cast<u4_any*>(o) = v;
               } else {
@@ -421,7 +422,7 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
             f4 v = *reinterpret_cast<const f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2));
             const int n = n0 + (row >> 5) * 16 * TN + 16 * j0 + (row & 31), m = m0 + 4 * c;
             if (n >= N || m >= g.M) continue;
-            float* o = out + (int64_t)n * g.ldo + m;
+            float* o = out + (int64_t)(g.rows ? g.rows[n] : n) * g.ldo + m;
             if (m + 4 <= g.M) {
               if (g.add) v += *reinterpret_cast<const f4_any*>(o);
               *reinterpret_cast<f4_any*>(o) = v;
@@ -865,49 +866,52 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(con
   static_assert(TPR % 64 == 0, "whole waves");
   __shared__ float2 red[RPW * WAVES];
   __shared__ float hits[RPW];
-  const int kept = state[S_KEPT], blocks = max((kept + RPW - 1) / RPW, 1);
+  const int kept = state[S_KEPT], blocks = min(max((kept + RPW - 1) / RPW, 1), (int)gridDim.x);
   if ((int)blockIdx.x >= blocks) return;
-  const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR, row = blockIdx.x * RPW + sub;
-  const int t = row < kept ? state[S_ROWS + N + row] : -1;
-  if (lane == 0) hits[sub] = NAN;                             // stays so where the target is no class
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  if (row < kept) {
-    const float* p = slabs + (int64_t)row * ldz;
-    for (int c = lane * 4; c < V; c += TPR * 4) {
-      const f4_any z = slab_logits(p, S, (int64_t)N * ldz, bias, c, V);
-      const float m = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), top), ref = m == -INFINITY ? 0.f : m;
-      sum *= exp_fine(top - ref);
+  const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
+  double share = 0;
+  for (int base = blockIdx.x * RPW; base < kept; base += blocks * RPW) {
+    const int row = base + sub, t = row < kept ? state[S_ROWS + N + row] : -1;
+    __syncthreads();
+    if (lane == 0) hits[sub] = NAN;                           // stays so where the target is no class
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+    if (row < kept) {
+      const float* p = slabs + (int64_t)row * ldz;
+      for (int c = lane * 4; c < V; c += TPR * 4) {
+        const f4_any z = slab_logits(p, S, (int64_t)N * ldz, bias, c, V);
+        const float m = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), top), ref = m == -INFINITY ? 0.f : m;
+        sum *= exp_fine(top - ref);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (c + e < V) sum += exp_fine(z[e] - ref);
-        if (c + e == t) hits[sub] = z[e];
+        for (int e = 0; e < 4; ++e) {
+          if (c + e < V) sum += exp_fine(z[e] - ref);
+          if (c + e == t) hits[sub] = z[e];
+        }
+        top = m;
       }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const float ot = __shfl_xor(top, o, 64), os = __shfl_xor(sum, o, 64), m = fmaxf(top, ot), ref = m == -INFINITY ? 0.f : m;
+      sum = sum * exp_fine(top - ref) + os * exp_fine(ot - ref);
       top = m;
     }
-  }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
+    __syncthreads();
+    if (lane == 0 && row < kept) {
+      float m = -INFINITY;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const float ot = __shfl_xor(top, o, 64), os = __shfl_xor(sum, o, 64), m = fmaxf(top, ot), ref = m == -INFINITY ? 0.f : m;
-    sum = sum * exp_fine(top - ref) + os * exp_fine(ot - ref);
-    top = m;
-  }
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
-  __syncthreads();
-  double share = 0;
-  if (lane == 0 && row < kept) {
-    float m = -INFINITY;
+      for (int i = 0; i < WAVES; ++i) m = fmaxf(m, red[sub * WAVES + i].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+      sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) m = fmaxf(m, red[sub * WAVES + i].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < WAVES; ++i) sum += red[sub * WAVES + i].y * exp_fine(red[sub * WAVES + i].x - ref);
-    const float lse = m + logf(sum);
-    reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
-    const float v = (lse - hits[sub]) * (!cw || t < 0 ? 1.f : cw[t]);
-    if (reduction == VAE_CE_NONE) loss[state[S_ROWS + row]] = v;
-    share = (double)v;
+      for (int i = 0; i < WAVES; ++i) sum += red[sub * WAVES + i].y * exp_fine(red[sub * WAVES + i].x - ref);
+      const float lse = m + logf(sum);
+      reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
+      const float v = (lse - hits[sub]) * (!cw || t < 0 ? 1.f : cw[t]);
+      if (reduction == VAE_CE_NONE) loss[state[S_ROWS + row]] = v;
+      share += (double)v;
+    }
   }
   if (reduction != VAE_CE_NONE) sum_losses(share, blocks, state, reduction, sums, loss);
 }
@@ -959,8 +963,8 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(const float* __restrict_
 //   db: the sums of d over the rows of every tile, added up.  64 classes to a workgroup of 4 waves, each of which adds every
 //       4th tile, eight loads in flight; the 4 sums are added in order
 //   dW: its slabs, where there are several, added in order
-//   dx: behind the last piece, the slabs (S, N, D) of a packed row added in order and put at its original row; ignored rows are
-//       zero.  A workgroup per row, four columns per thread
+//   dx: behind the last piece, the slabs (S, N, D) of a packed row, where there are any, added in order and put at its original
+//       row; ignored rows are zero.  A workgroup per row, four columns per thread
 struct Finish {
   int db_blocks, dw_blocks, dx_blocks;
   const int* state;
@@ -1022,7 +1026,7 @@ template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(Fi
   }
   block -= f.dw_blocks;
   const int64_t slab = (int64_t)f.N * f.D;
-  for (int row = block; row < kept; row += f.dx_blocks) {
+  for (int row = block; f.dx_slabs && row < kept; row += f.dx_blocks) {
     T* o = reinterpret_cast<T*>(f.dx) + (int64_t)f.state[S_ROWS + row] * f.D;
     const float* p = f.dx_slabs + (int64_t)row * f.D;
     for (int c = threadIdx.x * 4; c < f.D; c += 1024) {
@@ -1308,7 +1312,7 @@ struct Plan {
   Tiles z_tiles, d_tiles;                             // (of a pass)
   int64_t ldz;                                        // of partial logits
   int sum_rows;                                       // rows to a sum in d_sums
-  bool grads_big;
+  bool grads_big, dx_slabs;                           // (dx is written as it is where it takes one product with one part)
   int dx_split, dw_split;
   // byte offsets in the workspaces
   int64_t x, w, partial, tlogit, sums, g, scale, z, d, d_sums, slabs, slabs_w, bytes;
@@ -1326,7 +1330,7 @@ void grads_for(const vae_linear_ce* a, Plan& p) {
   for (int big = 0; big < 2; ++big) {
     const int64_t slots = big ? 256 : 512;
     for (int sx = 1; sx <= 64 && (sx == 1 || kx / sx >= 4); sx = next(sx)) {
-      const Tiles x = tiles_at(big, sx, a->D, a->N, kx, true, 8.0);
+      const Tiles x = tiles_at(big, sx, a->D, a->N, kx, p.piece < a->V, 8.0);
       if (sx > 1 && x.wgs > 2 * slots) break;
       for (int sw = 1; sw <= 64 && (sw == 1 || kw / sw >= 4); sw = next(sw)) {
         const Tiles w = tiles_at(big, sw, a->D, p.piece, kw, false, 8.0);
@@ -1375,7 +1379,8 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.sum_rows = p.d_tiles.split > 1 ? SLAB_ROWS : p.d_tiles.big ? 256 : 128;
     p.z = take(p.d_tiles.split > 1 ? p.d_tiles.split * a->N * p.ldz * 4 : 0);
     grads_for(a, p);
-    p.slabs = take((int64_t)p.dx_split * a->N * a->D * 4);
+    p.dx_slabs = p.dx_split > 1 || p.piece < a->V;
+    p.slabs = take(p.dx_slabs ? (int64_t)p.dx_split * a->N * a->D * 4 : 0);
     p.slabs_w = take(p.dw_split > 1 ? (int64_t)p.dw_split * p.piece * a->D * 4 : 0);
     p.d_sums = take(a->bias ? p.n_pad / p.sum_rows * p.piece * 4 : 0);
   }
@@ -1519,9 +1524,9 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
     VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
     const float* slabs = reinterpret_cast<const float*>(ws + p.partial);
 #define VAE_CE(T)                                                                                                                     \
-  if (a->V <= 1024) ce_slab_loss_kernel<T, 64><<<(unsigned)((a->N + 3) / 4), 256, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, \
+  if (a->V <= 1024) ce_slab_loss_kernel<T, 64><<<(unsigned)(a->N < 1024 ? (a->N + 3) / 4 : 256), 256, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, \
                                                                                 (int)a->N, (int)a->V, a->class_weight, reduction, sums, loss); \
-  else ce_slab_loss_kernel<T, 1024><<<(unsigned)a->N, 1024, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)a->V, \
+  else ce_slab_loss_kernel<T, 1024><<<(unsigned)(a->N < 512 ? a->N : 512), 1024, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)a->V, \
                                                                 a->class_weight, reduction, sums, loss)
     if (p.f32) { VAE_CE(float); }
     else if (a->dtype == VAE_ADAMW_BF16) { VAE_CE(__bf16); }
@@ -1608,7 +1613,9 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     gx.segs = z.segs;
     gx.dyn = s + S_KEPT;
     gx.d_scale = scale;
-    gx.out = slabs;
+    gx.out = p.dx_slabs ? (void*)slabs : dx;
+    gx.out_kind = p.dx_slabs ? 0 : p.f32 ? 2 : 1;
+    gx.rows = p.dx_slabs ? nullptr : s + S_ROWS;
     gx.ldo = a->D;
     gx.add = v0 > 0;
     gx.split = p.dx_split;
@@ -1654,7 +1661,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     }
     if (dx && v0 + n_v == a->V) {
       f.dx_blocks = (int)(a->N < 4096 ? a->N : 4096);
-      f.dx_slabs = slabs;
+      f.dx_slabs = p.dx_slabs ? slabs : nullptr;
       f.dx_split = p.dx_split;
       f.N = (int)a->N;
       f.D = (int)a->D;
