@@ -637,9 +637,10 @@ int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t wor
  * state: vae_linear_ce_state_bytes(N) bytes that the forward pass writes and the backward pass of the same arguments reads.
  * The backward pass takes the float gradient of the loss ((N) or (1)) and overwrites the dense dx (N, D), dw (V, D) and dbias
  * (V) that are not null, of the operands' type.  Ignored rows take no part at all: their dx is 0 and what their x holds
- * reaches nothing else.  The logits are never in memory; the workspace holds a packed copy of x, for fp32 (and for w that is
- * not 16-byte aligned with D and its stride multiples of 8) one of w, and up to 512 MiB of logit gradients.  Same bits every
- * time.                                                                                                                    */
+ * reaches nothing else.  The logits are not kept; the workspace holds a packed copy of x, for fp32 (and for w that is
+ * not 16-byte aligned with D and its stride multiples of 8) one of w, up to 512 MiB of logit gradients, and for few rows and
+ * classes over many features partial logits of at most 67 MB.  At most 2^24 tiles of 128 x 128 in N x V, N x D and V x D.  Same
+ * bits every time.                                                                                                          */
 enum { VAE_CE_NONE = 0, VAE_CE_SUM = 1, VAE_CE_MEAN = 2 };
 typedef struct {
   int64_t N, D, V;

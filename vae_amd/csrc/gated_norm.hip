@@ -13,7 +13,9 @@
 // writes dr, db and dgate, each once: a row lives in registers from its loads to its stores, in 32 bits.  A wave takes a row of
 // up to 64 16-byte pieces, a workgroup of up to 1024 threads a longer one, one to four pieces per thread.  A workgroup walks
 // over rows; the gradients of the vectors over columns are summed in registers over its rows, written once per workgroup, and
-// added up in a second launch in a fixed order (no atomics: same bits every time).
+// added up in a second launch in a fixed order (no atomics: same bits every time).  32768 x 4096 bf16 with a full gate: forward
+// 311 us = 4.3 TB/s, backward 455 us = 4.7 TB/s (a large copy: 4.9); without the next row's loads ahead of this row's work 373
+// and 712.
 #include "../../include/vae_amd.h"
 #include "common.h"
 
@@ -149,8 +151,9 @@ template <int NW, int K> __device__ __forceinline__ void row_sums(float (&v)[K],
   }
 }
 
-// Both within 3e-7 of themselves up to |v| = 4 (v * log2 e is rounded: |v| 2^-24 beyond): the hardware's exponential and reciprocal (an ulp each) leave the registers that the
-// correctly rounded division and the library's functions take, times 8 elements, to the loads.
+// Both within 3e-7 of themselves up to |v| = 4 (v * log2 e is rounded: |v| 2^-24 beyond): the hardware's exponential and
+// reciprocal (an ulp each) leave the registers that the correctly rounded division and the library's functions take, times 8
+// elements, to the loads.
 __device__ __forceinline__ float sigmoid_f(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
 }

@@ -1,5 +1,5 @@
 // Softmax cross entropy of a linear head, z = x W^T + b over N rows and V classes, with its gradients, without the logits
-// ever being in memory (gfx950).
+// being in memory (gfx950).
 //
 //   lse_i = log sum_v exp z_iv        nll_i = c[t_i] (lse_i - z_{i, t_i})
 //   d_iv  = g_i c[t_i] (exp(z_iv - lse_i) - [v = t_i])        dx = d W        dW = d^T x        db = sum_i d_i
@@ -11,17 +11,21 @@
 // Forward: a tile product of W with the packed x in which a lane owns a row of x and its accumulators run over classes.  The
 // running maximum and sum of a tile are then taken inside a lane's registers, and only one pair per row and 256 classes is
 // written.  Backward, for pieces of the classes whose d fits a fixed workspace: the same product again, whose epilogue turns
-// the logits into d (16 bits), then dx += d W and dW = d^T x.  4 products of 2 N D V operations, of which one is the recompute
-// that stands for keeping N V logits.  Bound by the matrix cores as soon as N and D are a few hundred.
+// the logits into d (16 bits) and sums it over its rows for db; then dx += d W and dW = d^T x, in one launch.  4 products of
+// 2 N D V operations, of which one is the recompute that stands for keeping N V logits.  Bound by the matrix cores as soon as N
+// and D are a few hundred: 8192 x 4096 x 131072 in bf16, loss 6.7 ms = 1.3 PFLOP/s, loss and gradients 26.9 ms = 1.3 PFLOP/s over
+// all four products (a product of that shape by the library: 1.48).  Only where the tiles of the logits are too few to fill the
+// chip is K split instead, and partial logits of at most 67 MB are written and read once (64 x 4000 x 900 bf16: both passes 70 us,
+// 129 without; 901 x 3014 x 1683 fp32 326 and 527).
 //
 // Types: bf16 and fp16 multiply as they are, sums in 32 bits; d is rounded to the same type (relative 2^-9 or 2^-12 of each
 // element, independent of each other, so that a sum of them is off by no more than its own rounding).  d is divided by the
 // largest factor g_i c[t_i] for that, and the products are multiplied by it in 32 bits: the term of the target, -1 in nearly
 // every row of a large vocabulary, is then exact, where the rounding of 1 / N itself would shift every gradient by the same
 // 2^-9 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
-// multiplied by 2^14 as well.  fp32 operands are split exactly
-// into three bf16 terms, and for every 64 of K the six products that matter run one after the other: the error
-// is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix instruction would give a sixteenth).
+// multiplied by 2^14 as well.  fp32 operands are split exactly into three bf16 terms, and for every 64 of K the six products
+// that matter run one after the other: the error is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix
+// instruction would give a sixteenth).
 #include "../../include/vae_amd.h"
 #include "common.h"
 
@@ -42,7 +46,8 @@ constexpr int ROW_PAD = 256;                            // packed rows and colum
 constexpr int K_PAD = 64;
 
 // the state of a forward pass that the backward pass reads: int32 / float words
-constexpr int S_KEPT = 0, S_TOTAL = 1, S_DONE = 2, S_ROWS = 4;   // kept rows, sum of c[t], finished workgroups; row index, class (-1: none) and lse, N each, of the kept rows
+// kept rows, sum of c[t], finished workgroups; row index, class (-1: none) and lse, N each, of the kept rows
+constexpr int S_KEPT = 0, S_TOTAL = 1, S_DONE = 2, S_ROWS = 4;
 
 enum { EPI_STATS = 0, EPI_D = 1, EPI_STORE = 2 };
 
@@ -857,7 +862,8 @@ template <typename T> __device__ __forceinline__ f4_any slab_logits(const float*
   for (int e = 0; e < 4; ++e) z[e] = c + e < V ? z[e] + (bias ? (float)bias[c + e] : 0.f) : -INFINITY;
   return z;
 }
-// lse and loss: TPR threads to a row
+// lse and loss: TPR threads to a row, a wave up to 1024 classes and a workgroup beyond (loss of 600 x 2000 x 900 bf16 34 us by waves,
+// 39 by workgroups; of 64 x 4000 x 4000 45 and 31)
 template <typename T, int TPR>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(const float* __restrict__ slabs, int S, int64_t ldz, const T* __restrict__ bias,
                                                                             int* __restrict__ state, int N, int V, const float* __restrict__ cw,
@@ -1049,7 +1055,7 @@ template <typename T> __global__ __launch_bounds__(256) void ce_finish_kernel(Fi
 // The products are too small for tiles and the dozen launches of the way above would be all that is waited for.  256 rows at a
 // time lie in LDS beside W, in 32 bits whatever the type; four lanes share a row, which they hold in registers, and take every
 // fourth class.  D is padded with zeros to DM columns.
-constexpr int SMALL_V = 64, SMALL_D = 64, SMALL_ROWS = 1024, SMALL_WORK = 1 << 19, CHUNK = 256;
+constexpr int SMALL_V = 64, SMALL_D = 64, SMALL_ROWS = 1024, SMALL_WORK = 1 << 18, CHUNK = 256;
 struct Small {
   int N, D, V, reduction;
   int64_t ldx, ldw, ignore;
@@ -1242,8 +1248,9 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_b
   if (a.db && oq == 0) reinterpret_cast<T*>(a.db)[ov] = (T)sum[4];
 }
 
-// One workgroup is the faster way up to some 2^19 products (both passes, fp32: 512 x 30 x 17 in 35 us against 99, 1024 x 30 x 17
-// in 63 against 80, 512 x 64 x 64, 2^21 products, in 115 against 74).
+// One workgroup is the faster way up to some 2^18 products (both passes on the GPU, fp32, against the way above: 64 x 32 x 32 16 us
+// and 46, 512 x 30 x 17 35 and 50, 1024 x 30 x 17, 2^19 products, 64 and 51; 1024 x 16 x 16 takes 55 and 37, but 3 launches less a
+// pass save their caller 24).
 bool small_head(const vae_linear_ce* a) {
   return a->V <= SMALL_V && a->D <= SMALL_D && a->N <= SMALL_ROWS && a->N * a->V * a->D <= SMALL_WORK;
 }
@@ -1510,7 +1517,8 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   int* s = reinterpret_cast<int*>(state);
   hipStream_t st = (hipStream_t)stream;
   float* tl = reinterpret_cast<float*>(ws + p.tlogit);
-  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, reduction == VAE_CE_NONE ? loss : nullptr);
+  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl,
+                                     reduction == VAE_CE_NONE ? loss : nullptr);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   pack(a, p, ws, s, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
@@ -1523,11 +1531,14 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
     store_logits(g, p.z_tiles, p.ldz, ws + p.partial, a->dtype, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
     const float* slabs = reinterpret_cast<const float*>(ws + p.partial);
-#define VAE_CE(T)                                                                                                                     \
-  if (a->V <= 1024) ce_slab_loss_kernel<T, 64><<<(unsigned)(a->N < 1024 ? (a->N + 3) / 4 : 256), 256, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, \
-                                                                                (int)a->N, (int)a->V, a->class_weight, reduction, sums, loss); \
-  else ce_slab_loss_kernel<T, 1024><<<(unsigned)(a->N < 512 ? a->N : 512), 1024, 0, st>>>(slabs, p.z_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)a->V, \
-                                                                a->class_weight, reduction, sums, loss)
+    const int S = p.z_tiles.split, N = (int)a->N, V = (int)a->V;
+    const unsigned narrow = N < 1024 ? (N + 3) / 4 : 256, wide = N < 512 ? N : 512;
+#define VAE_CE(T)                                                                                                                  \
+  const T* bias = reinterpret_cast<const T*>(a->bias);                                                                             \
+  if (V <= 1024)                                                                                                                   \
+    ce_slab_loss_kernel<T, 64><<<narrow, 256, 0, st>>>(slabs, S, p.ldz, bias, s, N, V, a->class_weight, reduction, sums, loss);     \
+  else                                                                                                                             \
+    ce_slab_loss_kernel<T, 1024><<<wide, 1024, 0, st>>>(slabs, S, p.ldz, bias, s, N, V, a->class_weight, reduction, sums, loss)
     if (p.f32) { VAE_CE(float); }
     else if (a->dtype == VAE_ADAMW_BF16) { VAE_CE(__bf16); }
     else { VAE_CE(_Float16); }
@@ -1565,7 +1576,8 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   const int* s = reinterpret_cast<const int*>(state);
   hipStream_t st = (hipStream_t)stream;
-  float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale), *slabs = reinterpret_cast<float*>(ws + p.slabs), *sums = reinterpret_cast<float*>(ws + p.d_sums);
+  float *gr = reinterpret_cast<float*>(ws + p.g), *scale = reinterpret_cast<float*>(ws + p.scale);
+  float *slabs = reinterpret_cast<float*>(ws + p.slabs), *sums = reinterpret_cast<float*>(ws + p.d_sums);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
   pack(a, p, ws, s, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
@@ -1588,9 +1600,11 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       store_logits(z, p.d_tiles, p.ldz, ws + p.z, a->dtype, st);
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
       const dim3 grid((unsigned)((up_to(n_v, 64) + 1023) / 1024), (unsigned)(up_to(a->N, 64) / SLAB_ROWS));
-#define VAE_CE(T)                                                                                                                              \
-  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(reinterpret_cast<const float*>(ws + p.z), p.d_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, \
-                                            gr, scale, d, p.piece, plane_d, dbias ? sums : nullptr)
+      const float* zs = reinterpret_cast<const float*>(ws + p.z);
+      float* to = dbias ? sums : nullptr;
+#define VAE_CE(T)                                                                                                               \
+  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(zs, p.d_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, gr, scale, d, \
+                                            p.piece, plane_d, to)
       if (p.f32) VAE_CE(float);
       else if (a->dtype == VAE_ADAMW_BF16) VAE_CE(__bf16);
       else VAE_CE(_Float16);

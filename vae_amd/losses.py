@@ -3,7 +3,7 @@ call signatures (src/losses.py:9-202).  Off by default in the reference (task.py
 config.py:80) and tiny (B x n_classes): plain torch, no kernels.
 
 ``linear_cross_entropy`` / ``LinearCrossEntropyLoss``: the cross entropy of the discrete cell-property heads
-(task.py:129-137) for heads with many classes, on the HIP kernels and without the logits in memory."""
+(task.py:129-137) for heads with many classes, on the HIP kernels and without keeping the logits."""
 from __future__ import annotations
 
 from typing import List, Optional
@@ -112,7 +112,7 @@ class GroupDRO:
 def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
                          weight: Optional[torch.Tensor] = None, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
     """``F.cross_entropy(x @ w.T + bias, target, weight, ignore_index=..., reduction=...)`` as float32, differentiable once in
-    ``x`` (..., D), ``w`` (V, D) and ``bias`` (V), without the (..., V) logits ever being in memory.
+    ``x`` (..., D), ``w`` (V, D) and ``bias`` (V), without the (..., V) logits being kept.
 
     ``x``, ``w`` and ``bias`` are float32, bfloat16 or float16, all of one type; sums, the softmax statistics and the loss are
     held in 32 bits.  ``target`` (...) int64; ``weight`` (V) float32 class weights.  Rows whose target is ``ignore_index`` take no
