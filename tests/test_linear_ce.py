@@ -191,6 +191,17 @@ def test_few_tiles_over_many_features(n, d, v, dtype, reduction):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", [(1, 70, 130), (2, 4099, 33), (16, 64, 5000), (17, 513, 1001), (33, 300, 2050), (64, 1030, 70), (8, 1024, 40000)])
+@pytest.mark.parametrize("off,bias,ignored", [(0, True, 0.0), (3, False, 0.4)])
+def test_few_rows(n, d, v, off, bias, ignored):
+    """fp32 rows in ones, sixteens and their neighbours, W read as it is, on and off 16-byte boundaries."""
+    s = _inputs(n, d, v, "fp32", bias, not bias, ignored, seed=n + d, off=off)
+    s["target"][n // 2] = v - 1
+    loss, grads = _run(s, "mean")
+    _check(s, "mean", loss, grads)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,d,v,dtype", [(40000, 72, 7000, "bf16"), (14000, 72, 6500, "fp32"), (8000, 520, 7100, "bf16"), (8200, 328, 7000, "fp16")])
 def test_large_tiles_and_pieces(n, d, v, dtype):
     """Hundreds of tiles of 256 x 256, few and many steps of K, and (the longest batches) a vocabulary in two pieces."""

@@ -921,10 +921,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(con
   }
   if (reduction != VAE_CE_NONE) sum_losses(share, blocks, state, reduction, sums, loss);
 }
-// d and the sums of SLAB_ROWS rows of it; zeros behind the last class and the last kept row, up to whole steps of K
+// d and the sums of SLAB_ROWS rows of it; zeros behind the last class and the last kept row, up to whole steps of K.  `keep`: d
+// also takes the place of the first slab
 constexpr int SLAB_ROWS = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void ce_slab_d_kernel(const float* __restrict__ slabs, int S, int64_t ldz, const T* __restrict__ bias,
+__global__ __launch_bounds__(256) void ce_slab_d_kernel(float* slabs, bool keep, int S, int64_t ldz, const T* __restrict__ bias,
                                                         const int* __restrict__ state, int N, int V, const float* __restrict__ gs,
                                                         const float* __restrict__ d_scale, uint16_t* __restrict__ d, int64_t ldd, int64_t plane,
                                                         float* __restrict__ sums) {
@@ -947,6 +948,7 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(const float* __restrict_
         total[e] += v[e];
       }
     }
+    if (keep && row < kept && c < V) *reinterpret_cast<f4_any*>(slabs + (int64_t)row * ldz + c) = f4_any{v[0], v[1], v[2], v[3]};
     uint16_t* o = d + (int64_t)row * ldd + c;
     if constexpr (sizeof(T) == 4) {
       union {
@@ -963,6 +965,125 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(const float* __restrict_
     }
   }
   if (sums) *reinterpret_cast<f4_any*>(sums + (int64_t)blockIdx.y * ldd + c) = total;
+}
+
+// ---- fp32, at most FEW_ROWS rows: W goes from memory straight into 32-bit matrix instructions ----
+// The three terms of W would be written and read again for a handful of rows.  Both kernels are bound by their one read of W; a
+// lane's four consecutive floats are four values of K (or four columns) whose order the other operand shares.
+constexpr int FEW_ROWS = 64;
+__device__ __forceinline__ f4_any load4(const float* p, int c, int n) {                // p[c .. c + 4), those from n on as zeros
+  if (c + 4 <= n) return *reinterpret_cast<const f4_any*>(p + c);
+  f4_any v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < n) v[e] = p[c + e];
+  return v;
+}
+// partial logits (part, N, ldz): a wave takes 32 classes and all rows, 16 to a tile, over `per` features (a multiple of 64)
+template <int NB>
+__global__ __launch_bounds__(256) void ce_few_z_kernel(const float* __restrict__ w, int64_t ldw, const float* __restrict__ x, int64_t ldx,
+                                                       const int* __restrict__ state, int N, int D, int V, int per, float* __restrict__ slabs,
+                                                       int64_t ldz) {
+  const int kept = state[S_KEPT], lane = threadIdx.x & 63, l15 = lane & 15, lj = lane >> 4;
+  const int v0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 32, k0 = blockIdx.y * per, k1 = min(k0 + per, D);
+  if (kept == 0 || v0 >= V) return;
+  const float *wr[2], *xr[NB];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) wr[t] = w + (int64_t)min(v0 + 16 * t + l15, V - 1) * ldw;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) xr[j] = x + (int64_t)state[S_ROWS + min(16 * j + l15, kept - 1)] * ldx;
+  f32x4 acc[2][NB];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[t][j] = (f32x4)0.f;
+  constexpr int AHEAD = NB <= 2 ? 4 : 2;                      // groups of 16 features in flight
+  for (int k = k0; k < k1; k += 16 * AHEAD) {
+    f4_any a[AHEAD][2], b[AHEAD][NB];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int c = k + 16 * u + 4 * lj;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) a[u][t] = load4(wr[t], c, k1);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[u][j] = load4(xr[j], c, k1);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][t][e], b[u][j][e], acc[t][j], 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int n = 16 * j + l15;
+    if (n >= kept) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int v = v0 + 16 * t + 4 * lj;
+      if (v < V) *reinterpret_cast<f32x4*>(slabs + ((int64_t)blockIdx.y * N + n) * ldz + v) = acc[t][j];       // (ldz: V in whole fours)
+    }
+  }
+}
+// dx slabs (part, N, D): a wave takes 64 columns and all rows over `per` classes (a multiple of 16); d (N, ldz) in 32 bits
+template <int NB>
+__global__ __launch_bounds__(256) void ce_few_dx_kernel(const float* __restrict__ w, int64_t ldw, const float* __restrict__ d, int64_t ldz,
+                                                        const int* __restrict__ state, int N, int D, int V, int per,
+                                                        const float* __restrict__ d_scale, float* __restrict__ slabs) {
+  const int kept = state[S_KEPT], lane = threadIdx.x & 63, l15 = lane & 15, lj = lane >> 4;
+  const int c = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64 + 4 * l15, k0 = blockIdx.y * per, k1 = min(k0 + per, V);
+  if (kept == 0 || c - 4 * l15 >= D) return;
+  const float* dr[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) dr[j] = d + (int64_t)min(16 * j + l15, kept - 1) * ldz;
+  f32x4 acc[4][NB];                                           // [column & 3]
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[t][j] = (f32x4)0.f;
+  constexpr int AHEAD = NB <= 2 ? 2 : 1;                      // groups of 16 classes in flight
+  for (int k = k0; k < k1; k += 16 * AHEAD) {
+    f4_any a[AHEAD][4], b[AHEAD][NB];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int v = k + 16 * u + 4 * lj;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[u][e] = load4(w + (int64_t)min(v + e, V - 1) * ldw, c, D);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) b[u][j] = load4(dr[j], v, k1);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][e][t], b[u][j][e], acc[t][j], 0, 0, 0);
+  }
+  const float inv = d_scale[1];
+  const int c0 = c - 4 * l15 + 16 * lj;                       // acc[t][j][r]: column c0 + 4 r + t
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int n = 16 * j + l15;
+    if (n >= kept) continue;
+    float* o = slabs + ((int64_t)blockIdx.y * N + n) * D;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f4_any v = f4_any{acc[0][j][r], acc[1][j][r], acc[2][j][r], acc[3][j][r]} * inv;
+      const int at = c0 + 4 * r;
+      if (at + 4 <= D) {
+        *reinterpret_cast<f4_any*>(o + at) = v;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (at + t < D) o[at + t] = v[t];
+      }
+    }
+  }
 }
 
 // What is left behind the products of a piece, in one launch:
@@ -1316,7 +1437,9 @@ struct Plan {
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
   int64_t planes;
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
+  bool few;                                           // fp32, few rows: W as it is
   Tiles z_tiles, d_tiles;                             // (of a pass)
+  int z_parts;                                        // slabs of partial logits; 0: the product's epilogue finishes them
   int64_t ldz;                                        // of partial logits
   int sum_rows;                                       // rows to a sum in d_sums
   bool grads_big, dx_slabs;                           // (dx is written as it is where it takes one product with one part)
@@ -1357,9 +1480,13 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.planes = p.f32 ? 3 : 1;
   p.n_pad = up_to(a->N, ROW_PAD);
   p.d_pad = up_to(a->D, K_PAD);
-  p.pack_w = p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w);
-  p.ldw = p.pack_w ? p.d_pad : a->ldw;
+  // waves enough to fill the chip, sums over at most 2048 features, partial logits of at most 64 MiB
+  const int64_t waves = (a->V + 31) / 32, want = (2047 + waves) / waves, most_parts = (a->D + 255) / 256, long_sums = (a->D + 2047) / 2048;
+  const int64_t parts = want > most_parts ? most_parts : want < long_sums ? long_sums : want;
   p.ldz = up_to(a->V, 4);
+  p.few = p.f32 && a->N <= FEW_ROWS && parts <= 64 && parts * a->N * p.ldz * 4 <= 64ll << 20 && a->V <= D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256;
+  p.pack_w = !p.few && (p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w));
+  p.ldw = p.pack_w ? p.d_pad : a->ldw;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -1370,7 +1497,8 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
   if (!bwd) {
     p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32, 8.0, 0.0);
-    p.partial = take(p.z_tiles.split > 1 ? p.z_tiles.split * a->N * p.ldz * 4 : up_to(a->V, 128) / 128 * p.n_pad * 8);
+    p.z_parts = p.few ? (int)parts : p.z_tiles.split > 1 ? p.z_tiles.split : 0;
+    p.partial = take(p.z_parts ? p.z_parts * a->N * p.ldz * 4 : up_to(a->V, 128) / 128 * p.n_pad * 8);
     p.tlogit = take(p.n_pad * 4);
     p.sums = take(p.n_pad * 8);
   } else {
@@ -1383,10 +1511,15 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
     p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, p.f32 ? 55.0 : 12.0, 5.0);
-    p.sum_rows = p.d_tiles.split > 1 ? SLAB_ROWS : p.d_tiles.big ? 256 : 128;
-    p.z = take(p.d_tiles.split > 1 ? p.d_tiles.split * a->N * p.ldz * 4 : 0);
+    p.z_parts = p.few ? (int)parts : p.d_tiles.split > 1 ? p.d_tiles.split : 0;
+    p.sum_rows = p.z_parts ? SLAB_ROWS : p.d_tiles.big ? 256 : 128;
+    p.z = take((int64_t)p.z_parts * a->N * p.ldz * 4);
     grads_for(a, p);
-    p.dx_slabs = p.dx_split > 1 || p.piece < a->V;
+    if (p.few) {                                      // (as above: waves of 64 columns)
+      const int64_t cols = (a->D + 63) / 64, fill = (2047 + cols) / cols, most_x = (a->V + 63) / 64, cap = most_x < 128 ? most_x : 128;
+      p.dx_split = (int)(fill < cap ? fill : cap);
+    }
+    p.dx_slabs = p.few || p.dx_split > 1 || p.piece < a->V;
     p.slabs = take(p.dx_slabs ? (int64_t)p.dx_split * a->N * a->D * 4 : 0);
     p.slabs_w = take(p.dw_split > 1 ? (int64_t)p.dw_split * p.piece * a->D * 4 : 0);
     p.d_sums = take(a->bias ? p.n_pad / p.sum_rows * p.piece * 4 : 0);
@@ -1449,6 +1582,22 @@ void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, 
   if (p.f32) ce_pack_kernel<float><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
   else ce_pack_kernel<uint16_t><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
 }
+
+#define VAE_FEW(KERNEL, ...)                                    \
+  if (a->N <= 16) KERNEL<1><<<grid, 256, 0, st>>>(__VA_ARGS__); \
+  else if (a->N <= 32) KERNEL<2><<<grid, 256, 0, st>>>(__VA_ARGS__); \
+  else KERNEL<4><<<grid, 256, 0, st>>>(__VA_ARGS__)
+void few_logits(const vae_linear_ce* a, const Plan& p, const int* state, float* slabs, hipStream_t st) {
+  const int per = (int)up_to((a->D + p.z_parts - 1) / p.z_parts, 64);
+  const dim3 grid((unsigned)((a->V + 127) / 128), (unsigned)p.z_parts);
+  VAE_FEW(ce_few_z_kernel, (const float*)a->w, p.ldw, (const float*)a->x, a->ldx, state, (int)a->N, (int)a->D, (int)a->V, per, slabs, p.ldz);
+}
+void few_dx(const vae_linear_ce* a, const Plan& p, const int* state, const float* d, const float* d_scale, float* slabs, hipStream_t st) {
+  const int per = (int)up_to((a->V + p.dx_split - 1) / p.dx_split, 16);
+  const dim3 grid((unsigned)((a->D + 255) / 256), (unsigned)p.dx_split);
+  VAE_FEW(ce_few_dx_kernel, (const float*)a->w, p.ldw, d, p.ldz, state, (int)a->N, (int)a->D, (int)a->V, per, d_scale, slabs);
+}
+#undef VAE_FEW
 
 int check(const vae_linear_ce* a, const char* who) {
   VAE_REQUIRE(a, "%s: null arguments", who);
@@ -1520,18 +1669,19 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl,
                                      reduction == VAE_CE_NONE ? loss : nullptr);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
-  pack(a, p, ws, s, Upstream{}, st);
+  if (!p.few) pack(a, p, ws, s, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   Gemm g = logits_gemm(a, p, ws, s);
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
   g.target_logit = tl;
   const bool big = p.z_tiles.big;
   double* sums = reinterpret_cast<double*>(ws + p.sums);
-  if (p.z_tiles.split > 1) {
-    store_logits(g, p.z_tiles, p.ldz, ws + p.partial, a->dtype, st);
+  if (p.z_parts) {
+    if (p.few) few_logits(a, p, s, reinterpret_cast<float*>(ws + p.partial), st);
+    else store_logits(g, p.z_tiles, p.ldz, ws + p.partial, a->dtype, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
     const float* slabs = reinterpret_cast<const float*>(ws + p.partial);
-    const int S = p.z_tiles.split, N = (int)a->N, V = (int)a->V;
+    const int S = p.z_parts, N = (int)a->N, V = (int)a->V;
     const unsigned narrow = N < 1024 ? (N + 3) / 4 : 256, wide = N < 512 ? N : 512;
 #define VAE_CE(T)                                                                                                                  \
   const T* bias = reinterpret_cast<const T*>(a->bias);                                                                             \
@@ -1596,14 +1746,15 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.ldd = p.piece;
     z.plane_d = plane_d;
     z.d_sums = dbias ? sums : nullptr;
-    if (p.d_tiles.split > 1) {                          // (one piece: the classes that do not fill the chip)
-      store_logits(z, p.d_tiles, p.ldz, ws + p.z, a->dtype, st);
+    if (p.z_parts) {                                    // (one piece: few rows, or classes that do not fill the chip)
+      if (p.few) few_logits(a, p, s, reinterpret_cast<float*>(ws + p.z), st);
+      else store_logits(z, p.d_tiles, p.ldz, ws + p.z, a->dtype, st);
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
       const dim3 grid((unsigned)((up_to(n_v, 64) + 1023) / 1024), (unsigned)(up_to(a->N, 64) / SLAB_ROWS));
-      const float* zs = reinterpret_cast<const float*>(ws + p.z);
+      float* zs = reinterpret_cast<float*>(ws + p.z);
       float* to = dbias ? sums : nullptr;
 #define VAE_CE(T)                                                                                                               \
-  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(zs, p.d_tiles.split, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, gr, scale, d, \
+  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(zs, p.few, p.z_parts, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, gr, scale, d, \
                                             p.piece, plane_d, to)
       if (p.f32) VAE_CE(float);
       else if (a->dtype == VAE_ADAMW_BF16) VAE_CE(__bf16);
@@ -1652,7 +1803,9 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     uint8_t* o = dw ? reinterpret_cast<uint8_t*>(dw) + v0 * a->D * esize : nullptr;
     gw.out = gw.split > 1 ? ws + p.slabs_w : o;
     gw.out_kind = gw.split > 1 ? 0 : p.f32 ? 2 : 1;
-    if (dx || dw) gradients(gx, gw, dx, dw, a->dtype, p.grads_big, st);
+    const bool tiled_dx = dx && !p.few;
+    if (dx && p.few) few_dx(a, p, s, reinterpret_cast<const float*>(ws + p.z), scale, slabs, st);
+    if (tiled_dx || dw) gradients(gx, gw, tiled_dx, dw, a->dtype, p.grads_big, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
     Finish f = {};
     f.state = s;
