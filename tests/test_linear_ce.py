@@ -191,7 +191,7 @@ def test_few_tiles_over_many_features(n, d, v, dtype, reduction):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,d,v", [(1, 70, 130), (2, 4099, 33), (16, 64, 5000), (17, 513, 1001), (33, 300, 2050), (64, 1030, 70), (8, 1024, 40000)])
+@pytest.mark.parametrize("n,d,v", [(1, 70, 130), (2, 4099, 33), (16, 64, 5000), (17, 513, 1001), (33, 300, 2050), (64, 1030, 70), (64, 1030, 2100), (8, 1024, 40000)])
 @pytest.mark.parametrize("off,bias,ignored", [(0, True, 0.0), (3, False, 0.4)])
 def test_few_rows(n, d, v, off, bias, ignored):
     """fp32 rows in ones, sixteens and their neighbours, W read as it is, on and off 16-byte boundaries."""

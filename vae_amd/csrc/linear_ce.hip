@@ -969,7 +969,11 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(float* slabs, bool keep,
 
 // ---- fp32, at most FEW_ROWS rows: W goes from memory straight into 32-bit matrix instructions ----
 // The three terms of W would be written and read again for a handful of rows.  Both kernels are bound by their one read of W; a
-// lane's four consecutive floats are four values of K (or four columns) whose order the other operand shares.
+// lane's four consecutive floats are four values of K (or four columns) whose order the other operand shares.  8 x 1024 x 40000:
+// partial logits 38 us = 4.3 TB/s of W, dx 28 us (W partly in the caches), a loss 52 us against 197 with three terms, loss and
+// gradients 211 against 530; 64 x 1024 x 40000 101 against 196 and 364 against 532 (the rows, read by every wave, are then half of
+// the traffic).  Worth its two launches more from V D of some 2^15 N on: 16 x 512 x 2000 61 us against 72, 64 x 512 x 4000 92 and
+// 91, 64 x 100 x 1000 68 and 57.
 constexpr int FEW_ROWS = 64;
 __device__ __forceinline__ f4_any load4(const float* p, int c, int n) {                // p[c .. c + 4), those from n on as zeros
   if (c + 4 <= n) return *reinterpret_cast<const f4_any*>(p + c);
@@ -997,17 +1001,24 @@ __global__ __launch_bounds__(256) void ce_few_z_kernel(const float* __restrict__
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[t][j] = (f32x4)0.f;
-  constexpr int AHEAD = NB <= 2 ? 4 : 2;                      // groups of 16 features in flight
-  for (int k = k0; k < k1; k += 16 * AHEAD) {
+  constexpr int AHEAD = NB <= 2 ? 4 : 2;                      // groups of 16 features at a time, the next ones on their way
+  struct In {
     f4_any a[AHEAD][2], b[AHEAD][NB];
+  } in, next;
+  auto fetch = [&](In& to, int k) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int c = k + 16 * u + 4 * lj;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) a[u][t] = load4(wr[t], c, k1);
+      for (int t = 0; t < 2; ++t) to.a[u][t] = load4(wr[t], c, k1);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) b[u][j] = load4(xr[j], c, k1);
+      for (int j = 0; j < NB; ++j) to.b[u][j] = load4(xr[j], c, k1);
     }
+  };
+  fetch(next, k0);
+  for (int k = k0; k < k1; k += 16 * AHEAD) {
+    in = next;
+    if (k + 16 * AHEAD < k1) fetch(next, k + 16 * AHEAD);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
@@ -1015,7 +1026,7 @@ __global__ __launch_bounds__(256) void ce_few_z_kernel(const float* __restrict__
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][t][e], b[u][j][e], acc[t][j], 0, 0, 0);
+          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(in.a[u][t][e], in.b[u][j][e], acc[t][j], 0, 0, 0);
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
@@ -1044,17 +1055,24 @@ __global__ __launch_bounds__(256) void ce_few_dx_kernel(const float* __restrict_
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[t][j] = (f32x4)0.f;
-  constexpr int AHEAD = NB <= 2 ? 2 : 1;                      // groups of 16 classes in flight
-  for (int k = k0; k < k1; k += 16 * AHEAD) {
+  constexpr int AHEAD = NB <= 2 ? 2 : 1;                      // groups of 16 classes at a time, the next ones on their way
+  struct In {
     f4_any a[AHEAD][4], b[AHEAD][NB];
+  } in, next;
+  auto fetch = [&](In& to, int k) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int v = k + 16 * u + 4 * lj;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) a[u][e] = load4(w + (int64_t)min(v + e, V - 1) * ldw, c, D);
+      for (int e = 0; e < 4; ++e) to.a[u][e] = load4(w + (int64_t)min(v + e, V - 1) * ldw, c, D);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) b[u][j] = load4(dr[j], v, k1);
+      for (int j = 0; j < NB; ++j) to.b[u][j] = load4(dr[j], v, k1);
     }
+  };
+  fetch(next, k0);
+  for (int k = k0; k < k1; k += 16 * AHEAD) {
+    in = next;
+    if (k + 16 * AHEAD < k1) fetch(next, k + 16 * AHEAD);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
@@ -1062,7 +1080,7 @@ __global__ __launch_bounds__(256) void ce_few_dx_kernel(const float* __restrict_
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][e][t], b[u][j][e], acc[t][j], 0, 0, 0);
+          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(in.a[u][e][t], in.b[u][j][e], acc[t][j], 0, 0, 0);
   }
   const float inv = d_scale[1];
   const int c0 = c - 4 * l15 + 16 * lj;                       // acc[t][j][r]: column c0 + 4 r + t
@@ -1481,10 +1499,10 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.n_pad = up_to(a->N, ROW_PAD);
   p.d_pad = up_to(a->D, K_PAD);
   // waves enough to fill the chip, sums over at most 2048 features, partial logits of at most 64 MiB
-  const int64_t waves = (a->V + 31) / 32, want = (2047 + waves) / waves, most_parts = (a->D + 255) / 256, long_sums = (a->D + 2047) / 2048;
+  const int64_t waves = (a->V + 31) / 32, want = (4095 + waves) / waves, most_parts = (a->D + 255) / 256, long_sums = (a->D + 2047) / 2048;
   const int64_t parts = want > most_parts ? most_parts : want < long_sums ? long_sums : want;
   p.ldz = up_to(a->V, 4);
-  p.few = p.f32 && a->N <= FEW_ROWS && parts <= 64 && parts * a->N * p.ldz * 4 <= 64ll << 20 && a->V <= D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256;
+  p.few = p.f32 && a->N <= FEW_ROWS && a->V * a->D >= a->N << 15 && parts <= 64 && parts * a->N * p.ldz * 4 <= 64ll << 20 && a->V <= D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256;
   p.pack_w = !p.few && (p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w));
   p.ldw = p.pack_w ? p.d_pad : a->ldw;
   int64_t at = 0;
@@ -1516,7 +1534,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.z = take((int64_t)p.z_parts * a->N * p.ldz * 4);
     grads_for(a, p);
     if (p.few) {                                      // (as above: waves of 64 columns)
-      const int64_t cols = (a->D + 63) / 64, fill = (2047 + cols) / cols, most_x = (a->V + 63) / 64, cap = most_x < 128 ? most_x : 128;
+      const int64_t cols = (a->D + 63) / 64, fill = (4095 + cols) / cols, most_x = (a->V + 63) / 64, cap = most_x < 128 ? most_x : 128;
       p.dx_split = (int)(fill < cap ? fill : cap);
     }
     p.dx_slabs = p.few || p.dx_split > 1 || p.piece < a->V;
