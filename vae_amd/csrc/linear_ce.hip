@@ -610,68 +610,88 @@ __global__ __launch_bounds__(64 * W_M * W_N, 2) void head_grads_kernel(Gemm dx, 
   else head_gemm<F16, false, false, BM, BN, W_M, W_N, EPI_STORE, false>(dw, smem, block - dx_blocks, (int)gridDim.x - dx_blocks);
 }
 
-// Rows that count, in order: rows[0 .. kept), kept, and the sum of their class weights, by one workgroup (8192 targets at a
-// time, 8 per thread).  An ignored row's loss is written as 0 where losses are returned by row.
-__global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict__ target, int N, int V, int64_t ignore,
-                                                       const float* __restrict__ cw, int* __restrict__ state,
-                                                       float* __restrict__ target_logit, float* __restrict__ loss_rows) {
-  __shared__ int wave_n[16];
+// Rows that count, in order, and the sum of their class weights, by one workgroup (ROWS_AT_ONCE targets at a time: a wave takes
+// 64 in a row, so that what it writes stands together) -> their number.  They go to `table`, or (`write`) to the state, and an ignored row's loss is written as 0 where losses are
+// returned by row.
+constexpr int ROWS_AT_ONCE = 8192, TABLE_ROWS = 4096;
+struct Rows {
+  const int64_t* target;
+  int N, V;
+  int64_t ignore;
+  const float* cw;
+  int* state;
+  float *target_logit, *loss_rows;
+};
+__device__ __forceinline__ int find_rows(const Rows& r, bool write, int* table) {
+  __shared__ int counts[129];                                 // of the waves' 64 targets, in order; then of those ahead of them
   __shared__ double wave_w[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, N = r.N, V = r.V;
   int before = 0;
   double weight = 0;
-  for (int base = 0; base < N; base += 8192) {
-    const int i0 = base + threadIdx.x * 8;
+  for (int base = 0; base < N; base += ROWS_AT_ONCE) {
     int64_t t[8];
-    int mine = 0;
+    uint64_t mask[8];
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      t[j] = i0 + j < N ? target[i0 + j] : ignore;
-      mine += t[j] != ignore;
-    }
-    int run = mine;                                           // inclusive scan over the wave
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(run, o, 64);
-      if (lane >= o) run += u;
-    }
-    __syncthreads();
-    if (lane == 63) wave_n[wave] = run;
-    __syncthreads();
-    int at = before + run - mine, all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) at += wave_n[w];
-      all += wave_n[w];
+      const int i = base + j * 1024 + (int)threadIdx.x;
+      t[j] = i < N ? r.target[i] : r.ignore;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (i0 + j >= N) continue;
-      if (t[j] != ignore) {
-        state[S_ROWS + at] = i0 + j;
-        state[S_ROWS + N + at] = t[j] < 0 || t[j] >= V ? -1 : (int)t[j];
-        target_logit[at] = NAN;                               // stays so where the target is no class
-        ++at;
-        weight += t[j] < 0 || t[j] >= V ? (double)NAN : cw ? (double)cw[t[j]] : 1.0;
-      } else if (loss_rows) {
-        loss_rows[i0 + j] = 0.f;
+      mask[j] = __ballot(t[j] != r.ignore);
+      if (lane == 0) counts[j * 16 + wave] = __popcll(mask[j]);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int a = counts[2 * lane], b = counts[2 * lane + 1];
+      int run = a + b;                                        // inclusive scan over the wave
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(run, o, 64);
+        if (lane >= o) run += u;
+      }
+      counts[2 * lane] = run - a - b;
+      counts[2 * lane + 1] = run - b;
+      if (lane == 63) counts[128] = run;
+    }
+    __syncthreads();
+    const int all = counts[128];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = base + j * 1024 + (int)threadIdx.x, at = before + counts[j * 16 + wave] + __popcll(mask[j] & ((1ull << lane) - 1));
+      if (i >= N) continue;
+      if (t[j] != r.ignore) {
+        if (table) table[at] = i;
+        if (write) {
+          const bool real = t[j] >= 0 && t[j] < V;
+          r.state[S_ROWS + at] = i;
+          r.state[S_ROWS + N + at] = real ? (int)t[j] : -1;
+          r.target_logit[at] = NAN;                           // stays so where the target is no class
+          weight += !real ? (double)NAN : r.cw ? (double)r.cw[t[j]] : 1.0;
+        }
+      } else if (write && r.loss_rows) {
+        r.loss_rows[i] = 0.f;
       }
     }
     before += all;
   }
+  if (write) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) weight += __shfl_xor(weight, o, 64);
+    for (int o = 32; o > 0; o >>= 1) weight += __shfl_xor(weight, o, 64);
+    if (lane == 0) wave_w[wave] = weight;
+  }
   __syncthreads();
-  if (lane == 0) wave_w[wave] = weight;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  if (write && threadIdx.x == 0) {
     double w = 0;
     for (int i = 0; i < 16; ++i) w += wave_w[i];
-    state[S_KEPT] = before;
-    state[S_DONE] = 0;
-    reinterpret_cast<float*>(state)[S_TOTAL] = (float)w;
+    r.state[S_KEPT] = before;
+    r.state[S_DONE] = 0;
+    reinterpret_cast<float*>(r.state)[S_TOTAL] = (float)w;
   }
+  return before;
 }
+__global__ __launch_bounds__(1024) void ce_rows_kernel(Rows r) { find_rows(r, true, nullptr); }
 
 // g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to); by one workgroup
 struct Upstream {
@@ -714,10 +734,9 @@ struct Pack {
   uint16_t* out;
   int64_t plane;
 };
-template <typename T> __device__ __forceinline__ void pack_rows(const Pack& p, int block, int D, int64_t ldo) {
+template <typename T, typename Index>
+__device__ __forceinline__ void pack_rows(const Pack& p, int block, int D, int64_t ldo, int kept, int padded, Index&& index) {
   const int per = (int)(ldo / 8);
-  const int kept = p.state ? p.state[S_KEPT] : p.rows;
-  const int padded = p.state ? (kept + ROW_PAD - 1) / ROW_PAD * ROW_PAD : p.rows;
   const int64_t all = (int64_t)padded * per;
   for (int64_t i = (int64_t)block * 1024 + threadIdx.x; i < all; i += (int64_t)p.blocks * 1024) {
     const int row = (int)(i / per), c = (int)(i - (int64_t)row * per) * 8;
@@ -729,7 +748,7 @@ template <typename T> __device__ __forceinline__ void pack_rows(const Pack& p, i
 #pragma unroll
     for (int q = 0; q < Q; ++q) v.q[q] = (u4)0;
     if (row < kept) {
-      const T* from = reinterpret_cast<const T*>(p.src) + (int64_t)(p.state ? p.state[S_ROWS + row] : row) * p.ld + c;
+      const T* from = reinterpret_cast<const T*>(p.src) + (int64_t)index(row) * p.ld + c;
       if (c + 8 <= D) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) v.q[q] = reinterpret_cast<const u4_any*>(from)[q];
@@ -754,12 +773,24 @@ template <typename T> __device__ __forceinline__ void pack_rows(const Pack& p, i
     }
   }
 }
-// All that comes ahead of the products, in one launch: the row factors, x, and w where it has to be packed.
-template <typename T> __global__ __launch_bounds__(1024) void ce_pack_kernel(Upstream u, Pack x, Pack w, int D, int64_t ldo) {
+// All that comes ahead of the products, in one launch: the row factors, x, and w where it has to be packed.  Where the rows that
+// count, of at most TABLE_ROWS, are to be found first, every workgroup of x does so for itself: a launch less (loss of 2000 x 300 x
+// 50 19.5 us and 21.2, called eagerly 26 and 30; of 8192 x 1024 x 500 47.8 and 43.8).
+template <typename T> __global__ __launch_bounds__(1024) void ce_pack_kernel(Rows r, Upstream u, Pack x, Pack w, int D, int64_t ldo) {
+  __shared__ int table[TABLE_ROWS];
   int block = blockIdx.x;
-  if (u.up && block-- == 0) upstream(u);
-  else if (block < x.blocks) pack_rows<T>(x, block, D, ldo);
-  else pack_rows<T>(w, block - x.blocks, D, ldo);
+  const auto padded = [](int kept) { return (kept + ROW_PAD - 1) / ROW_PAD * ROW_PAD; };
+  if (u.up && block-- == 0) {
+    upstream(u);
+  } else if (block >= x.blocks) {
+    pack_rows<T>(w, block - x.blocks, D, ldo, w.rows, w.rows, [](int row) { return row; });
+  } else if (r.target) {
+    const int kept = find_rows(r, block == 0, table);
+    pack_rows<T>(x, block, D, ldo, kept, padded(kept), [&](int row) { return table[row]; });
+  } else {
+    const int kept = x.state[S_KEPT];
+    pack_rows<T>(x, block, D, ldo, kept, padded(kept), [&](int row) { return x.state[S_ROWS + row]; });
+  }
 }
 
 // Sum and mean of the losses: every workgroup leaves the sum of its rows' (`share`, over its threads), and the one that finishes
@@ -869,19 +900,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(con
                                                                             int* __restrict__ state, int N, int V, const float* __restrict__ cw,
                                                                             int reduction, double* __restrict__ sums, float* __restrict__ loss) {
   constexpr int RPW = TPR < 256 ? 256 / TPR : 1, WAVES = TPR / 64;
-  static_assert(TPR % 64 == 0, "whole waves");
-  __shared__ float2 red[RPW * WAVES];
-  __shared__ float hits[RPW];
+  static_assert(TPR == 64 || RPW == 1, "a row to a wave or to a workgroup");
+  __shared__ float2 red[WAVES];
+  __shared__ float target_hit;
   const int kept = state[S_KEPT], blocks = min(max((kept + RPW - 1) / RPW, 1), (int)gridDim.x);
   if ((int)blockIdx.x >= blocks) return;
   const int sub = threadIdx.x / TPR, lane = threadIdx.x % TPR;
   double share = 0;
   for (int base = blockIdx.x * RPW; base < kept; base += blocks * RPW) {
     const int row = base + sub, t = row < kept ? state[S_ROWS + N + row] : -1;
-    __syncthreads();
-    if (lane == 0) hits[sub] = NAN;                           // stays so where the target is no class
-    __syncthreads();
-    float top = -INFINITY, sum = 0.f;
+    float top = -INFINITY, sum = 0.f, hit = NAN;              // (stays so where the target is no class)
     if (row < kept) {
       const float* p = slabs + (int64_t)row * ldz;
       for (int c = lane * 4; c < V; c += TPR * 4) {
@@ -891,7 +919,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(con
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (c + e < V) sum += exp_fine(z[e] - ref);
-          if (c + e == t) hits[sub] = z[e];
+          hit = c + e == t ? z[e] : hit;
         }
         top = m;
       }
@@ -902,19 +930,28 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void ce_slab_loss_kernel(con
       sum = sum * exp_fine(top - ref) + os * exp_fine(ot - ref);
       top = m;
     }
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
-    __syncthreads();
+    const int owner = t < 0 ? 0 : (t >> 2) % TPR;             // (whose hit is NaN where t < 0)
+    if (WAVES == 1) {
+      hit = __shfl(hit, owner, 64);
+    } else {
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(top, sum);
+      if (lane == owner) target_hit = hit;
+      __syncthreads();
+      if (lane == 0) {
+        hit = target_hit;
+        float m = top;
+        for (int i = 1; i < WAVES; ++i) m = fmaxf(m, red[i].x);
+        const float ref = m == -INFINITY ? 0.f : m;
+        sum *= exp_fine(top - ref);
+        for (int i = 1; i < WAVES; ++i) sum += red[i].y * exp_fine(red[i].x - ref);
+        top = m;
+      }
+    }
     if (lane == 0 && row < kept) {
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < WAVES; ++i) m = fmaxf(m, red[sub * WAVES + i].x);
-      const float ref = m == -INFINITY ? 0.f : m;
-      sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < WAVES; ++i) sum += red[sub * WAVES + i].y * exp_fine(red[sub * WAVES + i].x - ref);
-      const float lse = m + logf(sum);
+      const float lse = top + logf(sum);
       reinterpret_cast<float*>(state)[S_ROWS + 2 * N + row] = lse;
-      const float v = (lse - hits[sub]) * (!cw || t < 0 ? 1.f : cw[t]);
+      const float v = (lse - hit) * (!cw || t < 0 ? 1.f : cw[t]);
       if (reduction == VAE_CE_NONE) loss[state[S_ROWS + row]] = v;
       share += (double)v;
     }
@@ -1589,7 +1626,7 @@ void finish(const Finish& f, int dtype, hipStream_t st) {
   else ce_finish_kernel<_Float16><<<grid, 256, 0, st>>>(f);
 }
 
-void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, const Upstream& u, hipStream_t st) {
+void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, const Rows& r, const Upstream& u, hipStream_t st) {
   auto blocks = [&](int64_t rows) {
     const int64_t b = (rows * (p.d_pad / 8) + 1023) / 1024;
     return (int)(b < 1024 ? b : 1024);
@@ -1597,8 +1634,8 @@ void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, 
   const Pack x = {a->x, a->ldx, state, (int)a->N, blocks(p.n_pad), reinterpret_cast<uint16_t*>(ws + p.x), p.n_pad * p.d_pad};
   const Pack w = {a->w, a->ldw, nullptr, (int)a->V, p.pack_w ? blocks(a->V) : 0, reinterpret_cast<uint16_t*>(ws + p.w), a->V * p.d_pad};
   const int grid = (u.up ? 1 : 0) + x.blocks + w.blocks;
-  if (p.f32) ce_pack_kernel<float><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
-  else ce_pack_kernel<uint16_t><<<grid, 1024, 0, st>>>(u, x, w, (int)a->D, p.d_pad);
+  if (p.f32) ce_pack_kernel<float><<<grid, 1024, 0, st>>>(r, u, x, w, (int)a->D, p.d_pad);
+  else ce_pack_kernel<uint16_t><<<grid, 1024, 0, st>>>(r, u, x, w, (int)a->D, p.d_pad);
 }
 
 #define VAE_FEW(KERNEL, ...)                                    \
@@ -1684,10 +1721,11 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   int* s = reinterpret_cast<int*>(state);
   hipStream_t st = (hipStream_t)stream;
   float* tl = reinterpret_cast<float*>(ws + p.tlogit);
-  ce_rows_kernel<<<1, 1024, 0, st>>>(a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl,
-                                     reduction == VAE_CE_NONE ? loss : nullptr);
+  const Rows rows = {a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, reduction == VAE_CE_NONE ? loss : nullptr};
+  const bool apart = p.few || a->N > TABLE_ROWS;
+  if (apart) ce_rows_kernel<<<1, 1024, 0, st>>>(rows);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
-  if (!p.few) pack(a, p, ws, s, Upstream{}, st);
+  if (!p.few) pack(a, p, ws, s, apart ? Rows{} : rows, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   Gemm g = logits_gemm(a, p, ws, s);
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
@@ -1748,7 +1786,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   float *slabs = reinterpret_cast<float*>(ws + p.slabs), *sums = reinterpret_cast<float*>(ws + p.d_sums);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
-  pack(a, p, ws, s, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
+  pack(a, p, ws, s, Rows{}, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
   for (int64_t v0 = 0; v0 < a->V; v0 += p.piece) {
     const int64_t n_v = a->V - v0 < p.piece ? a->V - v0 : p.piece;
