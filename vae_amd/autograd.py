@@ -144,9 +144,6 @@ class LogLikFn(Function):
         return None, dmu, dth, dpi, None
 
 
-_GATED_NORM_GRADS = ("r", "b", "gate") + ops.GATED_NORM_VECTORS
-
-
 class GatedResidualNormFn(Function):
     """(y, h) = (r + scale * act(gate) * norm(b), norm(y)) over rows, in one pass each way (ops.gated_norm_fwd / _bwd).
     y and the (N, 4) row statistics are kept for the backward pass; r is not."""
@@ -163,15 +160,13 @@ class GatedResidualNormFn(Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh):
-        y, b, stats, gate, post_weight, post_bias, scale, norm_weight, norm_bias = ctx.saved_tensors
+        y, b, stats, gate, *vectors = ctx.saved_tensors
         if dy is None and dh is None:
             return (None,) * 11
-        dy, dh = (None if t is None else (t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()) for t in (dy, dh))
-        want = [n for n, need in zip(_GATED_NORM_GRADS, ctx.needs_input_grad) if need]
-        kind, gate_act, eps = ctx.how
-        g = ops.gated_norm_bwd(dy, dh, y, b, stats, gate, post_weight=post_weight, post_bias=post_bias, scale=scale,
-                               norm_weight=norm_weight, norm_bias=norm_bias, kind=kind, gate_act=gate_act, eps=eps, want=want)
-        return tuple(g.get(n) if n in want else None for n in _GATED_NORM_GRADS) + (None, None, None)
+        dy, dh = (t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (dy, dh))
+        need = ctx.needs_input_grad
+        g = ops.gated_norm_grads(dy, dh, y, b, stats, gate, vectors, *ctx.how, need[2], need[3:8])
+        return (g[0] if need[0] else None, g[1] if need[1] else None, *g[2:], None, None, None)
 
 
 class LinearCrossEntropyFn(Function):

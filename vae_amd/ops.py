@@ -693,6 +693,7 @@ GATED_NORM_MAX_D = 16384
 
 # what the C side reads as vae_gated_norm (include/vae_amd.h): packed at once, a ctypes structure costs three times that
 _GATED_NORM = struct.Struct("=2q5if26Q")
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -712,7 +713,7 @@ _HERE = _Here()
 
 def _on(device: torch.device):
     """Context in which ``device`` is the current one (a launch goes to its stream)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)
 
 
 def _at(t: Optional[torch.Tensor]) -> int:
@@ -783,7 +784,8 @@ def gated_norm_fwd(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.Tensor
     mode, f32 = _gated_norm_checks(r, b, gate, vectors, kind, gate_act, eps)
     (N, D), device = b.shape, b.device
     with _on(device):
-        y, h = torch.empty((N, D), dtype=b.dtype, device=device), torch.empty((N, D), dtype=b.dtype, device=device)
+        y = b.new_empty((N, D))
+        h = torch.empty_like(y)
         stats = torch.empty((N, 4), dtype=torch.float32, device=device) if want_stats else None
         rc = lib.vae_gated_norm_fwd(_GATED_NORM.pack(
             N, D, FLOAT_DTYPES[b.dtype], f32, NORM_KINDS[kind], mode, GATE_ACTS[gate_act], eps, r.data_ptr(), r.stride(0), b.data_ptr(),
@@ -800,46 +802,45 @@ def gated_norm_bwd(dy: Optional[torch.Tensor], dh: Optional[torch.Tensor], y: to
                    norm_weight: Optional[torch.Tensor] = None, norm_bias: Optional[torch.Tensor] = None, kind: str = "rms",
                    gate_act: str = "sigmoid", eps: float = 1e-5, want=("gate",) + GATED_NORM_VECTORS):
     """-> dict of gradients: r, b, and those of ``want`` whose tensor is given.  ``dy`` / ``dh`` None: zero."""
+    got = gated_norm_grads(dy, dh, y, b, stats, gate, (post_weight, post_bias, scale, norm_weight, norm_bias), kind, gate_act, eps,
+                           "gate" in want, [k in want for k in GATED_NORM_VECTORS])
+    return {k: t for k, t in zip(("r", "b", "gate") + GATED_NORM_VECTORS, got) if t is not None}
+
+
+def gated_norm_grads(dy, dh, y, b, stats, gate, vectors, kind, gate_act, eps, want_gate, want):
+    """``gated_norm_bwd`` -> gradients of r, b, the gate and the five vectors, None for those that are not there or not wanted."""
     lib = _lib.load()
-    vectors = (post_weight, post_bias, scale, norm_weight, norm_bias)
     mode, f32 = _gated_norm_checks(None, b, gate, vectors, kind, gate_act, eps)
-    (N, D), dtype, device = b.shape, b.dtype, b.device
-    for t, name, shape, of in ((y, "y", (N, D), dtype), (stats, "stats", (N, 4), torch.float32), (dy, "dy", (N, D), dtype),
-                               (dh, "dh", (N, D), dtype)):
-        if t is None:
-            continue
-        dense = t.is_contiguous() if name in ("y", "stats") else (D == 1 or N == 0 or t.stride(1) == 1)
-        if t.shape != shape or t.dtype != of or t.device != device or not dense:
-            raise ValueError(f"vae_amd.ops.gated_norm_bwd: {name} must be {shape} {of} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    shape, dtype, device = b.shape, b.dtype, b.device
+    N, D = shape
+    if y.shape != shape or y.dtype != dtype or y.device != device or not y.is_contiguous():
+        raise ValueError(f"vae_amd.ops.gated_norm_bwd: y must be contiguous {tuple(shape)} {dtype} on {device}, got {tuple(y.shape)} {y.dtype}")
+    if stats.shape != (N, 4) or stats.dtype != torch.float32 or stats.device != device or not stats.is_contiguous():
+        raise ValueError(f"vae_amd.ops.gated_norm_bwd: stats must be contiguous {(N, 4)} float32, got {tuple(stats.shape)} {stats.dtype}")
+    for t, name in ((dy, "dy"), (dh, "dh")):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(1) != 1 and D > 1 and N)):
+            raise ValueError(f"vae_amd.ops.gated_norm_bwd: {name} must be {tuple(shape)} {dtype} on {device}, got {tuple(t.shape)} {t.dtype}")
     with _on(device):
-        dr, db = torch.empty((N, D), dtype=dtype, device=device), torch.empty((N, D), dtype=dtype, device=device)
-        out = {"r": dr, "b": db}
-        dgate = None
-        if gate is not None and "gate" in want:
-            out["gate"] = dgate = torch.empty((N, D if mode == 2 else 1), dtype=dtype, device=device)
-        # the gradients of the vectors are rows of one allocation; dnorm_weight, dnorm_bias, dscale, dpost_weight, dpost_bias
-        names = [k for k, t in zip(GATED_NORM_VECTORS, vectors) if t is not None and k in want]
-        at = dict.fromkeys(GATED_NORM_VECTORS, 0)
-        nbytes, ws = 0, 0
-        if names:
-            sums = (torch.empty if N else torch.zeros)((len(names), D), dtype=torch.float32 if f32 else dtype, device=device)
-            out.update(zip(names, sums.unbind(0)))
-            for k in names:
-                at[k] = out[k].data_ptr()
+        dr, db, dgate = torch.empty_like(y), torch.empty_like(y), None
+        if gate is not None and want_gate:
+            dgate = torch.empty_like(y) if mode == 2 else y.new_empty((N, 1))
+        dv = [torch.empty_like(t) if t is not None and w else None for t, w in zip(vectors, want)]
         if N == 0:
-            return out
-        if names:                                       # scratch of this call alone: streams and captured graphs share none
+            return (dr, db, dgate, *(None if t is None else t.zero_() for t in dv))
+        nbytes, ws = 0, 0
+        if any(t is not None for t in dv):              # scratch of this call alone: streams and captured graphs share none
             nbytes = lib.vae_gated_norm_workspace_bytes(N, D, FLOAT_DTYPES[dtype])
-            scratch = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+            scratch = stats.new_empty(nbytes // 4)
             ws = scratch.data_ptr()
+        post_weight, post_bias, scale, norm_weight, norm_bias = map(_at, dv)
         rc = lib.vae_gated_norm_bwd(_GATED_NORM.pack(
             N, D, FLOAT_DTYPES[dtype], f32, NORM_KINDS[kind], mode, GATE_ACTS[gate_act], eps, 0, 0, b.data_ptr(), b.stride(0), _at(gate),
             0 if gate is None else gate.stride(0), *map(_at, vectors), y.data_ptr(), 0, stats.data_ptr(), _at(dy),
             0 if dy is None else dy.stride(0), _at(dh), 0 if dh is None else dh.stride(0), dr.data_ptr(), db.data_ptr(), _at(dgate),
-            at["norm_weight"], at["norm_bias"], at["scale"], at["post_weight"], at["post_bias"]), ws, nbytes, _raw_stream(device.index))
+            norm_weight, norm_bias, scale, post_weight, post_bias), ws, nbytes, _raw_stream(device.index))
     if rc:
         _lib.check(rc, "gated_norm_bwd")
-    return out
+    return (dr, db, dgate, *dv)
 
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
