@@ -263,19 +263,20 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
         if len(decay) != n:
             raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(decay)} weight decays")
     table: List[Union[int, float]] = []
-    at, live = 0, []
+    at, live, index = 0, [], dev.index
     for p, g, wd in zip(params, grads, decay):
         count = p.numel()
         if g is not None and count:
             dtype = p.dtype
-            if dtype not in _ADAMW_DTYPES or g.dtype != dtype:
+            kind = _ADAMW_DTYPES.get(dtype)
+            if kind is None or g.dtype is not dtype:
                 raise TypeError(f"vae_amd.optim.multi_tensor_adamw_: a parameter of {p.dtype} with a gradient of {g.dtype}; "
                                 "float32, bfloat16 and float16 are supported, both of the same type")
-            if p.device != dev or g.device != dev:
+            if p.get_device() != index or g.get_device() != index:      # (-1: on the CPU)
                 raise RuntimeError(f"vae_amd.optim.multi_tensor_adamw_: parameters, gradients and state must be on {dev}")
             if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
                 raise ValueError("vae_amd.optim.multi_tensor_adamw_: parameters and gradients must be contiguous and of one shape")
-            table += (p.data_ptr(), g.data_ptr(), count, at, wd, _ADAMW_DTYPES[dtype])
+            table += (p.data_ptr(), g.data_ptr(), count, at, wd, kind)
             live.append(p)
         at += -(-count // ADAMW_BLOCK)
     for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
