@@ -639,7 +639,7 @@ int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t wor
  * (V) that are not null, of the operands' type.  Ignored rows take no part at all: their dx is 0 and what their x holds
  * reaches nothing else.  The logits are not kept; the workspace holds a packed copy of x, for fp32 (and for w that is
  * not 16-byte aligned with D and its stride multiples of 8) one of w, up to 512 MiB of logit gradients, and for few rows and
- * classes over many features partial logits of at most 67 MB.  At most 2^24 tiles of 128 x 128 in N x V, N x D and V x D.  Same
+ * classes over many features partial logits of at most 134 MB.  At most 2^24 tiles of 128 x 128 in N x V, N x D and V x D.  Same
  * bits every time.                                                                                                          */
 enum { VAE_CE_NONE = 0, VAE_CE_SUM = 1, VAE_CE_MEAN = 2 };
 typedef struct {
