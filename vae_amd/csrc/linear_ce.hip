@@ -1004,14 +1004,18 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(float* slabs, bool keep,
   if (sums) *reinterpret_cast<f4_any*>(sums + (int64_t)blockIdx.y * ldd + c) = total;
 }
 
-// ---- fp32, at most FEW_ROWS rows: W goes from memory straight into 32-bit matrix instructions ----
+// ---- at most FEW_ROWS rows (fp32) or classes: the long operand goes from memory straight into matrix instructions ----
 // The three terms of W would be written and read again for a handful of rows.  Both kernels are bound by their one read of W; a
 // lane's four consecutive floats are four values of K (or four columns) whose order the other operand shares.  8 x 1024 x 40000:
 // partial logits 38 us = 4.3 TB/s of W, dx 28 us (W partly in the caches), a loss 52 us against 197 with three terms, loss and
 // gradients 211 against 530; 64 x 1024 x 40000 101 against 196 and 364 against 532 (the rows, read by every wave, are then half of
 // the traffic).  Worth its two launches more from V D of some 2^15 N on: 16 x 512 x 2000 61 us against 72, 64 x 512 x 4000 92 and
 // 91, 64 x 100 x 1000 68 and 57.
+// The loss of a head of at most as many classes on many rows reads x in the same way, in every type, where its packed copy would take
+// longer than the product: from 2^21 elements of x on (8192 x 4000 x 10 bf16 50 us and 70, 4096 x 3000 x 30 fp32 43 and 72, 8192 x 1024
+// x 10 bf16 32 and 46; 1000 x 1000 x 40 fp32 30 and 29).
 constexpr int FEW_ROWS = 64;
+constexpr int64_t HEAD_WORK = 1 << 21;
 __device__ __forceinline__ f4_any load4(const float* p, int c, int n) {                // p[c .. c + 4), those from n on as zeros
   if (c + 4 <= n) return *reinterpret_cast<const f4_any*>(p + c);
   f4_any v = {0.f, 0.f, 0.f, 0.f};
@@ -1020,59 +1024,101 @@ __device__ __forceinline__ f4_any load4(const float* p, int c, int n) {         
     if (c + e < n) v[e] = p[c + e];
   return v;
 }
-// partial logits (part, N, ldz): a wave takes 32 classes and all rows, 16 to a tile, over `per` features (a multiple of 64)
-template <int NB>
-__global__ __launch_bounds__(256) void ce_few_z_kernel(const float* __restrict__ w, int64_t ldw, const float* __restrict__ x, int64_t ldx,
+// 16 bytes of a row from feature c on, those from n on as zeros
+template <typename T> __device__ __forceinline__ u4 load16(const T* p, int c, int n) {
+  constexpr int P = 16 / (int)sizeof(T);
+  if (c + P <= n) return *reinterpret_cast<const u4_any*>(p + c);
+  union {
+    T t[P];
+    u4 q;
+  } v;
+  v.q = (u4)0;
+#pragma unroll
+  for (int e = 0; e < P; ++e)
+    if (c + e < n) v.t[e] = p[c + e];
+  return v.q;
+}
+template <typename T> __device__ __forceinline__ f32x4 mma16(u4 a, u4 b, f32x4 c) {      // 16 bytes of K to a lane
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  } else {
+    return mma<__is_same(T, _Float16)>(a, b, c);
+  }
+}
+// Partial logits (part, N, ldz) straight from memory.  A wave takes 32 rows of the long operand and all of the short one, at most 64
+// rows in tiles of 16, over `per` features (a multiple of 64).  HEAD: x is the long one and W the short, otherwise W is long.
+template <typename T, int NB, bool HEAD>
+__global__ __launch_bounds__(256) void ce_few_z_kernel(const T* __restrict__ w, int64_t ldw, const T* __restrict__ x, int64_t ldx,
                                                        const int* __restrict__ state, int N, int D, int V, int per, float* __restrict__ slabs,
                                                        int64_t ldz) {
   const int kept = state[S_KEPT], lane = threadIdx.x & 63, l15 = lane & 15, lj = lane >> 4;
-  const int v0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 32, k0 = blockIdx.y * per, k1 = min(k0 + per, D);
-  if (kept == 0 || v0 >= V) return;
-  const float *wr[2], *xr[NB];
+  const int m0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 32, k0 = blockIdx.y * per, k1 = min(k0 + per, D);
+  if (kept == 0 || m0 >= (HEAD ? kept : V)) return;
+  const auto row_of_x = [&](int n) { return x + (int64_t)state[S_ROWS + min(n, kept - 1)] * ldx; };
+  const auto row_of_w = [&](int v) { return w + (int64_t)min(v, V - 1) * ldw; };
+  const T *ar[2], *br[NB];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) wr[t] = w + (int64_t)min(v0 + 16 * t + l15, V - 1) * ldw;
+  for (int t = 0; t < 2; ++t) ar[t] = HEAD ? row_of_x(m0 + 16 * t + l15) : row_of_w(m0 + 16 * t + l15);
 #pragma unroll
-  for (int j = 0; j < NB; ++j) xr[j] = x + (int64_t)state[S_ROWS + min(16 * j + l15, kept - 1)] * ldx;
-  f32x4 acc[2][NB];
+  for (int j = 0; j < NB; ++j) br[j] = HEAD ? row_of_w(16 * j + l15) : row_of_x(16 * j + l15);
+  constexpr int PIECE = 16 / (int)sizeof(T), GROUP = 4 * PIECE;
+  constexpr int AHEAD = NB <= 2 ? 4 : 2;                      // groups of features at a time, the next ones on their way
+  f32x4 acc[AHEAD][2][NB];                                    // (a sum for each: a 32-bit one rounds at every product)
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[t][j] = (f32x4)0.f;
-  constexpr int AHEAD = NB <= 2 ? 4 : 2;                      // groups of 16 features at a time, the next ones on their way
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[u][t][j] = (f32x4)0.f;
   struct In {
-    f4_any a[AHEAD][2], b[AHEAD][NB];
+    u4 a[AHEAD][2], b[AHEAD][NB];
   } in, next;
   auto fetch = [&](In& to, int k) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int c = k + 16 * u + 4 * lj;
+      const int c = k + GROUP * u + PIECE * lj;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) to.a[u][t] = load4(wr[t], c, k1);
+      for (int t = 0; t < 2; ++t) to.a[u][t] = load16(ar[t], c, k1);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) to.b[u][j] = load4(xr[j], c, k1);
+      for (int j = 0; j < NB; ++j) to.b[u][j] = load16(br[j], c, k1);
     }
   };
   fetch(next, k0);
-  for (int k = k0; k < k1; k += 16 * AHEAD) {
+  for (int k = k0; k < k1; k += GROUP * AHEAD) {
     in = next;
-    if (k + 16 * AHEAD < k1) fetch(next, k + 16 * AHEAD);
+    if (k + GROUP * AHEAD < k1) fetch(next, k + GROUP * AHEAD);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(in.a[u][t][e], in.b[u][j][e], acc[t][j], 0, 0, 0);
+        for (int j = 0; j < NB; ++j) acc[u][t][j] = mma16<T>(in.a[u][t], in.b[u][j], acc[u][t][j]);
   }
 #pragma unroll
+  for (int h = AHEAD / 2; h > 0; h >>= 1)
+#pragma unroll
+    for (int u = 0; u < h; ++u)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[u][t][j] += acc[u + h][t][j];
+  float* out = slabs + (int64_t)blockIdx.y * N * ldz;
+#pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const int n = 16 * j + l15;
-    if (n >= kept) continue;
+    const int n = 16 * j + l15;                               // acc[0][t][j][r]: row m0 + 16 t + 4 lj + r of the long operand, n of the short
+    if (n >= (HEAD ? V : kept)) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int v = v0 + 16 * t + 4 * lj;
-      if (v < V) *reinterpret_cast<f32x4*>(slabs + ((int64_t)blockIdx.y * N + n) * ldz + v) = acc[t][j];       // (ldz: V in whole fours)
+      const int m = m0 + 16 * t + 4 * lj;
+      if constexpr (HEAD) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m + r < kept) out[(int64_t)(m + r) * ldz + n] = acc[0][t][j][r];
+      } else if (m < V) {
+        *reinterpret_cast<f32x4*>(out + (int64_t)n * ldz + m) = acc[0][t][j];       // (ldz: V in whole fours)
+      }
     }
   }
 }
@@ -1493,7 +1539,7 @@ struct Plan {
   int64_t n_pad, d_pad, ldw;                          // packed x: (n_pad, d_pad); W as it is, or packed to (V, d_pad)
   int64_t planes;
   int64_t piece;                                      // classes whose d is held at a time (a multiple of 256)
-  bool few;                                           // fp32, few rows: W as it is
+  bool few, head;                                     // fp32, few rows: W as it is; few classes (of a loss): x as it is
   Tiles z_tiles, d_tiles;                             // (of a pass)
   int z_parts;                                        // slabs of partial logits; 0: the product's epilogue finishes them
   int64_t ldz;                                        // of partial logits
@@ -1537,11 +1583,17 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.n_pad = up_to(a->N, ROW_PAD);
   p.d_pad = up_to(a->D, K_PAD);
   // waves enough to fill the chip, sums over at most 2048 features, partial logits of at most 64 MiB
-  const int64_t waves = (a->V + 31) / 32, want = (4095 + waves) / waves, most_parts = (a->D + 255) / 256, long_sums = (a->D + 2047) / 2048;
-  const int64_t parts = want > most_parts ? most_parts : want < long_sums ? long_sums : want;
   p.ldz = up_to(a->V, 4);
-  p.few = p.f32 && a->N <= FEW_ROWS && a->V * a->D >= a->N << 15 && parts <= 64 && parts * a->N * p.ldz * 4 <= 64ll << 20 && a->V <= D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256;
-  p.pack_w = !p.few && (p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w));
+  const auto parts_for = [&](int64_t rows) {
+    const int64_t waves = (rows + 31) / 32, want = (4095 + waves) / waves, most = (a->D + 255) / 256, least = (a->D + 2047) / 2048;
+    const int64_t parts = want > most ? most : want < least ? least : want;
+    return (int)(parts <= 64 && parts * a->N * p.ldz * 4 <= 64ll << 20 ? parts : 0);
+  };
+  const int few_parts = parts_for(a->V);
+  p.few = p.f32 && a->N <= FEW_ROWS && a->V * a->D >= a->N << 15 && few_parts &&
+          a->V <= D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256;
+  p.head = !p.few && !bwd && a->V <= FEW_ROWS && a->N * a->D >= HEAD_WORK && parts_for(a->N);
+  p.pack_w = !p.few && !p.head && (p.f32 || a->D % 8 || a->ldw % 8 || !vae_aligned16(a->w));
   p.ldw = p.pack_w ? p.d_pad : a->ldw;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1553,7 +1605,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   p.w = take(p.pack_w ? p.planes * a->V * p.d_pad * 2 : 0);
   if (!bwd) {
     p.z_tiles = tiles_for(a->V, a->N, a->D, p.f32, 8.0, 0.0);
-    p.z_parts = p.few ? (int)parts : p.z_tiles.split > 1 ? p.z_tiles.split : 0;
+    p.z_parts = p.few ? few_parts : p.head ? parts_for(a->N) : p.z_tiles.split > 1 ? p.z_tiles.split : 0;
     p.partial = take(p.z_parts ? p.z_parts * a->N * p.ldz * 4 : up_to(a->V, 128) / 128 * p.n_pad * 8);
     p.tlogit = take(p.n_pad * 4);
     p.sums = take(p.n_pad * 8);
@@ -1567,7 +1619,7 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
     p.piece = up_to((most + pieces - 1) / pieces, 256);
     p.d = take(p.planes * p.n_pad * p.piece * 2);
     p.d_tiles = tiles_for(p.piece, a->N, a->D, p.f32, p.f32 ? 55.0 : 12.0, 5.0);
-    p.z_parts = p.few ? (int)parts : p.d_tiles.split > 1 ? p.d_tiles.split : 0;
+    p.z_parts = p.few ? few_parts : p.d_tiles.split > 1 ? p.d_tiles.split : 0;
     p.sum_rows = p.z_parts ? SLAB_ROWS : p.d_tiles.big ? 256 : 128;
     p.z = take((int64_t)p.z_parts * a->N * p.ldz * 4);
     grads_for(a, p);
@@ -1639,21 +1691,22 @@ void pack(const vae_linear_ce* a, const Plan& p, uint8_t* ws, const int* state, 
   else ce_pack_kernel<uint16_t><<<grid, 1024, 0, st>>>(r, u, x, w, (int)a->D, p.d_pad);
 }
 
-#define VAE_FEW(KERNEL, ...)                                    \
-  if (a->N <= 16) KERNEL<1><<<grid, 256, 0, st>>>(__VA_ARGS__); \
-  else if (a->N <= 32) KERNEL<2><<<grid, 256, 0, st>>>(__VA_ARGS__); \
-  else KERNEL<4><<<grid, 256, 0, st>>>(__VA_ARGS__)
-void few_logits(const vae_linear_ce* a, const Plan& p, const int* state, float* slabs, hipStream_t st) {
-  const int per = (int)up_to((a->D + p.z_parts - 1) / p.z_parts, 64);
-  const dim3 grid((unsigned)((a->V + 127) / 128), (unsigned)p.z_parts);
-  VAE_FEW(ce_few_z_kernel, (const float*)a->w, p.ldw, (const float*)a->x, a->ldx, state, (int)a->N, (int)a->D, (int)a->V, per, slabs, p.ldz);
+template <typename T, bool HEAD> void few_logits(const vae_linear_ce* a, const Plan& p, const int* state, float* slabs, hipStream_t st) {
+  const int per = (int)up_to((a->D + p.z_parts - 1) / p.z_parts, 64), N = (int)a->N, D = (int)a->D, V = (int)a->V, few = HEAD ? V : N;
+  const dim3 grid((unsigned)(((HEAD ? a->N : a->V) + 127) / 128), (unsigned)p.z_parts);
+  const T *w = reinterpret_cast<const T*>(a->w), *x = reinterpret_cast<const T*>(a->x);
+  if (few <= 16) ce_few_z_kernel<T, 1, HEAD><<<grid, 256, 0, st>>>(w, a->ldw, x, a->ldx, state, N, D, V, per, slabs, p.ldz);
+  else if (few <= 32) ce_few_z_kernel<T, 2, HEAD><<<grid, 256, 0, st>>>(w, a->ldw, x, a->ldx, state, N, D, V, per, slabs, p.ldz);
+  else ce_few_z_kernel<T, 4, HEAD><<<grid, 256, 0, st>>>(w, a->ldw, x, a->ldx, state, N, D, V, per, slabs, p.ldz);
 }
 void few_dx(const vae_linear_ce* a, const Plan& p, const int* state, const float* d, const float* d_scale, float* slabs, hipStream_t st) {
-  const int per = (int)up_to((a->V + p.dx_split - 1) / p.dx_split, 16);
+  const int per = (int)up_to((a->V + p.dx_split - 1) / p.dx_split, 16), N = (int)a->N, D = (int)a->D, V = (int)a->V;
   const dim3 grid((unsigned)((a->D + 255) / 256), (unsigned)p.dx_split);
-  VAE_FEW(ce_few_dx_kernel, (const float*)a->w, p.ldw, d, p.ldz, state, (int)a->N, (int)a->D, (int)a->V, per, d_scale, slabs);
+  const float* w = reinterpret_cast<const float*>(a->w);
+  if (N <= 16) ce_few_dx_kernel<1><<<grid, 256, 0, st>>>(w, a->ldw, d, p.ldz, state, N, D, V, per, d_scale, slabs);
+  else if (N <= 32) ce_few_dx_kernel<2><<<grid, 256, 0, st>>>(w, a->ldw, d, p.ldz, state, N, D, V, per, d_scale, slabs);
+  else ce_few_dx_kernel<4><<<grid, 256, 0, st>>>(w, a->ldw, d, p.ldz, state, N, D, V, per, d_scale, slabs);
 }
-#undef VAE_FEW
 
 int check(const vae_linear_ce* a, const char* who) {
   VAE_REQUIRE(a, "%s: null arguments", who);
@@ -1723,10 +1776,10 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   hipStream_t st = (hipStream_t)stream;
   float* tl = reinterpret_cast<float*>(ws + p.tlogit);
   const Rows rows = {a->target, (int)a->N, (int)a->V, a->ignore_index, a->class_weight, s, tl, reduction == VAE_CE_NONE ? loss : nullptr};
-  const bool apart = p.few || a->N > TABLE_ROWS;
+  const bool unpacked = p.few || p.head, apart = unpacked || a->N > TABLE_ROWS;
   if (apart) ce_rows_kernel<<<1, 1024, 0, st>>>(rows);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
-  if (!p.few) pack(a, p, ws, s, apart ? Rows{} : rows, Upstream{}, st);
+  if (!unpacked) pack(a, p, ws, s, apart ? Rows{} : rows, Upstream{}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
   Gemm g = logits_gemm(a, p, ws, s);
   g.partial = reinterpret_cast<float2*>(ws + p.partial);
@@ -1734,7 +1787,11 @@ extern "C" int vae_linear_ce_fwd(const vae_linear_ce* a, int reduction, float* l
   const bool big = p.z_tiles.big;
   double* sums = reinterpret_cast<double*>(ws + p.sums);
   if (p.z_parts) {
-    if (p.few) few_logits(a, p, s, reinterpret_cast<float*>(ws + p.partial), st);
+    float* z = reinterpret_cast<float*>(ws + p.partial);
+    if (p.few) few_logits<float, false>(a, p, s, z, st);
+    else if (p.head && p.f32) few_logits<float, true>(a, p, s, z, st);
+    else if (p.head && a->dtype == VAE_ADAMW_BF16) few_logits<__bf16, true>(a, p, s, z, st);
+    else if (p.head) few_logits<_Float16, true>(a, p, s, z, st);
     else store_logits(g, p.z_tiles, p.ldz, ws + p.partial, a->dtype, st);
     VAE_CHECK_LAUNCH("vae_linear_ce_fwd");
     const float* slabs = reinterpret_cast<const float*>(ws + p.partial);
@@ -1804,7 +1861,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.plane_d = plane_d;
     z.d_sums = dbias ? sums : nullptr;
     if (p.z_parts) {                                    // (one piece: few rows, or classes that do not fill the chip)
-      if (p.few) few_logits(a, p, s, reinterpret_cast<float*>(ws + p.z), st);
+      if (p.few) few_logits<float, false>(a, p, s, reinterpret_cast<float*>(ws + p.z), st);
       else store_logits(z, p.d_tiles, p.ldz, ws + p.z, a->dtype, st);
       VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
       const dim3 grid((unsigned)((up_to(n_v, 64) + 1023) / 1024), (unsigned)(up_to(a->N, 64) / SLAB_ROWS));
