@@ -566,11 +566,11 @@ int vae_l1_penalty(const float* params, float* grads, int64_t n, const vae_adamw
  * state_bits = 8: they are OCP e4m3 bytes, exp_avg_sq holds the ROOT of the second moment, and a code times
  * scales[block] (exp_avg) / scales[n_blocks + block] (exp_avg_sq) is the value.  The first moment is rounded to nearest, the
  * root up or down at random from a hash of (seed, step, flat element index): the same call gives the same bits.  A block with
- * a moment that is not finite decodes as NaN throughout.
+ * a moment or a root that is not finite (the square of a finite gradient may overflow) decodes as NaN throughout.
  * master (nullable): float weights in the state's layout, which are updated instead; params receive their rounding and are
- * not read.  Weights are rounded to nearest.  A norm that is not finite reaches every weight, as with
- * torch.nn.utils.clip_grad_norm_.  Tensors that share memory with each other or with the state are rejected, and so are
- * tensors that share blocks.  The tensor array is read during the call only.
+ * not read.  Weights are rounded to nearest.  As with torch.nn.utils.clip_grad_norm_ a NaN norm makes every weight NaN, and an
+ * infinite one clips to 0: finite gradients count as 0 then, infinite ones give NaN.  Tensors that share memory with each other
+ * or with the state are rejected, and so are tensors that share blocks.  The tensor array is read during the call only.
  * workspace: needed when max_grad_norm > 0 or grad_norm_out is not null.                                            */
 #define VAE_ADAMW_BLOCK 256
 enum { VAE_ADAMW_F32 = 0, VAE_ADAMW_BF16 = 1, VAE_ADAMW_F16 = 2 };

@@ -299,3 +299,38 @@ def test_two_parameters_may_share_a_gradient():
     a.grad = b.grad = torch.randn(300, device="cuda")
     MultiTensorAdamW([a, b], state_bits=32).step()
     assert torch.equal(a, b) and not bool((a == 1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [1e20, -1e20, math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_a_block_that_is_not_finite_decodes_as_nan(bad, dtype):
+    """1e20 is finite and its square is not: m stays, the root is lost.  Zeros and ones beside it share the block's scale."""
+    from vae_amd.optim import MultiTensorAdamW
+    p = torch.ones(1000, device="cuda", dtype=DT[dtype])
+    opt = MultiTensorAdamW([p], state_bits=8)
+    p.grad = torch.ones_like(p)
+    p.grad[300], p.grad[301:310] = bad, 0.0
+    opt.step()
+    m, v = opt.moments(0)
+    inside = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    inside[256:512] = True
+    assert bool(torch.isnan(v[inside]).all()) and bool(torch.isfinite(v[~inside]).all())
+    assert bool((torch.isfinite(m) if math.isfinite(bad) else torch.isnan(m))[inside].all()) and bool(torch.isfinite(m[~inside]).all())
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert bool(torch.isnan(p[inside]).all()) and bool(torch.isfinite(p[~inside]).all())
+
+
+@pytest.mark.gpu
+def test_an_infinite_norm_clips_to_nothing():
+    """As torch's clip_grad_norm_: the coefficient is 0, finite gradients count as zeros and infinite ones become NaN."""
+    from vae_amd.optim import MultiTensorAdamW
+    p = torch.ones(600, device="cuda")
+    opt = MultiTensorAdamW([p], lr=0.5, weight_decay=0.5, state_bits=32, max_grad_norm=1.0)
+    p.grad = torch.ones(600, device="cuda")
+    p.grad[3] = math.inf
+    opt.step()
+    assert float(opt.grad_norm) == math.inf and bool(torch.isnan(p[3]))
+    p[3] = 0.75
+    assert bool((p == 0.75).all())

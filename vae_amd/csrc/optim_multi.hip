@@ -213,8 +213,10 @@ __device__ __forceinline__ void update(T* __restrict__ p, const T* __restrict__ 
         *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(em) + f) = make_uint2(wm[0], wm[1]);
         *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(ev) + f) = make_uint2(wv[0], wv[1]);
         if ((f & (BLK - 1)) == 0) {
-          scales[blk] = top_m * (float)(1.0 / 448.0);
-          scales[n_blocks + blk] = top_u * (float)(1.0 / 448.0);
+          // (an infinity is passed on as NaN: beside a finite gradient's overflowing square the block would otherwise come back as
+          // infinite roots, and weights that do not move any more)
+          scales[blk] = top_m < INFINITY ? top_m * (float)(1.0 / 448.0) : NAN;
+          scales[n_blocks + blk] = top_u < INFINITY ? top_u * (float)(1.0 / 448.0) : NAN;
         }
       }
     } else if (live) {
@@ -286,7 +288,8 @@ __global__ __launch_bounds__(256) void norm_partials_kernel(Tensors t, uint32_t 
   a = block_sum64(a, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = a;
 }
-// norm of grad_scale * g and min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_; a NaN norm is passed on
+// norm of grad_scale * g and min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_: a NaN norm is passed on, an
+// infinite one gives 0
 __global__ __launch_bounds__(256) void norm_finish_kernel(const double* __restrict__ partial, int n, double gscale, double max_norm,
                                                           float* __restrict__ coef, float* __restrict__ norm_out) {
   __shared__ double red[4];
