@@ -633,7 +633,8 @@ int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t wor
  * loss_i = class_weight[t_i] (logsumexp(z_i) - z_i[t_i]), 0 for rows whose target is ignore_index (nn.CrossEntropyLoss of the
  * cell-property heads, task.py:129-137, for heads too wide for vae_cell_heads_step).  reduction: VAE_CE_NONE -> loss (N),
  * VAE_CE_SUM, VAE_CE_MEAN (divided by the sum of the class weights that took part: NaN when no row does) -> loss (1); always
- * float.  A target that is neither a class nor ignore_index makes its row's loss and gradients NaN.
+ * float.  A target that is neither a class nor ignore_index makes its row's loss and dx NaN, and with them what is summed over
+ * rows: the reduced loss, dw and dbias.  The dx of the other rows is that of a batch in which the row is ignored.
  * state: vae_linear_ce_state_bytes(N) bytes that the forward pass writes and the backward pass of the same arguments reads.
  * The backward pass takes the float gradient of the loss ((N) or (1)) and overwrites the dense dx (N, D), dw (V, D) and dbias
  * (V) that are not null, of the operands' type.  Ignored rows take no part at all: their dx is 0 and what their x holds

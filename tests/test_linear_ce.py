@@ -369,3 +369,22 @@ def test_partial_gradients_empty_and_module():
     weighted = LinearCrossEntropyLoss(32, 40, weight=torch.rand(40, device="cuda")).cuda().bfloat16()    # takes the weights along
     weighted(s["x"].bfloat16(), s["target"]).backward()
     assert weighted.linear.weight.grad.dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("n,d,v", [(300, 64, 500), (300, 24, 10), (5000, 700, 12), (9, 2500, 3001)])
+@pytest.mark.parametrize("weight", [False, True])
+def test_a_target_that_is_no_class_spoils_its_row_alone(n, d, v, weight, reduction):
+    """The other rows' gradients are those of the batch without it (fp32: sums may be split another way, see above)."""
+    s = _inputs(n, d, v, "fp32", True, weight, 0.3 if n > 9 else 0.0, seed=n + d)
+    bad = {**s, "target": s["target"].clone()}
+    bad["target"][5], bad["target"][7], s["target"][[5, 7]] = v, -1, -100
+    loss, grads = _run(bad, reduction)
+    assert bool(torch.isnan(loss)) and all(bool(torch.isnan(grads[k]).all()) for k in ("w", "bias"))
+    rows = torch.ones(n, dtype=torch.bool, device="cuda")
+    rows[[5, 7]] = False
+    assert bool(torch.isnan(grads["x"][~rows]).all())
+    grads["x"][~rows] = 0
+    loss, _ = _run(s, reduction)
+    _check(s, reduction, loss, {"x": grads["x"]})

@@ -668,7 +668,7 @@ __device__ __forceinline__ int find_rows(const Rows& r, bool write, int* table) 
           r.state[S_ROWS + at] = i;
           r.state[S_ROWS + N + at] = real ? (int)t[j] : -1;
           r.target_logit[at] = NAN;                           // stays so where the target is no class
-          weight += !real ? (double)NAN : r.cw ? (double)r.cw[t[j]] : 1.0;
+          weight += !real ? 0.0 : r.cw ? (double)r.cw[t[j]] : 1.0;   // (no class has no weight: the divisor stays that of the others)
         }
       } else if (write && r.loss_rows) {
         r.loss_rows[i] = 0.f;
@@ -1362,8 +1362,9 @@ template <typename T, int DM> __global__ __launch_bounds__(1024) void ce_small_f
       hit += __shfl_xor(hit, o, 64);
     }
     if (part || row >= a.N) continue;
-    const float lse = top + logf(sum), c = !kept ? 0.f : t < 0 || t >= a.V ? NAN : a.cw ? a.cw[t] : 1.f;
-    const float loss = kept ? (lse - hit) * c : 0.f;
+    const bool real = kept && t >= 0 && t < a.V;
+    const float lse = top + logf(sum), c = !real ? 0.f : a.cw ? a.cw[t] : 1.f;
+    const float loss = real ? (lse - hit) * c : kept ? NAN : 0.f;
     reinterpret_cast<float*>(a.state)[S_ROWS + 2 * a.N + row] = lse;
     if (a.reduction == VAE_CE_NONE) a.loss[row] = loss;
     total += (double)loss;

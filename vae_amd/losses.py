@@ -116,8 +116,9 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
 
     ``x``, ``w`` and ``bias`` are float32, bfloat16 or float16, all of one type; sums, the softmax statistics and the loss are
     held in 32 bits.  ``target`` (...) int64; ``weight`` (V) float32 class weights.  Rows whose target is ``ignore_index`` take no
-    part: their loss and gradient are 0, and they cost next to nothing.  Any other target outside [0, V) makes its row's loss
-    and gradients NaN (torch stops with a device assertion).  "mean" divides by the sum of the class weights that took part
+    part: their loss and gradient are 0, and they cost next to nothing.  Any other target outside [0, V) makes its row's loss and
+    gradient in ``x`` NaN, and what sums over rows: the reduced loss and the gradients in ``w`` and ``bias`` (torch stops with a
+    device assertion).  "mean" divides by the sum of the class weights that took part
     (NaN when none did; the gradients are 0 then).  A class is ruled out by a bias of -inf or of the type's lowest value; what
     an infinity in ``w`` or in a row of ``x`` that takes part reaches is infinite or NaN."""
     from .autograd import LinearCrossEntropyFn
