@@ -91,6 +91,16 @@ def test_refusals_of_the_python_entry():
         linear_cross_entropy(x, w, t, weight=torch.zeros(4))
 
 
+def test_class_weights_keep_their_bits():
+    """A head that is moved to 16 bits takes its parameters along, not the class weights."""
+    from vae_amd.losses import LinearCrossEntropyLoss
+    c = torch.rand(40)
+    for to in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: torch.nn.Sequential(m).half()[0]):
+        m = to(LinearCrossEntropyLoss(32, 40, weight=c.clone()))
+        assert m.linear.weight.dtype != torch.float32 and m.weight.dtype == torch.float32 and torch.equal(m.weight, c)
+    assert m.to("meta").weight.device.type == "meta" and LinearCrossEntropyLoss(32, 40).half().weight is None
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 def _inputs(n, d, v, dtype, bias, weight, ignored, seed, off=0):
     g = torch.Generator(device="cuda").manual_seed(seed)

@@ -153,7 +153,15 @@ class LinearCrossEntropyLoss(nn.Module):
         self.register_buffer("weight", weight, persistent=False)
         self.ignore_index, self.reduction = ignore_index, reduction
 
+    def _apply(self, fn, recurse=True):
+        """The class weights follow the head to its device and not to its type (``.bfloat16()`` would round them)."""
+        weight = self.weight
+        super()._apply(fn, recurse)
+        if weight is not None and self.weight.dtype != weight.dtype:
+            self.weight = weight.to(self.weight.device)
+        return self
+
     def forward(self, x: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
-        weight = None if self.weight is None else self.weight.float()        # (.to(dtype) takes the buffer along)
+        weight = None if self.weight is None else self.weight.float()
         return linear_cross_entropy(x, self.linear.weight, target, bias=self.linear.bias, weight=weight,
                                     ignore_index=self.ignore_index, reduction=self.reduction)
