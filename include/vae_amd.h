@@ -562,10 +562,12 @@ int vae_l1_penalty(const float* params, float* grads, int64_t n, const vae_adamw
  * One step (same update as vae_adamw_step: decoupled decay, bias correction, optional clipping by the global norm) over
  * n_tensors contiguous tensors of fp32, bf16 or fp16, each with a gradient of its own type.  The moments are flat: tensor k
  * owns the blocks of VAE_ADAMW_BLOCK elements from tensors[k].first_block on (the last one padded), n_blocks in all.
+ * The bias correction goes by each tensor's own count of steps, as in torch.optim.AdamW, where a parameter without a gradient
+ * does not count a step.
  * state_bits = 32: exp_avg / exp_avg_sq are float (n_blocks * VAE_ADAMW_BLOCK).
  * state_bits = 8: they are OCP e4m3 bytes, exp_avg_sq holds the ROOT of the second moment, and a code times
  * scales[block] (exp_avg) / scales[n_blocks + block] (exp_avg_sq) is the value.  The first moment is rounded to nearest, the
- * root up or down at random from a hash of (seed, step, flat element index): the same call gives the same bits.  A block with
+ * root up or down at random from a hash of (seed, the tensor's step, flat element index): the same call gives the same bits.  A block with
  * a moment or a root that is not finite (the square of a finite gradient may overflow) decodes as NaN throughout.
  * master (nullable): float weights in the state's layout, which are updated instead; params receive their rounding and are
  * not read.  Weights are rounded to nearest.  As with torch.nn.utils.clip_grad_norm_ a NaN norm makes every weight NaN, and an
@@ -581,6 +583,7 @@ typedef struct {
   int64_t first_block;
   float weight_decay;
   int32_t dtype;
+  int64_t step;                  /* steps of this tensor, this one included; 0: those of the call */
 } vae_adamw_tensor;
 int64_t vae_adamw_multi_workspace_bytes(int64_t n_tensors);
 int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensors, int state_bits, void* exp_avg, void* exp_avg_sq,

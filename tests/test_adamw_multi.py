@@ -77,6 +77,14 @@ def test_refusals_of_the_python_entry():
         MultiTensorAdamW([p.double()])
 
 
+def test_refusals_of_the_counts_of_steps():
+    from vae_amd import _lib
+    lib = _lib.load()
+    base = 1 << 30
+    rc = lib.vae_adamw_multi(*_args(_lib, [_lib.AdamWTensor(base, base + (1 << 20), 100, 0, 0.0, 0, -1)]))
+    assert rc == 1 and "step counts from 1" in lib.vae_last_error().decode()
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 SIZES = {"ragged": [1, 255, 256, 257, 7, 2047, 2048, 2049, 4100, 65537], "one": [1], "empty": [0, 5, 0, 300, 0],
          "many": [3 + 37 * k % 400 for k in range(230)], "long": [2 ** 20 + 3, 9]}
@@ -334,3 +342,61 @@ def test_an_infinite_norm_clips_to_nothing():
     assert float(opt.grad_norm) == math.inf and bool(torch.isnan(p[3]))
     p[3] = 0.75
     assert bool((p == 0.75).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clip", [0.0, 0.1])
+@pytest.mark.parametrize("bits,master", [(32, False), (32, True), (8, False)])
+def test_a_parameter_counts_its_own_steps(clip, bits, master):
+    """Gradients that are absent now and then, 40 counts of steps among 120 tensors at the end: torch.optim.AdamW's weights, four
+    steps of 16 roundings each, and in 8 bits no further than a step of the moments' codes takes them (a quarter of lr a step)."""
+    from vae_amd.optim import MultiTensorAdamW
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    lr, steps, n = 1e-2, 42, 120
+    ours = [torch.randn(3 + 5 * k, generator=gen, device="cuda") for k in range(n)]
+    ref = [t.double().requires_grad_() for t in ours]
+    opt = MultiTensorAdamW(ours, lr=lr, state_bits=bits, master_weights=master, max_grad_norm=clip, weight_decay=0.1)
+    torch_opt = torch.optim.AdamW(ref, lr=lr, betas=(0.9, 0.998), eps=1e-7, weight_decay=0.1)
+    taken = [0] * n
+    for step in range(1, steps + 1):
+        for k in range(n):
+            # the first third joins late, tensor by tensor; of the others every fifth misses one step in three
+            absent = step <= k and k < 40 or (k >= 40 and k % 5 == 0 and step % 3 == 1)
+            ours[k].grad = None if absent else torch.randn(ours[k].shape, generator=gen, device="cuda")
+            ref[k].grad = None if absent else ours[k].grad.double()
+            taken[k] += not absent
+        if clip:
+            torch.nn.utils.clip_grad_norm_(ref, clip)
+        opt.step()
+        torch_opt.step()
+        if step == 40:                                                   # (the counts travel with the state)
+            other = MultiTensorAdamW(ours, lr=lr, state_bits=bits, master_weights=master, max_grad_norm=clip, weight_decay=0.1)
+            other.load_state_dict(opt.state_dict())
+            opt = other
+    assert opt.param_steps == taken and len(set(taken)) > 8 * 4 and opt.steps == steps
+    for a, b, t in zip(ours, ref, taken):
+        # an update is of at most 3 lr (its first ones: lr exactly); its error is 16 roundings of the moments' terms, in 8 bits
+        # the codes': an eighth of the root (at random, both ways) and a sixteenth of the first moment
+        tol = t * (16 * 2.0 ** -24 * (b.detach().abs().max() + 30 * lr) + (0.75 * lr if bits == 8 else 0))
+        assert float((a.double() - b.detach()).abs().max()) <= float(tol)
+
+
+@pytest.mark.gpu
+def test_a_late_parameter_starts_with_a_full_step():
+    """The first update of weights that had no gradient before is lr in the gradient's sign, not the 2.2 lr of three steps' bias."""
+    from vae_amd.optim import MultiTensorAdamW, multi_tensor_adamw_
+    a, b = torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda")
+    opt = MultiTensorAdamW([a, b], lr=1.0, eps=0.0, state_bits=8)
+    a.grad = torch.ones(300, device="cuda")
+    opt.step()
+    opt.step()
+    b.grad = -torch.ones(300, device="cuda")
+    opt.step()
+    assert float((b - 1).abs().max()) <= 16 * 2.0 ** -24 and opt.param_steps == [3, 1]
+    state = [torch.zeros(1024, device="cuda") for _ in range(2)]
+    with pytest.raises(ValueError, match="counts of steps"):
+        multi_tensor_adamw_([a, b], [a.grad, b.grad], *state, step=[1], lr=1.0)
+    with pytest.raises(ValueError, match="counts from 1"):
+        multi_tensor_adamw_([a, b], [a.grad, b.grad], *state, step=[1, 0], lr=1.0)
+    with pytest.raises(ValueError, match="does not fit|counts"):
+        opt.load_state_dict({**opt.state_dict(), "param_steps": [1]})

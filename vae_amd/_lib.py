@@ -127,7 +127,7 @@ class AdamWSegment(C.Structure):
 class AdamWTensor(C.Structure):
     """vae_adamw_tensor of include/vae_amd.h"""
     _fields_ = [("param", _ptr), ("grad", _ptr), ("n", C.c_int64), ("first_block", C.c_int64), ("weight_decay", C.c_float),
-                ("dtype", C.c_int32)]
+                ("dtype", C.c_int32), ("step", C.c_int64)]
 
 
 class GatedNorm(C.Structure):

@@ -41,16 +41,21 @@ struct Tensors {
   uint32_t first_block[PER_LAUNCH];
   uint32_t chunk_end[PER_LAUNCH];         // running total of chunks, this tensor's included
   float keep[PER_LAUNCH];                 // 1 - lr * weight_decay
-  uint8_t kind[PER_LAUNCH];               // dtype | 4: param and grad are 16-byte aligned
+  uint8_t kind[PER_LAUNCH];               // dtype | 4: param and grad are 16-byte aligned | 8 * index of its count of steps
   int32_t count;
   int32_t steps;                          // a chunk is steps * STEP_ELEMS elements
 };
-static_assert(sizeof(Tensors) < 3800, "kernel arguments are limited to 4 KB");
-
-struct Scalars {
-  float b1, omb1, b2, omb2, eps, step_size, inv_bc2, gscale;
+// What follows from a tensor's count of steps.  Tensors of a launch share a few counts: one, where all have had every gradient.
+constexpr int COUNTS = 8;
+struct Count {
+  float step_size, inv_bc2;
   uint32_t key;
 };
+struct Scalars {
+  float b1, omb1, b2, omb2, eps, gscale;
+  Count at[COUNTS];
+};
+static_assert(sizeof(Tensors) + sizeof(Scalars) + 48 <= 4096, "kernel arguments are limited to 4 KB");
 
 // Austin Appleby's 32-bit finaliser (MurmurHash3, public domain)
 __host__ __device__ __forceinline__ uint32_t mix32(uint32_t h) {
@@ -117,7 +122,7 @@ __device__ __forceinline__ int tensor_of(const Tensors& t, uint32_t b) {
 
 template <typename T, int BITS>
 __device__ __forceinline__ void update(T* __restrict__ p, const T* __restrict__ g, int64_t n, bool wide, int64_t from, int64_t to,
-                                       uint32_t first_block, float keep, float gs, const Scalars& s, void* __restrict__ em,
+                                       uint32_t first_block, float keep, float gs, const Scalars& s, const Count& c, void* __restrict__ em,
                                        void* __restrict__ ev, float* __restrict__ scales, int64_t n_blocks,
                                        float* __restrict__ master) {
   const int64_t flat0 = (int64_t)first_block * BLK;
@@ -165,7 +170,7 @@ __device__ __forceinline__ void update(T* __restrict__ p, const T* __restrict__ 
       m[j] = m[j] * s.b1 + gg * s.omb1;
       v[j] = v[j] * s.b2 + (gg * gg) * s.omb2;
       u[j] = sqrtf(v[j]);
-      const float moved = (m[j] / (u[j] * s.inv_bc2 + s.eps)) * s.step_size;
+      const float moved = (m[j] / (u[j] * c.inv_bc2 + s.eps)) * c.step_size;
       pw[j] = pw[j] * keep - moved;
       if (BITS == 8) {
         if (at + j >= n) m[j] = u[j] = 0.f;                            // padding holds zeros, whatever it held before
@@ -184,17 +189,17 @@ __device__ __forceinline__ void update(T* __restrict__ p, const T* __restrict__ 
       // below 1e-30 the reciprocal could overflow; such a block is held as zeros.  A NaN compares false: its scale says it
       const float im = top_m > 1e-30f ? (1.f / top_m) * 448.f : 0.f, iu = top_u > 1e-30f ? (1.f / top_u) * 448.f : 0.f;
       const uint32_t pair = (uint32_t)(f >> 1);                        // f is a multiple of 8: the four pairs share their upper half
-      const uint32_t key = mix32((uint32_t)(f >> 33) + s.key);
+      const uint32_t key = mix32((uint32_t)(f >> 33) + c.key);
       uint32_t wm[2], wv[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        int c = 0;
+        int code = 0;
         float q[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[j] = fminf(fmaxf(m[4 * h + j] * im, -448.f), 448.f);
-        c = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], c, false);
-        c = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], c, true);
-        wm[h] = (uint32_t)c;
+        code = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], code, false);
+        code = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], code, true);
+        wm[h] = (uint32_t)code;
         uint32_t w = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -239,7 +244,8 @@ __global__ __launch_bounds__(256) void adamw_multi_kernel(Tensors t, Scalars s, 
   const float gs = coef ? s.gscale * coef[0] : s.gscale;
   const int kind = t.kind[k];
   const bool wide = kind & 4;
-#define VAE_UPDATE(T) update<T, BITS>((T*)t.p[k], (const T*)t.g[k], n, wide, from, to, t.first_block[k], t.keep[k], gs, s, em, ev, scales, n_blocks, master)
+  const Count c = s.at[kind >> 3];
+#define VAE_UPDATE(T) update<T, BITS>((T*)t.p[k], (const T*)t.g[k], n, wide, from, to, t.first_block[k], t.keep[k], gs, s, c, em, ev, scales, n_blocks, master)
   switch (kind & 3) {
     case 0: VAE_UPDATE(float); break;
     case 1: VAE_UPDATE(__bf16); break;
@@ -357,6 +363,7 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
     else if (pb % esize || gb % esize) bad = "param or grad is not aligned to its element";
     else if (t.first_block < 0 || t.first_block > n_blocks || (t.n + BLK - 1) / BLK > n_blocks - t.first_block) bad = "does not fit the state";
     else if (!(t.weight_decay >= 0)) bad = "negative weight decay";
+    else if (t.step < 0) bad = "step counts from 1";
     else if (t.n) {
       spans[n_spans++] = {pb, pb + (uintptr_t)(t.n * esize)};
       blocks[n_live++] = {(uintptr_t)t.first_block, (uintptr_t)(t.first_block + (t.n + BLK - 1) / BLK)};
@@ -402,10 +409,11 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
   s.b2 = (float)beta2;
   s.omb2 = (float)(1.0 - beta2);
   s.eps = (float)eps;
-  s.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
-  s.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
   s.gscale = (float)grad_scale;
-  s.key = mix32(((uint32_t)seed ^ mix32((uint32_t)(seed >> 32))) ^ mix32((uint32_t)step * 0x9E3779B9u));
+  const auto count_of = [&](int64_t n) -> Count {
+    return {(float)(lr / (1.0 - pow(beta1, (double)n))), (float)(1.0 / sqrt(1.0 - pow(beta2, (double)n))),
+            mix32(((uint32_t)seed ^ mix32((uint32_t)(seed >> 32))) ^ mix32((uint32_t)n * 0x9E3779B9u))};
+  };
   double* partial = reinterpret_cast<double*>(workspace);
   float* coef = clip ? reinterpret_cast<float*>(partial + launches_of(n_tensors) * NORM_GROUPS) : nullptr;
   const float* use = max_grad_norm > 0 ? coef : nullptr;
@@ -413,12 +421,22 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
   for (int pass = clip ? 0 : 1; pass < 2; ++pass) {
     int64_t n_partials = 0;
     for (int64_t k = 0; k < n_tensors;) {
-      int64_t chunks = 0;
+      int64_t chunks = 0, counts[COUNTS];
+      int n_counts = 0;
       t.count = 0;
       t.steps = steps;
       for (; k < n_tensors && t.count < PER_LAUNCH; ++k) {
         const vae_adamw_tensor& e = tensors[k];
         if (e.n == 0) continue;
+        const int64_t own = e.step ? e.step : step;
+        int at = 0;
+        while (at < n_counts && counts[at] != own) ++at;
+        if (pass == 0) at = 0;                                         // (the norm asks for none: its launches stay launches_of())
+        else if (at == n_counts) {
+          if (at == COUNTS) break;                                     // (one count more than a launch holds: the next launch's)
+          counts[n_counts++] = own;
+          s.at[at] = count_of(own);
+        }
         const int i = t.count++;
         chunks += (e.n + chunk - 1) / chunk;
         t.p[i] = e.param;
@@ -427,7 +445,7 @@ extern "C" int vae_adamw_multi(const vae_adamw_tensor* tensors, int64_t n_tensor
         t.first_block[i] = (uint32_t)e.first_block;
         t.chunk_end[i] = (uint32_t)chunks;
         t.keep[i] = (float)(1.0 - lr * (double)e.weight_decay);
-        t.kind[i] = (uint8_t)(e.dtype | (vae_aligned16(e.param) && vae_aligned16(e.grad) ? 4 : 0));
+        t.kind[i] = (uint8_t)(e.dtype | (vae_aligned16(e.param) && vae_aligned16(e.grad) ? 4 : 0) | at << 3);
       }
       if (!t.count) break;
       if (pass == 0) {

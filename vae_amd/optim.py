@@ -229,23 +229,25 @@ def adamw_blocks(n: int) -> int:
 
 
 def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], exp_avg: torch.Tensor,
-                        exp_avg_sq: torch.Tensor, *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.998),
+                        exp_avg_sq: torch.Tensor, *, step: Union[int, Sequence[int]], lr: float, betas: Tuple[float, float] = (0.9, 0.998),
                         eps: float = 1e-7, weight_decay: Union[float, Sequence[float]] = 0.0, scales: Optional[torch.Tensor] = None,
                         master: Optional[torch.Tensor] = None, max_grad_norm: float = 0.0, grad_scale: float = 1.0, seed: int = 0,
                         return_norm: bool = False) -> Optional[torch.Tensor]:
     """One AdamW step in place over ``params`` (contiguous fp32 / bf16 / fp16 tensors on one GPU) in one launch for every 96 of
-    them (include/vae_amd.h, ``vae_adamw_multi``).  A parameter whose gradient is None is left alone, with its state.
+    them, or for every 8 counts of steps among them (include/vae_amd.h, ``vae_adamw_multi``).  A parameter whose gradient is
+    None is left alone, with its state.
 
     The state is flat, in the order of ``params``: every tensor starts a new block of ``ADAMW_BLOCK`` elements.  fp32
     ``exp_avg`` / ``exp_avg_sq``: 32-bit moments.  float8_e4m3fn ones: 8-bit moments, where ``exp_avg_sq`` holds the ROOT of
     the second moment and a code times ``scales[0 | 1, block]`` is the value; the root is rounded at random by
-    ``(seed, step, element)``, so equal calls give equal bits.  ``master``: fp32 weights in the same layout, which are updated in
-    the parameters' place; the parameters then receive their rounding.  Start all of them at zero (``master``: at the
-    parameters).
+    ``(seed, the tensor's step, element)``, so equal calls give equal bits.  ``master``: fp32 weights in the same layout, which
+    are updated in the parameters' place; the parameters then receive their rounding.  Start all of them at zero (``master``: at
+    the parameters).
 
-    ``step`` counts from 1.  ``weight_decay``: one value, or one for each tensor.  ``max_grad_norm`` > 0 clips by the norm over
-    all gradients; ``return_norm`` returns that norm (of ``grad_scale`` times the gradients, before clipping) as a 1-element
-    tensor.  The learning rate and the step count are host values: a captured graph would repeat them, so capturing raises."""
+    ``step`` counts from 1: one value, or a list with one for each tensor, by which its bias is corrected (``torch.optim.AdamW``
+    counts a parameter's own steps, and one without a gradient takes none).  ``weight_decay``: one value, or one for each
+    tensor.  ``max_grad_norm`` > 0 clips by the norm over all gradients; ``return_norm`` returns that norm (of ``grad_scale``
+    times the gradients, before clipping) as a 1-element tensor.  The learning rate and the step count are host values: a captured graph would repeat them, so capturing raises."""
     lib = _lib.load()
     n = len(params)
     if len(grads) != n:
@@ -262,9 +264,17 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
         decay = weight_decay
         if len(decay) != n:
             raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(decay)} weight decays")
+    if isinstance(step, (list, tuple)):
+        counts, step = step, 1
+        if len(counts) != n:
+            raise ValueError(f"vae_amd.optim.multi_tensor_adamw_: {n} params and {len(counts)} counts of steps")
+        if n and min(counts) < 1:
+            raise ValueError("vae_amd.optim.multi_tensor_adamw_: step counts from 1")
+    else:
+        counts = [0] * n                                                # (the call's)
     table: List[Union[int, float]] = []
     at, live, index = 0, [], dev.index
-    for p, g, wd in zip(params, grads, decay):
+    for p, g, wd, count_of in zip(params, grads, decay, counts):
         count = p.numel()
         if g is not None and count:
             dtype = p.dtype
@@ -276,7 +286,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
                 raise RuntimeError(f"vae_amd.optim.multi_tensor_adamw_: parameters, gradients and state must be on {dev}")
             if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
                 raise ValueError("vae_amd.optim.multi_tensor_adamw_: parameters and gradients must be contiguous and of one shape")
-            table += (p.data_ptr(), g.data_ptr(), count, at, wd, kind)
+            table += (p.data_ptr(), g.data_ptr(), count, at, wd, kind, count_of)
             live.append(p)
         at += -(-count // ADAMW_BLOCK)
     for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
@@ -300,7 +310,7 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
             return norm
         nbytes = lib.vae_adamw_multi_workspace_bytes(len(live)) if clip else 0
         ws = torch.empty(nbytes // 8, dtype=torch.float64, device=dev) if clip else None
-        rc = lib.vae_adamw_multi(struct.pack("=" + "QQqqfi" * len(live), *table), len(live), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+        rc = lib.vae_adamw_multi(struct.pack("=" + "QQqqfiq" * len(live), *table), len(live), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
                                  scales.data_ptr() if bits == 8 else None, at, None if master is None else master.data_ptr(), float(lr),
                                  float(betas[0]), float(betas[1]), float(eps), int(step), float(max_grad_norm), float(grad_scale),
                                  int(seed) & (2 ** 64 - 1), None if ws is None else ws.data_ptr(), nbytes,
@@ -343,7 +353,8 @@ class MultiTensorAdamW:
         self.base_lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
         self.max_grad_norm = float(max_grad_norm) if max_grad_norm else 0.0
         self.lr_lambda, self.seed, self.state_bits = lr_lambda, int(seed), state_bits
-        self.steps = 0
+        self.steps = 0                                     # calls of step(), by which the learning rate goes
+        self.param_steps = [0] * len(self.params)          # and in how many of them each parameter had a gradient
         self.starts, blocks = [], 0
         for p in self.params:
             self.starts.append(blocks * ADAMW_BLOCK)
@@ -375,10 +386,13 @@ class MultiTensorAdamW:
 
     def step(self, grad_scale: float = 1.0) -> None:
         """Update from ``p.grad``; ``grad_norm`` holds the unclipped norm afterwards when clipping is on."""
-        self.grad_norm = multi_tensor_adamw_(self.params, [p.grad for p in self.params], self.exp_avg, self.exp_avg_sq,
-                                             step=self.steps + 1, lr=self.lr, betas=self.betas, eps=self.eps, weight_decay=self.decay,
-                                             scales=self.scales, master=self.master, max_grad_norm=self.max_grad_norm,
-                                             grad_scale=grad_scale, seed=self.seed, return_norm=self.max_grad_norm > 0)
+        grads = [p.grad for p in self.params]
+        counts = [k + 1 for k in self.param_steps]
+        self.grad_norm = multi_tensor_adamw_(self.params, grads, self.exp_avg, self.exp_avg_sq, step=counts, lr=self.lr, betas=self.betas,
+                                             eps=self.eps, weight_decay=self.decay, scales=self.scales, master=self.master,
+                                             max_grad_norm=self.max_grad_norm, grad_scale=grad_scale, seed=self.seed,
+                                             return_norm=self.max_grad_norm > 0)
+        self.param_steps = [old if g is None else new for old, new, g in zip(self.param_steps, counts, grads)]
         self.steps += 1
 
     def moments(self, index: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -393,17 +407,21 @@ class MultiTensorAdamW:
         return m[:n].view(p.shape), v[:n].view(p.shape)
 
     def state_dict(self) -> Dict[str, object]:
-        return {"steps": self.steps, "seed": self.seed, "exp_avg": self.exp_avg, "exp_avg_sq": self.exp_avg_sq, "scales": self.scales,
-                "master": self.master}
+        return {"steps": self.steps, "param_steps": list(self.param_steps), "seed": self.seed, "exp_avg": self.exp_avg,
+                "exp_avg_sq": self.exp_avg_sq, "scales": self.scales, "master": self.master}
 
     def load_state_dict(self, sd: Dict[str, object]) -> None:
-        """State of an optimiser over the same parameters with the same ``state_bits``."""
+        """State of an optimiser over the same parameters with the same ``state_bits``.  One that was saved without the parameters'
+        own counts of steps: all of them took every step."""
         mine = {k: getattr(self, k) for k in ("exp_avg", "exp_avg_sq", "scales", "master")}
         for k, t in mine.items():
             s = sd[k]
             if (t is None) != (s is None) or (t is not None and (t.shape != s.shape or t.dtype != s.dtype)):
                 raise ValueError(f"vae_amd: MultiTensorAdamW.load_state_dict: {k} does not fit (other parameters, state_bits or master_weights)")
+        counts = [int(k) for k in sd.get("param_steps", [sd["steps"]] * len(self.params))]
+        if len(counts) != len(self.params):
+            raise ValueError(f"vae_amd: MultiTensorAdamW.load_state_dict: {len(counts)} counts of steps, {len(self.params)} parameters")
         for k, t in mine.items():
             if t is not None:
                 t.copy_(sd[k])
-        self.steps, self.seed = int(sd["steps"]), int(sd["seed"])
+        self.steps, self.param_steps, self.seed = int(sd["steps"]), counts, int(sd["seed"])
