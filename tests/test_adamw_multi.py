@@ -400,3 +400,12 @@ def test_a_late_parameter_starts_with_a_full_step():
         multi_tensor_adamw_([a, b], [a.grad, b.grad], *state, step=[1, 0], lr=1.0)
     with pytest.raises(ValueError, match="does not fit|counts"):
         opt.load_state_dict({**opt.state_dict(), "param_steps": [1]})
+
+
+@pytest.mark.gpu
+def test_moments_are_held_in_32_bits_unless_asked_otherwise():
+    from vae_amd.optim import MultiTensorAdamW
+    p = torch.ones(300, device="cuda")
+    opt = MultiTensorAdamW([p])
+    assert opt.exp_avg.dtype == opt.exp_avg_sq.dtype == torch.float32 and opt.scales is None
+    assert MultiTensorAdamW([p], state_bits=8).exp_avg.dtype == torch.float8_e4m3fn

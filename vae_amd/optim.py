@@ -322,13 +322,13 @@ def multi_tensor_adamw_(params: Sequence[torch.Tensor], grads: Sequence[Optional
 
 class MultiTensorAdamW:
     """AdamW over separate tensors of any of the three float types, beside ``FusedAdamW`` (which owns ONE fp32 arena): moments
-    in 8 or 32 bits, optional fp32 master weights, the reference's betas / eps by default (task.py:534-553).
+    in 32 or (asked for) 8 bits, optional fp32 master weights, the reference's betas / eps by default (task.py:534-553).
 
     ``params``: an iterable of tensors, or of dicts ``{"params": [...], "weight_decay": ...}``.  ``state_bits`` 8 keeps two bytes
     and 1/32 of a byte per parameter in place of eight (see ``multi_tensor_adamw_``)."""
 
     def __init__(self, params: Iterable, lr: float = 5e-4, betas: Tuple[float, float] = (0.9, 0.998), eps: float = 1e-7,
-                 weight_decay: float = 0.0, max_grad_norm: float = 0.0, state_bits: int = 8, master_weights: bool = False,
+                 weight_decay: float = 0.0, max_grad_norm: float = 0.0, state_bits: int = 32, master_weights: bool = False,
                  lr_lambda: Optional[Callable[[int], float]] = None, seed: int = 0):
         self.params: List[torch.Tensor] = []
         self.decay: List[float] = []
