@@ -87,6 +87,14 @@ def test_refusals_of_the_python_entry():
         gated_residual_norm(torch.zeros(1, 0), torch.zeros(1, 0))
 
 
+def test_strides_of_vectors_are_no_reason_to_refuse():
+    from vae_amd.functional import gated_residual_norm
+    x, v = torch.zeros(3, 8), torch.zeros(8, 2)
+    for call in (lambda: gated_residual_norm(x, x, scale=v[:, 0]), lambda: gated_residual_norm(x, x, norm_weight=torch.ones(1).expand(8))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 def _inputs(n, d, dtype, gate, post, scale, bias, vec32, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -320,3 +328,23 @@ def test_gradients_of_vectors_that_are_taken_as_one_or_zero(d):
     for got, ref in ((out[0], dh.double() * ny), (out[1], dh.double()), (out[2], dr.double() * x["b"].double())):
         tol = 2e-5 * float(ref.abs().max()) + 128 * 2.0 ** -24 * ref.abs().sum(0)        # (as the gradients of the vectors above)
         assert bool(((got.double() - ref.sum(0)).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+def test_strided_vectors():
+    from vae_amd.functional import gated_residual_norm
+    x, dy, dh = _inputs(9, 300, "bf16", "full", True, True, True, False, seed=3)
+    want, grads = _run(x, dy, dh, "layer", "sigmoid")
+    wide = torch.stack([x[k] for k in NAMES[3:]], 1).requires_grad_()                       # one parameter holds them side by side
+    y, h = gated_residual_norm(x["r"], x["b"], x["gate"], **{k: wide[:, i] for i, k in enumerate(NAMES[3:])}, kind="layer")
+    torch.autograd.backward([y, h], [dy, dh])
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    for i, k in enumerate(NAMES[3:]):
+        assert torch.equal(wide.grad[:, i], grads[k]), k
+    s = torch.full((1,), 0.5, device="cuda", dtype=torch.bfloat16, requires_grad=True)      # one value for all columns
+    x["scale"] = torch.full((300,), 0.5, device="cuda", dtype=torch.bfloat16)
+    _, grads = _run(x, dy, dh, "layer", "sigmoid")
+    y, h = gated_residual_norm(x["r"], x["b"], x["gate"], scale=s.expand(300), **{k: x[k] for k in NAMES[3:] if k != "scale"}, kind="layer")
+    torch.autograd.backward([y, h], [dy, dh])
+    total = grads["scale"].double()
+    assert abs(float(s.grad) - float(total.sum())) <= 2.0 ** -7 * float(total.abs().sum())  # (torch adds 300 of them in bf16's terms)

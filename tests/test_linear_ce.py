@@ -13,6 +13,7 @@ unit in the last place of a partial sum of some Z at most, that is 2^-24 Z, spre
 by 45 * 2^-24, half an ulp of 4 * 2^-24 eleven times over, where 8 + 4 Z is 31; S is 113.)  At the target p - 1 keeps the error of p
 however small p - 1 is, so this term takes the matrices of p and not those of d."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -89,6 +90,17 @@ def test_refusals_of_the_python_entry():
         linear_cross_entropy(x, w, t, weight=torch.zeros(5, requires_grad=True))
     with pytest.raises(ValueError, match="vector of 5"):
         linear_cross_entropy(x, w, t, weight=torch.zeros(4))
+
+
+def test_strides_are_no_reason_to_refuse():
+    """Targets, biases and class weights of any stride, and a column of weights that is one value: only the missing GPU stops them."""
+    from vae_amd.losses import linear_cross_entropy
+    x, w, t = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(6, dtype=torch.int64)[::2]
+    for call in (lambda: linear_cross_entropy(x, w, t), lambda: linear_cross_entropy(x, w, t, bias=torch.zeros(10)[::2]),
+                 lambda: linear_cross_entropy(x, w, t, weight=torch.zeros(1).expand(5)),
+                 lambda: linear_cross_entropy(x[:, :1], torch.zeros(1, 1).expand(5, 1), t)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
 
 
 def test_class_weights_keep_their_bits():
@@ -398,3 +410,19 @@ def test_a_target_that_is_no_class_spoils_its_row_alone(n, d, v, weight, reducti
     grads["x"][~rows] = 0
     loss, _ = _run(s, reduction)
     _check(s, reduction, loss, {"x": grads["x"]})
+
+
+@pytest.mark.gpu
+def test_strided_targets_biases_and_class_weights():
+    from vae_amd.losses import linear_cross_entropy
+    s = _inputs(60, 40, 90, "fp32", True, True, 0.2, seed=8)
+    want, grads = _run(s, "mean")
+    wide = {k: torch.stack((s[k], s[k]), 1) for k in ("bias", "weight", "target")}
+    bias = wide["bias"].requires_grad_()
+    got = linear_cross_entropy(s["x"], s["w"], wide["target"][:, 0], bias=bias[:, 1], weight=wide["weight"][:, 1])
+    got.backward()
+    assert torch.equal(got, want) and torch.equal(bias.grad[:, 1], grads["bias"]) and not bool(bias.grad[:, 0].any())
+    one = torch.ones(1, 1, device="cuda", requires_grad=True)
+    loss = linear_cross_entropy(s["x"][:, :1], one.expand(90, 1), s["target"])
+    loss.backward()
+    assert abs(float(loss) - math.log(90)) < 1e-5 and abs(float(one.grad)) < 1e-5           # all classes alike

@@ -61,9 +61,8 @@ def gated_residual_norm(r: torch.Tensor, b: torch.Tensor, gate: Optional[torch.T
         raise ValueError(f"vae_amd.gated_residual_norm: r is {tuple(r.shape)}, b is {tuple(b.shape)}")
     if gate is not None and tuple(gate.shape[:-1]) != tuple(b.shape[:-1]):
         raise ValueError(f"vae_amd.gated_residual_norm: gate is {tuple(gate.shape)}, b is {tuple(b.shape)}")
-
-    y, h = _gated_residual_norm()(_rows(r), _rows(b), None if gate is None else _rows(gate), post_weight, post_bias, scale, norm_weight,
-                                  norm_bias, kind, gate_act, eps)
+    vectors = (t if t is None else t.contiguous() for t in (post_weight, post_bias, scale, norm_weight, norm_bias))
+    y, h = _gated_residual_norm()(_rows(r), _rows(b), None if gate is None else _rows(gate), *vectors, kind, gate_act, eps)
     return (y, h) if b.dim() == 2 else (y.view(b.shape), h.view(b.shape))
 
 

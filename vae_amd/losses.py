@@ -129,8 +129,9 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.numel() and rows.stride(1) != 1 and rows.shape[1] > 1:
         rows = rows.contiguous()
-    if w.dim() == 2 and w.shape[1] > 1 and (w.stride(1) != 1 or (w.shape[0] > 1 and w.stride(0) < w.shape[1])):
+    if w.dim() == 2 and ((w.shape[1] > 1 and w.stride(1) != 1) or (w.shape[0] > 1 and w.stride(0) < w.shape[1])):
         w = w.contiguous()
+    bias, weight = (t if t is None else t.contiguous() for t in (bias, weight))
     if rows.shape[0] == 0 and w.dim() == 2 and w.shape[1] == rows.shape[1]:   # as torch: nothing, 0 or 0 / 0, with zero gradients
         if reduction not in ("none", "sum", "mean"):
             raise ValueError(f"vae_amd.linear_cross_entropy: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
@@ -138,7 +139,7 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
             raise RuntimeError("vae_amd.linear_cross_entropy: all tensors must live on one GPU (no CPU fallback)")
         zero = (rows.float().sum() + 0.0 * sum(t.float().flatten()[:1].sum() for t in (w, bias) if t is not None))
         return rows.float().sum(1).view(target.shape) if reduction == "none" else zero if reduction == "sum" else zero + float("nan")
-    loss = LinearCrossEntropyFn.apply(rows, w, bias, target.reshape(-1), weight, ignore_index, reduction)
+    loss = LinearCrossEntropyFn.apply(rows, w, bias, target.reshape(-1).contiguous(), weight, ignore_index, reduction)
     return loss.view(target.shape) if reduction == "none" else loss
 
 
