@@ -426,3 +426,86 @@ def test_strided_targets_biases_and_class_weights():
     loss = linear_cross_entropy(s["x"][:, :1], one.expand(90, 1), s["target"])
     loss.backward()
     assert abs(float(loss) - math.log(90)) < 1e-5 and abs(float(one.grad)) < 1e-5           # all classes alike
+
+
+def _check_uneven(s, reduction, up, grads):
+    """fp16 gradients where the rows' factors g span many powers of two.  d is held in steps of 2^-24 times 2^s top / (2^14 2^s)
+    (top: the largest |g|; s = 0 to 10 by how far a row is below it), so that besides the bounds of _check a row's d is off by half
+    a step, 2^-25 2^-14 2^-s top; and dW takes x 2^-s, off by 2^-25 in those units."""
+    _, ref = _oracle(s, reduction, up)
+    kept = s["target"] != -100
+    cw = kept.double() * (1 if s["weight"] is None else s["weight"].double()[s["target"].clamp(min=0)])
+    g = cw * up.double() / (cw.sum() if reduction == "mean" else 1)
+    top = g.abs().max()
+    below = torch.where(g > 0, torch.log2(top / g.clamp(min=1e-300)).round(), torch.zeros_like(g))
+    shift = (below - 6 - 1).clamp(0, 10)                # (an exponent's difference may be one less than the ratio's logarithm)
+    step = torch.where(g > 0, 2.0 ** (-25 - 14 - shift) * top, torch.zeros_like(g))
+    x, w = s["x"].double().abs(), s["w"].double().abs()
+    x = torch.where(kept[:, None], x, torch.zeros_like(x))
+    z = s["x"].double() @ s["w"].double().t() + (0 if s["bias"] is None else s["bias"].double())
+    d = torch.softmax(z, 1)
+    d.scatter_add_(1, s["target"].clamp(min=0)[:, None], -torch.ones_like(d[:, :1]))
+    d = torch.where(kept[:, None], d.abs() * g[:, None], torch.zeros_like(d))
+    shifted = (shift > 0).double() * 2.0 ** (-25 + (shift + 1).clamp(max=10))
+    extra = {"x": step[:, None] * w.sum(0), "w": (step[:, None] * x).sum(0) + (d * shifted[:, None]).sum(0)[:, None], "bias": 0.0}
+    eps = 2.0 ** -11
+    for k, got in grads.items():
+        val, mag, off = ref[k]
+        k_len = s["w"].shape[0] if k == "x" else s["x"].shape[0]
+        tol = off + max(32.0, 2 * (6 * k_len / 16) ** 0.5) * 2.0 ** -24 * mag + eps * mag + 1.01 * eps * val.abs() + extra[k] + 2.0 ** -25
+        bad = (got.double() - val).abs() - tol
+        assert float(bad.max()) <= 0, (k, float(bad.max()), float(val.abs().max()))
+
+
+UNEVEN = [(128, 64, 30000), (300, 72, 5000), (64, 4000, 900), (2500, 136, 3001), (700, 1000, 40), (40000, 72, 7000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", UNEVEN)
+@pytest.mark.parametrize("how", ["none", "mean"])
+def test_fp16_factors_far_apart(n, d, v, how):
+    """Upstream gradients, or class weights, over eight powers of ten; the weights have a common part, so that probabilities that
+    are lost shift a row's gradient instead of averaging out."""
+    s = _inputs(n, d, v, "fp16", True, how == "mean", 0.2, seed=n)
+    s["x"].mul_(0.3)
+    s["w"] = (s["w"].float() + 0.3).half()
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    if how == "none":
+        up = 512.0 * 10.0 ** (-8 * torch.rand(n, generator=gen, device="cuda"))
+    else:
+        s["weight"], up = 10.0 ** (-8 * torch.rand(v, generator=gen, device="cuda")), torch.tensor(512.0, device="cuda")
+    _, grads = _run(s, how, up)
+    _check_uneven(s, how, up, grads)
+
+
+@pytest.mark.gpu
+def test_fp16_rows_far_below_the_largest_keep_their_gradient():
+    """At 1e-7 of the largest factor a row's gradient over 30000 classes was off by 30 % once: each of its 30000 probabilities is
+    held to 2^-9 or better (8 bits and more), and so is the row."""
+    s = _inputs(128, 64, 30000, "fp16", False, False, 0.0, seed=1)
+    s["w"], s["x"] = (s["w"].float() + 0.3).half(), (0.1 * s["x"].float()).half()
+    up = torch.full((128,), 2048.0, device="cuda")
+    up[1::2] *= 1e-7
+    _, grads = _run(s, "none", up)
+    _, ref = _oracle(s, "none", up)
+    off = (grads["x"].double() - ref["x"][0]).norm(dim=1) / ref["x"][0].norm(dim=1)
+    assert float(off.max()) < 2.0 ** -8, float(off.max())
+
+
+@pytest.mark.gpu
+def test_fp16_factors_in_a_graph():
+    """The factors' unevenness is found on the device: a captured pass follows new ones."""
+    n, d, v = 700, 136, 3000
+    static = _inputs(n, d, v, "fp16", True, False, 0.2, seed=3)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    up = torch.ones(n, device="cuda")
+    _run(static, "none", up)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grads = _run(static, "none", up)
+    for k in range(3):
+        up.copy_(10.0 ** (-2 * k * torch.rand(n, generator=gen, device="cuda")))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _run(static, "none", up)
+        assert torch.equal(loss, want[0]) and all(torch.equal(grads[name], want[1][name]) for name in grads)

@@ -23,7 +23,8 @@
 // largest factor g_i c[t_i] for that, and the products are multiplied by it in 32 bits: the term of the target, -1 in nearly
 // every row of a large vocabulary, is then exact, where the rounding of 1 / N itself would shift every gradient by the same
 // 2^-9 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
-// multiplied by 2^14 as well.  fp32 operands are split exactly into three bf16 terms, and for every 64 of K the six products
+// multiplied by 2^14 as well, and where factors differ from row to row (see FACTOR_FREE) a row far below the largest one by a
+// power of two of its own.  fp32 operands are split exactly into three bf16 terms, and for every 64 of K the six products
 // that matter run one after the other: the error is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix
 // instruction would give a sixteenth).
 #include "../../include/vae_amd.h"
@@ -70,6 +71,7 @@ struct Gemm {
   const float* lse;             // by packed row
   const float* g;               // by packed row: upstream * class weight (0: an exactly zero row)
   const float* d_scale;         // what d is multiplied by, and its reciprocal
+  const float* row_factor;      // fp16: null, or what row n of d has to be multiplied by besides (EPI_STORE: row n of the result)
   uint16_t* d;                  // [N padded][ldd], planes at plane_d
   int64_t ldd, plane_d;
   float* d_sums;                // null, or (tile_n, ldd): sums of d over a tile's rows
@@ -386,12 +388,16 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
       }
     };
     if constexpr (EPI == EPI_STORE) {
-      const float inv = g.d_scale ? g.d_scale[1] : 1.f;
+      const float all = g.d_scale ? g.d_scale[1] : 1.f;
+      float inv[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) inv[j] = F16 && g.row_factor && nw + 16 * j < N ? all * g.row_factor[nw + 16 * j] : all;
       if (g.out_kind == 1) {
         uint16_t* out = reinterpret_cast<uint16_t*>(g.out);
         rows_out16(
             [&](int i, int j) {
-              return make_uint2(pack2<F16>(acc[i][j][0] * inv, acc[i][j][1] * inv), pack2<F16>(acc[i][j][2] * inv, acc[i][j][3] * inv));
+              const f32x4 v = acc[i][j] * inv[j];
+              return make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
             },
             [&](int row, int c, u4 v) {
               const int n = n0 + row, m = m0 + 8 * c;
@@ -419,7 +425,7 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
               const int row = wn * 32 + 16 * (j - j0) + l15, c = wm * 4 * TM + 4 * i + lj;
-              *reinterpret_cast<f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2)) = acc[i][j] * inv;
+              *reinterpret_cast<f4*>(lds + row * BM + (((c ^ (4 * row)) % CPR) << 2)) = acc[i][j] * inv[j];
             }
           __syncthreads();
           for (int x = threadIdx.x; x < ROWS * CPR; x += 64 * NW) {
@@ -553,6 +559,19 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
         }
       if (g.d_sums) {                                         // (of d as it is, before its rounding)
         float* red = reinterpret_cast<float*>(smem);          // [W_N][BM]
+        // (factors are powers of two: taken off for the sums and put back without a rounding)
+        auto times_factor = [&](bool back) {
+          if (!F16 || !g.row_factor) return;
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const float f = nw + 16 * j < N ? g.row_factor[nw + 16 * j] : 1.f, by = back ? 1.f / f : f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][r] *= by;
+          }
+        };
+        times_factor(false);
         wait_and_meet<0>();
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -571,6 +590,7 @@ __device__ __forceinline__ void head_gemm(Gemm g, uint16_t* smem, int block, int
           for (int w = 0; w < W_N; ++w) s += red[w * BM + c];
           g.d_sums[(int64_t)(n0 / BN) * g.ldd + m0 + c] = s;
         }
+        times_factor(true);
       }
 #pragma unroll
       for (int plane = 0; plane < (FINE ? 3 : 1); ++plane)
@@ -693,14 +713,22 @@ __device__ __forceinline__ int find_rows(const Rows& r, bool write, int* table) 
 }
 __global__ __launch_bounds__(1024) void ce_rows_kernel(Rows r) { find_rows(r, true, nullptr); }
 
-// g[i] = upstream * class weight / total of the kept rows; d_scale: (to / max |g|, max |g| / to); by one workgroup
+// fp16: d of a row whose factor g is 2^-k of the largest would sink into the subnormals with it (at 1e-7 of the largest the
+// gradient of a row of 30000 classes was off by 30 %).  Past FACTOR_FREE such a row's d is multiplied by 2^s, s up to FACTOR_MOST;
+// dx is multiplied by 2^-s where it is stored, and dW takes the row of x times 2^-s, which is exact down to |x| = 2^-4 or so
+// (s = 10) and off by 2^-25 below.  Rows down to 2^-16 of the largest so keep 11 bits of every probability from 2^-22 on, and a row
+// at 2^-24 from 2^-14 on.  Nothing of this where all factors are equal (one upstream gradient, no class weights);
+// elsewhere the copy of x times 2^-s takes 1 % (4093 x 1000 x 30011, reduction "none", 1074 and 1085 us).
+constexpr int FACTOR_FREE = 6, FACTOR_MOST = 10;
+// g[i] = upstream * class weight / total of the kept rows (times 2^s); d_scale: (to / max |g|, max |g| / to); factor: 2^-s by row;
+// by one workgroup
 struct Upstream {
   const float* up;                                            // null: nothing to do
   const int* state;
   int reduction, N;
   const float* cw;
   float to;
-  float *g, *d_scale;
+  float *g, *d_scale, *factor;                                // factor: null where it is 1 throughout
 };
 __device__ __forceinline__ void upstream(const Upstream& u) {
   __shared__ float red[16];
@@ -717,8 +745,17 @@ __device__ __forceinline__ void upstream(const Upstream& u) {
     top = fmaxf(top, fabsf(v));
   }
   top = block_max<16>(top, red);
+  const bool usable = top > 1e-30f && top < INFINITY;         // (nothing to do without a gradient; infinities reach the result)
+  if (u.factor) {
+    const auto exponent = [](float v) { return (int)(__float_as_uint(v) >> 23 & 255u); };
+    for (int i = threadIdx.x; i < kept; i += 1024) {
+      const float v = u.g[i];                                 // (this thread's own)
+      const int s = usable && v != 0.f ? min(max(exponent(top) - exponent(v) - FACTOR_FREE, 0), FACTOR_MOST) : 0;
+      u.g[i] = ldexpf(v, s);
+      u.factor[i] = ldexpf(1.f, -s);
+    }
+  }
   if (threadIdx.x == 0) {
-    const bool usable = top > 1e-30f && top < INFINITY;       // (nothing to do without a gradient; infinities reach the result)
     u.d_scale[0] = usable ? u.to / top : 1.f;
     u.d_scale[1] = usable ? top / u.to : 1.f;
   }
@@ -771,6 +808,16 @@ __device__ __forceinline__ void pack_rows(const Pack& p, int block, int D, int64
     } else {
       *reinterpret_cast<u4*>(o) = v.q[0];
     }
+  }
+}
+// fp16: out = the packed rows of x (rows, ldo) times their factors, 8 elements per thread
+__global__ __launch_bounds__(256) void ce_scale_rows_kernel(const _Float16* __restrict__ x, const float* __restrict__ factor,
+                                                            const int* __restrict__ state, int64_t ldo, _Float16* __restrict__ out) {
+  const int per = (int)(ldo / 8);
+  const int64_t all = (int64_t)state[S_KEPT] * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const _Float16 f = (_Float16)factor[i / per];             // (a power of two from 2^-10 on: exact)
+    reinterpret_cast<f16x8*>(out)[i] = reinterpret_cast<const f16x8*>(x)[i] * f;
   }
 }
 // All that comes ahead of the products, in one launch: the row factors, x, and w where it has to be packed.  Where the rows that
@@ -964,8 +1011,8 @@ constexpr int SLAB_ROWS = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void ce_slab_d_kernel(float* slabs, bool keep, int S, int64_t ldz, const T* __restrict__ bias,
                                                         const int* __restrict__ state, int N, int V, const float* __restrict__ gs,
-                                                        const float* __restrict__ d_scale, uint16_t* __restrict__ d, int64_t ldd, int64_t plane,
-                                                        float* __restrict__ sums) {
+                                                        const float* __restrict__ d_scale, const float* __restrict__ factor,
+                                                        uint16_t* __restrict__ d, int64_t ldd, int64_t plane, float* __restrict__ sums) {
   const int kept = state[S_KEPT], rows = (kept + 63) / 64 * 64, c = (blockIdx.x * 256 + threadIdx.x) * 4;
   const int first = blockIdx.y * SLAB_ROWS;
   if (first >= rows || c >= (V + 63) / 64 * 64) return;
@@ -978,11 +1025,12 @@ __global__ __launch_bounds__(256) void ce_slab_d_kernel(float* slabs, bool keep,
       const f4_any z = slab_logits(slabs + (int64_t)row * ldz, S, (int64_t)N * ldz, bias, c, V);
       const float lse = reinterpret_cast<const float*>(state)[S_ROWS + 2 * N + row];
       const int at = state[S_ROWS + N + row] - c;
+      const float of = factor ? factor[row] : 1.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p = exp_fine(z[e] - lse);
         v[e] = c + e < V ? (at == e ? p - 1.f : p) * g : 0.f;
-        total[e] += v[e];
+        total[e] = fmaf(v[e], of, total[e]);
       }
     }
     if (keep && row < kept && c < V) *reinterpret_cast<f4_any*>(slabs + (int64_t)row * ldz + c) = f4_any{v[0], v[1], v[2], v[3]};
@@ -1548,7 +1596,7 @@ struct Plan {
   bool grads_big, dx_slabs;                           // (dx is written as it is where it takes one product with one part)
   int dx_split, dw_split;
   // byte offsets in the workspaces
-  int64_t x, w, partial, tlogit, sums, g, scale, z, d, d_sums, slabs, slabs_w, bytes;
+  int64_t x, w, partial, tlogit, sums, g, scale, factor, scaled, z, d, d_sums, slabs, slabs_w, bytes;
 };
 
 constexpr int64_t D_BYTES = 512ll << 20;              // workspace for d, at most (but at least one tile of classes)
@@ -1613,6 +1661,9 @@ Plan plan_of(const vae_linear_ce* a, bool bwd) {
   } else {
     p.g = take(p.n_pad * 4);
     p.scale = take(8);
+    const bool f16 = a->dtype == VAE_ADAMW_F16;       // (which of its calls have factors by row is not known here)
+    p.factor = take(f16 ? p.n_pad * 4 : 0);
+    p.scaled = take(f16 ? p.n_pad * p.d_pad * 2 : 0);
     const int64_t fit = D_BYTES / (p.planes * p.n_pad * 2) / 256 * 256, most = up_to(a->V, 256);
     p.piece = fit < 256 ? 256 : fit < most ? fit : most;
     // pieces of equal length
@@ -1658,7 +1709,7 @@ template <int EPI> void logits(Gemm g, int dtype, bool big, hipStream_t st) {
 // partial logits, float slabs (split, N, ldz)
 void store_logits(Gemm g, const Tiles& t, int64_t ldz, void* slabs, int dtype, hipStream_t st) {
   g.split = t.split;
-  g.d_scale = nullptr;
+  g.d_scale = g.row_factor = nullptr;
   g.out = slabs;
   g.ldo = ldz;
   logits<EPI_STORE>(g, dtype, t.big, st);
@@ -1845,8 +1896,17 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
   float *slabs = reinterpret_cast<float*>(ws + p.slabs), *sums = reinterpret_cast<float*>(ws + p.d_sums);
   uint16_t *xp = reinterpret_cast<uint16_t*>(ws + p.x), *d = reinterpret_cast<uint16_t*>(ws + p.d);
   const int64_t plane_d = p.n_pad * p.piece, esize = p.f32 ? 4 : 2;
-  pack(a, p, ws, s, Rows{}, {grad, s, reduction, (int)a->N, a->class_weight, a->dtype == VAE_ADAMW_F16 ? 16384.f : 1.f, gr, scale}, st);
+  const bool f16 = a->dtype == VAE_ADAMW_F16;
+  float* factor = f16 && (reduction == VAE_CE_NONE || a->class_weight) ? reinterpret_cast<float*>(ws + p.factor) : nullptr;
+  pack(a, p, ws, s, Rows{}, {grad, s, reduction, (int)a->N, a->class_weight, f16 ? 16384.f : 1.f, gr, scale, factor}, st);
   VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+  if (factor && dw) {
+    const int64_t blocks = (a->N * (p.d_pad / 8) + 255) / 256;
+    ce_scale_rows_kernel<<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, st>>>(reinterpret_cast<const _Float16*>(xp), factor, s, p.d_pad,
+                                                                                   reinterpret_cast<_Float16*>(ws + p.scaled));
+    VAE_CHECK_LAUNCH("vae_linear_ce_bwd");
+    xp = reinterpret_cast<uint16_t*>(ws + p.scaled);
+  }
   for (int64_t v0 = 0; v0 < a->V; v0 += p.piece) {
     const int64_t n_v = a->V - v0 < p.piece ? a->V - v0 : p.piece;
     Gemm z = logits_gemm(a, p, ws, s);
@@ -1857,6 +1917,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     z.lse = reinterpret_cast<const float*>(s) + S_ROWS + 2 * a->N;
     z.g = gr;
     z.d_scale = scale;
+    z.row_factor = factor;
     z.d = d;
     z.ldd = p.piece;
     z.plane_d = plane_d;
@@ -1869,7 +1930,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
       float* zs = reinterpret_cast<float*>(ws + p.z);
       float* to = dbias ? sums : nullptr;
 #define VAE_CE(T)                                                                                                               \
-  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(zs, p.few, p.z_parts, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, gr, scale, d, \
+  ce_slab_d_kernel<T><<<grid, 256, 0, st>>>(zs, p.few, p.z_parts, p.ldz, (const T*)a->bias, s, (int)a->N, (int)n_v, gr, scale, factor, d, \
                                             p.piece, plane_d, to)
       if (p.f32) VAE_CE(float);
       else if (a->dtype == VAE_ADAMW_BF16) VAE_CE(__bf16);
@@ -1893,6 +1954,7 @@ extern "C" int vae_linear_ce_bwd(const vae_linear_ce* a, int reduction, const fl
     gx.segs = z.segs;
     gx.dyn = s + S_KEPT;
     gx.d_scale = scale;
+    gx.row_factor = factor;
     gx.out = p.dx_slabs ? (void*)slabs : dx;
     gx.out_kind = p.dx_slabs ? 0 : p.f32 ? 2 : 1;
     gx.rows = p.dx_slabs ? nullptr : s + S_ROWS;
