@@ -641,10 +641,17 @@ int vae_gated_norm_bwd(const vae_gated_norm* args, float* workspace, int64_t wor
  * state: vae_linear_ce_state_bytes(N) bytes that the forward pass writes and the backward pass of the same arguments reads.
  * The backward pass takes the float gradient of the loss ((N) or (1)) and overwrites the dense dx (N, D), dw (V, D) and dbias
  * (V) that are not null, of the operands' type.  Ignored rows take no part at all: their dx is 0 and what their x holds
- * reaches nothing else.  The logits are not kept; the workspace holds a packed copy of x, for fp32 (and for w that is
- * not 16-byte aligned with D and its stride multiples of 8) one of w, up to 512 MiB of logit gradients, and for few rows and
- * classes over many features partial logits of at most 134 MB.  At most 2^24 tiles of 128 x 128 in N x V, N x D and V x D.  Same
- * bits every time.                                                                                                          */
+ * reaches nothing else.  Same bits every time.  At most 2^24 tiles of 128 x 128 in N x V, N x D and V x D.
+ * Sums, the softmax statistics and the loss are held in 32 bits.  The gradients of the logits, divided by their row's factor
+ * (upstream gradient times class weight), are rounded to the operands' type ahead of the products that give dx and dw (fp32: to
+ * three bf16 terms, 24 bits), each off by half a step of its own and independently of the others; dbias sums them unrounded.
+ * fp16 holds a probability in 11 bits from 2^-22 of 1 on in rows whose factor is 2^-16 of the largest or more, and in fewer below.
+ * The logits are not kept.  The workspace holds x packed to multiples of 256 rows and 64 columns, for fp32 (and for w that is not
+ * 16-byte aligned with D and its stride multiples of 8) w packed to multiples of 64 columns, 6 bytes an element for fp32 and 2
+ * otherwise.  Forward: 8 bytes a row for every 128 classes, and 12 bytes a row.  Backward: gradients of logits, of 2 bytes (fp32:
+ * 6), for all rows and as many classes at a time as 512 MiB hold, 256 at least; where there is a bias, sums of them over 8 or 128 rows; in
+ * fp16 a second copy of x; float parts of dx and of dw, each of at most 134 MB, or N x D floats for dx where that is more.  Either way
+ * partial logits of at most 134 MB where there are few rows or classes over many features, and some bytes a row.              */
 enum { VAE_CE_NONE = 0, VAE_CE_SUM = 1, VAE_CE_MEAN = 2 };
 typedef struct {
   int64_t N, D, V;

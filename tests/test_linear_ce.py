@@ -63,6 +63,46 @@ def test_refusals_of_the_c_entry():
     assert lib.vae_linear_ce_workspace_bytes(C.byref(big), 1) < (512 << 20) + 4 * 8192 * 4096 + 2 * 8192 * 4096 + (1 << 20)
 
 
+def _workspace_bound(n, d, v, dtype, bias, packed, backward):
+    """The parts that include/vae_amd.h lists, each rounded up to 256 bytes."""
+    up = lambda a, b: -(-a // b) * b  # noqa: E731
+    e, rows, cols, part = 6 if dtype == 0 else 2, up(n, 256), up(d, 64), 134_217_728 + 256
+    total = e * rows * cols + (e * v * cols if packed else 0) + 12 * 256
+    if not backward:
+        return total + max(8 * rows * (up(v, 128) // 128), part) + 12 * rows
+    classes = min(up(v, 256), max(256, (512 << 20) // (e * rows)))
+    total += e * rows * classes + 8 * rows + (2 * rows * cols if dtype == 2 else 0)
+    total += (max(4 * classes * (rows // 128), 4 * classes * (rows // 8) if rows * classes <= 1 << 26 else 0) if bias else 0)
+    return total + max(part, 4 * n * d) + part + part
+
+
+def test_workspaces_are_what_the_header_says():
+    """Random sizes up to the limits, long batches among them (which hold 256 classes however many bytes these take)."""
+    import random
+    from vae_amd import _lib
+    lib, rng, seen = _lib.load(), random.Random(1), 0
+    sizes = [(1 << 21, 64, 1000), (1 << 20, 4096, 500), (1 << 24, 1, 100), (1, 1 << 20, 7), (64, 1 << 20, 1000), (8192, 4096, 1 << 20)]
+    sizes += [tuple(int(2 ** rng.uniform(0, k)) for k in (24, 20, 24)) for _ in range(3000)]
+    for n, d, v in sizes:
+        tiles = [-(-a // 128) * -(-b // 128) for a, b in ((n, v), (n, d), (v, d))]
+        if max(tiles) >= 1 << 24:
+            continue
+        seen += 1
+        for dtype in range(3):
+            for bias in (None, 4096):
+                for backward in (0, 1):
+                    ldw = d + rng.randrange(2)
+                    a = _lib.LinearCE(N=n, D=d, V=v, dtype=dtype, x=4096, ldx=d, w=8192, ldw=ldw, target=4096, bias=bias, ignore_index=-100)
+                    if ldw >= 1 << 22:
+                        continue
+                    got = lib.vae_linear_ce_workspace_bytes(C.byref(a), backward)
+                    packed = dtype == 0 or d % 8 != 0 or ldw % 8 != 0
+                    assert 0 <= got <= _workspace_bound(n, d, v, dtype, bias, packed, backward), (n, d, v, dtype, bias, backward, got)
+    assert seen > 1000
+    long = _lib.LinearCE(N=1 << 21, D=64, V=1000, dtype=1, x=4096, ldx=64, w=8192, ldw=64, target=4096, ignore_index=-100)
+    assert lib.vae_linear_ce_workspace_bytes(C.byref(long), 1) > (1 << 30)               # 256 classes of 2^21 rows
+
+
 def test_refusals_of_the_python_entry():
     from vae_amd.losses import linear_cross_entropy
     x, w, t = torch.zeros(3, 8), torch.zeros(5, 8), torch.zeros(3, dtype=torch.int64)
