@@ -348,3 +348,33 @@ def test_strided_vectors():
     torch.autograd.backward([y, h], [dy, dh])
     total = grads["scale"].double()
     assert abs(float(s.grad) - float(total.sum())) <= 2.0 ** -7 * float(total.abs().sum())  # (torch adds 300 of them in bf16's terms)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,n", [(700, 4500), (1000, 4500), (2000, 2300), (1531, 2100), (5000, 800), (8192, 700), (9001, 600), (16384, 520)])
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kind,gate,bias", [("layer", "full", True), ("rms", "row", False)])
+def test_workgroups_that_walk_over_several_rows(d, n, dtype, kind, gate, bias):
+    """More rows than workgroups on two, four, eight and sixteen waves: loads ahead of their row, and column sums over rows."""
+    x, dy, dh = _inputs(n, d, dtype, gate, True, True, bias, d % 2 == 1, seed=d)
+    out, grads = _run(x, dy, dh, kind, "tanh")
+    ref, rgrads = _oracle(x, dy, dh, kind, "tanh", out[0])
+    for name, a, b in zip(("y", "h"), out, ref):
+        _close(name, a, b, DT[dtype])
+    for k, g in grads.items():
+        _close(k, g, rgrads[k], g.dtype)
+
+
+@pytest.mark.gpu
+def test_the_kernel_entries_beside_autograd():
+    """ops.gated_norm_fwd / gated_norm_bwd give what the differentiable form gives, and only what is asked for."""
+    from vae_amd import ops
+    x, dy, dh = _inputs(33, 300, "bf16", "full", True, True, True, False, seed=4)
+    out, grads = _run(x, dy, dh, "layer", "sigmoid")
+    vectors = {k: x[k] for k in NAMES[3:]}
+    y, h, stats = ops.gated_norm_fwd(x["r"], x["b"], x["gate"], **vectors, kind="layer")
+    assert torch.equal(y, out[0]) and torch.equal(h, out[1])
+    got = ops.gated_norm_bwd(dy, dh, y, x["b"], stats, x["gate"], **vectors, kind="layer")
+    assert set(got) == set(grads) and all(torch.equal(got[k], grads[k]) for k in grads)
+    some = ops.gated_norm_bwd(dy, dh, y, x["b"], stats, x["gate"], **vectors, kind="layer", want=("scale",))
+    assert set(some) == {"r", "b", "scale"} and all(torch.equal(some[k], grads[k]) for k in some)

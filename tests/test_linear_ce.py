@@ -143,6 +143,47 @@ def test_strides_are_no_reason_to_refuse():
             call()
 
 
+def _rms(t):
+    return float(t.double().square().mean().sqrt())
+
+
+def _expected_loss_error(z_t, lse, loss, steps):
+    """Root mean square over the rows of what the roundings of a loss come to, with a quarter to spare.
+
+    z_t: a running sum over ``steps`` of matrix instructions, each of which rounds it once or twice.  A rounding has a standard
+    deviation of ulp / sqrt(12), over the mantissas 2^-25.2 of the value; the mean square of the partial sums is at most half that
+    of the whole, whether it grows steadily (a third) or as a random walk (a half): 2^-25.2 sqrt(2 steps / 2) rms(z_t).
+    Else: five roundings of lse's size (maximum, scaled logit and its offset, logarithm, sum), two of z_t's and one of the
+    loss's, of 2^-24 / sqrt(3) each."""
+    sums = 1.25 * 2.0 ** -25.2 * steps ** 0.5 * _rms(z_t)
+    return (sums ** 2 + (5 * _rms(lse) ** 2 + 2 * _rms(z_t) ** 2 + _rms(loss) ** 2) * 2.0 ** -48 / 3) ** 0.5
+
+
+def _three_terms(t):
+    h = t.bfloat16().float()
+    m = (t - h).bfloat16().float()
+    return h.double(), m.double(), (t - h - m).bfloat16().double()
+
+
+@pytest.mark.parametrize("d", [64, 512, 4096])
+def test_the_expected_error_shows_a_missing_product_of_terms(d):
+    """fp32 operands as three bf16 terms: without even the smallest of the six products the loss is off by more than that."""
+    g = torch.Generator().manual_seed(0)
+    n, v = 1000, 500
+    w = torch.randn(v, d, generator=g) / d ** 0.5
+    t = torch.randint(0, v, (n,), generator=g)
+    x = torch.randn(n, d, generator=g) + 2 * w[t]
+    z = x.double() @ w.double().t()
+    pick = lambda q: (q.logsumexp(1), q.gather(1, t[:, None])[:, 0])  # noqa: E731
+    lse, z_t = pick(z)
+    bound = _expected_loss_error(z_t, lse, lse - z_t, 6 * d / 32)
+    xs, ws = _three_terms(x), _three_terms(w)
+    six = [(0, 0), (0, 1), (1, 0), (0, 2), (2, 0), (1, 1)]
+    for left_out in (None, (1, 1), (0, 2), (2, 0)):
+        a, b = pick(sum(xs[i] @ ws[j].t() for i, j in six if (i, j) != left_out))
+        assert (_rms(a - b - lse + z_t) > bound) == (left_out is not None), left_out
+
+
 def test_class_weights_keep_their_bits():
     """A head that is moved to 16 bits takes its parameters along, not the class weights."""
     from vae_amd.losses import LinearCrossEntropyLoss
@@ -549,3 +590,56 @@ def test_fp16_factors_in_a_graph():
         torch.cuda.synchronize()
         want = _run(static, "none", up)
         assert torch.equal(loss, want[0]) and all(torch.equal(grads[name], want[1][name]) for name in grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v,dtype", [(2048, 512, 3000, "fp32"), (1000, 4096, 500, "fp32"), (64, 1024, 40000, "fp32"), (4096, 3000, 30, "fp32"),
+                                         (2048, 512, 3000, "bf16"), (600, 2000, 900, "fp16"), (8192, 4000, 10, "bf16"), (3000, 1536, 9000, "fp16")])
+def test_losses_are_as_exact_as_their_sums(n, d, v, dtype):
+    """The mean error of the losses of many rows, where single ones are held to the bound of the largest (test_shapes).  A sum's
+    steps: products of 32 of D, six of them for fp32; where fp32 goes into 32-bit instructions (few rows or classes) one for every
+    feature, in two sums at least."""
+    s = _inputs(n, d, v, dtype, False, False, 0.0, seed=n)
+    z = s["x"].double() @ s["w"].double().t()
+    lse, z_t = z.logsumexp(1), z.gather(1, s["target"][:, None])[:, 0]
+    got, _ = _run(s, "none", torch.ones(n, device="cuda"))
+    steps = d / 2 if dtype == "fp32" and min(n, v) <= 64 else 6 * d / 32 if dtype == "fp32" else d / 32
+    assert _rms(got.double() - lse + z_t) <= _expected_loss_error(z_t, lse, lse - z_t, steps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", [(600, 512, 500), (2048, 256, 1500), (64, 1024, 4000)])
+def test_fp32_gradients_are_as_exact_as_their_sums(n, d, v):
+    """As above for dx and dW.  Their terms are products of d, whose p is off by the error of z - lse, its own in every class and one
+    for the row, and which is held in 24 bits; a sum rounds at the size of its value or of its terms' root sum of squares; the
+    result, its factors and d are rounded four times."""
+    s = _inputs(n, d, v, "fp32", False, False, 0.0, seed=n)
+    x, w, t = s["x"].double(), s["w"].double(), s["target"]
+    z = x @ w.t()
+    lse, z_t = z.logsumexp(1), z.gather(1, t[:, None])[:, 0]
+    few = n <= 64
+    off = _expected_loss_error(z_t, lse, lse - z_t, d / 2 if few else 6 * d / 32)
+    p = torch.softmax(z, 1)
+    dl = p.clone()
+    dl[torch.arange(n), t] -= 1
+    _, grads = _run(s, "sum")
+    for name, a, b, pa, steps in (("x", dl, w, p, v / 2 if few else 6 * v / 32), ("w", dl.t(), x, p.t(), 6 * n / 32)):
+        val = a @ b
+        size = val.square() + a.square() @ b.square()
+        bound = ((1.25 * 2.0 ** -25.2) ** 2 * steps + 4 * 2.0 ** -48 / 3) * size + off ** 2 * (pa.square() @ b.square() + (pa @ b).square())
+        assert _rms(grads[name].double() - val) <= float(bound.mean().sqrt()), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,v", [(5000, 40, 30000), (4100, 64, 20000), (3000, 7, 9000), (130, 60, 70000), (100, 33, 80000), (9000, 1, 7000)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("ignored", [0.0, 0.6])
+def test_one_step_of_features_and_many_tiles(n, d, v, dtype, ignored):
+    """Workgroups that stay for several tiles of one step: both loads on the way belong to tiles other than the one in work."""
+    s = _inputs(n, d, v, dtype, True, False, ignored, seed=n + d)
+    s["target"][n // 2] = v - 1
+    loss, grads = _run(s, "mean")
+    _check(s, "mean", loss, grads)
+    got, _ = _run(s, "none", torch.ones(n, device="cuda"))
+    ref, _ = _oracle(s, "none")
+    assert bool(((got.double() - ref).abs() <= 2e-6 * ref + 1e-6).all())
