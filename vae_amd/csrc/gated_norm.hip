@@ -14,8 +14,10 @@
 // up to 64 16-byte pieces, a workgroup of up to 1024 threads a longer one, one to four pieces per thread.  A workgroup walks
 // over rows; the gradients of the vectors over columns are summed in registers over its rows, written once per workgroup, and
 // added up in a second launch in a fixed order (no atomics: same bits every time).  32768 x 4096 bf16 with a full gate: forward
-// 311 us = 4.3 TB/s, backward 455 us = 4.7 TB/s (a large copy: 4.9); without the next row's loads ahead of this row's work 373
-// and 712.
+// 269 us = 4.9 TB/s, backward 440 us = 4.8 TB/s (a large copy: 4.9); without the next row's loads ahead of this row's work
+// some 60 and 260 us more.  Rows on 16 waves (16 bits or fp32 beyond 4096 or 2048 columns) have no room for those loads, and from
+// 4097 columns on the backward pass keeps part of its column sums in scratch: 16384 x 8192 bf16 forward 361 us, both 1646; 8192 x
+// 16384 293 and 2425.
 #include "../../include/vae_amd.h"
 #include "common.h"
 

@@ -18,11 +18,11 @@
 // chip is K split instead, and partial logits of at most 134 MB are written and read once (64 x 4000 x 900 bf16: both passes 70 us,
 // 129 without; 901 x 3014 x 1683 fp32 326 and 527).
 //
-// Types: bf16 and fp16 multiply as they are, sums in 32 bits; d is rounded to the same type (relative 2^-9 or 2^-12 of each
+// Types: bf16 and fp16 multiply as they are, sums in 32 bits; d is rounded to the same type (by at most 2^-8 or 2^-11 of each
 // element, independent of each other, so that a sum of them is off by no more than its own rounding).  d is divided by the
 // largest factor g_i c[t_i] for that, and the products are multiplied by it in 32 bits: the term of the target, -1 in nearly
 // every row of a large vocabulary, is then exact, where the rounding of 1 / N itself would shift every gradient by the same
-// 2^-9 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
+// part, up to 2^-8 (error against 64 bits 3.7e-3 with it, 1.7e-3 without).  fp16 could not hold d, which goes down to 1e-12: it is
 // multiplied by 2^14 as well, and where factors differ from row to row (see FACTOR_FREE) a row far below the largest one by a
 // power of two of its own.  fp32 operands are split exactly into three bf16 terms, and for every 64 of K the six products
 // that matter run one after the other: the error is that of 32-bit sums, at a sixth of the 16-bit rate (a 32-bit matrix
@@ -90,7 +90,8 @@ __device__ __forceinline__ void split3(float v, __bf16& h, __bf16& m, __bf16& l)
   l = (__bf16)(r - (float)m);
 }
 
-// exp to an ulp or so for v <= 88, 0 far below, NaN for NaN: the rounding error of v * log2 e is fed back
+// exp to an ulp or so for v <= 88, 0 far below: the rounding error of v * log2 e is fed back.  As vae_exp_acc, which takes a NaN for
+// -inf, where this one passes it on (a NaN logit has to show in its row's loss)
 __device__ __forceinline__ float exp_fine(float v) {
   v = v < -100.f ? -100.f : v;
   const float t = v * 1.44269504088896341f;

@@ -13,9 +13,9 @@
 // HBM-bound: (p, g, m, v) are read and (p, m, v) written once, 28 bytes per fp32 parameter with 32-bit moments, 16 with
 // 8-bit ones; gradient clipping reads g once more.  A wave takes 512 elements, 8 per lane: 16-byte accesses for 16-bit
 // types and 32 lanes = one quantisation block, whose two maxima are five DPP / swizzle steps.  The tensors travel as kernel
-// arguments, up to 96 to a launch: nothing has to be uploaded or kept between calls.  1e9 bf16 parameters in 300 tensors with
-// fp32 master weights and 8-bit moments: 3.21 ms = 5.0 TB/s; 18 M fp32 ones with 32-bit moments and clipping: 122 us, of which
-// the norm 27 (a large copy: 4.9 TB/s).
+// arguments, up to 96 and up to eight counts of steps to a launch: nothing has to be uploaded or kept between calls.  1e9 bf16
+// parameters in 300 tensors with fp32 master weights and 8-bit moments: 3.22 ms = 5.0 TB/s; 18 M fp32 ones with 32-bit moments and
+// clipping: 123 us, of which the norm 26 (a large copy: 4.9 TB/s).
 #include "../../include/vae_amd.h"
 #include "common.h"
 

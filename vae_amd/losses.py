@@ -116,12 +116,12 @@ def linear_cross_entropy(x: torch.Tensor, w: torch.Tensor, target: torch.Tensor,
 
     ``x``, ``w`` and ``bias`` are float32, bfloat16 or float16, all of one type; sums, the softmax statistics and the loss are
     held in 32 bits.  The gradients of the logits are rounded to that type (float32: to 24 bits) ahead of the products that
-    give those of ``x`` and ``w``, as the backward pass of a linear layer in 16 bits does.  ``target`` (...) int64; ``weight`` (V) float32 class weights.  Rows whose target is ``ignore_index`` take no
-    part: their loss and gradient are 0, and they cost next to nothing.  Any other target outside [0, V) makes its row's loss and
-    gradient in ``x`` NaN, and what sums over rows: the reduced loss and the gradients in ``w`` and ``bias`` (torch stops with a
-    device assertion).  "mean" divides by the sum of the class weights that took part (NaN when none did; the gradients are 0
-    then).  A class is ruled out by a bias of -inf or of the type's lowest value; what an infinity in ``w`` or in a row of
-    ``x`` that takes part reaches is infinite or NaN.
+    give those of ``x`` and ``w``, as the backward pass of a linear layer in 16 bits does.  ``target`` (...) int64; ``weight`` (V)
+    float32 class weights.  Rows whose target is ``ignore_index`` take no part: their loss and gradient are 0, and they cost
+    next to nothing.  Any other target outside [0, V) makes its row's loss and gradient in ``x`` NaN, and what sums over rows:
+    the reduced loss and the gradients in ``w`` and ``bias`` (torch stops with a device assertion).  "mean" divides by the sum of
+    the class weights that took part (NaN when none did; the gradients are 0 then).  A class is ruled out by a bias of -inf or
+    of the type's lowest value; what an infinity in ``w`` or in a row of ``x`` that takes part reaches is infinite or NaN.
 
     The backward pass holds the logits' gradients of all rows and as many classes as 512 MiB take, 256 at least: a batch of
     millions of rows is better given in parts (include/vae_amd.h lists the workspaces)."""
